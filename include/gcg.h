@@ -515,6 +515,43 @@ GCG_API int gcg_bwd_time_major(const void *dy, const void *x, const void *B, con
             void *workspace, size_t workspace_bytes,
             int64_t bs, int64_t L, int32_t g, int32_t dg, int32_t hl, int32_t dtype, void *stream);
 
+/*
+ * Activation checkpoints in 8 bits: a contiguous (rows, D) tensor as codes (rows, D) and fp32 scales
+ * (rows, ceil(D / GCG_BLOCK8)), of which gcg_unpack8 makes a tensor again for the backward pass.
+ * Blocks of GCG_BLOCK8 elements along a row share a scale (a row's last block may be shorter):
+ *
+ *     top = max |x|;  scale = top * fp32(1 / 127);  code = rint(x * (127 / top));  value = code * scale
+ *
+ * in fp32 arithmetic, the value rounded once to the tensor's type.  Both kernels are exact functions of their
+ * inputs, the same on every run.  A block with top < 2^-100 is kept as zeros, one that holds an infinity or a NaN
+ * comes back as NaN throughout.  Any D, any alignment of the element type.  dtype: GCG_F32, GCG_BF16, GCG_F16.
+ */
+enum { GCG_BLOCK8 = 128 };
+GCG_API int gcg_pack8(const void *x, int8_t *codes, float *scales, int64_t rows, int64_t D, int32_t dtype, void *stream);
+GCG_API int gcg_unpack8(const int8_t *codes, const float *scales, void *x, int64_t rows, int64_t D, int32_t dtype, void *stream);
+
+/*
+ * Layer norm over the last dimension of a contiguous (rows, D) tensor, and its backward:
+ *
+ *     y = (x - mean) * rstd * w + b,   mean = sum x / D,   rstd = (sum (x - mean)^2 / D + eps)^-1/2
+ *     g = dy * w;  dx = rstd * (g - mean(g) - xh * mean(g * xh)), xh = (x - mean) * rstd;  dw = sum dy * xh;  db = sum dy
+ *
+ * Statistics and sums are fp32, y and dx are rounded once.  w, b (D) may be null (1 and 0); they and dw, db have the
+ * tensors' type, or are fp32 with 16-bit tensors (GCG_BF16_F32, GCG_F16_F32).  stats: (rows, 2) fp32, mean and rstd, which
+ * the backward needs; may be null in the forward.  codes, scales: both or neither.  In the forward they take x's 8-bit
+ * checkpoint (gcg_pack8's, bit for bit) from the same pass; in the backward they are given instead of x, and xh is formed of the
+ * checkpoint's values with the exact row's mean and rstd.  dw, db may be null.  dw, db are overwritten and
+ * bit-reproducible.  workspace: gcg_layer_norm_bwd_workspace_bytes, 256-byte aligned; not needed if dw and db are null.
+ * D up to GCG_NORM_MAX_WIDTH, else GCG_ERR_UNSUPPORTED.
+ */
+enum { GCG_NORM_MAX_WIDTH = 16384 };
+GCG_API int gcg_layer_norm_fwd(const void *x, const void *w, const void *b, void *y, float *stats, int8_t *codes, float *scales,
+            int64_t rows, int32_t D, float eps, int32_t dtype, void *stream);
+GCG_API size_t gcg_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t D, int32_t dtype);
+GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *codes, const float *scales, const float *stats,
+            const void *w, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
+            int64_t rows, int32_t D, int32_t dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

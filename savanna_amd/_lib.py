@@ -40,6 +40,7 @@ EXPORTS = (
     "gcg_mixer_mr_fwd", "gcg_mixer_mr_bwd_workspace_bytes", "gcg_mixer_mr_bwd_scratch_bytes", "gcg_mixer_mr_bwd", "gcg_mixer_mr_fwd_decay", "gcg_mixer_mr_bwd_decay",
     "gcg_mixer_mr_fwd_planar", "gcg_mixer_mr_bwd_planar", "gcg_mixer_mr_fwd_planar_decay", "gcg_mixer_mr_bwd_planar_decay", "gcg_fwd_time_major", "gcg_bwd_time_major_workspace_bytes", "gcg_bwd_time_major",
     "gcg_fwd_decay", "gcg_bwd_decay", "gcg_fwd_interleaved_decay", "gcg_bwd_interleaved_decay",
+    "gcg_pack8", "gcg_unpack8", "gcg_layer_norm_fwd", "gcg_layer_norm_bwd_workspace_bytes", "gcg_layer_norm_bwd",
 )
 
 _lock = threading.Lock()
@@ -147,6 +148,16 @@ def load() -> ctypes.CDLL:
         lib.gcg_fwd_interleaved_decay.restype = ctypes.c_int
         lib.gcg_bwd_interleaved_decay.argtypes = [vp] * 4 + [i32] + [vp] * 3 + [sz, i64, i64, i32, i32, i32, i32, i32, vp]
         lib.gcg_bwd_interleaved_decay.restype = ctypes.c_int
+        lib.gcg_pack8.argtypes = [vp] * 3 + [i64, i64, i32, vp]
+        lib.gcg_pack8.restype = ctypes.c_int
+        lib.gcg_unpack8.argtypes = lib.gcg_pack8.argtypes
+        lib.gcg_unpack8.restype = ctypes.c_int
+        lib.gcg_layer_norm_fwd.argtypes = [vp] * 7 + [i64, i32, ctypes.c_float, i32, vp]
+        lib.gcg_layer_norm_fwd.restype = ctypes.c_int
+        lib.gcg_layer_norm_bwd_workspace_bytes.argtypes = [i64, i32, i32]
+        lib.gcg_layer_norm_bwd_workspace_bytes.restype = sz
+        lib.gcg_layer_norm_bwd.argtypes = [vp] * 10 + [sz, i64, i32, i32, vp]
+        lib.gcg_layer_norm_bwd.restype = ctypes.c_int
         _lib = lib
         return lib
 
@@ -980,3 +991,143 @@ def select_algo(bs, L, g, dg, hl, dtype: torch.dtype, backward=False) -> str:
     if rc < 0:
         check(rc, "gcg_select_algo")
     return {v: k for k, v in ALGO_NAMES.items()}[rc]
+
+
+# ---- 8-bit activation checkpoints and layer norm ----------------------------------------------------
+
+BLOCK8 = 128                        # GCG_BLOCK8
+NORM_MAX_WIDTH = 16384              # GCG_NORM_MAX_WIDTH
+
+
+def _check_rows(t: torch.Tensor, name: str = "x") -> None:
+    if t.dim() < 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of at least one dimension")
+
+
+def _scale_shape(shape) -> tuple:
+    return (*shape[:-1], (shape[-1] + BLOCK8 - 1) // BLOCK8)
+
+
+def _check_codes(codes, scales) -> None:
+    _check_rows(codes, "codes")
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not scales.is_contiguous() \
+            or tuple(scales.shape) != _scale_shape(codes.shape) or scales.device != codes.device:
+        raise ValueError(f"codes must be int8, and scales contiguous float32 with one element for every {BLOCK8} codes of a row")
+
+
+def pack8(x):
+    """(codes, scales) of a contiguous tensor's 8-bit checkpoint; blocks of 128 along the last dimension."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.pack8, x)
+    lib = load()
+    _check_rows(x)
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty(_scale_shape(x.shape), dtype=torch.float32, device=x.device)
+    code = dtype_code(x.dtype)
+    if x.numel() == 0:
+        return codes, scales
+    D = x.shape[-1]
+    with _on_device(x.device):
+        rc = lib.gcg_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // D, D, code,
+                           torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_pack8")
+    return codes, scales
+
+
+def unpack8(codes, scales, dtype: torch.dtype):
+    """The tensor of ``dtype`` that an 8-bit checkpoint stands for."""
+    _require_gpu(codes)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.unpack8, codes, scales, dtype)
+    lib = load()
+    _check_codes(codes, scales)
+    x = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    code = dtype_code(dtype)
+    if x.numel() == 0:
+        return x
+    D = x.shape[-1]
+    with _on_device(codes.device):
+        rc = lib.gcg_unpack8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), x.numel() // D, D, code,
+                             torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_unpack8")
+    return x
+
+
+def _norm_code(x, w, b) -> int:
+    code, wide = dtype_code(x.dtype), False
+    _check_rows(x)
+    if not 0 < x.shape[-1] <= NORM_MAX_WIDTH:
+        raise ValueError(f"layer norm over {x.shape[-1]} elements; 1 to {NORM_MAX_WIDTH} are supported")
+    for p in (w, b):
+        if p is None:
+            continue
+        if p.dim() != 1 or p.shape[0] != x.shape[-1] or p.device != x.device or not p.is_contiguous():
+            raise ValueError("weight and bias must be contiguous, on x's device and of the size of x's last dimension")
+        if p.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"weight and bias must have x's dtype or be float32; got {p.dtype} with {x.dtype}")
+        wide = p.dtype != x.dtype
+    if w is not None and b is not None and w.dtype != b.dtype:
+        raise TypeError("weight and bias must share one dtype")
+    return code if not wide else GCG_BF16_F32 if code == GCG_BF16 else GCG_F16_F32
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def layer_norm_fwd(x, w, b, eps: float, save_8bit: bool = False, stats: bool = True):
+    """(y, stats, codes, scales) over the last dimension of a contiguous x; w, b may be None.  ``stats`` (mean and rstd of
+    every row) is what the backward needs; codes and scales, x's 8-bit checkpoint, are empty without ``save_8bit``."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        if not (stats or save_8bit):
+            return _run(torch.ops.gcg.layer_norm_infer, x, w, b, eps), None, None, None
+        return _run(torch.ops.gcg.layer_norm_fwd, x, w, b, eps, save_8bit)
+    lib = load()
+    code = _norm_code(x, w, b)
+    y, f32 = torch.empty_like(x), dict(dtype=torch.float32, device=x.device)
+    kept = torch.empty((*x.shape[:-1], 2), **f32) if stats or save_8bit else None
+    codes = torch.empty(x.shape if save_8bit else (0,), dtype=torch.int8, device=x.device)
+    scales = torch.empty(_scale_shape(x.shape) if save_8bit else (0,), **f32)
+    if x.numel():
+        D = x.shape[-1]
+        with _on_device(x.device):
+            rc = lib.gcg_layer_norm_fwd(x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(kept),
+                                        codes.data_ptr() if save_8bit else None, scales.data_ptr() if save_8bit else None,
+                                        x.numel() // D, D, eps, code, torch.cuda.current_stream().cuda_stream)
+        check(rc, "gcg_layer_norm_fwd")
+    return y, kept, codes, scales
+
+
+def layer_norm_bwd(dy, x, codes, scales, stats, w, b):
+    """(dx, dw, db); x, or its 8-bit checkpoint and None in x's place.  w and b say which gradients are wanted."""
+    _require_gpu(dy)
+    if TORCH_OPS:
+        return torch.ops.gcg.layer_norm_bwd(dy, x, codes, scales, stats, w, b)
+    lib = load()
+    code = _norm_code(dy, w, b)
+    if (codes is None) != (scales is None) or (x is None) == (codes is None):
+        raise ValueError("the backward takes either x, or its codes and scales")
+    if codes is not None:
+        _check_codes(codes, scales)
+    source = x if x is not None else codes
+    if source.shape != dy.shape or source.device != dy.device or not source.is_contiguous() or (x is not None and x.dtype != dy.dtype):
+        raise ValueError("dy must be a contiguous tensor with the shape, dtype and device of x")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (*dy.shape[:-1], 2) or not stats.is_contiguous() or stats.device != dy.device:
+        raise ValueError("stats must be the forward's")
+    D = dy.shape[-1]
+    rows = dy.numel() // D
+    dx = torch.empty_like(dy)
+    dw = torch.empty_like(w) if w is not None else None
+    db = torch.empty_like(b) if b is not None else None
+    if rows == 0:
+        return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
+    nbytes = lib.gcg_layer_norm_bwd_workspace_bytes(rows, D, code)
+    with _on_device(dy.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+        rc = lib.gcg_layer_norm_bwd(dy.data_ptr(), _ptr(x), _ptr(codes), _ptr(scales), stats.data_ptr(), _ptr(w), dx.data_ptr(),
+                                    _ptr(dw), _ptr(db), ws.data_ptr(), nbytes, rows, D, code,
+                                    torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_layer_norm_bwd")
+    return dx, dw, db

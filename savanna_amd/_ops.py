@@ -37,10 +37,11 @@ OP_NAMES = (
     "mixer_se_fwd", "mixer_se_bwd", "filter_decay_fwd", "filter_decay_bwd",
     "mixer_mr_fwd", "mixer_mr_bwd", "mixer_mr_fwd_decay", "mixer_mr_bwd_decay", "fwd_time_major", "bwd_time_major", "fwd_decay", "bwd_decay", "fwd_interleaved_decay", "bwd_interleaved_decay",
     "fwd_planar", "bwd_planar",
+    "pack8", "unpack8", "layer_norm_fwd", "layer_norm_infer", "layer_norm_bwd",
 )
 
 # differentiable as they are: C++ autograd nodes around operators above, which a trace sees in their place
-NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay")
+NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay", "layer_norm")
 
 
 # ---- autograd --------------------------------------------------------------------------------------------
@@ -123,10 +124,24 @@ def _register_autograd():
         return dfeat, dw, None, None, None
     reg("gcg::fwd_interleaved_decay", interleaved_decay, setup_context=save(0, 1, 2))
 
+    def norm_setup(ctx, inputs, output):     # layer_norm_fwd(x, w, b, eps, save_8bit) -> y, stats, codes, scales
+        x, w, b, _, ctx.save_8bit = inputs
+        _, stats, codes, scales = output
+        ctx.save_for_backward(*((None, codes, scales) if ctx.save_8bit else (x, None, None)), stats, w, b)
+
+    def norm(ctx, dy, *_):
+        w, b = ctx.saved_tensors[4:]
+        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), *ctx.saved_tensors)
+        return dx, dw if w is not None else None, db if b is not None else None, None, None
+    reg("gcg::layer_norm_fwd", norm, setup_context=norm_setup)
+
     def refuse(name, hint):
         def backward(ctx, *grads):
             raise RuntimeError(f"torch.ops.gcg.{name} is not differentiable; {hint}")
         return backward
+    nothing = lambda ctx, inputs, output: None                                       # noqa: E731
+    reg("gcg::layer_norm_infer", refuse("layer_norm_infer", "use torch.ops.gcg.layer_norm"), setup_context=nothing)
+    reg("gcg::pack8", refuse("pack8", "a checkpoint is what a backward pass reads"), setup_context=nothing)
     reg("gcg::fwd_full", refuse("fwd_full", "use torch.ops.gcg.fwd for a differentiable y"), setup_context=lambda ctx, inputs, output: None)
 
 

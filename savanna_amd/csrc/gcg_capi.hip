@@ -876,4 +876,67 @@ GCG_API int gcg_filter_decay_bwd(const void *dh, const float *decay, float *dw, 
     return finish(gcg::filter_bwd_launch(dtype, dh, decay, dw, g, l_cache, hl, (hipStream_t)stream));
 }
 
+// ---- 8-bit activation checkpoints and layer norm ---------------------------------------------------
+
+GCG_API int gcg_pack8(const void *x, int8_t *codes, float *scales, int64_t rows, int64_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !codes || !scales || rows <= 0 || D <= 0) return GCG_ERR_BAD_ARG;
+    if (dtype != GCG_F32 && dtype != GCG_BF16 && dtype != GCG_F16) return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::pack8_launch(dtype, x, codes, scales, rows, D, (hipStream_t)stream));
+}
+
+GCG_API int gcg_unpack8(const int8_t *codes, const float *scales, void *x, int64_t rows, int64_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !codes || !scales || rows <= 0 || D <= 0) return GCG_ERR_BAD_ARG;
+    if (dtype != GCG_F32 && dtype != GCG_BF16 && dtype != GCG_F16) return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::unpack8_launch(dtype, codes, scales, x, rows, D, (hipStream_t)stream));
+}
+
+namespace {
+int norm_check(int64_t rows, int32_t D, int32_t dtype)
+{
+    if (rows <= 0 || D <= 0 || dtype < GCG_F32 || dtype > GCG_F16_F32) return GCG_ERR_BAD_ARG;
+    return D > GCG_NORM_MAX_WIDTH ? GCG_ERR_UNSUPPORTED : GCG_OK;
+}
+} // namespace
+
+GCG_API int gcg_layer_norm_fwd(const void *x, const void *w, const void *b, void *y, float *stats, int8_t *codes, float *scales,
+                               int64_t rows, int32_t D, float eps, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !y || (codes == nullptr) != (scales == nullptr) || !(eps >= 0.f)) return GCG_ERR_BAD_ARG;
+    int rc = norm_check(rows, D, dtype);
+    if (rc) return rc;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::layer_norm_fwd_launch(dtype, x, w, b, y, stats, codes, scales, rows, D, eps, (hipStream_t)stream));
+}
+
+GCG_API size_t gcg_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t D, int32_t dtype)
+{
+    if (norm_check(rows, D, dtype)) return 0;
+    return (gcg::layer_norm_bwd_workspace(rows, D) + 255) & ~(size_t)255;
+}
+
+GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *codes, const float *scales, const float *stats,
+                               const void *w, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
+                               int64_t rows, int32_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!dy || !stats || !dx || (codes == nullptr) != (scales == nullptr) || (x == nullptr) == (codes == nullptr)) return GCG_ERR_BAD_ARG;
+    int rc = norm_check(rows, D, dtype);
+    if (rc) return rc;
+    if ((dw || db) && (!workspace || workspace_bytes < gcg_layer_norm_bwd_workspace_bytes(rows, D, dtype) || ((uintptr_t)workspace & 255)))
+        return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::layer_norm_bwd_launch(dtype, dy, x, codes, scales, stats, w, dx, dw, db, workspace, rows, D, (hipStream_t)stream));
+}
+
 } // extern "C"

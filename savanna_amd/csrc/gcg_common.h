@@ -415,4 +415,13 @@ int filter_fwd_launch(int dtype, const float *w, const float *decay, void *h, in
 int filter_bwd_launch(int dtype, const void *dh, const float *decay, float *dw, int g, int l_cache, int hl,
                       hipStream_t st);
 
+// 8-bit activation checkpoints of a (rows, D) tensor, and layer norm with or without one
+int pack8_launch(int dtype, const void *x, int8_t *codes, float *scales, int64_t rows, int64_t D, hipStream_t st);
+int unpack8_launch(int dtype, const int8_t *codes, const float *scales, void *x, int64_t rows, int64_t D, hipStream_t st);
+int layer_norm_fwd_launch(int dtype, const void *x, const void *w, const void *b, void *y, float *stats, int8_t *codes, float *scales,
+                          int64_t rows, int D, float eps, hipStream_t st);
+size_t layer_norm_bwd_workspace(int64_t rows, int D);
+int layer_norm_bwd_launch(int dtype, const void *dy, const void *x, const int8_t *codes, const float *scales, const float *stats,
+                          const void *w, void *dx, void *dw, void *db, void *ws, int64_t rows, int D, hipStream_t st);
+
 } // namespace gcg

@@ -10,30 +10,11 @@
 // This is the counterpart of the Triton launch wrappers two_pass_fwd_grouped /
 // two_pass_bwd_refactor (savanna/kernels/triton_src/cgcg/src/fwd.py:13-233, src/bwd.py:347-474)
 // as TwoPassChunkedGateConvGate calls them (cgcg/interface.py:27-127).
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
-#include <torch/types.h>
-
 #include <tuple>
 
-#include "../../include/gcg.h"
+#include "gcg_torch_common.h"
 
 namespace {
-
-using at::Tensor;
-using DeviceGuard = at::hip::OptionalHIPGuardMasqueradingAsCUDA;
-
-int dtype_code(at::ScalarType t)
-{
-    switch (t) {
-    case at::kFloat: return GCG_F32;
-    case at::kBFloat16: return GCG_BF16;
-    case at::kHalf: return GCG_F16;
-    default: TORCH_CHECK(false, "gcg: unsupported dtype ", t, "; expected float32, bfloat16 or float16");
-    }
-}
 
 // dtype code of the gated operator: the tensors' dtype, or 16-bit tensors with an fp32 filter
 int gated_code(const Tensor &x, const Tensor &h)
@@ -44,22 +25,6 @@ int gated_code(const Tensor &x, const Tensor &h)
                 "gcg: the filter must have the tensors' dtype, or be float32 with bfloat16 / float16 tensors; got ", t,
                 " tensors and a ", f, " filter");
     return t == at::kBFloat16 ? GCG_BF16_F32 : GCG_F16_F32;
-}
-
-void *stream_of(const Tensor &t)
-{
-    return (void *)at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
-
-void check_rc(int rc, const char *what)
-{
-    TORCH_CHECK(rc == 0, what, ": ", gcg_strerror(rc), " (code ", rc, ", hipError ", gcg_last_hip_error(), ")");
-}
-
-void require_gpu(const Tensor &t, const char *name)
-{
-    TORCH_CHECK(t.is_cuda(), "gcg: ", name, " is on ", t.device(),
-                "; the kernels run on an MI355X (gfx950) device only and there is no CPU path");
 }
 
 // x, B, C (and dy): contiguous (bs, L, g, dg) of one dtype on one device; h: contiguous (g, 1, hl)
@@ -92,12 +57,6 @@ void check_feat(const Tensor &feat, const Tensor &h)
                 "gcg: h must be a contiguous (g, 1, hl) tensor");
     TORCH_CHECK(h.device() == feat.device(), "gcg: feat and h must be on one device");
     (void)gated_code(feat, h);
-}
-
-Tensor workspace(size_t bytes, const Tensor &like, const char *what)
-{
-    TORCH_CHECK(bytes > 0, what, ": arguments rejected (shape not supported by the requested kernel family)");
-    return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
 }
 
 // ---- gated convolution on separate tensors ----------------------------------------------------
@@ -863,14 +822,6 @@ std::tuple<Tensor, Tensor, Tensor> mixer_mr_bwd_meta(const Tensor &dy, const Ten
 // The autograd functions of the layers (savanna_amd/kernels, savanna_amd/operators) as C++ nodes: same operators, same
 // tensors saved, but the backward runs on autograd's device thread without the interpreter, whose lock that thread and the
 // caller otherwise hand to and fro.  Forward and backward call the operators above through the dispatcher, so modes see them.
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-template <typename F> c10::TypedOperatorHandle<F> op(const char *name)
-{
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
-}
-
 struct GatedConvGate : torch::autograd::Function<GatedConvGate> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &B, const Tensor &C, const Tensor &h)
     {
