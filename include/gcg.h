@@ -552,6 +552,39 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
             const void *w, void *dx, void *dw, void *db, void *workspace, size_t workspace_bytes,
             int64_t rows, int32_t D, int32_t dtype, void *stream);
 
+/*
+ * Linear attention with a decay for each head.  With f = exp(log_decay[h]) and a state S (dk, dv), fp32, a batch entry and head:
+ *
+ *     S_t = f S_{t-1} + k_t v_t^T,     o_t = scale * q_t S_t
+ *
+ * q, k (bs, L, H, dk), v, o (bs, L, H, dv), the last dimension contiguous; `strides` holds the others' strides in elements,
+ * batch, time and head, of q, k, v, o in this order (of do, q, k, v, dq, dk, dv in the backward; batch and head of q, k, v, o in
+ * the step).  log_decay (H) fp32, a constant, at most 0 in use (-inf: no memory).  initial, final, dfinal, dinitial and state are
+ * contiguous (bs, H, dk, dv) fp32.  initial and dfinal may be null (zeros), final and dinitial too (not wanted).
+ * lengths (bs) int32, or null: an entry's rows from its length on (clamped to 0 .. L) are not read, their outputs and gradients
+ * are zero, and final is the state after the last row inside.
+ *
+ * gcg_linear_attn_step takes one token: the state is moved on in place.
+ *
+ * A row of v that holds an infinity or a NaN also makes NaN of outputs up to 31 rows before it (forward; as of do
+ * for dk and dv's rows after it): it meets them in one matrix instruction, times zero.
+ *
+ * dk, dv up to GCG_LINEAR_MAX_DIM, bs * H up to GCG_LINEAR_MAX_HEADS, else GCG_ERR_UNSUPPORTED.  scale: finite, not 0.  dtype:
+ * GCG_F32, GCG_BF16, GCG_F16.  workspace: gcg_linear_attn_workspace_bytes (0: none), 256-byte aligned.  Results are the same on
+ * every run.
+ */
+enum { GCG_LINEAR_MAX_DIM = 256, GCG_LINEAR_MAX_HEADS = 65535 };
+GCG_API size_t gcg_linear_attn_workspace_bytes(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, int32_t backward);
+GCG_API int gcg_linear_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, const float *log_decay,
+            const float *initial, const int32_t *lengths, void *o, float *final, void *workspace, size_t workspace_bytes,
+            int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream);
+GCG_API int gcg_linear_attn_bwd(const void *d_o, const void *q, const void *k, const void *v, const int64_t *strides,
+            const float *log_decay, const float *initial, const int32_t *lengths, const float *dfinal,
+            void *dq, void *d_k, void *d_v, float *dinitial, void *workspace, size_t workspace_bytes,
+            int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream);
+GCG_API int gcg_linear_attn_step(const void *q, const void *k, const void *v, void *o, const int64_t *strides, const float *log_decay,
+            float *state, int64_t bs, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

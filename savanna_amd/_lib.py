@@ -41,6 +41,7 @@ EXPORTS = (
     "gcg_mixer_mr_fwd_planar", "gcg_mixer_mr_bwd_planar", "gcg_mixer_mr_fwd_planar_decay", "gcg_mixer_mr_bwd_planar_decay", "gcg_fwd_time_major", "gcg_bwd_time_major_workspace_bytes", "gcg_bwd_time_major",
     "gcg_fwd_decay", "gcg_bwd_decay", "gcg_fwd_interleaved_decay", "gcg_bwd_interleaved_decay",
     "gcg_pack8", "gcg_unpack8", "gcg_layer_norm_fwd", "gcg_layer_norm_bwd_workspace_bytes", "gcg_layer_norm_bwd",
+    "gcg_linear_attn_workspace_bytes", "gcg_linear_attn_fwd", "gcg_linear_attn_bwd", "gcg_linear_attn_step",
 )
 
 _lock = threading.Lock()
@@ -158,6 +159,14 @@ def load() -> ctypes.CDLL:
         lib.gcg_layer_norm_bwd_workspace_bytes.restype = sz
         lib.gcg_layer_norm_bwd.argtypes = [vp] * 10 + [sz, i64, i32, i32, vp]
         lib.gcg_layer_norm_bwd.restype = ctypes.c_int
+        lib.gcg_linear_attn_workspace_bytes.argtypes = [i64, i64, i32, i32, i32, i32]
+        lib.gcg_linear_attn_workspace_bytes.restype = sz
+        lib.gcg_linear_attn_fwd.argtypes = [vp] * 10 + [sz, i64, i64, i32, i32, i32, ctypes.c_float, i32, vp]
+        lib.gcg_linear_attn_fwd.restype = ctypes.c_int
+        lib.gcg_linear_attn_bwd.argtypes = [vp] * 14 + [sz, i64, i64, i32, i32, i32, ctypes.c_float, i32, vp]
+        lib.gcg_linear_attn_bwd.restype = ctypes.c_int
+        lib.gcg_linear_attn_step.argtypes = [vp] * 7 + [i64, i32, i32, i32, ctypes.c_float, i32, vp]
+        lib.gcg_linear_attn_step.restype = ctypes.c_int
         _lib = lib
         return lib
 
@@ -1131,3 +1140,157 @@ def layer_norm_bwd(dy, x, codes, scales, stats, w, b):
                                     torch.cuda.current_stream().cuda_stream)
     check(rc, "gcg_layer_norm_bwd")
     return dx, dw, db
+
+
+# ---- linear attention with a decay for each head --------------------------------------------------------
+
+LINEAR_MAX_DIM = 256                # GCG_LINEAR_MAX_DIM
+
+
+def _check_linear(q, k, v, log_decay, dim) -> None:
+    if q.dim() != dim or q.shape != k.shape or v.shape[:-1] != q.shape[:-1]:
+        raise ValueError("q and k must be (bs, L, H, dk), v (bs, L, H, dv)" if dim == 4 else "q and k must be (bs, H, dk), v (bs, H, dv)")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("q, k and v must share dtype and device")
+    dtype_code(q.dtype)
+    if log_decay.shape != (q.shape[-2],) or log_decay.dtype != torch.float32 or not log_decay.is_contiguous() \
+            or log_decay.device != q.device:
+        raise ValueError("log_decay must be a contiguous float32 tensor of one element a head on q's device")
+    if not (0 < q.shape[-1] <= LINEAR_MAX_DIM and 0 < v.shape[-1] <= LINEAR_MAX_DIM):
+        raise ValueError(f"head dimensions are 1 to {LINEAR_MAX_DIM}")
+
+
+def _check_state(t, q, v, name) -> None:
+    if t is not None and (t.shape != (q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]) or t.dtype != torch.float32
+                          or not t.is_contiguous() or t.device != q.device):
+        raise ValueError(f"{name} must be a contiguous (bs, H, dk, dv) float32 tensor on q's device")
+
+
+def _check_lengths(t, q) -> None:
+    if t is not None and (t.shape != (q.shape[0],) or t.dtype != torch.int32 or not t.is_contiguous() or t.device != q.device):
+        raise ValueError("lengths must be a contiguous int32 tensor of one element a batch entry on q's device")
+
+
+def _rows(t):
+    """The tensor with a contiguous last dimension, as the kernels read it."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(n: int, *tensors):
+    s = [t.stride(i) for t in tensors for i in range(n)]
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def _passed_on(source, to):
+    return None if to is None else to.copy_(source) if source is not None else to.zero_()
+
+
+def _linear_workspace(lib, q, v, backward):
+    n = lib.gcg_linear_attn_workspace_bytes(q.shape[0], q.shape[1], q.shape[2], q.shape[3], v.shape[3], int(backward))
+    return n, (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None)
+
+
+def linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale: float, final: bool):
+    """(o, final state or None) of q, k (bs, L, H, dk), v (bs, L, H, dv); initial (bs, H, dk, dv) fp32 and lengths (bs) int32 may
+    be None."""
+    _require_gpu(q)
+    if TORCH_OPS:
+        o, last = _run(torch.ops.gcg.linear_attn_fwd, q, k, v, log_decay, initial, lengths, scale, final)
+        return o, (last if final else None)
+    lib = load()
+    _check_linear(q, k, v, log_decay, 4)
+    _check_state(initial, q, v, "initial_state")
+    _check_lengths(lengths, q)
+    bs, L, H, dk = q.shape
+    dv = v.shape[-1]
+    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    last = torch.empty(bs, H, dk, dv, dtype=torch.float32, device=q.device) if final else None
+    if o.numel() == 0:
+        return o, _passed_on(initial, last)
+    with _on_device(q.device):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        n, ws = _linear_workspace(lib, q, v, False)
+        rc = lib.gcg_linear_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, q, k, v, o), log_decay.data_ptr(),
+                                     _ptr(initial), _ptr(lengths), o.data_ptr(), _ptr(last), _ptr(ws), n, bs, L, H, dk, dv, scale,
+                                     dtype_code(q.dtype), torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_linear_attn_fwd")
+    return o, last
+
+
+def _linear_bwd_into(do, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, dk, dv, dinitial) -> None:
+    lib = load()
+    if do.shape != v.shape or do.dtype != v.dtype or do.device != v.device:
+        raise ValueError("do must have the shape, dtype and device of v")
+    with _on_device(q.device):
+        do, q, k, v = _rows(do), _rows(q), _rows(k), _rows(v)
+        n, ws = _linear_workspace(lib, q, v, True)
+        rc = lib.gcg_linear_attn_bwd(do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, do, q, k, v, dq, dk, dv),
+                                     log_decay.data_ptr(), _ptr(initial), _ptr(lengths), _ptr(dfinal), dq.data_ptr(), dk.data_ptr(),
+                                     dv.data_ptr(), _ptr(dinitial), _ptr(ws), n, *q.shape, v.shape[-1], scale, dtype_code(q.dtype),
+                                     torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_linear_attn_bwd")
+
+
+def linear_attn_bwd(do, q, k, v, log_decay, initial, lengths, dfinal, scale: float, need_dinitial: bool):
+    """(dq, dk, dv, gradient of the initial state or None); dfinal, the final state's gradient, may be None."""
+    _require_gpu(q)
+    if TORCH_OPS:
+        dq, dk, dv, di = torch.ops.gcg.linear_attn_bwd(do, q, k, v, log_decay, initial, lengths, dfinal, scale, need_dinitial)
+        return dq, dk, dv, (di if need_dinitial else None)
+    _check_linear(q, k, v, log_decay, 4)
+    _check_state(initial, q, v, "initial_state")
+    _check_state(dfinal, q, v, "the final state's gradient")
+    _check_lengths(lengths, q)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    di = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=q.device) if need_dinitial else None
+    if do.numel() == 0:
+        return dq, dk, dv, _passed_on(dfinal, di)
+    _linear_bwd_into(do, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, dk, dv, di)
+    return dq, dk, dv, di
+
+
+def _split_features(features, heads: int):
+    if features.dim() != 3 or not features.is_contiguous() or heads <= 0 or features.shape[2] % (3 * heads):
+        raise ValueError("features must be a contiguous (bs, L, 3 * H * d) tensor")
+    return features.view(*features.shape[:2], 3, heads, -1).unbind(2)
+
+
+def linear_attn_packed_fwd(features, heads: int, log_decay, scale: float):
+    """o (bs, L, H, d) of the projected features (bs, L, 3 * H * d), laid out "(p h d)" with p = q, k, v."""
+    _require_gpu(features)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.linear_attn_packed_fwd, features, heads, log_decay, scale)
+    return linear_attn_fwd(*_split_features(features, heads), log_decay, None, None, scale, False)[0]
+
+
+def linear_attn_packed_bwd(do, features, heads: int, log_decay, scale: float):
+    """The features' gradient, in their layout."""
+    _require_gpu(features)
+    if TORCH_OPS:
+        return torch.ops.gcg.linear_attn_packed_bwd(do, features, heads, log_decay, scale)
+    q, k, v = _split_features(features, heads)
+    _check_linear(q, k, v, log_decay, 4)
+    df = torch.empty_like(features)
+    if df.numel():
+        _linear_bwd_into(do, q, k, v, log_decay, None, None, None, scale, *_split_features(df, heads), None)
+    return df
+
+
+def linear_attn_step(q, k, v, log_decay, state, scale: float):
+    """o (bs, H, dv) of one token, q, k (bs, H, dk), v (bs, H, dv); state (bs, H, dk, dv) fp32 moves on in place."""
+    _require_gpu(q)
+    if TORCH_OPS:
+        return torch.ops.gcg.linear_attn_step(q, k, v, log_decay, state, scale)
+    lib = load()
+    _check_linear(q, k, v, log_decay, 3)
+    _check_state(state, q, v, "state")
+    o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if o.numel() == 0:
+        return o
+    with _on_device(q.device):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        rc = lib.gcg_linear_attn_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _strides(2, q, k, v, o),
+                                      log_decay.data_ptr(), state.data_ptr(), *q.shape, v.shape[-1], scale, dtype_code(q.dtype),
+                                      torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_linear_attn_step")
+    return o

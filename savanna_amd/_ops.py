@@ -38,10 +38,12 @@ OP_NAMES = (
     "mixer_mr_fwd", "mixer_mr_bwd", "mixer_mr_fwd_decay", "mixer_mr_bwd_decay", "fwd_time_major", "bwd_time_major", "fwd_decay", "bwd_decay", "fwd_interleaved_decay", "bwd_interleaved_decay",
     "fwd_planar", "bwd_planar",
     "pack8", "unpack8", "layer_norm_fwd", "layer_norm_infer", "layer_norm_bwd",
+    "linear_attn_fwd", "linear_attn_bwd", "linear_attn_packed_fwd", "linear_attn_packed_bwd", "linear_attn_step",
 )
 
 # differentiable as they are: C++ autograd nodes around operators above, which a trace sees in their place
-NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay", "layer_norm")
+NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay", "layer_norm", "linear_attn",
+              "linear_attn_packed")
 
 
 # ---- autograd --------------------------------------------------------------------------------------------
@@ -134,6 +136,25 @@ def _register_autograd():
         dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), *ctx.saved_tensors)
         return dx, dw if w is not None else None, db if b is not None else None, None, None
     reg("gcg::layer_norm_fwd", norm, setup_context=norm_setup)
+
+    def linear_setup(ctx, inputs, output):   # linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale, final) -> o, state
+        ctx.save_for_backward(*inputs[:6])
+        ctx.scale, ctx.final = inputs[6:]
+        ctx.set_materialize_grads(False)
+
+    def linear(ctx, do, dfinal):
+        q, k, v, log_decay, initial, lengths = ctx.saved_tensors
+        do = do if do is not None else torch.zeros_like(v)
+        dfinal = dfinal.contiguous() if ctx.final and dfinal is not None else None
+        need = initial is not None and ctx.needs_input_grad[4]
+        dq, dk, dv, di = ops.linear_attn_bwd(do, q, k, v, log_decay, initial, lengths, dfinal, ctx.scale, need)
+        return dq, dk, dv, None, di if need else None, None, None, None
+    reg("gcg::linear_attn_fwd", linear, setup_context=linear_setup)
+
+    def linear_packed(ctx, do):              # linear_attn_packed_fwd(features, H, log_decay, scale)
+        features, log_decay = ctx.saved_tensors
+        return ops.linear_attn_packed_bwd(do, features, ctx.rest[1], log_decay, ctx.rest[3]), None, None, None
+    reg("gcg::linear_attn_packed_fwd", linear_packed, setup_context=save(0, 2))
 
     def refuse(name, hint):
         def backward(ctx, *grads):

@@ -939,4 +939,68 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
     return finish(gcg::layer_norm_bwd_launch(dtype, dy, x, codes, scales, stats, w, dx, dw, db, workspace, rows, D, (hipStream_t)stream));
 }
 
+// ---- linear attention with a decay for each head ------------------------------------------------------
+
+namespace {
+int linear_check(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype)
+{
+    if (bs <= 0 || L <= 0 || H <= 0 || dk <= 0 || dv <= 0) return GCG_ERR_BAD_ARG;
+    if (dtype != GCG_F32 && dtype != GCG_BF16 && dtype != GCG_F16) return GCG_ERR_BAD_ARG;
+    if (!(scale - scale == 0.f) || scale == 0.f) return GCG_ERR_BAD_ARG;
+    // heads and batch index the grid together
+    return dk > GCG_LINEAR_MAX_DIM || dv > GCG_LINEAR_MAX_DIM || bs > GCG_LINEAR_MAX_HEADS || bs * H > GCG_LINEAR_MAX_HEADS ? GCG_ERR_UNSUPPORTED : GCG_OK;
+}
+bool missing(const void *ws, size_t have, size_t need) { return need && (!ws || have < need || ((uintptr_t)ws & 255)); }
+} // namespace
+
+GCG_API size_t gcg_linear_attn_workspace_bytes(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, int32_t backward)
+{
+    if (linear_check(bs, L, H, dk, dv, 1.f, GCG_F32)) return 0;
+    return (gcg::linear_attn_workspace(bs, L, H, dk, dv, backward != 0) + 255) & ~(size_t)255;
+}
+
+GCG_API int gcg_linear_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, const float *log_decay,
+                                const float *initial, const int32_t *lengths, void *o, float *final, void *workspace,
+                                size_t workspace_bytes, int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float scale,
+                                int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!q || !k || !v || !strides || !log_decay || !o) return GCG_ERR_BAD_ARG;
+    int rc = linear_check(bs, L, H, dk, dv, scale, dtype);
+    if (rc) return rc;
+    if (missing(workspace, workspace_bytes, gcg_linear_attn_workspace_bytes(bs, L, H, dk, dv, 0))) return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::linear_attn_fwd_launch(dtype, q, k, v, strides, log_decay, initial, lengths, o, final, workspace, bs, L, H, dk, dv,
+                                              scale, (hipStream_t)stream));
+}
+
+GCG_API int gcg_linear_attn_bwd(const void *d_o, const void *q, const void *k, const void *v, const int64_t *strides,
+                                const float *log_decay, const float *initial, const int32_t *lengths, const float *dfinal, void *dq,
+                                void *d_k, void *d_v, float *dinitial, void *workspace, size_t workspace_bytes, int64_t bs, int64_t L,
+                                int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!d_o || !q || !k || !v || !strides || !log_decay || !dq || !d_k || !d_v) return GCG_ERR_BAD_ARG;
+    int rc = linear_check(bs, L, H, dk, dv, scale, dtype);
+    if (rc) return rc;
+    if (missing(workspace, workspace_bytes, gcg_linear_attn_workspace_bytes(bs, L, H, dk, dv, 1))) return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::linear_attn_bwd_launch(dtype, d_o, q, k, v, strides, log_decay, initial, lengths, dfinal, dq, d_k, d_v, dinitial,
+                                              workspace, bs, L, H, dk, dv, scale, (hipStream_t)stream));
+}
+
+GCG_API int gcg_linear_attn_step(const void *q, const void *k, const void *v, void *o, const int64_t *strides, const float *log_decay,
+                                 float *state, int64_t bs, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!q || !k || !v || !o || !strides || !log_decay || !state) return GCG_ERR_BAD_ARG;
+    int rc = linear_check(bs, 1, H, dk, dv, scale, dtype);
+    if (rc) return rc;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::linear_attn_step_launch(dtype, q, k, v, o, strides, log_decay, state, bs, H, dk, dv, scale, (hipStream_t)stream));
+}
+
 } // extern "C"

@@ -424,4 +424,16 @@ size_t layer_norm_bwd_workspace(int64_t rows, int D);
 int layer_norm_bwd_launch(int dtype, const void *dy, const void *x, const int8_t *codes, const float *scales, const float *stats,
                           const void *w, void *dx, void *dw, void *db, void *ws, int64_t rows, int D, hipStream_t st);
 
+// linear attention with a decay for each head; strides: batch, time and head of q, k, v, o (do, q, k, v, dq, dk, dv), in elements
+size_t linear_attn_workspace(int64_t bs, int64_t L, int H, int dk, int dv, bool backward);
+int linear_attn_fwd_launch(int dtype, const void *q, const void *k, const void *v, const int64_t *strides, const float *log_decay,
+                           const float *initial, const int32_t *lengths, void *o, float *final, void *ws, int64_t bs, int64_t L, int H,
+                           int dk, int dv, float scale, hipStream_t st);
+int linear_attn_bwd_launch(int dtype, const void *d_o, const void *q, const void *k, const void *v, const int64_t *strides,
+                           const float *log_decay, const float *initial, const int32_t *lengths, const float *dfinal, void *dq, void *d_k,
+                           void *d_v, float *dinitial, void *ws, int64_t bs, int64_t L, int H, int dk, int dv, float scale, hipStream_t st);
+// one token; strides: batch and head of q, k, v, o
+int linear_attn_step_launch(int dtype, const void *q, const void *k, const void *v, void *o, const int64_t *strides, const float *log_decay,
+                            float *state, int64_t bs, int H, int dk, int dv, float scale, hipStream_t st);
+
 } // namespace gcg

@@ -1,8 +1,12 @@
-// PyTorch binding of the operators around the convolution (include/gcg.h): 8-bit activation checkpoints and layer norm.
+// PyTorch binding of the operators around the convolution (include/gcg.h): 8-bit activation checkpoints, layer norm, linear
+// attention with a decay for each head.
 // As in gcg_torch.cpp: device and meta implementations of torch.ops.gcg.*, and C++ autograd nodes around them for eager
 // training steps.
+#include <algorithm>
+#include <array>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "gcg_torch_common.h"
 
@@ -247,6 +251,272 @@ Tensor layer_norm(const Tensor &x, const OptTensor &w, const OptTensor &b, doubl
     return LayerNormNode::apply(x, w, b, eps, save_8bit);
 }
 
+// ---- linear attention with a decay for each head ------------------------------------------------------
+
+void add_strides(std::vector<int64_t> &s, const Tensor &t) { s.insert(s.end(), {t.stride(0), t.stride(1), t.stride(2)}); }
+
+// a tensor whose last dimension is contiguous, as the kernels read it
+Tensor rows_of(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+void check_heads(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, int64_t dim)
+{
+    TORCH_CHECK(q.dim() == dim && k.dim() == dim && v.dim() == dim && q.sizes() == k.sizes() &&
+                    v.sizes().slice(0, dim - 1) == q.sizes().slice(0, dim - 1),
+                dim == 4 ? "gcg: q and k must be (bs, L, H, dk), v (bs, L, H, dv)" : "gcg: q and k must be (bs, H, dk), v (bs, H, dv)");
+    TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                    v.device() == q.device(),
+                "gcg: q, k and v must share dtype and device");
+    (void)dtype_code(q.scalar_type());
+    TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == q.size(dim - 2) && log_decay.scalar_type() == at::kFloat &&
+                    log_decay.is_contiguous() && log_decay.device() == q.device(),
+                "gcg: log_decay must be a contiguous float32 tensor of one element a head on q's device");
+    TORCH_CHECK(q.size(-1) <= GCG_LINEAR_MAX_DIM && v.size(-1) <= GCG_LINEAR_MAX_DIM && q.size(-1) > 0 && v.size(-1) > 0,
+                "gcg: head dimensions are 1 to ", (int)GCG_LINEAR_MAX_DIM);
+}
+
+void check_state(const OptTensor &t, const Tensor &q, const Tensor &v, const char *name)
+{
+    if (!given(t)) return;
+    TORCH_CHECK(t->dim() == 4 && t->size(0) == q.size(0) && t->size(1) == q.size(-2) && t->size(2) == q.size(-1) &&
+                    t->size(3) == v.size(-1) && t->scalar_type() == at::kFloat && t->is_contiguous() && t->device() == q.device(),
+                "gcg: ", name, " must be a contiguous (bs, H, dk, dv) float32 tensor on q's device");
+}
+
+void check_lengths(const OptTensor &t, const Tensor &q)
+{
+    if (!given(t)) return;
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == q.size(0) && t->scalar_type() == at::kInt && t->is_contiguous() && t->device() == q.device(),
+                "gcg: lengths must be a contiguous int32 tensor of one element a batch entry on q's device");
+}
+
+Tensor new_state(const Tensor &q, const Tensor &v, bool wanted)
+{
+    const auto f32 = q.options().dtype(at::kFloat);
+    return wanted ? at::empty({q.size(0), q.size(-2), q.size(-1), v.size(-1)}, f32) : at::empty({0}, f32);
+}
+
+Tensor linear_workspace(const Tensor &q, const Tensor &v, bool backward, size_t *bytes)
+{
+    *bytes = gcg_linear_attn_workspace_bytes(q.size(0), q.size(1), (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), backward);
+    return *bytes ? at::empty({(int64_t)*bytes}, q.options().dtype(at::kByte)) : Tensor();
+}
+
+// a sequence of no rows: the state is the one given
+Tensor passed_on(const OptTensor &from, Tensor to) { return to.numel() == 0 ? to : given(from) ? to.copy_(*from) : to.zero_(); }
+
+std::tuple<Tensor, Tensor> linear_attn_fwd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                           const OptTensor &initial, const OptTensor &lengths, double scale, bool final)
+{
+    require_gpu(q, "q");
+    check_heads(q, k, v, log_decay, 4);
+    check_state(initial, q, v, "initial_state");
+    check_lengths(lengths, q);
+    DeviceGuard guard(q.device());
+    Tensor o = at::empty({v.size(0), v.size(1), v.size(2), v.size(3)}, v.options());
+    Tensor last = new_state(q, v, final);
+    if (o.numel() == 0) return {o, passed_on(initial, last)};
+    const Tensor a = rows_of(q), b = rows_of(k), c = rows_of(v);
+    std::vector<int64_t> s;
+    for (const Tensor *t : {&a, &b, &c, (const Tensor *)&o}) add_strides(s, *t);
+    size_t bytes;
+    Tensor ws = linear_workspace(q, v, false, &bytes);
+    check_rc(gcg_linear_attn_fwd(a.data_ptr(), b.data_ptr(), c.data_ptr(), s.data(), (const float *)log_decay.data_ptr(),
+                                 (const float *)ptr(initial), (const int32_t *)ptr(lengths), o.data_ptr(),
+                                 final ? (float *)last.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, q.size(0), q.size(1),
+                                 (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), (float)scale, dtype_code(q.scalar_type()),
+                                 stream_of(q)),
+             "gcg_linear_attn_fwd");
+    return {o, last};
+}
+
+void linear_bwd_launch(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                       const OptTensor &initial, const OptTensor &lengths, const OptTensor &dfinal, double scale, const Tensor &dq,
+                       const Tensor &d_k, const Tensor &d_v, float *dinitial)
+{
+    const Tensor g = rows_of(d_o), a = rows_of(q), b = rows_of(k), c = rows_of(v);
+    std::vector<int64_t> s;
+    for (const Tensor *t : {&g, &a, &b, &c, &dq, &d_k, &d_v}) add_strides(s, *t);
+    size_t bytes;
+    Tensor ws = linear_workspace(q, v, true, &bytes);
+    check_rc(gcg_linear_attn_bwd(g.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), s.data(), (const float *)log_decay.data_ptr(),
+                                 (const float *)ptr(initial), (const int32_t *)ptr(lengths), (const float *)ptr(dfinal), dq.data_ptr(),
+                                 d_k.data_ptr(), d_v.data_ptr(), dinitial, bytes ? ws.data_ptr() : nullptr, bytes, q.size(0), q.size(1),
+                                 (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), (float)scale, dtype_code(q.scalar_type()),
+                                 stream_of(q)),
+             "gcg_linear_attn_bwd");
+}
+
+void check_do(const Tensor &d_o, const Tensor &v)
+{
+    TORCH_CHECK(d_o.sizes() == v.sizes() && d_o.scalar_type() == v.scalar_type() && d_o.device() == v.device(),
+                "gcg: do must have the shape, dtype and device of v");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attn_bwd(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v,
+                                                           const Tensor &log_decay, const OptTensor &initial, const OptTensor &lengths,
+                                                           const OptTensor &dfinal, double scale, bool need_dinitial)
+{
+    require_gpu(q, "q");
+    check_heads(q, k, v, log_decay, 4);
+    check_do(d_o, v);
+    check_state(initial, q, v, "initial_state");
+    check_state(dfinal, q, v, "the final state's gradient");
+    check_lengths(lengths, q);
+    DeviceGuard guard(q.device());
+    Tensor dq = at::empty(q.sizes(), q.options()), d_k = at::empty(k.sizes(), k.options()), d_v = at::empty(v.sizes(), v.options());
+    Tensor dinitial = new_state(q, v, need_dinitial);
+    if (d_o.numel() == 0) return {dq, d_k, d_v, passed_on(dfinal, dinitial)};
+    linear_bwd_launch(d_o, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, d_k, d_v,
+                      need_dinitial ? (float *)dinitial.data_ptr() : nullptr);
+    return {dq, d_k, d_v, dinitial};
+}
+
+// the projected features (bs, L, 3 * H * d), laid out "(p h d)" with p = q, k, v
+std::array<Tensor, 3> split_features(const Tensor &features, int64_t H)
+{
+    TORCH_CHECK(features.dim() == 3 && features.is_contiguous() && H > 0 && features.size(2) % (3 * H) == 0,
+                "gcg: features must be a contiguous (bs, L, 3 * H * d) tensor");
+    const Tensor f = features.view({features.size(0), features.size(1), 3, H, features.size(2) / (3 * H)});
+    return {f.select(2, 0), f.select(2, 1), f.select(2, 2)};
+}
+
+Tensor linear_attn_packed_fwd(const Tensor &features, int64_t H, const Tensor &log_decay, double scale)
+{
+    const auto [q, k, v] = split_features(features, H);
+    return std::get<0>(linear_attn_fwd(q, k, v, log_decay, OptTensor(), OptTensor(), scale, false));
+}
+
+Tensor linear_attn_packed_bwd(const Tensor &d_o, const Tensor &features, int64_t H, const Tensor &log_decay, double scale)
+{
+    require_gpu(features, "features");
+    const auto [q, k, v] = split_features(features, H);
+    check_heads(q, k, v, log_decay, 4);
+    check_do(d_o, v);
+    DeviceGuard guard(q.device());
+    Tensor df = at::empty_like(features);
+    if (df.numel() == 0) return df;
+    const auto [dq, d_k, d_v] = split_features(df, H);
+    linear_bwd_launch(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, dq, d_k, d_v, nullptr);
+    return df;
+}
+
+Tensor linear_attn_step(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, Tensor &state, double scale)
+{
+    require_gpu(q, "q");
+    check_heads(q, k, v, log_decay, 3);
+    check_state(state, q, v, "state");
+    DeviceGuard guard(q.device());
+    Tensor o = at::empty(v.sizes(), v.options());
+    if (o.numel() == 0) return o;
+    const Tensor a = rows_of(q), b = rows_of(k), c = rows_of(v);
+    const int64_t s[8] = {a.stride(0), a.stride(1), b.stride(0), b.stride(1), c.stride(0), c.stride(1), o.stride(0), o.stride(1)};
+    check_rc(gcg_linear_attn_step(a.data_ptr(), b.data_ptr(), c.data_ptr(), o.data_ptr(), s, (const float *)log_decay.data_ptr(),
+                                  (float *)state.data_ptr(), q.size(0), (int32_t)q.size(1), (int32_t)q.size(2), (int32_t)v.size(2),
+                                  (float)scale, dtype_code(q.scalar_type()), stream_of(q)),
+             "gcg_linear_attn_step");
+    return o;
+}
+
+std::tuple<Tensor, Tensor> linear_attn_fwd_meta(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                                const OptTensor &initial, const OptTensor &lengths, double, bool final)
+{
+    check_heads(q, k, v, log_decay, 4);
+    check_state(initial, q, v, "initial_state");
+    check_lengths(lengths, q);
+    return {at::empty(v.sizes(), v.options()), new_state(q, v, final)};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attn_bwd_meta(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v,
+                                                                const Tensor &log_decay, const OptTensor &, const OptTensor &,
+                                                                const OptTensor &, double, bool need_dinitial)
+{
+    check_heads(q, k, v, log_decay, 4);
+    check_do(d_o, v);
+    return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(v.sizes(), v.options()),
+            new_state(q, v, need_dinitial)};
+}
+Tensor linear_attn_packed_fwd_meta(const Tensor &features, int64_t H, const Tensor &log_decay, double)
+{
+    const auto [q, k, v] = split_features(features, H);
+    check_heads(q, k, v, log_decay, 4);
+    return at::empty({features.size(0), features.size(1), H, features.size(2) / (3 * H)}, features.options());
+}
+Tensor linear_attn_packed_bwd_meta(const Tensor &, const Tensor &features, int64_t H, const Tensor &, double)
+{
+    (void)split_features(features, H);
+    return at::empty_like(features);
+}
+Tensor linear_attn_step_meta(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, Tensor &state, double)
+{
+    check_heads(q, k, v, log_decay, 3);
+    check_state(state, q, v, "state");
+    return at::empty(v.sizes(), v.options());
+}
+
+struct LinearAttnNode : torch::autograd::Function<LinearAttnNode> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
+                                 const OptTensor &initial, const OptTensor &lengths, double scale, bool final)
+    {
+        static const auto f = op<std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                           const OptTensor &, const OptTensor &, double, bool)>("gcg::linear_attn_fwd");
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, v, log_decay, or_empty(initial), or_empty(lengths)});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["dinitial"] = given(initial) && initial->requires_grad();
+        auto [o, last] = f.call(q, k, v, log_decay, initial, lengths, scale, final);
+        if (final) return {o, last};
+        return {o};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g)
+    {
+        static const auto f = op<std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                                           const Tensor &, const OptTensor &, const OptTensor &,
+                                                                           const OptTensor &, double, bool)>("gcg::linear_attn_bwd");
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor d_o = g[0].defined() ? g[0] : at::zeros(s[2].sizes(), s[2].options());
+        const Tensor dfinal = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+        const bool need = ctx->saved_data["dinitial"].toBool();
+        auto [dq, d_k, d_v, dinitial] = f.call(d_o, s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), opt(dfinal),
+                                               ctx->saved_data["scale"].toDouble(), need);
+        return {dq, d_k, d_v, Tensor(), need ? dinitial : Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+struct PackedLinearAttnNode : torch::autograd::Function<PackedLinearAttnNode> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &features, int64_t H, const Tensor &log_decay, double scale, bool save_8bit)
+    {
+        static const auto f = op<Tensor(const Tensor &, int64_t, const Tensor &, double)>("gcg::linear_attn_packed_fwd");
+        static const auto pack = op<std::tuple<Tensor, Tensor>(const Tensor &)>("gcg::pack8");
+        at::AutoDispatchBelowADInplaceOrView below;
+        Tensor codes, scales;
+        if (save_8bit) std::tie(codes, scales) = pack.call(features);
+        ctx->save_for_backward({save_8bit ? Tensor() : features, codes, scales, log_decay});
+        ctx->saved_data["H"] = H;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["dtype"] = (int64_t)features.scalar_type();
+        return f.call(features, H, log_decay, scale);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g)
+    {
+        static const auto f = op<Tensor(const Tensor &, const Tensor &, int64_t, const Tensor &, double)>("gcg::linear_attn_packed_bwd");
+        static const auto unpack = op<Tensor(const Tensor &, const Tensor &, at::ScalarType)>("gcg::unpack8");
+        const variable_list s = ctx->get_saved_variables();
+        const Tensor features = s[0].defined() ? s[0] : unpack.call(s[1], s[2], (at::ScalarType)ctx->saved_data["dtype"].toInt());
+        return {f.call(g[0], features, ctx->saved_data["H"].toInt(), s[3], ctx->saved_data["scale"].toDouble()), Tensor(), Tensor(),
+                Tensor(), Tensor()};
+    }
+};
+
+std::vector<Tensor> linear_attn(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const OptTensor &initial,
+                                const OptTensor &lengths, double scale, bool final)
+{
+    return LinearAttnNode::apply(q, k, v, log_decay, initial, lengths, scale, final);
+}
+Tensor linear_attn_packed(const Tensor &features, int64_t H, const Tensor &log_decay, double scale, bool save_8bit)
+{
+    return PackedLinearAttnNode::apply(features, H, log_decay, scale, save_8bit);
+}
+
 } // namespace
 
 TORCH_LIBRARY_FRAGMENT(gcg, m)
@@ -258,6 +528,16 @@ TORCH_LIBRARY_FRAGMENT(gcg, m)
     m.def("layer_norm_bwd(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor stats, Tensor? w, Tensor? b)"
           " -> (Tensor, Tensor, Tensor)");
     m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, bool save_8bit) -> Tensor", &layer_norm);
+    m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial, Tensor? lengths, float scale, bool final)"
+          " -> (Tensor, Tensor)");
+    m.def("linear_attn_bwd(Tensor d_o, Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial, Tensor? lengths, Tensor? dfinal,"
+          " float scale, bool need_dinitial) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("linear_attn_packed_fwd(Tensor features, int H, Tensor log_decay, float scale) -> Tensor");
+    m.def("linear_attn_packed_bwd(Tensor d_o, Tensor features, int H, Tensor log_decay, float scale) -> Tensor");
+    m.def("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) -> Tensor");
+    m.def("linear_attn(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial, Tensor? lengths, float scale, bool final)"
+          " -> Tensor[]", &linear_attn);
+    m.def("linear_attn_packed(Tensor features, int H, Tensor log_decay, float scale, bool save_8bit) -> Tensor", &linear_attn_packed);
 }
 
 TORCH_LIBRARY_IMPL(gcg, CUDA, m)
@@ -267,6 +547,11 @@ TORCH_LIBRARY_IMPL(gcg, CUDA, m)
     m.impl("layer_norm_fwd", &layer_norm_fwd);
     m.impl("layer_norm_infer", &layer_norm_infer);
     m.impl("layer_norm_bwd", &layer_norm_bwd);
+    m.impl("linear_attn_fwd", &linear_attn_fwd);
+    m.impl("linear_attn_bwd", &linear_attn_bwd);
+    m.impl("linear_attn_packed_fwd", &linear_attn_packed_fwd);
+    m.impl("linear_attn_packed_bwd", &linear_attn_packed_bwd);
+    m.impl("linear_attn_step", &linear_attn_step);
 }
 
 TORCH_LIBRARY_IMPL(gcg, Meta, m)
@@ -276,4 +561,9 @@ TORCH_LIBRARY_IMPL(gcg, Meta, m)
     m.impl("layer_norm_fwd", &layer_norm_fwd_meta);
     m.impl("layer_norm_infer", &layer_norm_infer_meta);
     m.impl("layer_norm_bwd", &layer_norm_bwd_meta);
+    m.impl("linear_attn_fwd", &linear_attn_fwd_meta);
+    m.impl("linear_attn_bwd", &linear_attn_bwd_meta);
+    m.impl("linear_attn_packed_fwd", &linear_attn_packed_fwd_meta);
+    m.impl("linear_attn_packed_bwd", &linear_attn_packed_bwd_meta);
+    m.impl("linear_attn_step", &linear_attn_step_meta);
 }
