@@ -569,11 +569,13 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
  * A row of v that holds an infinity or a NaN also makes NaN of outputs up to 31 rows before it (forward; as of do
  * for dk and dv's rows after it): it meets them in one matrix instruction, times zero.
  *
- * dk, dv up to GCG_LINEAR_MAX_DIM, bs * H up to GCG_LINEAR_MAX_HEADS, else GCG_ERR_UNSUPPORTED.  scale: finite, not 0.  dtype:
+ * dk, dv up to GCG_LINEAR_MAX_DIM, multiples of 8 (GCG_F32: of 4; the step takes any), bs * H up to GCG_LINEAR_MAX_HEADS, time strides up to GCG_LINEAR_MAX_TIME_STRIDE elements,
+ * L up to GCG_LINEAR_MAX_ROWS, else GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, not 0.  dtype:
  * GCG_F32, GCG_BF16, GCG_F16.  workspace: gcg_linear_attn_workspace_bytes (0: none), 256-byte aligned.  Results are the same on
  * every run.
  */
-enum { GCG_LINEAR_MAX_DIM = 256, GCG_LINEAR_MAX_HEADS = 65535 };
+enum { GCG_LINEAR_MAX_DIM = 256, GCG_LINEAR_MAX_HEADS = 65535, GCG_LINEAR_MAX_TIME_STRIDE = 1 << 22,
+       GCG_LINEAR_MAX_ROWS = 1 << 30 };
 GCG_API size_t gcg_linear_attn_workspace_bytes(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, int32_t backward);
 GCG_API int gcg_linear_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, const float *log_decay,
             const float *initial, const int32_t *lengths, void *o, float *final, void *workspace, size_t workspace_bytes,

@@ -1171,9 +1171,13 @@ def _check_lengths(t, q) -> None:
         raise ValueError("lengths must be a contiguous int32 tensor of one element a batch entry on q's device")
 
 
+LINEAR_MAX_TIME_STRIDE = 1 << 22    # GCG_LINEAR_MAX_TIME_STRIDE
+
+
 def _rows(t):
-    """The tensor with a contiguous last dimension, as the kernels read it."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+    """The tensor with a contiguous last dimension and rows near enough to each other, as the kernels read it."""
+    in_place = (t.shape[-1] == 1 or t.stride(-1) == 1) and (t.dim() < 4 or t.stride(1) <= LINEAR_MAX_TIME_STRIDE)
+    return t if in_place else t.contiguous()
 
 
 def _strides(n: int, *tensors):
@@ -1183,6 +1187,23 @@ def _strides(n: int, *tensors):
 
 def _passed_on(source, to):
     return None if to is None else to.copy_(source) if source is not None else to.zero_()
+
+
+def _to_whole(q, d: int) -> int:
+    """Zeros that a head dimension lacks to whole vectors: to a multiple of 8 (4 is enough in float32)."""
+    return 0 if q.dtype == torch.float32 and d % 4 == 0 else -d % 8
+
+
+def _padded(n: int, *tensors):
+    return [torch.nn.functional.pad(t, (0, n)) if n else t for t in tensors]
+
+
+def _padded_state(t, pk: int, pv: int):
+    return torch.nn.functional.pad(t, (0, pv, 0, pk)) if t is not None else None
+
+
+def _cut_state(t, dk: int, dv: int):
+    return t[:, :, :dk, :dv].contiguous() if t is not None else None
 
 
 def _linear_workspace(lib, q, v, backward):
@@ -1207,6 +1228,10 @@ def linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale: float, final: b
     last = torch.empty(bs, H, dk, dv, dtype=torch.float32, device=q.device) if final else None
     if o.numel() == 0:
         return o, _passed_on(initial, last)
+    pk, pv = _to_whole(q, dk), _to_whole(q, dv)
+    if pk or pv:
+        o, last = linear_attn_fwd(*_padded(pk, q, k), *_padded(pv, v), log_decay, _padded_state(initial, pk, pv), lengths, scale, final)
+        return o[..., :dv].contiguous(), _cut_state(last, dk, dv)
     with _on_device(q.device):
         q, k, v = _rows(q), _rows(k), _rows(v)
         n, ws = _linear_workspace(lib, q, v, False)
@@ -1245,6 +1270,13 @@ def linear_attn_bwd(do, q, k, v, log_decay, initial, lengths, dfinal, scale: flo
     di = torch.empty(q.shape[0], q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=q.device) if need_dinitial else None
     if do.numel() == 0:
         return dq, dk, dv, _passed_on(dfinal, di)
+    nk, nv = q.shape[-1], v.shape[-1]
+    pk, pv = _to_whole(q, nk), _to_whole(q, nv)
+    if pk or pv:
+        do, v, q, k = *_padded(pv, do, v), *_padded(pk, q, k)
+        dq, dk, dv, di = linear_attn_bwd(do, q, k, v, log_decay, _padded_state(initial, pk, pv), lengths, _padded_state(dfinal, pk, pv),
+                                         scale, need_dinitial)
+        return dq[..., :nk].contiguous(), dk[..., :nk].contiguous(), dv[..., :nv].contiguous(), _cut_state(di, nk, nv)
     _linear_bwd_into(do, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, dk, dv, di)
     return dq, dk, dv, di
 
@@ -1271,7 +1303,10 @@ def linear_attn_packed_bwd(do, features, heads: int, log_decay, scale: float):
     q, k, v = _split_features(features, heads)
     _check_linear(q, k, v, log_decay, 4)
     df = torch.empty_like(features)
-    if df.numel():
+    if df.numel() and _to_whole(q, q.shape[-1]):
+        for part, g in zip(_split_features(df, heads), linear_attn_bwd(do, q, k, v, log_decay, None, None, None, scale, False)):
+            part.copy_(g)
+    elif df.numel():
         _linear_bwd_into(do, q, k, v, log_decay, None, None, None, scale, *_split_features(df, heads), None)
     return df
 

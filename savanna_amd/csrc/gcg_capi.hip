@@ -942,20 +942,32 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
 // ---- linear attention with a decay for each head ------------------------------------------------------
 
 namespace {
+// L: 0 for a single token
 int linear_check(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype)
 {
-    if (bs <= 0 || L <= 0 || H <= 0 || dk <= 0 || dv <= 0) return GCG_ERR_BAD_ARG;
+    if (bs <= 0 || L < 0 || H <= 0 || dk <= 0 || dv <= 0) return GCG_ERR_BAD_ARG;
     if (dtype != GCG_F32 && dtype != GCG_BF16 && dtype != GCG_F16) return GCG_ERR_BAD_ARG;
     if (!(scale - scale == 0.f) || scale == 0.f) return GCG_ERR_BAD_ARG;
-    // heads and batch index the grid together
-    return dk > GCG_LINEAR_MAX_DIM || dv > GCG_LINEAR_MAX_DIM || bs > GCG_LINEAR_MAX_HEADS || bs * H > GCG_LINEAR_MAX_HEADS ? GCG_ERR_UNSUPPORTED : GCG_OK;
+    // rows are read in vectors (the step reads by elements); heads and batch index the grid together
+    const int vec = dtype == GCG_F32 ? 4 : 8;
+    if (L != 0 && (dk % vec || dv % vec)) return GCG_ERR_UNSUPPORTED;
+    return L > GCG_LINEAR_MAX_ROWS || dk > GCG_LINEAR_MAX_DIM || dv > GCG_LINEAR_MAX_DIM || bs > GCG_LINEAR_MAX_HEADS || bs * H > GCG_LINEAR_MAX_HEADS ? GCG_ERR_UNSUPPORTED : GCG_OK;
+}
+// a chunk's rows are addressed by 32-bit offsets
+int strides_check(const int64_t *s, int tensors, int dims)
+{
+    for (int i = 0; i < tensors * dims; ++i)
+        if (s[i] < 0) return GCG_ERR_BAD_ARG;
+    for (int i = 0; dims == 3 && i < tensors; ++i)
+        if (s[3 * i + 1] > GCG_LINEAR_MAX_TIME_STRIDE) return GCG_ERR_UNSUPPORTED;
+    return GCG_OK;
 }
 bool missing(const void *ws, size_t have, size_t need) { return need && (!ws || have < need || ((uintptr_t)ws & 255)); }
 } // namespace
 
 GCG_API size_t gcg_linear_attn_workspace_bytes(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, int32_t backward)
 {
-    if (linear_check(bs, L, H, dk, dv, 1.f, GCG_F32)) return 0;
+    if (L <= 0 || linear_check(bs, L, H, dk, dv, 1.f, GCG_F32)) return 0;
     return (gcg::linear_attn_workspace(bs, L, H, dk, dv, backward != 0) + 255) & ~(size_t)255;
 }
 
@@ -966,7 +978,8 @@ GCG_API int gcg_linear_attn_fwd(const void *q, const void *k, const void *v, con
 {
     TimerScope timer_scope;
     if (!q || !k || !v || !strides || !log_decay || !o) return GCG_ERR_BAD_ARG;
-    int rc = linear_check(bs, L, H, dk, dv, scale, dtype);
+    int rc = L <= 0 ? GCG_ERR_BAD_ARG : linear_check(bs, L, H, dk, dv, scale, dtype);
+    if (!rc) rc = strides_check(strides, 4, 3);
     if (rc) return rc;
     if (missing(workspace, workspace_bytes, gcg_linear_attn_workspace_bytes(bs, L, H, dk, dv, 0))) return GCG_ERR_WORKSPACE;
     rc = check_device();
@@ -982,7 +995,8 @@ GCG_API int gcg_linear_attn_bwd(const void *d_o, const void *q, const void *k, c
 {
     TimerScope timer_scope;
     if (!d_o || !q || !k || !v || !strides || !log_decay || !dq || !d_k || !d_v) return GCG_ERR_BAD_ARG;
-    int rc = linear_check(bs, L, H, dk, dv, scale, dtype);
+    int rc = L <= 0 ? GCG_ERR_BAD_ARG : linear_check(bs, L, H, dk, dv, scale, dtype);
+    if (!rc) rc = strides_check(strides, 7, 3);
     if (rc) return rc;
     if (missing(workspace, workspace_bytes, gcg_linear_attn_workspace_bytes(bs, L, H, dk, dv, 1))) return GCG_ERR_WORKSPACE;
     rc = check_device();
@@ -996,7 +1010,8 @@ GCG_API int gcg_linear_attn_step(const void *q, const void *k, const void *v, vo
 {
     TimerScope timer_scope;
     if (!q || !k || !v || !o || !strides || !log_decay || !state) return GCG_ERR_BAD_ARG;
-    int rc = linear_check(bs, 1, H, dk, dv, scale, dtype);
+    int rc = linear_check(bs, 0, H, dk, dv, scale, dtype);
+    if (!rc) rc = strides_check(strides, 4, 2);
     if (rc) return rc;
     rc = check_device();
     if (rc) return rc;

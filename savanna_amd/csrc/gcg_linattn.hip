@@ -32,7 +32,6 @@ constexpr int CHUNK = 64, COLS = 32;        // rows of a chunk; columns of c a w
 constexpr int THREADS = 256;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 
 // ---- operands of the matrix instructions ------------------------------------------------------------------
 // A fragment is a lane's part of a 16 x KF operand: row (of the first operand) or column (of the second) lane % 16, and in
@@ -74,28 +73,53 @@ template <> struct Mat<float> {
     }
 };
 
-// KF rows of a tile in LDS as the inner dimension, 16 of its columns as the operand's rows: rows row0 + 4 g .. + 3 (and, in 16
-// bits, row0 + 16 + 4 g .. + 3), the order in which a lane holds four results of a product in each of two tiles.  The columns are
-// col0 + lane % 16, or, SPREAD, col0 + 8 (lane % 16 / 4) + lane % 4, so that two such tiles four columns apart give a lane eight
-// columns side by side.  In 16 bits by the transposing LDS load, which hands lane i of 16 the i-th column of four rows of
-// four lanes' 8 bytes each.
-template <typename T, bool SPREAD>
-__device__ __forceinline__ u32x4 inner_rows(const T *tile, int stride, int row0, int col0, int lane)
+// ---- tiles in LDS -------------------------------------------------------------------------------------------
+// A tile's rows lie one after the other without padding; inside a row, 16-byte pieces (in b and the state's copy) or halves (in
+// c and the weighted c) change places by the row, so that the lanes that one LDS cycle serves touch every bank once.  Measured
+// with 16 waves, cycles a wave: 16-byte reads of 16 rows 4.0 (rows padded by 16 bytes: 8.0); transposing reads 2.3 (padded,
+// rows in their own order: 4.0).
+//
+// b, and the state's copy with a slice's columns as rows: rows of DA elements
+template <typename T, int DA> __device__ __forceinline__ int wide_at(int row, int piece)
 {
-    const int l = lane & 15, g = lane >> 4;
-    if constexpr (sizeof(T) == 2) {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s4 *lds_p;
-        const T *p = tile + (row0 + 4 * g + (l >> 2)) * stride + col0 + (SPREAD ? 8 : 4) * (l & 3);
-        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 16 * stride)));
-        return u32x4{lo[0], lo[1], hi[0], hi[1]};
-    } else {
-        const int col = SPREAD ? 8 * (l >> 2) + (l & 3) : l;
-        const float *p = (const float *)tile + (row0 + 4 * g) * stride + col0 + col;
-        return u32x4{__float_as_uint(p[0]), __float_as_uint(p[stride]), __float_as_uint(p[2 * stride]), __float_as_uint(p[3 * stride])};
-    }
+    const int swap = DA * sizeof(T) >= 256 ? row & 15 : (row & 2) | (row & 8) >> 1 | (row >> 2 & 1);
+    return row * DA + (piece ^ swap) * Mat<T>::V;
 }
+// c and the weighted c: rows of COLS elements (fp32: padded by 16 bytes, which serves its plain loads)
+template <typename T> constexpr int kSliceRow = sizeof(T) == 2 ? COLS : COLS + 4;
+template <typename T, int BIT> __device__ __forceinline__ int slice_at(int row, int col)
+{
+    if constexpr (sizeof(T) == 2) return row * COLS + (col ^ (row >> BIT & 1) << 4);
+    else return row * kSliceRow<T> + col;
+}
+constexpr int C_BIT = 2, W_BIT = 3;
+
+// The order of a tile's 16 rows as a product's inner dimension: lane group g takes four of them, its lanes' results or loads in
+// this order on both sides.  The scores' (and c's) order is that of the product that makes them; the state's update has
+// one that suits both b's and the weighted c's banks.
+__device__ __forceinline__ int score_row(int g, int i) { return 4 * g + i; }
+template <typename T> __device__ __forceinline__ int update_row(int g, int i)
+{
+    return sizeof(T) == 2 ? 8 * (g & 1) + 2 * i + ((i >> 1 ^ g >> 1) & 1) : 4 * g + i;
+}
+// A lane's part of KF rows at p (the lane's own element there) as the inner dimension, 16 columns as the operand's rows.  In 16
+// bits by the transposing load, which hands lane i of 16 the i-th column of four rows, of which four lanes each
+// address 8 bytes; `far` is the distance of the next 16 rows.  In fp32 by the offsets of the group's four rows.
+template <typename T> __device__ __forceinline__ u32x4 load_inner(const T *p, int far)
+{
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 *lds_p;
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + far)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+__device__ __forceinline__ u32x4 load_inner(const float *p, const int (&row)[4])
+{
+    return u32x4{__float_as_uint(p[row[0]]), __float_as_uint(p[row[1]]), __float_as_uint(p[row[2]]), __float_as_uint(p[row[3]])};
+}
+// Where column n of a slice lies in LDS as a row of the state's copy and as a column of c: a product's 16 of them side by side
+// give a lane columns 8 g .. 8 g + 3, the next 16 columns 8 g + 4 .. 8 g + 7 of the output.
+__device__ __forceinline__ int spread(int n) { return 16 * ((n >> 2) & 1) + 4 * (n >> 3) + (n & 3); }
 
 // The powers of two that bring a largest magnitude to 1/2 .. 1 and back; 1 for none, infinities and NaN.
 struct Range { float down, up; };
@@ -130,7 +154,7 @@ struct Walks {
     const int32_t *lengths;     // of the batch entries, or null: L
     float *seg;                 // states of the segments, [walk][bs][H][segment][da][dc]
     int64_t seg_walk[3];        // where a walk's begin
-    int64_t L, seg_rows;        // seg_rows: multiple of 64
+    int32_t L, seg_rows;        // seg_rows: multiple of 64
     int32_t n, bs, H, segments;
     int64_t groups;             // n * bs * H * segments
 };
@@ -145,21 +169,6 @@ __device__ __forceinline__ void power(float g, int n, float &hi, float &lo)
     lo = (float)(p - (double)hi);
 }
 
-// vector of row elements at column c of D; FULL: the caller knows that all are there
-template <typename T, bool FULL> __device__ __forceinline__ u32x4 load_cols(const T *row, int c, int D)
-{
-    constexpr int V = Mat<T>::V;
-    if (FULL || c + V <= D) return *(const u32x4_any *)(row + c);
-    u32x4 r = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (c + i < D) {
-            if constexpr (sizeof(T) == 2) r[i / 2] |= (uint32_t)((const uint16_t *)row)[c + i] << (16 * (i & 1));
-            else r[i] = ((const uint32_t *)row)[c + i];
-        }
-    return r;
-}
-
 // (group, slice) of a workgroup: the slices of a head follow one another on one XCD, whose L2 then holds the a and b they share
 __device__ __forceinline__ void place(int64_t id, int slices, int64_t &group, int &slice)
 {
@@ -169,158 +178,164 @@ __device__ __forceinline__ void place(int64_t id, int slices, int64_t &group, in
     group = block * 8 + (rest & 7);
 }
 
-// OUT: the walk with its output; otherwise the state alone, of a segment that starts from nothing.  PARTS: 16-bit parts of the
-// weighted c.  FULL: da is DA and dc a multiple of COLS.
-template <typename T, int DA, bool OUT, int PARTS, bool FULL>
-__global__ __launch_bounds__(THREADS) void walk_kernel(Walks args, int slices)
-{
+// One workgroup's walk: its place, its rows in memory and in LDS, and the parts of a chunk's work.
+//
+// OUT: with an output; otherwise the state alone, of a segment that starts from nothing.  PARTS: 16-bit parts of the weighted
+// c.  FULL: da is DA and dc a multiple of COLS; otherwise both are multiples of a vector.
+template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     typedef Mat<T> M;
-    constexpr int V = M::V, KF = M::KF, KB = DA / KF, KG = CHUNK / KF;
-    constexpr int BS = DA + V, CS = COLS + 16 / (int)sizeof(T), SS = DA + V;       // LDS row strides: 16 bytes past the row
-    constexpr int SETS = (size_t)2 * (CHUNK * BS + (PARTS + 1) * CHUNK * CS + (OUT ? COLS * SS : 0)) * sizeof(T) <= 160 * 1024 ? 2 : 1;
+    static constexpr bool F16 = __is_same(T, f16_t);
+    static constexpr int V = M::V, KF = M::KF, KB = DA / KF, KG = CHUNK / KF;
+    static constexpr int CS = kSliceRow<T>;
+    static constexpr size_t ONE = (size_t)(CHUNK * DA + (PARTS + OUT) * CHUNK * CS + (OUT ? COLS * DA : 0)) * sizeof(T);
+    static constexpr int SETS = 2 * ONE <= 160 * 1024 - 256 ? 2 : 1;
+    static_assert(SETS * ONE <= 160 * 1024 - 256, "workgroup exceeds the 160 KB of LDS");
     // 16-row tiles of the state a wave keeps, and of its two 16-column ones: whole blocks of KF rows in 16 bits
-    constexpr int NW = DA == 64 ? 1 : 2, MT = DA == 64 ? 2 : DA / 64;
-    constexpr bool F16 = __is_same(T, f16_t);
-    constexpr size_t LDS = (size_t)SETS * (CHUNK * BS + (PARTS + 1) * CHUNK * CS + (OUT ? COLS * SS : 0)) * sizeof(T);
-    static_assert(LDS <= 160 * 1024, "workgroup exceeds the 160 KB of LDS");
-    __shared__ __align__(16) unsigned char lds_raw[LDS];
-    __shared__ float lds_range[SETS][F16 && OUT ? KB : 1][2];
-    T *const lds_b = (T *)lds_raw, *const lds_c = lds_b + SETS * CHUNK * BS, *const lds_w = lds_c + SETS * CHUNK * CS,
-            *const lds_s = lds_w + SETS * PARTS * CHUNK * CS;
+    static constexpr int NW = DA == 64 ? 1 : 2, MT = DA == 64 ? 2 : DA / 64;
+    static constexpr bool DEEP = DA * sizeof(T) <= 256;     // registers for the rows of two chunks ahead (else one)
+    static constexpr int BT = DA / V, BR = 256 / BT, BP = CHUNK / BR;      // b: threads a row, rows a pass, passes
+    static constexpr int CT = COLS / V, CR = 256 / CT, CP = CHUNK / CR;    // c
 
-    int64_t group;
-    int slice;
-    place(blockIdx.x, slices, group, slice);
-    if (group >= args.groups) return;
-    const int seg = (int)(group % args.segments);
-    group /= args.segments;
-    const int h = (int)(group % args.H);
-    group /= args.H;
-    const int b = (int)(group % args.bs), job = (int)(group / args.bs);
-    const Walk &wk = args.w[job];
-    const int da = wk.da, dc = wk.dc, n0 = slice * COLS;
-    if (n0 >= dc) return;
-    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, g4 = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-    int64_t length = args.L;
-    if (args.lengths) {
-        length = args.lengths[b];
-        length = length < 0 ? 0 : length > args.L ? args.L : length;
-    }
-    const int64_t from = seg * args.seg_rows, to = from + args.seg_rows < length ? from + args.seg_rows : length;
-    const T *const pa = (const T *)wk.a.p + b * wk.a.sb + h * wk.a.sh, *const pb = (const T *)wk.b.p + b * wk.b.sb + h * wk.b.sh,
-                  *const pc = (const T *)wk.c.p + b * wk.c.sb + h * wk.c.sh;
-    T *const po = (T *)wk.out.p + b * wk.out.sb + h * wk.out.sh;
-    const auto row_of = [&](int64_t r) { return wk.reverse ? length - 1 - r : r; };     // walk's row -> time
-    const float decay = clamp_decay(args.log_decay[h]), l2 = decay * 1.44269504f;
-    const int64_t state_at = (int64_t)(b * args.H + h) * da * dc;
-
-    // ---- what does not change from chunk to chunk
-    float f[4][4];              // OUT: f^(t-s) of this wave's rows (lane % 16) and the four columns of each score tile
-    float row_mul = 0.f;
-    if constexpr (OUT) {
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int d = 16 * (wave - st) + l16 - 4 * g4 - i;
-                f[st][i] = d >= 0 ? exp2f(l2 * d) : 0.f;
-            }
-        row_mul = exp2f(l2 * (16 * wave + l16));
-    }
-    float chunk_hi, chunk_lo;
-    power(decay, CHUNK, chunk_hi, chunk_lo);
-
-    // ---- the state: tile (mt, nw) holds rows m0 + 16 mt + 4 g4 .. + 3 of the slice's column c0 + 16 nw + l16
-    const int m0 = DA == 64 ? (wave >> 1) * 32 : wave * (DA / 4), c0 = DA == 64 ? (wave & 1) * 16 : 0;
-    f32x4 S[MT][NW];
-    const float *first = nullptr;
-    int64_t fi = wk.si, fj = wk.sj;
-    float first_mul = 1.f;
-    int lead = 1;
-    if (OUT && args.segments > 1) {         // (the segments' states are joined: each begins from its own)
-        first = args.seg + args.seg_walk[job] + ((int64_t)(b * args.H + h) * args.segments + seg) * da * dc;
-        fi = dc; fj = 1;
-        lead = seg == 0 ? wk.lead : 1;
-    } else if (OUT && wk.first) {
-        first = wk.first + state_at;
-        first_mul = wk.first_mul;
-        lead = wk.lead;
-    }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nw = 0; nw < NW; ++nw)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int m = m0 + 16 * mt + 4 * g4 + i, n = n0 + c0 + 16 * nw + l16;
-                S[mt][nw][i] = first && m < da && n < dc ? first[m * fi + n * fj] * first_mul : 0.f;
-            }
-    const auto publish = [&](int set) {     // the state's rounded copy, columns as rows
-        if constexpr (OUT) {
-#pragma unroll
-            for (int nw = 0; nw < NW; ++nw) {
-                float by[MT / 2 ? MT / 2 : 1];
-                if constexpr (F16) {
-#pragma unroll
-                    for (int kb = 0; kb < MT / 2; ++kb) {
-                        float top = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(S[2 * kb + i / 4][nw][i & 3]));
-                        const Range r = range(wave_max(top));
-                        by[kb] = r.down;
-                        if (lane == 0) lds_range[set][m0 / KF + kb][c0 / 16 + nw] = r.up;
-                    }
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    T *to = lds_s + set * COLS * SS + (c0 + 16 * nw + l16) * SS + m0 + 16 * mt + 4 * g4;
-                    f32x4 v = S[mt][nw];
-                    if constexpr (F16) v *= by[mt / 2];
-                    if constexpr (sizeof(T) == 2) *(u32x2 *)to = u32x2{M::pack(v[0], v[1]), M::pack(v[2], v[3])};
-                    else *(f32x4 *)to = v;
-                }
-            }
-        }
+    struct Lds {
+        __align__(16) T b[SETS][CHUNK * DA];
+        __align__(16) T c[SETS][OUT ? CHUNK * CS : 1];
+        __align__(16) T w[SETS][PARTS][CHUNK * CS];
+        __align__(16) T s[SETS][OUT ? COLS * DA : 1];
+        float range[SETS][F16 && OUT ? KB : 1][2];
     };
 
-    // ---- rows from memory: b in passes over the chunk's rows, c's 32 columns, and a's fragments of this wave's rows
-    constexpr int BT = DA / V, BR = THREADS / BT, BP = CHUNK / BR;      // threads a row, rows a pass, passes
-    constexpr int CT = COLS / V, CR = THREADS / CT, CP = CHUNK / CR;
-    const int b_row = tid / BT, b_col = tid % BT * V, c_row = tid / CT, c_col = tid % CT * V;
-    u32x4 rb[BP], rc[CP], ra[OUT ? KB : 1];
-    const auto request = [&](int64_t at) {                              // the chunk of rows at ..; rows past the end repeat the last one
-#pragma unroll
-        for (int i = 0; i < BP; ++i) {
-            const int64_t r = at + b_row + i * BR;
-            rb[i] = load_cols<T, FULL>(pb + row_of(r < to ? r : to - 1) * wk.b.st, b_col, da);
+    const Walks &args;
+    const Walk &wk;
+    Lds &lds;
+    int b, h, seg, job, da, dc, n0, lane, l16, g4, wave, tid;
+    int length, from, rows;     // of the sequence; the segment's first row and its rows
+    int64_t state_at;
+    float decay, l2;
+    int lead;                   // of the first chunk
+
+    __device__ Walker(const Walks &args_, const Walk &wk_, Lds &lds_) : args(args_), wk(wk_), lds(lds_) {}
+
+    // ---- rows in memory
+    // A chunk of one tensor is a window from its lowest row to its highest row's last column; a lane's place in it is a 32-bit
+    // offset that does not change from chunk to chunk but for a shift (a chunk of fewer rows, walked backwards).  Rows past the end
+    // lie outside the window, and so do columns past the row's end, whose lanes hold an offset beyond any window: such
+    // loads return zero and such stores are dropped, so no access is conditional, and the waits before the use of one chunk's rows
+    // leave the next chunks' requests in flight.  A stream hands out the windows of one chunk after the other; what it needs is in
+    // scalar registers (through readfirstlane, or the compiler loads it from the kernel's arguments again in every chunk and
+    // waits for that).
+    static constexpr uint32_t NOWHERE = 0xc0000000u;
+    struct Chunk { win_t win; uint32_t shift; };
+    struct Stream {
+        uint64_t base;          // of the chunk's lowest row, if the chunk is full
+        int64_t step;
+        int unit, tail, left;   // bytes from row to row, and of a row; rows from this chunk on
+        bool reverse;
+        __device__ __forceinline__ Chunk next()
+        {
+            const int rows = left < 0 ? 0 : left < CHUNK ? left : CHUNK;
+            const int absent = reverse ? (CHUNK - rows) * unit : 0;
+            const Chunk c = {make_window((const void *)(base + (uint32_t)absent), rows ? (rows - 1) * unit + tail : 0), 0u - (uint32_t)absent};
+            base += step;
+            left -= CHUNK;
+            return c;
         }
+    };
+    static __device__ __forceinline__ uint64_t uniform(uint64_t x)
+    {
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32 |
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+    }
+    __device__ __forceinline__ Stream stream(const Rows &r, int cols) const
+    {
+        Stream s;
+        const int64_t row = wk.reverse ? (int64_t)length - from - CHUNK : from;
+        s.reverse = __builtin_amdgcn_readfirstlane(wk.reverse) != 0;
+        s.base = uniform((uint64_t)r.p + (uint64_t)((b * r.sb + h * r.sh + row * r.st) * (int64_t)sizeof(T)));
+        s.unit = __builtin_amdgcn_readfirstlane((int)r.st * (int)sizeof(T));
+        s.step = s.reverse ? -(int64_t)CHUNK * s.unit : (int64_t)CHUNK * s.unit;
+        s.tail = __builtin_amdgcn_readfirstlane(cols * (int)sizeof(T));
+        s.left = __builtin_amdgcn_readfirstlane(rows);
+        return s;
+    }
+    __device__ __forceinline__ uint32_t offset(const Rows &r, int i, int col, int cols) const
+    {
+        if (!FULL && col >= cols) return NOWHERE;
+        return (uint32_t)(wk.reverse ? CHUNK - 1 - i : i) * (uint32_t)r.st * (uint32_t)sizeof(T) + (uint32_t)(col * sizeof(T));
+    }
+    static __device__ __forceinline__ u32x4 load(const Chunk &c, uint32_t off) { return win_load_aux<0, u32x4>(c.win, off + c.shift); }
+    __device__ __forceinline__ int rows_in(int chunk) const { return rows - chunk * CHUNK < CHUNK ? rows - chunk * CHUNK : CHUNK; }
+
+    // ---- the state waves: rows into LDS, the state from chunk to chunk
+    struct Fetch { u32x4 b[BP], c[CP]; };
+    uint32_t ob[BP], oc[CP];
+    int b_row, b_col, c_row, c_col;
+    float first_hi, first_lo, chunk_hi, chunk_lo, last_hi, last_lo;     // f^rows of the first, a full and the last chunk
+    int m0, c0;                 // tile (mt, nw): rows m0 + 16 mt + 4 g4 .. + 3, the slice's column c0 + 16 nw + l16
+    f32x4 S[NW][MT];
+
+    __device__ __forceinline__ void state_setup(int t)
+    {
+        b_row = t / BT; b_col = t % BT * V; c_row = t / CT; c_col = t % CT * V;
+        sb = stream(wk.b, da);
+        sc = stream(wk.c, dc);
+#pragma unroll
+        for (int i = 0; i < BP; ++i) ob[i] = offset(wk.b, b_row + i * BR, b_col, da);
 #pragma unroll
         for (int i = 0; i < CP; ++i) {
-            const int64_t r = at + c_row + i * CR;
-            rc[i] = load_cols<T, FULL>(pc + row_of(r < to ? r : to - 1) * wk.c.st, n0 + c_col, dc);
+            oc[i] = offset(wk.c, c_row + i * CR, n0 + c_col, dc);
         }
-        if constexpr (OUT) {
-            const int64_t r = at + 16 * wave + l16;
-            const T *row = pa + row_of(r < to ? r : to - 1) * wk.a.st;
-#pragma unroll
-            for (int k = 0; k < KB; ++k) ra[k] = load_cols<T, FULL>(row, k * KF + g4 * V, da);
+        const int early = lead == 0 ? 1 : 0, last_rows = rows > 0 ? (rows - 1) % CHUNK + 1 : 0;
+        power(decay, CHUNK - early, first_hi, first_lo);
+        power(decay, CHUNK, chunk_hi, chunk_lo);
+        power(decay, last_rows - (rows <= CHUNK ? early : 0), last_hi, last_lo);
+        const int q = t / 64;
+        m0 = DA == 64 ? (q >> 1) * 32 : q * (DA / 4);
+        c0 = DA == 64 ? (q & 1) * 16 : 0;
+        const float *first = nullptr;
+        int64_t fi = wk.si, fj = wk.sj;
+        float mul = 1.f;
+        if (OUT && args.segments > 1) {     // (the segments' states are joined: each begins from its own)
+            first = args.seg + args.seg_walk[job] + ((int64_t)(b * args.H + h) * args.segments + seg) * da * dc;
+            fi = dc; fj = 1;
+        } else if (OUT && wk.first) {
+            first = wk.first + state_at;
+            mul = wk.first_mul;
         }
-    };
-    // into LDS: b, c and c weighted by f^(rows - 1 - r); rows past the end count for nothing
-    const auto deposit = [&](int set, int rows) {
 #pragma unroll
-        for (int i = 0; i < BP; ++i) *(u32x4 *)(lds_b + (set * CHUNK + b_row + i * BR) * BS + b_col) = rb[i];
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nw = 0; nw < NW; ++nw)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int m = m0 + 16 * mt + 4 * g4 + i, n = n0 + c0 + 16 * nw + l16;
+                    S[nw][mt][i] = first && m < da && n < dc ? first[m * fi + n * fj] * mul : 0.f;
+                }
+    }
+    Stream sb, sc;
+    __device__ __forceinline__ void fetch(Fetch &f)
+    {
+        const Chunk cb = sb.next(), cc = sc.next();
+#pragma unroll
+        for (int i = 0; i < BP; ++i) f.b[i] = load(cb, ob[i]);
+#pragma unroll
+        for (int i = 0; i < CP; ++i) f.c[i] = load(cc, oc[i]);
+    }
+    // b, c and c weighted by f^(rows - 1 - r); rows past the end count for nothing
+    __device__ __forceinline__ void deposit(int set, const Fetch &f, int rows) const
+    {
+#pragma unroll
+        for (int i = 0; i < BP; ++i) *(u32x4 *)(lds.b[set] + wide_at<T, DA>(b_row + i * BR, b_col / V)) = f.b[i];
 #pragma unroll
         for (int i = 0; i < CP; ++i) {
             const int r = c_row + i * CR;
             const float w = r < rows ? exp2f(l2 * (rows - 1 - r)) : 0.f;
-            u32x4 v = rc[i];
-            if (r >= rows) v = u32x4{0, 0, 0, 0};
-            T *const to_c = lds_c + (set * CHUNK + r) * CS + c_col;
-            if constexpr (OUT) *(u32x4 *)to_c = v;
-            T *const to_w = lds_w + (set * PARTS * CHUNK + r) * CS + c_col;
+            u32x4 v = f.c[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = r < rows ? v[j] : 0;
+            if constexpr (OUT) {
+                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col))) = u32x2{v[0], v[1]};
+                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col + V / 2))) = u32x2{v[2], v[3]};
+            }
             if constexpr (sizeof(T) == 2) {
                 u32x4 part[PARTS];
 #pragma unroll
@@ -336,205 +351,399 @@ __global__ __launch_bounds__(THREADS) void walk_kernel(Walks args, int slices)
                     }
                 }
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) *(u32x4 *)(to_w + p * CHUNK * CS) = part[p];
+                for (int p = 0; p < PARTS; ++p) *(u32x4 *)(lds.w[set][p] + slice_at<T, W_BIT>(r, c_col)) = part[p];
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * w);
-                *(u32x4 *)to_w = v;
+                *(u32x4 *)(lds.w[set][0] + slice_at<T, W_BIT>(r, c_col)) = v;
             }
         }
-    };
-
-    u32x4 a[OUT ? KB : 1];
-    if (from < to) {
-        request(from);
-        const int rows = (int)(to - from < CHUNK ? to - from : CHUNK);
-        deposit(0, rows);
-        publish(0);
-        __syncthreads();
     }
-    int set = 0;
-    for (int64_t at = from; at < to; at += CHUNK) {
-        const int rows = (int)(to - at < CHUNK ? to - at : CHUNK);
-        const bool more = at + CHUNK < to;
+    // the state's rounded copy, columns as rows
+    __device__ __forceinline__ void publish(int set) const
+    {
         if constexpr (OUT) {
 #pragma unroll
-            for (int k = 0; k < KB; ++k) a[k] = ra[k];
-        }
-        if (more) request(at + CHUNK);
-        const T *const tb = lds_b + set * CHUNK * BS, *const tc = lds_c + set * CHUNK * CS, *const tw = lds_w + set * PARTS * CHUNK * CS,
-                      *const ts = lds_s + set * COLS * SS;
-        if constexpr (OUT) {
-            // scores, transposed: rows 16 st + .. of b by this wave's rows of a
-            f32x4 P[4];
+            for (int nw = 0; nw < NW; ++nw) {
+                float by[MT / 2];
+                if constexpr (F16) {
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                P[st] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (st <= wave) {
+                    for (int kb = 0; kb < MT / 2; ++kb) {
+                        float top = 0.f;
 #pragma unroll
-                    for (int k = 0; k < KB; ++k)
-                        P[st] = M::mul(*(const u32x4 *)(tb + (16 * st + l16) * BS + k * KF + g4 * V), a[k], P[st]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) P[st][i] = f[st][i] != 0.f ? P[st][i] * f[st][i] : 0.f;
-                }
-            }
-            // output, transposed: this wave's rows by columns 8 g4 .. + 7 of the slice
-            f32x4 O[2];
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                O[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
-                const int n = 8 * (l16 >> 2) + (l16 & 3) + 4 * nt;
-#pragma unroll
-                for (int k = 0; k < KB; ++k) {
-                    const u32x4 x = *(const u32x4 *)(ts + n * SS + k * KF + g4 * V);
-                    if constexpr (F16) O[nt] += M::mul(x, a[k], f32x4{0.f, 0.f, 0.f, 0.f}) * lds_range[set][k][g4 >> 1];
-                    else O[nt] = M::mul(x, a[k], O[nt]);
-                }
-                const float m = row_mul * (at == from && lead == 0 ? 1.f : exp2f(l2));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) O[nt][i] *= m;
-            }
-            // (f16: the scores of a row, like the state's copy, by a power of two that brings the largest to about 1)
-            f32x4 inside[2] = {O[0], O[1]};
-            float up = 1.f;
-            if constexpr (F16) {
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(P[i >> 2][i & 3]));
-                top = fmaxf(top, __shfl_xor(top, 16));
-                const Range r = range(fmaxf(top, __shfl_xor(top, 32)));
-                up = r.up;
-#pragma unroll
-                for (int st = 0; st < 4; ++st) P[st] *= r.down;
-                inside[0] = inside[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-#pragma unroll
-            for (int p = 0; p < KG; ++p) {
-                u32x4 x;
-                if constexpr (sizeof(T) == 2) {
-                    if (2 * p > wave) continue;
-                    x = u32x4{M::pack(P[2 * p][0], P[2 * p][1]), M::pack(P[2 * p][2], P[2 * p][3]), M::pack(P[2 * p + 1][0], P[2 * p + 1][1]),
-                              M::pack(P[2 * p + 1][2], P[2 * p + 1][3])};
-                } else {
-                    if (p > wave) continue;
-                    x = __builtin_bit_cast(u32x4, P[p]);
-                }
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) inside[nt] = M::mul(inner_rows<T, true>(tc, CS, p * KF, 4 * nt, lane), x, inside[nt]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt) O[nt] = F16 ? O[nt] + inside[nt] * up : inside[nt];
-            if (16 * wave + l16 < rows) {
-                T *row = po + row_of(at + 16 * wave + l16) * wk.out.st;
-                const int n = n0 + 8 * g4;
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = O[i >> 2][i & 3] * wk.out_mul;
-                if (FULL || n + 8 <= dc) {
-                    if constexpr (sizeof(T) == 2) {
-                        *(u32x4_any *)(row + n) = u32x4{M::pack(v[0], v[1]), M::pack(v[2], v[3]), M::pack(v[4], v[5]), M::pack(v[6], v[7])};
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            *(u32x4_any *)(row + n + 4 * j) = u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                                                                    __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])};
+                        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(S[nw][2 * kb + i / 4][i & 3]));
+                        const Range r = range(wave_max(top));
+                        by[kb] = r.down;
+                        if (lane == 0) lds.range[set][m0 / KF + kb][c0 / 16 + nw] = r.up;
                     }
-                } else {
+                }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (n + i < dc) Elem<T>::store(row + n + i, v[i]);
+                for (int mt = 0; mt < MT; ++mt) {
+                    constexpr int LANES = V / 4;            // lane groups that share a piece
+                    T *to = lds.s[set] + wide_at<T, DA>(spread(c0 + 16 * nw + l16), (m0 + 16 * mt) / V + g4 / LANES) + g4 % LANES * 4;
+                    f32x4 v = S[nw][mt];
+                    if constexpr (F16) v *= by[mt / 2];
+                    if constexpr (sizeof(T) == 2) *(u32x2 *)to = u32x2{M::pack(v[0], v[1]), M::pack(v[2], v[3])};
+                    else *(f32x4 *)to = v;
                 }
             }
         }
-        // the state moves on
-        float hi = chunk_hi, lo = chunk_lo;
-        const int turns = rows - (at == from && lead == 0 ? 1 : 0);
-        if (turns != CHUNK) power(decay, turns, hi, lo);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int nw = 0; nw < NW; ++nw)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[mt][nw][i] = fmaf(S[mt][nw][i], hi, S[mt][nw][i] * lo);
-        if constexpr (F16) {
-            // parts after the first are stored 2^12, 2^24 times larger and added up on their own, the smallest first
-            f32x4 R[MT][NW];
-#pragma unroll
-            for (int part = PARTS - 1; part >= 0; --part) {
-                if (part == PARTS - 1) {
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int nw = 0; nw < NW; ++nw) R[mt][nw] = f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-#pragma unroll
-                for (int p = 0; p < KG; ++p)
-#pragma unroll
-                    for (int nw = 0; nw < NW; ++nw) {
-                        const u32x4 y = inner_rows<T, false>(tw + part * CHUNK * CS, CS, p * KF, c0 + 16 * nw, lane);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) R[mt][nw] = M::mul(inner_rows<T, false>(tb, BS, p * KF, m0 + 16 * mt, lane), y, R[mt][nw]);
-                    }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int nw = 0; nw < NW; ++nw) {
-                        if (part > 0) R[mt][nw] *= 0x1p-12f;
-                        else S[mt][nw] += R[mt][nw];
-                    }
-            }
+    }
+    // fragments of b and of the weighted c, rows as the inner dimension
+    __device__ __forceinline__ u32x4 inner_b(int set, int p, int mt) const
+    {
+        if constexpr (sizeof(T) == 2) {
+            const int at = wide_at<T, DA>(update_row<T>(g4, l16 >> 2), (m0 + 16 * mt) / V + (l16 >> 1 & 1)) + (l16 & 1) * 4;
+            return load_inner(lds.b[set] + p * KF * DA + at, 16 * DA);
         } else {
+            int at[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) at[i] = wide_at<T, DA>(update_row<T>(g4, i), (m0 + 16 * mt + l16) / V) + l16 % V;
+            return load_inner(lds.b[set] + p * KF * DA, at);
+        }
+    }
+    __device__ __forceinline__ u32x4 inner_w(int set, int part, int p, int nw) const
+    {
+        if constexpr (sizeof(T) == 2) {
+            const int at = slice_at<T, W_BIT>(update_row<T>(g4, l16 >> 2), c0 + 16 * nw + 4 * (l16 & 3));
+            return load_inner(lds.w[set][part] + p * KF * CS + at, 16 * CS);
+        } else {
+            const int at[4] = {4 * g4 * CS, (4 * g4 + 1) * CS, (4 * g4 + 2) * CS, (4 * g4 + 3) * CS};
+            return load_inner(lds.w[set][part] + p * KF * CS + c0 + 16 * nw + l16, at);
+        }
+    }
+    __device__ __forceinline__ u32x4 inner_c(int set, int p, int nt) const
+    {
+        if constexpr (sizeof(T) == 2) {
+            const int at = slice_at<T, C_BIT>(score_row(g4, l16 >> 2), 16 * nt + 4 * (l16 & 3));
+            return load_inner(lds.c[set] + p * KF * CS + at, 16 * CS);
+        } else {
+            const int at[4] = {4 * g4 * CS, (4 * g4 + 1) * CS, (4 * g4 + 2) * CS, (4 * g4 + 3) * CS};
+            return load_inner(lds.c[set] + p * KF * CS + 16 * nt + l16, at);
+        }
+    }
+    // S = f^rows S + (weighted c)^T b of the chunk in `set`.  Where registers allow it (DEEP) its fragments are requested before
+    // anything else of the turn; otherwise one inner block at a time.
+    struct Frags { u32x4 x[KG][MT], y[PARTS][KG][NW]; };
+    __device__ __forceinline__ void gather(Frags &f, int set) const
+    {
+        if constexpr (DEEP) {
 #pragma unroll
             for (int p = 0; p < KG; ++p) {
-                u32x4 x[MT];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) x[mt] = inner_rows<T, false>(tb, BS, p * KF, m0 + 16 * mt, lane);
+                for (int mt = 0; mt < MT; ++mt) f.x[p][mt] = inner_b(set, p, mt);
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part)
 #pragma unroll
-                    for (int nw = 0; nw < NW; ++nw) {
-                        const u32x4 y = inner_rows<T, false>(tw + part * CHUNK * CS, CS, p * KF, c0 + 16 * nw, lane);
+                    for (int nw = 0; nw < NW; ++nw) f.y[part][p][nw] = inner_w(set, part, p, nw);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // to[mt] += (weighted c's part)^T b, columns nw
+    __device__ __forceinline__ void update(const Frags &f, int set, int part, int nw, f32x4 (&to)[MT]) const
+    {
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) S[mt][nw] = M::mul(x[mt], y, S[mt][nw]);
-                    }
+        for (int p = 0; p < KG; ++p) {
+            const u32x4 y = DEEP ? f.y[part][p][nw] : inner_w(set, part, p, nw);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) to[mt] = M::mul(DEEP ? f.x[p][mt] : inner_b(set, p, mt), y, to[mt]);
+            if constexpr (!DEEP) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __device__ __forceinline__ void move_on(const Frags &f, int set, float hi, float lo)
+    {
+#pragma unroll
+        for (int nw = 0; nw < NW; ++nw)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[nw][mt][i] = fmaf(S[nw][mt][i], hi, S[nw][mt][i] * lo);
+#pragma unroll
+        for (int nw = 0; nw < NW; ++nw) {
+            if constexpr (F16) {
+                // parts after the first are stored 2^12, 2^24 times larger and added up on their own, the smallest first
+                f32x4 R[MT];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) R[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int part = PARTS - 1; part > 0; --part) {
+                    update(f, set, part, nw, R);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) R[mt] *= 0x1p-12f;
+                }
+                update(f, set, 0, nw, R);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) S[nw][mt] += R[mt];
+            } else {
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) update(f, set, part, nw, S[nw]);
             }
         }
-        if (more) {
-            if constexpr (SETS == 1) __syncthreads();
-            else set ^= 1;
-            deposit(set, (int)(to - at - CHUNK < CHUNK ? to - at - CHUNK : CHUNK));
-            publish(set);
-            __syncthreads();
+    }
+    __device__ __forceinline__ void store_last() const
+    {
+        float *last = nullptr;
+        int64_t li = wk.si, lj = wk.sj;
+        float mul = 1.f;
+        if (!OUT) {
+            last = args.seg + args.seg_walk[job] + ((int64_t)(b * args.H + h) * args.segments + seg) * da * dc;
+            li = dc; lj = 1;
+        } else if (args.segments == 1 && wk.last) {
+            last = wk.last + state_at;
+            mul = wk.last_mul * (wk.last_decays && length > 0 ? exp2f(l2) : 1.f);
         }
-    }
-
-    // ---- the state after the last row
-    float *last = nullptr;
-    int64_t li = wk.si, lj = wk.sj;
-    float last_mul = 1.f;
-    if (!OUT) {
-        last = args.seg + args.seg_walk[job] + ((int64_t)(b * args.H + h) * args.segments + seg) * da * dc;
-        li = dc; lj = 1;
-    } else if (args.segments == 1 && wk.last) {
-        last = wk.last + state_at;
-        last_mul = wk.last_mul * (wk.last_decays && length > 0 ? exp2f(l2) : 1.f);
-    }
-    if (last) {
+        if (!last) return;
+        int place = m0 + 4 * g4, column = n0 + c0 + l16;
+        asm("" : "+v"(place), "+v"(column));    // (or what state_setup computed of them is kept in registers all the way)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nw = 0; nw < NW; ++nw)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int m = m0 + 16 * mt + 4 * g4 + i, n = n0 + c0 + 16 * nw + l16;
-                    if (m < da && n < dc) last[m * li + n * lj] = S[mt][nw][i] * last_mul;
+                    const int m = place + 16 * mt + i, n = column + 16 * nw;
+                    if (m < da && n < dc) last[m * li + n * lj] = S[nw][mt][i] * mul;
                 }
     }
+    // One chunk: `next` holds the rows of the chunk after it (none after the last), and takes the next ones not yet requested.
+    template <int PARITY> __device__ __forceinline__ void state_turn(int chunk, int chunks, Fetch &next)
+    {
+        constexpr int SET = SETS == 2 ? PARITY : 0, OTHER = SETS == 2 ? PARITY ^ 1 : 0;
+        Frags f;
+        gather(f, SET);
+        if constexpr (SETS == 2) {
+            deposit(OTHER, next, rows_in(chunk + 1));
+            fetch(next);
+        }
+        const bool last = chunk + 1 == chunks;
+        move_on(f, SET, last ? last_hi : chunk == 0 ? first_hi : chunk_hi, last ? last_lo : chunk == 0 ? first_lo : chunk_lo);
+        if constexpr (SETS == 1) {
+            __syncthreads();
+            deposit(OTHER, next, rows_in(chunk + 1));
+            fetch(next);
+        }
+        publish(OTHER);
+        __syncthreads();
+    }
+    __device__ __forceinline__ void state_walk(int t)
+    {
+        state_setup(t);
+        if (rows > 0) {
+            const int chunks = (rows + CHUNK - 1) / CHUNK;
+            Fetch even, second, &odd = DEEP ? second : even;
+            fetch(even);
+            if constexpr (DEEP) fetch(odd);
+            deposit(0, even, rows_in(0));
+            fetch(even);
+            publish(0);
+            __syncthreads();
+            for (int chunk = 0; chunk < chunks; chunk += 2) {
+                state_turn<0>(chunk, chunks, odd);
+                if (chunk + 1 < chunks) state_turn<1>(chunk + 1, chunks, even);
+            }
+        }
+        store_last();
+    }
+
+    // ---- the output waves: rows 16 W .. 16 W + 15 of every chunk
+    struct RowsA { u32x4 k[KB]; };
+    float row_mul, step_mul;
+    float f[4][4];              // f^(t-s) of this wave's rows (lane % 16) and of the rows of each score tile
+    uint32_t oa[FULL ? 1 : KB], oo;
+
+    Stream sa, so;
+    float out_mul;
+
+    __device__ __forceinline__ void fetch_a(RowsA &a)
+    {
+        const Chunk c = sa.next();
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+            a.k[k] = load(c, FULL ? oa[0] + (uint32_t)(k * KF * sizeof(T)) : oa[FULL ? 0 : k]);
+    }
+    template <int W, int PARITY> __device__ __forceinline__ void out_turn(int chunk, RowsA &a)
+    {
+        constexpr int SET = SETS == 2 ? PARITY : 0;
+        const T *const tb = lds.b[SET], *const ts = lds.s[SET];
+        // Scores, transposed (rows 16 st + .. of b by this wave's rows of a), and what comes from before the chunk, transposed (the
+        // state's columns 8 g4 .. + 7 by this wave's rows).  All of a block's fragments are requested before the first product: left
+        // to itself the compiler keeps one or two reads ahead, and a wave then waits for LDS at every product.
+        f32x4 P[W + 1], O[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int st = 0; st <= W; ++st) P[st] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int BLOCK = KB < 4 || !DEEP ? 2 : 4;
+#pragma unroll
+        for (int kb = 0; kb < KB; kb += BLOCK) {
+            u32x4 xb[BLOCK][W + 1], xs[BLOCK][2];
+#pragma unroll
+            for (int k = 0; k < BLOCK; ++k) {
+                const int at_k = wide_at<T, DA>(l16, 4 * (kb + k) + g4);
+#pragma unroll
+                for (int st = 0; st <= W; ++st) xb[k][st] = *(const u32x4 *)(tb + 16 * st * DA + at_k);
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) xs[k][nt] = *(const u32x4 *)(ts + 16 * nt * DA + at_k);
+            }
+            if constexpr (DEEP) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < BLOCK; ++k) {
+#pragma unroll
+                for (int st = 0; st <= W; ++st) P[st] = M::mul(xb[k][st], a.k[kb + k], P[st]);
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    if constexpr (F16) O[nt] += M::mul(xs[k][nt], a.k[kb + k], f32x4{0.f, 0.f, 0.f, 0.f}) * lds.range[SET][kb + k][g4 >> 1];
+                    else O[nt] = M::mul(xs[k][nt], a.k[kb + k], O[nt]);
+                }
+            }
+        }
+        constexpr int GROUPS = sizeof(T) == 2 ? W / 2 + 1 : W + 1;
+        u32x4 xc[GROUPS][2];
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p)
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) xc[p][nt] = inner_c(SET, p, nt);
+        if constexpr (DEEP) __builtin_amdgcn_sched_barrier(0);
+        fetch_a(a);
+        const float mul = row_mul * (chunk == 0 && lead == 0 ? 1.f : step_mul);
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) O[nt] *= mul;
+#pragma unroll
+        for (int st = 0; st < W; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) P[st][i] *= f[st][i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) P[W][i] = l16 >= score_row(g4, i) ? P[W][i] * f[W][i] : 0.f;
+        // (f16: the scores of a row, like the state's copy, by a power of two that brings the largest to about 1)
+        f32x4 near[2] = {O[0], O[1]};
+        float up = 1.f;
+        if constexpr (F16) {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4 * (W + 1); ++i) top = fmaxf(top, fabsf(P[i >> 2][i & 3]));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            const Range r = range(fmaxf(top, __shfl_xor(top, 32)));
+            up = r.up;
+#pragma unroll
+            for (int st = 0; st <= W; ++st) P[st] *= r.down;
+            near[0] = near[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int p = 0; p < GROUPS; ++p) {
+            u32x4 x;
+            if constexpr (sizeof(T) == 2) {
+                x[0] = M::pack(P[2 * p][0], P[2 * p][1]);
+                x[1] = M::pack(P[2 * p][2], P[2 * p][3]);
+                x[2] = 2 * p + 1 <= W ? M::pack(P[2 * p + 1 <= W ? 2 * p + 1 : 0][0], P[2 * p + 1 <= W ? 2 * p + 1 : 0][1]) : 0;
+                x[3] = 2 * p + 1 <= W ? M::pack(P[2 * p + 1 <= W ? 2 * p + 1 : 0][2], P[2 * p + 1 <= W ? 2 * p + 1 : 0][3]) : 0;
+            } else {
+                x = __builtin_bit_cast(u32x4, P[p]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) near[nt] = M::mul(xc[p][nt], x, near[nt]);
+        }
+        const Chunk to_rows = so.next();
+        const uint32_t off = oo + to_rows.shift;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (F16 ? fmaf(near[i >> 2][i & 3], up, O[i >> 2][i & 3]) : near[i >> 2][i & 3]) * out_mul;
+        if constexpr (sizeof(T) == 2) {
+            win_store_aux<0>(to_rows.win, off, u32x4{M::pack(v[0], v[1]), M::pack(v[2], v[3]), M::pack(v[4], v[5]), M::pack(v[6], v[7])});
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                win_store_aux<0>(to_rows.win, FULL || n0 + 8 * g4 + 4 * j < dc ? off + 16 * j : NOWHERE,
+                                 u32x4{__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])});
+        }
+    }
+    __device__ __forceinline__ void between() const
+    {
+        if constexpr (SETS == 1) __syncthreads();
+        __syncthreads();
+    }
+    template <int W> __device__ __forceinline__ void out_walk()
+    {
+#pragma unroll
+        for (int k = 0; k < (FULL ? 1 : KB); ++k) oa[k] = offset(wk.a, 16 * W + l16, k * KF + g4 * V, da);
+        oo = offset(wk.out, 16 * W + l16, n0 + 8 * g4, dc);
+        row_mul = exp2f(l2 * (16 * W + l16));
+        step_mul = exp2f(l2);
+#pragma unroll
+        for (int st = 0; st <= W; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[st][i] = exp2f(l2 * (16 * (W - st) + l16 - score_row(g4, i)));
+        if (rows <= 0) return;
+        sa = stream(wk.a, da);
+        so = stream(wk.out, dc);
+        out_mul = wk.out_mul;
+        const int chunks = (rows + CHUNK - 1) / CHUNK;
+        RowsA even, second, &odd = DEEP ? second : even;
+        fetch_a(even);
+        if constexpr (DEEP) fetch_a(odd);
+        __syncthreads();
+        for (int chunk = 0; chunk < chunks; chunk += 2) {
+            out_turn<W, 0>(chunk, even);
+            between();
+            if (chunk + 1 == chunks) break;
+            out_turn<W, 1>(chunk + 1, odd);
+            between();
+        }
+    }
     // rows of the segment's time span past the sequence's end
+    __device__ __forceinline__ void clear_rest(int t, int threads) const
+    {
+        const int end = from + args.seg_rows < args.L ? from + args.seg_rows : args.L;
+        T *const po = (T *)wk.out.p + b * wk.out.sb + h * wk.out.sh;
+        for (int r = (from > length ? from : length) + (t >> 5); r < end; r += threads / 32)
+            if (n0 + (t & 31) < dc) Elem<T>::store(po + r * wk.out.st + n0 + (t & 31), 0.f);
+    }
+};
+
+// Waves 0 - 3 make the output, waves 4 - 7 move the state on and fetch rows: a chunk's two halves depend on each other only
+// from chunk to chunk, so they run side by side, two waves a SIMD.
+template <typename T, int DA, bool OUT, int PARTS, bool FULL>
+__global__ __launch_bounds__(OUT ? 512 : 256) void walk_kernel(Walks args, int slices)
+{
+    typedef Walker<T, DA, OUT, PARTS, FULL> W;
+    __shared__ typename W::Lds lds;
+    int64_t group;
+    int slice;
+    place(blockIdx.x, slices, group, slice);
+    if (group >= args.groups) return;
+    const int seg = (int)(group % args.segments);
+    group /= args.segments;
+    const int h = (int)(group % args.H);
+    group /= args.H;
+    const int b = (int)(group % args.bs), job = (int)(group / args.bs);
+    W w(args, args.w[job], lds);
+    w.b = b; w.h = h; w.seg = seg; w.job = job;
+    w.da = w.wk.da; w.dc = w.wk.dc; w.n0 = slice * COLS;
+    if (w.n0 >= w.dc) return;
+    w.tid = threadIdx.x;
+    w.lane = w.tid & 63; w.l16 = w.lane & 15; w.g4 = w.lane >> 4;
+    w.wave = __builtin_amdgcn_readfirstlane(w.tid >> 6);
+    int length = args.L;
+    if (args.lengths) {
+        length = __builtin_amdgcn_readfirstlane(args.lengths[b]);
+        length = length < 0 ? 0 : length > args.L ? args.L : length;
+    }
+    w.length = length;
+    w.from = seg * args.seg_rows;
+    w.rows = length - w.from < args.seg_rows ? length - w.from : args.seg_rows;
+    w.decay = clamp_decay(args.log_decay[h]);
+    w.l2 = w.decay * 1.44269504f;
+    w.state_at = (int64_t)(b * args.H + h) * w.da * w.dc;
+    w.lead = OUT && seg == 0 && w.wk.first ? w.wk.lead : 1;
     if constexpr (OUT) {
-        const int64_t end = from + args.seg_rows < args.L ? from + args.seg_rows : args.L;
-        for (int64_t t = (from > length ? from : length) + (tid >> 5); t < end; t += THREADS / 32)
-            if (n0 + (tid & 31) < dc) Elem<T>::store(po + t * wk.out.st + n0 + (tid & 31), 0.f);
+        switch (w.wave) {
+        case 0: w.template out_walk<0>(); break;
+        case 1: w.template out_walk<1>(); break;
+        case 2: w.template out_walk<2>(); break;
+        case 3: w.template out_walk<3>(); break;
+        default: w.state_walk(w.tid - 256);
+        }
+        w.clear_rest(w.tid, 512);
+    } else {
+        w.state_walk(w.tid);
     }
 }
 
@@ -547,20 +756,19 @@ __global__ __launch_bounds__(THREADS) void join_kernel(Walks args)
     const Walk &wk = args.w[job];
     const int e = blockIdx.x * THREADS + threadIdx.x, size = wk.da * wk.dc;
     if (e >= size || bh >= heads) return;
-    int64_t length = args.L;
+    int length = args.L;
     if (args.lengths) {
         length = args.lengths[bh / args.H];
         length = length < 0 ? 0 : length > args.L ? args.L : length;
     }
     const float decay = clamp_decay(args.log_decay[bh % args.H]);
     float whole_hi, whole_lo;
-    power(decay, (int)args.seg_rows, whole_hi, whole_lo);
+    power(decay, args.seg_rows, whole_hi, whole_lo);
     const int64_t at = bh * size + (e / wk.dc) * wk.si + (e % wk.dc) * wk.sj;
     float s = wk.first ? wk.first[at] * wk.first_mul : 0.f;
     float *p = args.seg + args.seg_walk[job] + bh * args.segments * size + e;
     for (int i = 0; i < args.segments; ++i, p += size) {
-        const int64_t left = length - i * args.seg_rows;
-        const int rows = (int)(left < 0 ? 0 : left < args.seg_rows ? left : args.seg_rows);
+        const int left = length - i * args.seg_rows, rows = left < 0 ? 0 : left < args.seg_rows ? left : args.seg_rows;
         const bool final = i + 1 == args.segments;
         const float add = final && !wk.last ? 0.f : *p;
         *p = s;
@@ -655,7 +863,7 @@ template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void s
 template <typename T, int DA, bool OUT, int PARTS> int walk_go(const Walks &w, int slices, bool full, hipStream_t st)
 {
     const int64_t blocks = (w.groups + 7) / 8 * 8 * slices;
-    const dim3 grid((unsigned)blocks), block(THREADS);
+    const dim3 grid((unsigned)blocks), block(OUT ? 512 : 256);
     if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidConfiguration;
     if (full) return launch_plain(walk_kernel<T, DA, OUT, PARTS, true>, grid, block, st, w, slices);
     return launch_plain(walk_kernel<T, DA, OUT, PARTS, false>, grid, block, st, w, slices);
@@ -709,9 +917,9 @@ int64_t seg_rows_of(int64_t L, int segments) { return ((L + segments - 1) / segm
 void plan(Walks &w, int64_t L, int dc)
 {
     w.segments = segments_of(w.n, w.bs, L, w.H, dc);
-    w.seg_rows = seg_rows_of(L, w.segments);
+    w.seg_rows = (int32_t)seg_rows_of(L, w.segments);
     w.segments = (int)((L + w.seg_rows - 1) / w.seg_rows);
-    w.L = L;
+    w.L = (int32_t)L;
     w.groups = (int64_t)w.n * w.bs * w.H * w.segments;
     int64_t at = 0;
     for (int i = 0; i < w.n; ++i) {

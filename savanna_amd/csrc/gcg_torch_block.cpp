@@ -255,8 +255,12 @@ Tensor layer_norm(const Tensor &x, const OptTensor &w, const OptTensor &b, doubl
 
 void add_strides(std::vector<int64_t> &s, const Tensor &t) { s.insert(s.end(), {t.stride(0), t.stride(1), t.stride(2)}); }
 
-// a tensor whose last dimension is contiguous, as the kernels read it
-Tensor rows_of(const Tensor &t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// a tensor whose last dimension is contiguous and whose rows are near enough to each other, as the kernels read it
+Tensor rows_of(const Tensor &t)
+{
+    const bool in_place = (t.size(-1) == 1 || t.stride(-1) == 1) && (t.dim() < 4 || t.stride(1) <= GCG_LINEAR_MAX_TIME_STRIDE);
+    return in_place ? t : t.contiguous();
+}
 
 void check_heads(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, int64_t dim)
 {
@@ -304,6 +308,15 @@ Tensor linear_workspace(const Tensor &q, const Tensor &v, bool backward, size_t 
 // a sequence of no rows: the state is the one given
 Tensor passed_on(const OptTensor &from, Tensor to) { return to.numel() == 0 ? to : given(from) ? to.copy_(*from) : to.zero_(); }
 
+// Head dimensions that the kernels' vectors do not divide: the tensors with zeros up to the next multiple of 8, which add nothing
+// to any product, and the results without them.
+int64_t to_whole(const Tensor &q, int64_t d) { return q.scalar_type() == at::kFloat && d % 4 == 0 ? 0 : (8 - d % 8) % 8; }
+bool odd_heads(const Tensor &q, const Tensor &v) { return to_whole(q, q.size(-1)) || to_whole(q, v.size(-1)); }
+Tensor padded(const Tensor &t, int64_t n) { return n ? at::constant_pad_nd(t, {0, n}) : t; }
+OptTensor padded_state(const OptTensor &t, int64_t dk, int64_t dv) { return given(t) ? OptTensor(at::constant_pad_nd(*t, {0, dv, 0, dk})) : t; }
+Tensor cut(const Tensor &t, int64_t d) { return t.size(-1) == d ? t : t.slice(-1, 0, d).contiguous(); }
+Tensor cut_state(const Tensor &t, int64_t dk, int64_t dv) { return t.numel() ? t.slice(2, 0, dk).slice(3, 0, dv).contiguous() : t; }
+
 std::tuple<Tensor, Tensor> linear_attn_fwd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                            const OptTensor &initial, const OptTensor &lengths, double scale, bool final)
 {
@@ -315,6 +328,12 @@ std::tuple<Tensor, Tensor> linear_attn_fwd(const Tensor &q, const Tensor &k, con
     Tensor o = at::empty({v.size(0), v.size(1), v.size(2), v.size(3)}, v.options());
     Tensor last = new_state(q, v, final);
     if (o.numel() == 0) return {o, passed_on(initial, last)};
+    if (odd_heads(q, v)) {
+        const int64_t dk = q.size(-1), dv = v.size(-1), pk = to_whole(q, dk), pv = to_whole(q, dv);
+        const auto [po, pl] = linear_attn_fwd(padded(q, pk), padded(k, pk), padded(v, pv), log_decay, padded_state(initial, pk, pv), lengths,
+                                              scale, final);
+        return {cut(po, dv), cut_state(pl, dk, dv)};
+    }
     const Tensor a = rows_of(q), b = rows_of(k), c = rows_of(v);
     std::vector<int64_t> s;
     for (const Tensor *t : {&a, &b, &c, (const Tensor *)&o}) add_strides(s, *t);
@@ -366,6 +385,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attn_bwd(const Tensor &d_o, co
     Tensor dq = at::empty(q.sizes(), q.options()), d_k = at::empty(k.sizes(), k.options()), d_v = at::empty(v.sizes(), v.options());
     Tensor dinitial = new_state(q, v, need_dinitial);
     if (d_o.numel() == 0) return {dq, d_k, d_v, passed_on(dfinal, dinitial)};
+    if (odd_heads(q, v)) {
+        const int64_t dk = q.size(-1), dv = v.size(-1), pk = to_whole(q, dk), pv = to_whole(q, dv);
+        const auto [pq, pkk, pvv, pi] = linear_attn_bwd(padded(d_o, pv), padded(q, pk), padded(k, pk), padded(v, pv), log_decay,
+                                                        padded_state(initial, pk, pv), lengths, padded_state(dfinal, pk, pv), scale,
+                                                        need_dinitial);
+        return {cut(pq, dk), cut(pkk, dk), cut(pvv, dv), cut_state(pi, dk, dv)};
+    }
     linear_bwd_launch(d_o, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, d_k, d_v,
                       need_dinitial ? (float *)dinitial.data_ptr() : nullptr);
     return {dq, d_k, d_v, dinitial};
@@ -396,6 +422,13 @@ Tensor linear_attn_packed_bwd(const Tensor &d_o, const Tensor &features, int64_t
     Tensor df = at::empty_like(features);
     if (df.numel() == 0) return df;
     const auto [dq, d_k, d_v] = split_features(df, H);
+    if (odd_heads(q, v)) {
+        const auto [pq, pk, pv, pi] = linear_attn_bwd(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, false);
+        dq.copy_(pq);
+        d_k.copy_(pk);
+        d_v.copy_(pv);
+        return df;
+    }
     linear_bwd_launch(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, dq, d_k, d_v, nullptr);
     return df;
 }
