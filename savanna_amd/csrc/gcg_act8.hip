@@ -8,10 +8,12 @@ namespace gcg {
 namespace {
 
 // A wave's vectors lie wave * 64 .. + 63 in the row-major list of a row's vectors; rows of whole blocks are one long row.
-// Each lane walks (row, vector) by a fixed step, whose parts the host divides.
+// Each lane takes UNROLL of them, a fixed step apart, whose parts in rows and vectors the host divides (a loop over more of them in
+// fewer workgroups is slower: 16384 x 12288 bf16 110 us, 104 this way).
+constexpr int UNROLL = 2;
 struct Walk { int64_t rows; int64_t D; int64_t per_row; int64_t step_row, step_vec; };
 
-template <typename T, bool TAIL, int UNROLL>
+template <typename T, bool TAIL, bool STREAM>
 __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, int8_t *__restrict__ codes, float *__restrict__ scales,
                                                     Walk w)
 {
@@ -31,7 +33,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, int
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             raw[u] = u32x4{0, 0, 0, 0};
-            if (r[u] < w.rows) raw[u] = load_row_vec<T, TAIL>(x + r[u] * w.D + c[u] * V, 0, (int)(w.D - c[u] * V < V ? w.D - c[u] * V : V));
+            if (r[u] < w.rows) raw[u] = load_row_vec<T, TAIL, STREAM>(x + r[u] * w.D + c[u] * V, 0, (int)(w.D - c[u] * V < V ? w.D - c[u] * V : V));
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
@@ -47,8 +49,8 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, int
             if (D > 0) {
                 int8_t *to = codes + r[u] * w.D + at;
                 if (D == V) {
-                    if constexpr (V == 8) *(u32x2_any *)to = u32x2{word[0], word[1]};
-                    else *(u32_any *)to = word[0];
+                    if constexpr (V == 8) put<STREAM>((u32x2_any *)to, u32x2{word[0], word[1]});
+                    else put<STREAM>((u32_any *)to, word[0]);
                 } else if (TAIL) {
 #pragma unroll
                     for (int i = 0; i < V; ++i)
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(const T *__restrict__ x, int
     }
 }
 
-template <typename T, bool TAIL, int UNROLL>
+template <typename T, bool TAIL, bool STREAM>
 __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__ codes, const float *__restrict__ scales,
                                                       T *__restrict__ x, Walk w)
 {
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__
             scale[u] = 0.f;
             if (r[u] < w.rows && c[u] < w.D) {
                 const int64_t left = w.D - c[u];
-                raw[u] = load_codes8<V, TAIL>(codes + r[u] * w.D + c[u], 0, (int)(left < V ? left : V));
+                raw[u] = load_codes8<V, TAIL, STREAM>(codes + r[u] * w.D + c[u], 0, (int)(left < V ? left : V));
                 scale[u] = scales[r[u] * nb + c[u] / kBlock8];
             }
         }
@@ -94,12 +96,12 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const int8_t *__restrict__
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) values8(raw[u][i], scale[u], v + 4 * i);
             const int64_t left = w.D - c[u];
-            if (r[u] < w.rows && left > 0) store_row_vec<T, TAIL>(x + r[u] * w.D + c[u], 0, (int)(left < V ? left : V), v);
+            if (r[u] < w.rows && left > 0) store_row_vec<T, TAIL, STREAM>(x + r[u] * w.D + c[u], 0, (int)(left < V ? left : V), v);
         }
     }
 }
 
-template <typename T> Walk make_walk(int64_t rows, int64_t D, int64_t *blocks, int unroll)
+template <typename T> Walk make_walk(int64_t rows, int64_t D, int64_t *blocks)
 {
     constexpr int V = kVec<T>;
     Walk w;
@@ -107,8 +109,8 @@ template <typename T> Walk make_walk(int64_t rows, int64_t D, int64_t *blocks, i
     w.rows = rows;
     w.D = D;
     w.per_row = (D + kBlock8 - 1) / kBlock8 * (kBlock8 / V);
-    const int64_t total = rows * w.per_row, most = 256 * 8;
-    *blocks = (total + 256 * unroll - 1) / (256 * unroll);
+    const int64_t total = rows * w.per_row, most = 1 << 23;         // (a launch holds 2^32 threads)
+    *blocks = (total + 256 * UNROLL - 1) / (256 * UNROLL);
     if (*blocks > most) *blocks = most;
     const int64_t step = *blocks * 256;
     w.step_row = step / w.per_row;
@@ -116,21 +118,23 @@ template <typename T> Walk make_walk(int64_t rows, int64_t D, int64_t *blocks, i
     return w;
 }
 
+template <typename T> bool streams(int64_t rows, int64_t D) { return rows * D * (int64_t)sizeof(T) > kStreamBytes; }
+
 template <typename T> int pack_t(const void *x, int8_t *codes, float *scales, int64_t rows, int64_t D, hipStream_t st)
 {
     int64_t blocks;
-    const Walk w = make_walk<T>(rows, D, &blocks, 4);
-    const dim3 grid((unsigned)blocks), block(256);
-    if (D % kVec<T>) return launch_main(pack8_kernel<T, true, 4>, grid, block, st, (const T *)x, codes, scales, w);
-    return launch_main(pack8_kernel<T, false, 4>, grid, block, st, (const T *)x, codes, scales, w);
+    const Walk w = make_walk<T>(rows, D, &blocks);
+    const auto go = [&](auto kernel) { return launch_main(kernel, dim3((unsigned)blocks), dim3(256), st, (const T *)x, codes, scales, w); };
+    if (D % kVec<T>) return streams<T>(rows, D) ? go(pack8_kernel<T, true, true>) : go(pack8_kernel<T, true, false>);
+    return streams<T>(rows, D) ? go(pack8_kernel<T, false, true>) : go(pack8_kernel<T, false, false>);
 }
 template <typename T> int unpack_t(const int8_t *codes, const float *scales, void *x, int64_t rows, int64_t D, hipStream_t st)
 {
     int64_t blocks;
-    const Walk w = make_walk<T>(rows, D, &blocks, 4);
-    const dim3 grid((unsigned)blocks), block(256);
-    if (D % kVec<T>) return launch_main(unpack8_kernel<T, true, 4>, grid, block, st, codes, scales, (T *)x, w);
-    return launch_main(unpack8_kernel<T, false, 4>, grid, block, st, codes, scales, (T *)x, w);
+    const Walk w = make_walk<T>(rows, D, &blocks);
+    const auto go = [&](auto kernel) { return launch_main(kernel, dim3((unsigned)blocks), dim3(256), st, codes, scales, (T *)x, w); };
+    if (D % kVec<T>) return streams<T>(rows, D) ? go(unpack8_kernel<T, true, true>) : go(unpack8_kernel<T, true, false>);
+    return streams<T>(rows, D) ? go(unpack8_kernel<T, false, true>) : go(unpack8_kernel<T, false, false>);
 }
 
 } // namespace

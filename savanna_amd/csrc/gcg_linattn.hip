@@ -201,12 +201,17 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
         __align__(16) T c[SETS][OUT ? CHUNK * CS : 1];
         __align__(16) T w[SETS][PARTS][CHUNK * CS];
         __align__(16) T s[SETS][OUT ? COLS * DA : 1];
-        float range[SETS][F16 && OUT ? KB : 1][2];
     };
 
     const Walks &args;
     const Walk &wk;
     Lds &lds;
+    // f16: by how much the blocks of the state's copy are smaller (a workgroup without them has no place for it either)
+    static __device__ __forceinline__ float &range_of(int set, int block, int half)
+    {
+        __shared__ float place[SETS][KB][2];
+        return place[set][block][half];
+    }
     int b, h, seg, job, da, dc, n0, lane, l16, g4, wave, tid;
     int length, from, rows;     // of the sequence; the segment's first row and its rows
     int64_t state_at;
@@ -319,6 +324,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
         for (int i = 0; i < BP; ++i) f.b[i] = load(cb, ob[i]);
 #pragma unroll
         for (int i = 0; i < CP; ++i) f.c[i] = load(cc, oc[i]);
+        __builtin_amdgcn_sched_barrier(0);      // requests stay in order, which is what the waits count by
     }
     // b, c and c weighted by f^(rows - 1 - r); rows past the end count for nothing
     __device__ __forceinline__ void deposit(int set, const Fetch &f, int rows) const
@@ -374,7 +380,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(S[nw][2 * kb + i / 4][i & 3]));
                         const Range r = range(wave_max(top));
                         by[kb] = r.down;
-                        if (lane == 0) lds.range[set][m0 / KF + kb][c0 / 16 + nw] = r.up;
+                        if (lane == 0) range_of(set, m0 / KF + kb, c0 / 16 + nw) = r.up;
                     }
                 }
 #pragma unroll
@@ -538,10 +544,12 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
             fetch(even);
             publish(0);
             __syncthreads();
-            for (int chunk = 0; chunk < chunks; chunk += 2) {
+            // (in pairs, an odd chunk after the loop: were a turn skipped on one way through it, the waits would have to suit both ways)
+            for (int chunk = 0; chunk + 1 < chunks; chunk += 2) {
                 state_turn<0>(chunk, chunks, odd);
-                if (chunk + 1 < chunks) state_turn<1>(chunk + 1, chunks, even);
+                state_turn<1>(chunk + 1, chunks, even);
             }
+            if (chunks & 1) state_turn<0>(chunks - 1, chunks, odd);
         }
         store_last();
     }
@@ -561,6 +569,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
 #pragma unroll
         for (int k = 0; k < KB; ++k)
             a.k[k] = load(c, FULL ? oa[0] + (uint32_t)(k * KF * sizeof(T)) : oa[FULL ? 0 : k]);
+        __builtin_amdgcn_sched_barrier(0);
     }
     template <int W, int PARITY> __device__ __forceinline__ void out_turn(int chunk, RowsA &a)
     {
@@ -591,7 +600,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                 for (int st = 0; st <= W; ++st) P[st] = M::mul(xb[k][st], a.k[kb + k], P[st]);
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-                    if constexpr (F16) O[nt] += M::mul(xs[k][nt], a.k[kb + k], f32x4{0.f, 0.f, 0.f, 0.f}) * lds.range[SET][kb + k][g4 >> 1];
+                    if constexpr (F16) O[nt] += M::mul(xs[k][nt], a.k[kb + k], f32x4{0.f, 0.f, 0.f, 0.f}) * range_of(SET, kb + k, g4 >> 1);
                     else O[nt] = M::mul(xs[k][nt], a.k[kb + k], O[nt]);
                 }
             }
@@ -677,14 +686,26 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
         out_mul = wk.out_mul;
         const int chunks = (rows + CHUNK - 1) / CHUNK;
         RowsA even, second, &odd = DEEP ? second : even;
+        // A store that is dropped after each request, as one follows each in the loop: the waits of the first turn, which are the
+        // loop's too, then count alike.
+        const Chunk none = {make_window(nullptr, 0), 0};
         fetch_a(even);
-        if constexpr (DEEP) fetch_a(odd);
+        win_store_aux<0>(none.win, NOWHERE, u32x4{0, 0, 0, 0});
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (DEEP) {
+            fetch_a(odd);
+            win_store_aux<0>(none.win, NOWHERE, u32x4{0, 0, 0, 0});
+        }
+        __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
-        for (int chunk = 0; chunk < chunks; chunk += 2) {
+        for (int chunk = 0; chunk + 1 < chunks; chunk += 2) {
             out_turn<W, 0>(chunk, even);
             between();
-            if (chunk + 1 == chunks) break;
             out_turn<W, 1>(chunk + 1, odd);
+            between();
+        }
+        if (chunks & 1) {
+            out_turn<W, 0>(chunks - 1, even);
             between();
         }
     }

@@ -25,7 +25,7 @@ __device__ __forceinline__ void load_param(const void *p, bool f32, int c, int D
         for (int i = 0; i < V; ++i)
             if (!TAIL || c + i < D) v[i] = ((const float *)p)[c + i];
     } else {
-        unpack_vec(load_row_vec<T, TAIL>((const T *)p, c, D), v, T{});
+        unpack_vec(load_row_vec<T, TAIL, false>((const T *)p, c, D), v, T{});
     }
 }
 
@@ -66,7 +66,7 @@ struct NormFwd {
 
 // TPR lanes hold a row, K vectors each; a workgroup of max(TPR, 256) threads walks over rows, the next row's loads in flight
 // while one is worked on.
-template <typename T, int TPR, int K, bool BITS8, bool TAIL>
+template <typename T, int TPR, int K, bool BITS8, bool TAIL, bool STREAM>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(NormFwd a)
 {
     constexpr int V = kVec<T>, THREADS = TPR > 256 ? TPR : 256, GROUPS = THREADS / TPR;
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(N
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         next[k] = u32x4{0, 0, 0, 0};
-        if (row < a.rows) next[k] = load_row_vec<T, TAIL>((const T *)a.x + row * D, (k * TPR + t) * V, D);
+        if (row < a.rows) next[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.x + row * D, (k * TPR + t) * V, D);
     }
     float w[K][V], b[K][V];
 #pragma unroll
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(N
         for (int k = 0; k < K; ++k) unpack_vec(next[k], v[k], T{});
         if (row + step < a.rows) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) next[k] = load_row_vec<T, TAIL>((const T *)a.x + (row + step) * D, (k * TPR + t) * V, D);
+            for (int k = 0; k < K; ++k) next[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.x + (row + step) * D, (k * TPR + t) * V, D);
         }
         float s[1] = {0.f};
 #pragma unroll
@@ -121,8 +121,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(N
                 float y[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) y[i] = fmaf((v[k][i] - mean) * rstd, w[k][i], b[k][i]);
-                store_row_vec<T, TAIL>((T *)a.y + row * D, c, D, y);
-                if constexpr (BITS8) store_codes8<V, TAIL>(a.codes + row * D, a.scales + row * nb, c, D, v[k]);
+                store_row_vec<T, TAIL, STREAM>((T *)a.y + row * D, c, D, y);
+                if constexpr (BITS8) store_codes8<V, TAIL, STREAM>(a.codes + row * D, a.scales + row * nb, c, D, v[k]);
             }
             if (a.stats && t == 0) *(float2 *)(a.stats + 2 * row) = float2{mean, rstd};
         }
@@ -142,13 +142,15 @@ struct NormBwd {
     int32_t param_f32;
 };
 
-// A lane keeps 16 columns (K vectors) of its row and, over all rows it walks, of dw and db, and requests the next row while one
-// is worked on.  Above 8192 columns it has 32, and registers for neither the next row nor w.
-template <typename T, int TPR, int K, bool BITS8, bool TAIL>
+// A lane keeps 8 columns (K vectors) of its row and, over all rows it walks, of dw and db, and requests the next row while one
+// is worked on: 16 waves a CU with two rows each in flight.  (16 columns a lane leave room for 8 waves: 15009 x 2560 f16 51 us
+// instead of 49, 32768 x 8192 from 8 bits 382 instead of 328, 16384 x 4096 bf16 80 and 79.)  Above 8192 columns it has 32, and registers for neither the
+// next row nor w.
+template <typename T, int TPR, int K, bool BITS8, bool TAIL, bool STREAM>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(NormBwd a)
 {
     constexpr int V = kVec<T>, THREADS = TPR > 256 ? TPR : 256, GROUPS = THREADS / TPR;
-    constexpr bool AHEAD = K * V <= 16;
+    constexpr bool AHEAD = K * V <= 8;
     __shared__ float slots[2][2 * THREADS / kWave];
     __shared__ float sums[GROUPS > 1 ? 2 * TPR * K * V : 1];
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, D = a.D;
@@ -165,12 +167,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(N
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * TPR + t) * V;
-            next_dy[k] = load_row_vec<T, TAIL>((const T *)a.dy + r * D, c, D);
+            next_dy[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.dy + r * D, c, D);
             if constexpr (BITS8) {
-                next_codes[k] = load_codes8<V, TAIL>(a.codes + r * D, c, D);
+                next_codes[k] = load_codes8<V, TAIL, STREAM>(a.codes + r * D, c, D);
                 next_scale[k] = c < D ? a.scales[r * nb + c / kBlock8] : 0.f;
             } else {
-                next_x[k] = load_row_vec<T, TAIL>((const T *)a.x + r * D, c, D);
+                next_x[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.x + r * D, c, D);
             }
         }
     };
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(N
                 float dx[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) dx[i] = rstd * (fmaf(dy[at][i], w[at][i], -c1) - xh[at][i] * c2);
-                store_row_vec<T, TAIL>((T *)a.dx + row * D, (k * TPR + t) * V, D, dx);
+                store_row_vec<T, TAIL, STREAM>((T *)a.dx + row * D, (k * TPR + t) * V, D, dx);
             }
         }
     }
@@ -288,21 +290,26 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(N
     }
 }
 
-// dw and db from the workgroups' partial sums, in a fixed order: 64 columns a workgroup, 16 threads a column.
+// dw and db from the workgroups' partial sums, in a fixed order: 32 columns a workgroup, 32 threads a column.  (A few megabytes, so
+// what counts is that all of them are on the way at once: 512 sets of 4096 columns 9.3 us with 64 columns and 16 threads, 4.0 now.)
 template <typename P> __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float *partial, int n, int D, P *dw, P *db)
 {
-    __shared__ float part[16][64];
-    const int c = blockIdx.x * 64 + threadIdx.x % 64, slice = threadIdx.x / 64;
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x % 32, slice = threadIdx.x / 32, c = blockIdx.x * 32 + lane;
     float s = 0.f;
-    if (c < 2 * D)
-        for (int i = slice; i < n; i += 16) s += partial[(int64_t)i * 2 * D + c];
-    part[slice][threadIdx.x % 64] = s;
+    if (c < 2 * D) {
+#pragma unroll 8
+        for (int i = slice; i < n; i += 32) s += partial[(int64_t)i * 2 * D + c];
+    }
+    part[slice][lane] = s;
     __syncthreads();
-    if (slice == 0 && c < 2 * D) {
+    s = part[lane][slice];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
-        P *to = c < D ? dw : db;
-        if (to) Elem<P>::store(to + (c < D ? c : c - D), s);
+    for (int d = 16; d > 0; d /= 2) s += __shfl_xor(s, d);
+    const int out = blockIdx.x * 32 + slice;
+    if (lane == 0 && out < 2 * D) {
+        P *to = out < D ? dw : db;
+        if (to) Elem<P>::store(to + (out < D ? out : out - D), s);
     }
 }
 
@@ -312,8 +319,13 @@ template <typename T, int TPR, int K, bool BITS8> int fwd_launch(const NormFwd &
     constexpr int THREADS = TPR > 256 ? TPR : 256;
     const int64_t need = (a.rows + THREADS / TPR - 1) / (THREADS / TPR), most = 256 * 2048 / THREADS;
     const dim3 grid((unsigned)(need < most ? need : most)), block(THREADS);
-    if (a.D % kVec<T>) return launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, true>, grid, block, st, a);
-    return launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, false>, grid, block, st, a);
+    const bool tail = a.D % kVec<T>, stream = a.rows * a.D * (int64_t)sizeof(T) > kStreamBytes;
+    if (tail) {
+        return stream ? launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, true, true>, grid, block, st, a)
+                      : launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, true, false>, grid, block, st, a);
+    }
+    return stream ? launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, false, true>, grid, block, st, a)
+                  : launch_main(layer_norm_fwd_kernel<T, TPR, K, BITS8, false, false>, grid, block, st, a);
 }
 template <typename T, bool BITS8> int fwd_width(const NormFwd &a, hipStream_t st)
 {
@@ -332,22 +344,27 @@ template <typename T> int fwd_t(const NormFwd &a, hipStream_t st) { return a.cod
 int bwd_lanes(int D)
 {
     int tpr = 64;
-    while (tpr * 16 < D && tpr < 512) tpr *= 2;
-    return tpr;
+    while (tpr * 8 < D && tpr < 1024) tpr *= 2;
+    return D > 8192 ? 512 : tpr;
 }
-// Workgroups of the backward: two of 256 threads a CU (or as many threads in larger ones); each writes a set of partial sums.
+// Workgroups of the backward, each of which writes a set of partial sums: two a CU, one of 1024 threads.
 int bwd_blocks(int64_t rows, int D)
 {
     const int tpr = bwd_lanes(D), threads = tpr > 256 ? tpr : 256;
-    const int64_t need = (rows + threads / tpr - 1) / (threads / tpr), most = 512 * 256 / threads;
+    const int64_t need = (rows + threads / tpr - 1) / (threads / tpr), most = threads >= 1024 || D > 8192 ? 256 : 512;
     return (int)(need < most ? need : most);
 }
-template <typename T, int TPR, bool BITS8, int COLUMNS = 16> int bwd_launch(const NormBwd &a, hipStream_t st)
+template <typename T, int TPR, bool BITS8, int COLUMNS = 8> int bwd_launch(const NormBwd &a, hipStream_t st)
 {
     constexpr int K = COLUMNS / kVec<T>;
     const dim3 grid((unsigned)bwd_blocks(a.rows, a.D)), block(TPR > 256 ? TPR : 256);
-    if (a.D % kVec<T>) return launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, true>, grid, block, st, a);
-    return launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, false>, grid, block, st, a);
+    const bool tail = a.D % kVec<T>, stream = a.rows * a.D * (int64_t)sizeof(T) > kStreamBytes;
+    if (tail) {
+        return stream ? launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, true, true>, grid, block, st, a)
+                      : launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, true, false>, grid, block, st, a);
+    }
+    return stream ? launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, false, true>, grid, block, st, a)
+                  : launch_main(layer_norm_bwd_kernel<T, TPR, K, BITS8, false, false>, grid, block, st, a);
 }
 template <typename T, bool BITS8> int bwd_width(const NormBwd &a, hipStream_t st)
 {
@@ -355,8 +372,9 @@ template <typename T, bool BITS8> int bwd_width(const NormBwd &a, hipStream_t st
     case 64: return bwd_launch<T, 64, BITS8>(a, st);
     case 128: return bwd_launch<T, 128, BITS8>(a, st);
     case 256: return bwd_launch<T, 256, BITS8>(a, st);
+    case 512: return a.D <= 8192 ? bwd_launch<T, 512, BITS8>(a, st) : bwd_launch<T, 512, BITS8, 32>(a, st);
+    default: return bwd_launch<T, 1024, BITS8>(a, st);
     }
-    return a.D <= 512 * 16 ? bwd_launch<T, 512, BITS8>(a, st) : bwd_launch<T, 512, BITS8, 32>(a, st);
 }
 template <typename T> int bwd_t(const NormBwd &a, hipStream_t st) { return a.codes ? bwd_width<T, true>(a, st) : bwd_width<T, false>(a, st); }
 
@@ -389,7 +407,7 @@ int layer_norm_bwd_launch(int dtype, const void *dy, const void *x, const int8_t
     default: rc = bwd_t<f16_t>(a, st); break;
     }
     if (rc || !a.partial) return rc;
-    const dim3 grid((unsigned)((2 * D + 63) / 64)), block(1024);
+    const dim3 grid((unsigned)((2 * D + 31) / 32)), block(1024);
     const int n = bwd_blocks(rows, D);
     switch (dtype) {
     case GCG_BF16: return launch_plain(layer_norm_reduce_kernel<bf16_t>, grid, block, st, (const float *)ws, n, D, (bf16_t *)dw, (bf16_t *)db);

@@ -12,6 +12,21 @@ typedef uint32_t u32_any __attribute__((aligned(1)));
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);          // elements of a vector
 
+// Accesses with the streaming hint, for tensors that the last-level cache (256 MB) does not hold from one kernel to the next
+// anyway: 16384 x 12288 bf16 into 8 bits and back 128 + 124 us without, 104 + 103 with; norm of 32768 x 8192 203 and 192, its
+// backward 295 and 273, from 8 bits 320 and 312.  Smaller ones gain nothing, and the next kernel finds them in the cache.
+constexpr int64_t kStreamBytes = 256ll << 20;
+template <bool STREAM, typename P> __device__ __forceinline__ P fetch(const P *p)
+{
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool STREAM, typename P, typename X> __device__ __forceinline__ void put(P *p, const X &v)
+{
+    if constexpr (STREAM) __builtin_nontemporal_store((P)v, p);
+    else *p = v;
+}
+
 __device__ __forceinline__ void unpack_vec(const u32x4 &r, float (&v)[4], float)
 {
 #pragma unroll
@@ -45,11 +60,12 @@ __device__ __forceinline__ u32x4 pack_vec(const float (&v)[8], f16_t)
 
 // The vector of row elements c .. c + kVec - 1, of which those at D and beyond are absent (zeros).  TAIL: D is not a multiple
 // of the vector, so one lane of a row has a vector that ends inside it and goes element by element.
-template <typename T, bool TAIL> __device__ __forceinline__ u32x4 load_row_vec(const T *row, int c, int D)
+// STREAM: with the streaming hint.
+template <typename T, bool TAIL, bool STREAM> __device__ __forceinline__ u32x4 load_row_vec(const T *row, int c, int D)
 {
     constexpr int V = kVec<T>;
     u32x4 r = {0, 0, 0, 0};
-    if (c + V <= D) r = *(const u32x4_any *)(row + c);
+    if (c + V <= D) r = fetch<STREAM>((const u32x4_any *)(row + c));
     else if (TAIL && c < D) {
         float v[V];
 #pragma unroll
@@ -58,10 +74,11 @@ template <typename T, bool TAIL> __device__ __forceinline__ u32x4 load_row_vec(c
     }
     return r;
 }
-template <typename T, bool TAIL> __device__ __forceinline__ void store_row_vec(T *row, int c, int D, const float (&v)[kVec<T>])
+template <typename T, bool TAIL, bool STREAM>
+__device__ __forceinline__ void store_row_vec(T *row, int c, int D, const float (&v)[kVec<T>])
 {
     constexpr int V = kVec<T>;
-    if (c + V <= D) *(u32x4_any *)(row + c) = pack_vec(v, T{});
+    if (c + V <= D) put<STREAM>((u32x4_any *)(row + c), pack_vec(v, T{}));
     else if (TAIL && c < D) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -151,7 +168,7 @@ template <int V> __device__ __forceinline__ uint32_t top_of(const float (&v)[V])
     return m;
 }
 // Codes of one vector a lane, at row elements c ..; the 128 / V lanes of a block hold it side by side (absent elements zero).
-template <int V, bool TAIL>
+template <int V, bool TAIL, bool STREAM>
 __device__ __forceinline__ void store_codes8(int8_t *codes, float *scales, int c, int D, const float (&v)[V])
 {
     const Scale8 s = scale8(lanes_max<kBlock8 / V>(top_of<V>(v)));
@@ -159,8 +176,8 @@ __device__ __forceinline__ void store_codes8(int8_t *codes, float *scales, int c
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) w[i] = codes8(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s.inv);
     if (c + V <= D) {
-        if constexpr (V == 8) *(u32x2_any *)(codes + c) = u32x2{w[0], w[1]};
-        else *(u32_any *)(codes + c) = w[0];
+        if constexpr (V == 8) put<STREAM>((u32x2_any *)(codes + c), u32x2{w[0], w[1]});
+        else put<STREAM>((u32_any *)(codes + c), w[0]);
     } else if (TAIL) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -169,12 +186,12 @@ __device__ __forceinline__ void store_codes8(int8_t *codes, float *scales, int c
     if (c < D && (c & (kBlock8 - 1)) == 0) scales[c / kBlock8] = s.scale;
 }
 // The words of a vector's codes, absent ones zero.
-template <int V, bool TAIL> __device__ __forceinline__ u32x2 load_codes8(const int8_t *codes, int c, int D)
+template <int V, bool TAIL, bool STREAM> __device__ __forceinline__ u32x2 load_codes8(const int8_t *codes, int c, int D)
 {
     u32x2 w = {0, 0};
     if (c + V <= D) {
-        if constexpr (V == 8) w = *(const u32x2_any *)(codes + c);
-        else w[0] = *(const u32_any *)(codes + c);
+        if constexpr (V == 8) w = fetch<STREAM>((const u32x2_any *)(codes + c));
+        else w[0] = fetch<STREAM>((const u32_any *)(codes + c));
     } else if (TAIL && c < D) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
