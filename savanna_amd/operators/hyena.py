@@ -317,21 +317,36 @@ class CausalDepthwiseConv1d(nn.Module):
         return self.forward_bld(x.permute(0, 2, 1)).permute(0, 2, 1)
 
 
+def _keep(ctx, raw, save_8bit, *rest):
+    """Saves a mixer's features and its parameters; with ``save_8bit`` the features' 8-bit checkpoint (act8.py), taken over
+    whole rows of (b, l, 3 * hidden)."""
+    ctx.kept = (raw.shape, raw.dtype) if save_8bit else None
+    ctx.save_for_backward(*(_lib.pack8(raw.flatten(2)) if save_8bit else (raw, None)), *rest)
+
+
+def _kept(ctx):
+    raw, scales, *rest = ctx.saved_tensors
+    if ctx.kept is not None:
+        shape, dtype = ctx.kept
+        raw = _lib.unpack8(raw, scales, dtype).reshape(shape)
+    return raw, *rest
+
+
 class _FeaturizedShortGateConvGate(torch.autograd.Function):
     """z = gated short convolution of the featurized projection, raw (b, l, g, dg, 3) -> (b, l, g, dg),
     in one kernel each way; the featurized tensor exists in registers only.  ``planar``: raw is (b, l, 3, g, dg)."""
 
     @staticmethod
-    def forward(ctx, raw, wf, h, planar=False):
+    def forward(ctx, raw, wf, h, planar=False, save_8bit=False):
         raw, wf, h = (t if t.is_contiguous() else t.contiguous() for t in (raw, wf, h))
-        ctx.save_for_backward(raw, wf, h)
+        _keep(ctx, raw, save_8bit, wf, h)
         ctx.planar = planar
         return _lib.mixer_se_fwd(raw, wf, h, planar)
 
     @staticmethod
     def backward(ctx, dz):
-        raw, wf, h = ctx.saved_tensors
-        return _lib.mixer_se_bwd(dz if dz.is_contiguous() else dz.contiguous(), raw, wf, h, ctx.planar) + (None,)
+        raw, wf, h = _kept(ctx)
+        return _lib.mixer_se_bwd(dz if dz.is_contiguous() else dz.contiguous(), raw, wf, h, ctx.planar) + (None, None)
 
 
 class _FeaturizedGateConvGate(torch.autograd.Function):
@@ -341,16 +356,16 @@ class _FeaturizedGateConvGate(torch.autograd.Function):
     ``planar``: raw is (b, l, 3, g, dg)."""
 
     @staticmethod
-    def forward(ctx, raw, wf, h, planar=False):
+    def forward(ctx, raw, wf, h, planar=False, save_8bit=False):
         raw, wf, h = (t if t.is_contiguous() else t.contiguous() for t in (raw, wf, h))
-        ctx.save_for_backward(raw, wf, h)
+        _keep(ctx, raw, save_8bit, wf, h)
         ctx.planar = planar
         return _lib.mixer_mr_fwd(raw, wf, h, planar)
 
     @staticmethod
     def backward(ctx, dz):
-        raw, wf, h = ctx.saved_tensors
-        return _lib.mixer_mr_bwd(dz if dz.is_contiguous() else dz.contiguous(), raw, wf, h, ctx.planar) + (None,)
+        raw, wf, h = _kept(ctx)
+        return _lib.mixer_mr_bwd(dz if dz.is_contiguous() else dz.contiguous(), raw, wf, h, ctx.planar) + (None, None)
 
 
 class _FeaturizedDecayedGateConvGate(torch.autograd.Function):
@@ -359,25 +374,45 @@ class _FeaturizedDecayedGateConvGate(torch.autograd.Function):
     part is one kernel each way, and the backward returns the gradient of the filter parameter itself."""
 
     @staticmethod
-    def forward(ctx, raw, wf, w, decay, hl, filt, planar=False):
+    def forward(ctx, raw, wf, w, decay, hl, filt, planar=False, save_8bit=False):
         raw, wf, w, decay = (t if t.is_contiguous() else t.contiguous() for t in (raw, wf, w, decay))
-        ctx.save_for_backward(raw, wf, w, decay)
+        _keep(ctx, raw, save_8bit, wf, w, decay)
         ctx.hl, ctx.filt, ctx.planar = hl, filt, planar
         return _lib.mixer_mr_fwd_decay(raw, wf, w, decay, hl, filt, planar)
 
     @staticmethod
     def backward(ctx, dz):
-        raw, wf, w, decay = ctx.saved_tensors
+        raw, wf, w, decay = _kept(ctx)
         draw, dwf, dw = _lib.mixer_mr_bwd_decay(dz if dz.is_contiguous() else dz.contiguous(), raw, wf, w, decay,
                                                 ctx.hl, ctx.filt, ctx.planar)
-        return draw, dwf, dw, None, None, None, None
+        return draw, dwf, dw, None, None, None, None, None
 
 
-def _featurized(entry, function, tensors, *rest):
-    """The entry point itself, or its Python autograd function (``_lib.native_nodes``)."""
-    if _lib.native_nodes(tensors[0]):
+def _featurized(entry, function, tensors, *rest, save_8bit=False):
+    """The entry point itself, or its Python autograd function (``_lib.native_nodes``; an 8-bit checkpoint is the latter's)."""
+    if _lib.native_nodes(tensors[0]) and not save_8bit:
         return entry(*(t if t.is_contiguous() else t.contiguous() for t in tensors), *rest)
-    return function.apply(*tensors, *rest)
+    return function.apply(*tensors, *rest, save_8bit)
+
+
+class _Recomputed8(torch.autograd.Function):
+    """``run(features)`` of which only the features' 8-bit checkpoint is kept: the backward runs it again on that."""
+
+    @staticmethod
+    def forward(ctx, run, features, *params):
+        ctx.run, ctx.dtype = run, features.dtype
+        ctx.save_for_backward(*_lib.pack8(features.contiguous()), *params)
+        return run(features)
+
+    @staticmethod
+    def backward(ctx, dz):
+        codes, scales, *params = ctx.saved_tensors
+        features = _lib.unpack8(codes, scales, ctx.dtype).requires_grad_(True)
+        with torch.enable_grad():
+            z = ctx.run(features)
+        inputs = [features] + [p for p in params if p.requires_grad]
+        grads = iter(torch.autograd.grad(z, inputs, dz, allow_unused=True))
+        return None, next(grads), *(next(grads) if p.requires_grad else None for p in params)
 
 
 class HyenaMixer(nn.Module):
@@ -392,15 +427,20 @@ class HyenaMixer(nn.Module):
     (9 to 128 taps) and a featurizer of at most 3 taps the featurized tensor is never stored (``fuse_medium``):
     the operator's kernels make its rows from the projection output, forward and backward, with the chain's results,
     and form the decayed filter themselves where the operator allows it (``HyenaMROperator.fuse_filter``).
-    ``interleave_projections=False`` takes the features laid out "(p g dg)" instead (block.py:881-884)."""
+    ``interleave_projections=False`` takes the features laid out "(p g dg)" instead (block.py:881-884).
+
+    ``save_8bit``: of the features only their 8-bit checkpoint (act8.py) is kept for the backward, half of their bytes, and the
+    gradients are those at its values.  The one-kernel routes read it as they read the features; the others run their
+    forward again on it, and so keep no featurized tensor either."""
 
     def __init__(self, operator: _CgcgOperatorBase, short_conv_L: int = 3, dtype=torch.float32, device=None,
-                 fuse_short: bool = True, fuse_medium: bool = True, interleave_projections: bool = True):
+                 fuse_short: bool = True, fuse_medium: bool = True, interleave_projections: bool = True, save_8bit: bool = False):
         super().__init__()
         self.mixer = operator
         self.fuse_short = fuse_short
         self.fuse_medium = fuse_medium
         self.interleave_projections = interleave_projections        # global_config.py:270
+        self.save_8bit = save_8bit
         self.hyena_proj_conv = CausalDepthwiseConv1d(3 * operator.hidden_size, short_conv_L, dtype=dtype, device=device)
 
     def _fusable(self, features: torch.Tensor, hl: int) -> bool:
@@ -423,7 +463,7 @@ class HyenaMixer(nn.Module):
         shape = (bs, seqlen, 3, g, dg) if planar else (bs, seqlen, g, dg, 3)
         z = _FeaturizedShortGateConvGate.apply(features.reshape(shape),
                                                self.hyena_proj_conv.short_conv_weight.to(features.dtype),
-                                               h.to(op.cgcg_dtype), planar)
+                                               h.to(op.cgcg_dtype), planar, self._save_8bit())
         z = z.reshape(bs, seqlen, g * dg)
         return z.to(dtype) if cast else z
 
@@ -451,11 +491,15 @@ class HyenaMixer(nn.Module):
             return op.cgcg_dtype == features.dtype or op._fp32_inside(features.dtype, features)
         return op.cgcg_dtype == features.dtype and features.dtype in (torch.bfloat16, torch.float16)
 
+    def _save_8bit(self) -> bool:
+        return self.save_8bit and torch.is_grad_enabled()
+
     def forward(self, features: torch.Tensor) -> torch.Tensor:
         op, conv = self.mixer, self.hyena_proj_conv
         bs, seqlen, d3 = features.shape
         g, dg = op.num_groups, op.group_dim
         assert d3 == 3 * g * dg
+        save_8bit = self._save_8bit()
         planar = not self.interleave_projections
         shape = (bs, seqlen, 3, g, dg) if planar else (bs, seqlen, g, dg, 3)
         # Hyena-MR: one kernel each way, with the decayed filter formed inside it where the operator allows that
@@ -463,16 +507,18 @@ class HyenaMixer(nn.Module):
         if fused is not None and self._medium(features, fused[0]):
             z = _featurized(_lib.mixer_mr_fwd_decay, _FeaturizedDecayedGateConvGate,
                             (features.reshape(shape), conv.short_conv_weight.to(features.dtype), op.filter.h, op.filter.decay),
-                            fused[0], fused[1], planar)
+                            fused[0], fused[1], planar, save_8bit=save_8bit)
             return z.reshape(bs, seqlen, g * dg)
         h = op._filter(seqlen)
         if self._medium(features, h.shape[-1]):
             z = _featurized(_lib.mixer_mr_fwd, _FeaturizedGateConvGate,
-                            (features.reshape(shape), conv.short_conv_weight.to(features.dtype), h.to(op.cgcg_dtype)), planar)
+                            (features.reshape(shape), conv.short_conv_weight.to(features.dtype), h.to(op.cgcg_dtype)), planar,
+                            save_8bit=save_8bit)
             return z.reshape(bs, seqlen, g * dg)
         # Hyena-SE: one kernel each way
         if self._fusable(features, h.shape[-1]):
             return self._fused_short(features, h, planar)
         # otherwise the featurizer kernel, then the operator on its output where it lies (two kernels each way)
-        return op.forward_features(conv.forward_bld(features, feeds_operator=True), from_featurizer=True,
-                                   interleaved=not planar)
+        run = lambda f: op.forward_features(conv.forward_bld(f, feeds_operator=True), from_featurizer=True,  # noqa: E731
+                                            interleaved=not planar)
+        return _Recomputed8.apply(run, features, *self.parameters()) if save_8bit else run(features)
