@@ -12,11 +12,23 @@
 // the state, out += f^(r+1) a S, and the state moves on by S = f^64 S + (b * f^(63-r))^T c.  Only non-negative powers
 // of f are formed, so no decay over- or underflows into a wrong result (f = 0 and f = 1 included).
 //
-// A workgroup of four waves walks one head's rows for 32 columns of c, with its da x 32 state in fp32 in the waves' accumulation
-// registers.  Wave w makes rows 16 w .. 16 w + 15 of P and of the output, and keeps a quarter of the state's rows.  P passes from
-// one product to the next in registers: the scores are made transposed, so that a lane's four results of a tile are four
-// consecutive positions of the next product's inner dimension; the products run over those positions in that order on both sides.
-// b, c, the weighted c and the state's rounded copy are in LDS, two sets of each, so one barrier a chunk is enough.
+// A workgroup of twelve waves walks one head's rows for 32 columns of c: four waves make the output, 16 rows of a chunk each, four
+// hold the da x 32 state in fp32 in their accumulation registers and move it on, and four bring rows from memory, two chunks
+// ahead, into LDS.  The three meet at one barrier a chunk; b, c, the weighted c and the state's rounded copy have two sets in
+// LDS.  P passes from one product to the next in registers: the scores are made transposed, so that a lane's four results of a
+// tile are four consecutive positions of the next product's inner dimension; the products run over those positions in that order
+// on both sides.  Narrow slices fill the card from few heads (2 sequences of 32 heads of 128: 256 workgroups) and keep the
+// state small; a and b, which a head's slices share, come from the XCD's L2, where they are put side by side.
+//
+// Measured, bf16, 2 x 8192 rows of 32 heads of 128: forward 150 us, backward (three walks in one launch) 474 us, 3.6 and 3.4
+// TB/s of what it has to move.  Of the forward's time 115 us are left when every head reads the same rows from L2: a chunk's
+// chain -- LDS reads (35 % of its time), two dependent products, rounding, the next state's copy, the barrier -- and not the
+// matrix units (24 %) or LDS bounds it; the rest is HBM latency that shows through (rows of 256 bytes, 8 KB apart).  Tried: two
+// workgroups of 128 registers a CU, three sets in LDS with the scores and the state's operands a chunk ahead, and other orders
+// of heads over XCDs, all within 5 % or slower; waves for both the state and the rows (8 a workgroup) 165 and 510 us.
+//
+// Few heads, long sequences: the rows are cut into segments whose states are made first, each from nothing, and joined by a scan
+// over segments; then all segments run at once (8 heads, 131072 rows: 486 us in three launches; in one segment 2.0 ms).
 //
 // Rounding of 16-bit walks: the matrix instructions take 16-bit operands, so P and the state's copy are rounded to the type once,
 // as the output is; the weighted c is given as a sum of two 16-bit parts (three where the state itself is a result), whose
@@ -193,6 +205,10 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     // 16-row tiles of the state a wave keeps, and of its two 16-column ones: whole blocks of KF rows in 16 bits
     static constexpr int NW = DA == 64 ? 1 : 2, MT = DA == 64 ? 2 : DA / 64;
     static constexpr bool DEEP = DA * sizeof(T) <= 256;     // registers for the rows of two chunks ahead (else one)
+    // The output's, the state's and the fetching waves, four each: 168 registers a lane.  Walks with rows of more than 256 bytes do
+    // not fit in that but for bf16's; there the state's waves fetch too (JOINT).
+    static constexpr bool JOINT = OUT && !DEEP && !__is_same(T, bf16_t);
+    static constexpr int WAVES = 4 + (OUT ? 4 : 0) + (JOINT ? 0 : 4);
     static constexpr int BT = DA / V, BR = 256 / BT, BP = CHUNK / BR;      // b: threads a row, rows a pass, passes
     static constexpr int CT = COLS / V, CR = 256 / CT, CP = CHUNK / CR;    // c
 
@@ -270,15 +286,73 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     static __device__ __forceinline__ u32x4 load(const Chunk &c, uint32_t off) { return win_load_aux<0, u32x4>(c.win, off + c.shift); }
     __device__ __forceinline__ int rows_in(int chunk) const { return rows - chunk * CHUNK < CHUNK ? rows - chunk * CHUNK : CHUNK; }
 
-    // ---- the state waves: rows into LDS, the state from chunk to chunk
+    // ---- the fetching waves: rows into LDS
     struct Fetch { u32x4 b[BP], c[CP]; };
     uint32_t ob[BP], oc[CP];
     int b_row, b_col, c_row, c_col;
-    float first_hi, first_lo, chunk_hi, chunk_lo, last_hi, last_lo;     // f^rows of the first, a full and the last chunk
-    int m0, c0;                 // tile (mt, nw): rows m0 + 16 mt + 4 g4 .. + 3, the slice's column c0 + 16 nw + l16
-    f32x4 S[NW][MT];
+    Stream sb, sc;
 
-    __device__ __forceinline__ void state_setup(int t)
+    __device__ __forceinline__ void fetch(Fetch &f)
+    {
+        const Chunk cb = sb.next(), cc = sc.next();
+#pragma unroll
+        for (int i = 0; i < BP; ++i) f.b[i] = load(cb, ob[i]);
+#pragma unroll
+        for (int i = 0; i < CP; ++i) f.c[i] = load(cc, oc[i]);
+        __builtin_amdgcn_sched_barrier(0);      // requests stay in order, which is what the waits count by
+    }
+    __device__ __forceinline__ void deposit_b(int set, const Fetch &f) const
+    {
+#pragma unroll
+        for (int i = 0; i < BP; ++i) *(u32x4 *)(lds.b[set] + wide_at<T, DA>(b_row + i * BR, b_col / V)) = f.b[i];
+    }
+    // b, c and c weighted by f^(rows - 1 - r); rows past the end count for nothing.  Waves that do nothing else weight c first, while
+    // the others' reads have LDS to themselves.
+    __device__ __forceinline__ void deposit(int set, const Fetch &f, int rows) const
+    {
+        if constexpr (JOINT) deposit_b(set, f);
+        u32x4 v[CP], part[CP][sizeof(T) == 2 ? PARTS : 1];
+#pragma unroll
+        for (int i = 0; i < CP; ++i) {
+            const int r = c_row + i * CR;
+            const float w = r < rows ? exp2f(l2 * (rows - 1 - r)) : 0.f;
+            v[i] = f.c[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[i][j] = r < rows ? v[i][j] : 0;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float lo = M::low(v[i][j]) * w, hi = M::high(v[i][j]) * w;
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        part[i][p][j] = M::pack(lo, hi);
+                        // the remainder is that of the part as stored, not of one that the compiler rounds again from the exact
+                        // product (its mixed-precision f16 instructions do, an f16 step apart now and then)
+                        asm("" : "+v"(part[i][p][j]));
+                        if (p + 1 < PARTS) { lo = (lo - M::low(part[i][p][j])) * M::MORE; hi = (hi - M::high(part[i][p][j])) * M::MORE; }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) part[i][0][j] = __float_as_uint(__uint_as_float(v[i][j]) * w);
+            }
+        }
+        if constexpr (!JOINT) {
+            __builtin_amdgcn_sched_barrier(0);
+            deposit_b(set, f);
+        }
+#pragma unroll
+        for (int i = 0; i < CP; ++i) {
+            const int r = c_row + i * CR;
+            if constexpr (OUT) {
+                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col))) = u32x2{v[i][0], v[i][1]};
+                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col + V / 2))) = u32x2{v[i][2], v[i][3]};
+            }
+#pragma unroll
+            for (int p = 0; p < (sizeof(T) == 2 ? PARTS : 1); ++p) *(u32x4 *)(lds.w[set][p] + slice_at<T, W_BIT>(r, c_col)) = part[i][p];
+        }
+    }
+    __device__ __forceinline__ void fetch_setup(int t)
     {
         b_row = t / BT; b_col = t % BT * V; c_row = t / CT; c_col = t % CT * V;
         sb = stream(wk.b, da);
@@ -286,9 +360,52 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
 #pragma unroll
         for (int i = 0; i < BP; ++i) ob[i] = offset(wk.b, b_row + i * BR, b_col, da);
 #pragma unroll
-        for (int i = 0; i < CP; ++i) {
-            oc[i] = offset(wk.c, c_row + i * CR, n0 + c_col, dc);
+        for (int i = 0; i < CP; ++i) oc[i] = offset(wk.c, c_row + i * CR, n0 + c_col, dc);
+    }
+    // `even` and `odd` hold the rows of the next two chunks (not DEEP: one is both)
+    __device__ __forceinline__ void fetch_first(Fetch &even, Fetch &odd)
+    {
+        fetch(even);
+        if constexpr (DEEP) fetch(odd);
+        deposit(0, even, rows_in(0));
+        fetch(even);
+    }
+    // in chunk's turn: `next`, the rows of the chunk after it (none after the last), into LDS, and the next ones not yet requested
+    template <int PARITY> __device__ __forceinline__ void supply(int chunk, Fetch &next)
+    {
+        deposit(SETS == 2 ? PARITY ^ 1 : 0, next, rows_in(chunk + 1));
+        fetch(next);
+    }
+    template <int PARITY> __device__ __forceinline__ void fetch_turn(int chunk, Fetch &next)
+    {
+        if constexpr (SETS == 1) __syncthreads();
+        supply<PARITY>(chunk, next);
+        __syncthreads();
+    }
+    __device__ __forceinline__ void fetch_walk(int t)
+    {
+        if (rows <= 0) return;
+        __builtin_amdgcn_s_setprio(2);          // the turn's longest way is theirs (7B training step: 181 -> 173, 479 -> 469 us)
+        fetch_setup(t);
+        const int chunks = (rows + CHUNK - 1) / CHUNK;
+        Fetch even, second, &odd = DEEP ? second : even;
+        fetch_first(even, odd);
+        __syncthreads();
+        // (in pairs, an odd chunk after the loop: were a turn skipped on one way through it, the waits would have to suit both ways)
+        for (int chunk = 0; chunk + 1 < chunks; chunk += 2) {
+            fetch_turn<0>(chunk, odd);
+            fetch_turn<1>(chunk + 1, even);
         }
+        if (chunks & 1) fetch_turn<0>(chunks - 1, odd);
+    }
+
+    // ---- the state waves: the state from chunk to chunk
+    float first_hi, first_lo, chunk_hi, chunk_lo, last_hi, last_lo;     // f^rows of the first, a full and the last chunk
+    int m0, c0;                 // tile (mt, nw): rows m0 + 16 mt + 4 g4 .. + 3, the slice's column c0 + 16 nw + l16
+    f32x4 S[NW][MT];
+
+    __device__ __forceinline__ void state_setup(int t)
+    {
         const int early = lead == 0 ? 1 : 0, last_rows = rows > 0 ? (rows - 1) % CHUNK + 1 : 0;
         power(decay, CHUNK - early, first_hi, first_lo);
         power(decay, CHUNK, chunk_hi, chunk_lo);
@@ -315,55 +432,6 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                     const int m = m0 + 16 * mt + 4 * g4 + i, n = n0 + c0 + 16 * nw + l16;
                     S[nw][mt][i] = first && m < da && n < dc ? first[m * fi + n * fj] * mul : 0.f;
                 }
-    }
-    Stream sb, sc;
-    __device__ __forceinline__ void fetch(Fetch &f)
-    {
-        const Chunk cb = sb.next(), cc = sc.next();
-#pragma unroll
-        for (int i = 0; i < BP; ++i) f.b[i] = load(cb, ob[i]);
-#pragma unroll
-        for (int i = 0; i < CP; ++i) f.c[i] = load(cc, oc[i]);
-        __builtin_amdgcn_sched_barrier(0);      // requests stay in order, which is what the waits count by
-    }
-    // b, c and c weighted by f^(rows - 1 - r); rows past the end count for nothing
-    __device__ __forceinline__ void deposit(int set, const Fetch &f, int rows) const
-    {
-#pragma unroll
-        for (int i = 0; i < BP; ++i) *(u32x4 *)(lds.b[set] + wide_at<T, DA>(b_row + i * BR, b_col / V)) = f.b[i];
-#pragma unroll
-        for (int i = 0; i < CP; ++i) {
-            const int r = c_row + i * CR;
-            const float w = r < rows ? exp2f(l2 * (rows - 1 - r)) : 0.f;
-            u32x4 v = f.c[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = r < rows ? v[j] : 0;
-            if constexpr (OUT) {
-                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col))) = u32x2{v[0], v[1]};
-                *(u32x2 *)(lds.c[set] + slice_at<T, C_BIT>(r, spread(c_col + V / 2))) = u32x2{v[2], v[3]};
-            }
-            if constexpr (sizeof(T) == 2) {
-                u32x4 part[PARTS];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float lo = M::low(v[j]) * w, hi = M::high(v[j]) * w;
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        part[p][j] = M::pack(lo, hi);
-                        // the remainder is that of the part as stored, not of one that the compiler rounds again from the exact
-                        // product (its mixed-precision f16 instructions do, an f16 step apart now and then)
-                        asm("" : "+v"(part[p][j]));
-                        if (p + 1 < PARTS) { lo = (lo - M::low(part[p][j])) * M::MORE; hi = (hi - M::high(part[p][j])) * M::MORE; }
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < PARTS; ++p) *(u32x4 *)(lds.w[set][p] + slice_at<T, W_BIT>(r, c_col)) = part[p];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * w);
-                *(u32x4 *)(lds.w[set][0] + slice_at<T, W_BIT>(r, c_col)) = v;
-            }
-        }
     }
     // the state's rounded copy, columns as rows
     __device__ __forceinline__ void publish(int set) const
@@ -512,44 +580,36 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                     if (m < da && n < dc) last[m * li + n * lj] = S[nw][mt][i] * mul;
                 }
     }
-    // One chunk: `next` holds the rows of the chunk after it (none after the last), and takes the next ones not yet requested.
     template <int PARITY> __device__ __forceinline__ void state_turn(int chunk, int chunks, Fetch &next)
     {
         constexpr int SET = SETS == 2 ? PARITY : 0, OTHER = SETS == 2 ? PARITY ^ 1 : 0;
         Frags f;
         gather(f, SET);
-        if constexpr (SETS == 2) {
-            deposit(OTHER, next, rows_in(chunk + 1));
-            fetch(next);
-        }
+        if constexpr (JOINT && SETS == 2) supply<PARITY>(chunk, next);
         const bool last = chunk + 1 == chunks;
         move_on(f, SET, last ? last_hi : chunk == 0 ? first_hi : chunk_hi, last ? last_lo : chunk == 0 ? first_lo : chunk_lo);
         if constexpr (SETS == 1) {
             __syncthreads();
-            deposit(OTHER, next, rows_in(chunk + 1));
-            fetch(next);
+            if constexpr (JOINT) supply<PARITY>(chunk, next);
         }
         publish(OTHER);
         __syncthreads();
     }
     __device__ __forceinline__ void state_walk(int t)
     {
+        if constexpr (JOINT) fetch_setup(t);
         state_setup(t);
         if (rows > 0) {
             const int chunks = (rows + CHUNK - 1) / CHUNK;
-            Fetch even, second, &odd = DEEP ? second : even;
-            fetch(even);
-            if constexpr (DEEP) fetch(odd);
-            deposit(0, even, rows_in(0));
-            fetch(even);
+            Fetch next;
+            if constexpr (JOINT) fetch_first(next, next);
             publish(0);
             __syncthreads();
-            // (in pairs, an odd chunk after the loop: were a turn skipped on one way through it, the waits would have to suit both ways)
             for (int chunk = 0; chunk + 1 < chunks; chunk += 2) {
-                state_turn<0>(chunk, chunks, odd);
-                state_turn<1>(chunk + 1, chunks, even);
+                state_turn<0>(chunk, chunks, next);
+                state_turn<1>(chunk + 1, chunks, next);
             }
-            if (chunks & 1) state_turn<0>(chunks - 1, chunks, odd);
+            if (chunks & 1) state_turn<0>(chunks - 1, chunks, next);
         }
         store_last();
     }
@@ -581,7 +641,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
         f32x4 P[W + 1], O[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int st = 0; st <= W; ++st) P[st] = f32x4{0.f, 0.f, 0.f, 0.f};
-        constexpr int BLOCK = KB < 4 || !DEEP ? 2 : 4;
+        constexpr int BLOCK = 2;
 #pragma unroll
         for (int kb = 0; kb < KB; kb += BLOCK) {
             u32x4 xb[BLOCK][W + 1], xs[BLOCK][2];
@@ -719,10 +779,10 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     }
 };
 
-// Waves 0 - 3 make the output, waves 4 - 7 move the state on and fetch rows: a chunk's two halves depend on each other only
-// from chunk to chunk, so they run side by side, two waves a SIMD.
+// Waves 0 - 3 make the output, waves 4 - 7 move the state on, waves 8 - 11 fetch rows: a chunk's parts depend on each other only
+// from chunk to chunk, so they run side by side, three waves a SIMD.  Without an output the state's waves come first.
 template <typename T, int DA, bool OUT, int PARTS, bool FULL>
-__global__ __launch_bounds__(OUT ? 512 : 256) void walk_kernel(Walks args, int slices)
+__global__ __launch_bounds__((Walker<T, DA, OUT, PARTS, FULL>::WAVES * 64)) void walk_kernel(Walks args, int slices)
 {
     typedef Walker<T, DA, OUT, PARTS, FULL> W;
     __shared__ typename W::Lds lds;
@@ -760,11 +820,15 @@ __global__ __launch_bounds__(OUT ? 512 : 256) void walk_kernel(Walks args, int s
         case 1: w.template out_walk<1>(); break;
         case 2: w.template out_walk<2>(); break;
         case 3: w.template out_walk<3>(); break;
-        default: w.state_walk(w.tid - 256);
+        case 4: case 5: case 6: case 7: w.state_walk(w.tid - 256); break;
+        default:
+            if constexpr (!W::JOINT) w.fetch_walk(w.tid - 512);
         }
-        w.clear_rest(w.tid, 512);
-    } else {
+        w.clear_rest(w.tid, W::WAVES * 64);
+    } else if (w.wave < 4) {
         w.state_walk(w.tid);
+    } else {
+        w.fetch_walk(w.tid - 256);
     }
 }
 
@@ -815,7 +879,8 @@ struct Step {
 };
 
 // A workgroup takes some columns of one head's state: each thread four columns of every R-th row, read, moved on, written back and
-// multiplied with q on the way; the threads of a column add up through LDS.  ALIGNED: dv is a multiple of 4.
+// multiplied with q on the way; the threads of a column add up through LDS.  ALIGNED: dv is a multiple of 4.  Bound by the state's
+// bytes: 128 sequences of 64 heads of 128 x 128 in 204 us, 5.3 TB/s; one sequence of 32 heads in 5.2 us, hardly more than a launch.
 template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void step_kernel(Step a)
 {
     __shared__ float lq[GCG_LINEAR_MAX_DIM], lk[GCG_LINEAR_MAX_DIM];
@@ -884,7 +949,7 @@ template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void s
 template <typename T, int DA, bool OUT, int PARTS> int walk_go(const Walks &w, int slices, bool full, hipStream_t st)
 {
     const int64_t blocks = (w.groups + 7) / 8 * 8 * slices;
-    const dim3 grid((unsigned)blocks), block(OUT ? 512 : 256);
+    const dim3 grid((unsigned)blocks), block(Walker<T, DA, OUT, PARTS, true>::WAVES * 64);
     if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidConfiguration;
     if (full) return launch_plain(walk_kernel<T, DA, OUT, PARTS, true>, grid, block, st, w, slices);
     return launch_plain(walk_kernel<T, DA, OUT, PARTS, false>, grid, block, st, w, slices);
@@ -924,16 +989,29 @@ template <typename T> int run_walks(const Walks &w, bool states, hipStream_t st)
     return walk_parts<T, true>(w, states && w.segments == 1, st);
 }
 
-// Segments of a walk: as many as give every CU two workgroups, of at least 512 rows, where the heads alone do not.
+int64_t seg_rows_of(int64_t L, int segments) { return ((L + segments - 1) / segments + CHUNK - 1) / CHUNK * CHUNK; }
+
+// Segments of a walk.  A CU takes one workgroup of a walk at a time, so a launch costs (rounds of 256 workgroups) * (chunks of a
+// segment), half as much again where the segments' states are made first, and two more launches and the join, about 10 chunks.
+// Segments are taken where that is below 3/4 of the walk in one piece, the fewest within 3 % of the best, four chunks at least.
+// Measured in us (bf16, 1 sequence, heads of 128): 8 heads of 131072 rows, forward, 1 segment 1961, 8 538, 16 525; backward, 1
+// segment 1890, 3 1841, 6 1429, 8 1289; 16 heads of 8192 rows, forward, 1 segment 103, 4 60, 8 71; backward, 1 segment 115, 2
+// 171; 8 heads of 1024 rows, forward, 1 segment 19, 2 26.
 int segments_of(int64_t walks, int64_t bs, int64_t L, int H, int dc)
 {
-    const int64_t units = walks * bs * H * ((dc + COLS - 1) / COLS);
-    if (units >= 256) return 1;
-    int64_t n = (512 + units - 1) / units, most = L / 512;
-    n = n < most ? n : most;
-    return n < 1 ? 1 : (int)n;
+    const int64_t units = walks * bs * H * ((dc + COLS - 1) / COLS), chunks = (L + CHUNK - 1) / CHUNK;
+    const auto rounds = [&](int64_t n) { return (units * n + 255) / 256; };
+    int64_t best = rounds(1) * chunks * 3 / 2;
+    int segments = 1;
+    for (int64_t n = 2; n <= chunks / 4 && units * n <= 768; ++n) {
+        const int64_t cost = rounds(n) * (seg_rows_of(L, (int)n) / CHUNK) * 3 + 20;
+        if (cost * 100 < best * 97) {
+            best = cost;
+            segments = (int)n;
+        }
+    }
+    return segments;
 }
-int64_t seg_rows_of(int64_t L, int segments) { return ((L + segments - 1) / segments + CHUNK - 1) / CHUNK * CHUNK; }
 
 void plan(Walks &w, int64_t L, int dc)
 {

@@ -116,7 +116,8 @@ def test_lengths_of_the_sequence(gcg_lib, L, dtype):
 @pytest.mark.parametrize("L", [1024, 1500, 2049])
 def test_split_sequences(gcg_lib, L, dtype):
     """Few heads: the sequence is walked in segments that are joined (their workspace is not empty), states included."""
-    assert gcg_lib.gcg_linear_attn_workspace_bytes(1, L, 2, 64, 64, 0) > 0 and gcg_lib.gcg_linear_attn_workspace_bytes(1, L, 2, 64, 64, 1) > 0
+    for backward in (0, 1):        # (1024 rows are walked in one piece)
+        assert (gcg_lib.gcg_linear_attn_workspace_bytes(1, L, 2, 64, 64, backward) > 0) == (L > 1024)
     q, k, v, do, initial, dfinal = data(1, L, 2, 64, 64, dtype, seed=L)
     ld = torch.tensor([-0.01, -0.0003], device=DEV)
     check(step(q, k, v, do, ld, None, initial, dfinal), reference(q, k, v, do, ld, 0.125, initial, dfinal), f"split {L} {dtype}")
@@ -288,9 +289,10 @@ def test_empty(gcg_lib):
                                  torch.zeros(0, 2, 16, 8, device=DEV)).shape == (0, 2, 8)
 
 
-def test_captured_in_a_graph(gcg_lib):
-    """A split prompt and a token after it, replayed with new inputs."""
-    q, k, v, do, initial, dfinal = data(1, 1100, 2, 64, 64, torch.bfloat16, seed=11)
+@pytest.mark.parametrize("L", [1100, 3000])
+def test_captured_in_a_graph(gcg_lib, L):
+    """A prompt, in one piece and split, and a token after it, replayed with new inputs."""
+    q, k, v, do, initial, dfinal = data(1, L, 2, 64, 64, torch.bfloat16, seed=11)
     ld = torch.tensor([-0.01, -0.001], device=DEV)
     state = torch.zeros_like(initial)
     def call():
@@ -306,7 +308,7 @@ def test_captured_in_a_graph(gcg_lib):
         out = call()
     torch.cuda.current_stream().wait_stream(side)
     for seed in range(3):
-        for t, new in zip((q, k, v, do, initial, dfinal), data(1, 1100, 2, 64, 64, torch.bfloat16, seed=20 + seed)):
+        for t, new in zip((q, k, v, do, initial, dfinal), data(1, L, 2, 64, 64, torch.bfloat16, seed=20 + seed)):
             t.copy_(new)
         eager = [t.clone() for t in call()] + [state.clone()]
         torch.cuda.synchronize()
