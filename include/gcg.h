@@ -570,7 +570,7 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
  * for dk and dv's rows after it): it meets them in one matrix instruction, times zero.
  *
  * dk, dv up to GCG_LINEAR_MAX_DIM, multiples of 8 (GCG_F32: of 4; the step takes any), bs * H up to GCG_LINEAR_MAX_HEADS, time strides up to GCG_LINEAR_MAX_TIME_STRIDE elements,
- * L up to GCG_LINEAR_MAX_ROWS, else GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, not 0.  dtype:
+ * L up to GCG_LINEAR_MAX_ROWS, else GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, as is its inverse.  dtype:
  * GCG_F32, GCG_BF16, GCG_F16.  workspace: gcg_linear_attn_workspace_bytes (0: none), 256-byte aligned.  Results are the same on
  * every run.
  */

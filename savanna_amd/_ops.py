@@ -37,13 +37,16 @@ OP_NAMES = (
     "mixer_se_fwd", "mixer_se_bwd", "filter_decay_fwd", "filter_decay_bwd",
     "mixer_mr_fwd", "mixer_mr_bwd", "mixer_mr_fwd_decay", "mixer_mr_bwd_decay", "fwd_time_major", "bwd_time_major", "fwd_decay", "bwd_decay", "fwd_interleaved_decay", "bwd_interleaved_decay",
     "fwd_planar", "bwd_planar",
+)
+# the operators around the convolution
+BLOCK_OP_NAMES = (
     "pack8", "unpack8", "layer_norm_fwd", "layer_norm_infer", "layer_norm_bwd",
     "linear_attn_fwd", "linear_attn_bwd", "linear_attn_packed_fwd", "linear_attn_packed_bwd", "linear_attn_step",
 )
 
 # differentiable as they are: C++ autograd nodes around operators above, which a trace sees in their place
-NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay", "layer_norm", "linear_attn",
-              "linear_attn_packed")
+NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay")
+BLOCK_NODE_NAMES = ("layer_norm", "linear_attn", "linear_attn_packed")
 
 
 # ---- autograd --------------------------------------------------------------------------------------------

@@ -2,6 +2,8 @@
 //
 // Bound by memory: s + 1 + 1/32 bytes an element each way, against a dozen vector instructions.  A lane holds one 16-byte
 // vector of a block, so a block is 16 lanes (32 in fp32) and its maximum a few lane exchanges; no shared memory, no barrier.
+// Measured, 16384 x 12288 bf16: 98 us each way, 6.2 TB/s, more than a copy of that size reaches (5.2); small tensors (701 x 1001
+// fp32: 3.6 and 3.4 us) are bound by the launch.
 #include "gcg_row.h"
 
 namespace gcg {
@@ -9,7 +11,7 @@ namespace {
 
 // A wave's vectors lie wave * 64 .. + 63 in the row-major list of a row's vectors; rows of whole blocks are one long row.
 // Each lane takes UNROLL of them, a fixed step apart, whose parts in rows and vectors the host divides (a loop over more of them in
-// fewer workgroups is slower: 16384 x 12288 bf16 110 us, 104 this way).
+// fewer workgroups is slower: 16384 x 12288 bf16 110 us, 98 this way).
 constexpr int UNROLL = 2;
 struct Walk { int64_t rows; int64_t D; int64_t per_row; int64_t step_row, step_vec; };
 

@@ -947,7 +947,7 @@ int linear_check(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float
 {
     if (bs <= 0 || L < 0 || H <= 0 || dk <= 0 || dv <= 0) return GCG_ERR_BAD_ARG;
     if (dtype != GCG_F32 && dtype != GCG_BF16 && dtype != GCG_F16) return GCG_ERR_BAD_ARG;
-    if (!(scale - scale == 0.f) || scale == 0.f) return GCG_ERR_BAD_ARG;
+    if (!(scale - scale == 0.f) || !(1.f / scale - 1.f / scale == 0.f)) return GCG_ERR_BAD_ARG;    // (the backward divides by it)
     // rows are read in vectors (the step reads by elements); heads and batch index the grid together
     const int vec = dtype == GCG_F32 ? 4 : 8;
     if (L != 0 && (dk % vec || dv % vec)) return GCG_ERR_UNSUPPORTED;

