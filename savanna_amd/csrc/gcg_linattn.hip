@@ -66,7 +66,8 @@ template <> struct Mat<f16_t> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int V = 8, KF = 32;
-    static constexpr float MORE = 4096.f;
+    // (rounding is off by at most 16, which 2^11 brings to 32768: the next part and its own rounding stay in range for every f16)
+    static constexpr float MORE = 2048.f;
     static __device__ __forceinline__ f32x4 mul(const u32x4 &a, const u32x4 &b, const f32x4 &c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -537,7 +538,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
 #pragma unroll
         for (int nw = 0; nw < NW; ++nw) {
             if constexpr (F16) {
-                // parts after the first are stored 2^12, 2^24 times larger and added up on their own, the smallest first
+                // parts after the first are stored 2^11, 2^22 times larger and added up on their own, the smallest first
                 f32x4 R[MT];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) R[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -545,7 +546,7 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                 for (int part = PARTS - 1; part > 0; --part) {
                     update(f, set, part, nw, R);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) R[mt] *= 0x1p-12f;
+                    for (int mt = 0; mt < MT; ++mt) R[mt] *= 0x1p-11f;
                 }
                 update(f, set, 0, nw, R);
 #pragma unroll
