@@ -33,9 +33,9 @@
 //
 // Rounding of 16-bit walks: the matrix instructions take 16-bit operands, so P and the state's copy are rounded to the type once,
 // as the output is; the weighted c is given as a sum of two 16-bit parts (three where the state itself is a result), whose
-// remainder, 2^-16 (2^-24), does not show in the fp32 state.  f16 has no range to spare: rows of P and blocks of the
-// state's copy are scaled by powers of two, and the later parts of the weighted c too, so that neither large states nor
-// small gradients leave it.  fp32 walks run on the fp32 matrix instructions, with nothing rounded.
+// remainder, 2^-16 (2^-24), does not show in the fp32 state.  f16 has no range to spare: rows of P and the
+// columns of the state's copy, 32 rows at a time, are scaled by powers of two, and the later parts of the weighted c too, so that neither
+// large states nor small gradients leave it.  fp32 walks run on the fp32 matrix instructions, with nothing rounded.
 #include "gcg_common.h"
 
 namespace gcg {
@@ -143,11 +143,6 @@ __device__ __forceinline__ Range range(float top)
     if (e < 20 || e > 230) return {1.f, 1.f};
     return {__uint_as_float((253 - e) << 23), __uint_as_float((e + 1) << 23)};
 }
-__device__ __forceinline__ float wave_max(float x)
-{
-    for (int d = 1; d < 64; d *= 2) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
 
 // ---- arguments ----------------------------------------------------------------------------------------------
 struct Rows { const void *p; int64_t sb, st, sh; };                    // strides of batch, time and head in elements
@@ -201,9 +196,10 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     static constexpr bool F16 = __is_same(T, f16_t);
     static constexpr int V = M::V, KF = M::KF, KB = DA / KF, KG = CHUNK / KF;
     static constexpr int CS = kSliceRow<T>;
-    static constexpr size_t ONE = (size_t)(CHUNK * DA + (PARTS + OUT) * CHUNK * CS + (OUT ? COLS * DA : 0)) * sizeof(T);
-    static constexpr int SETS = 2 * ONE <= 160 * 1024 - 256 ? 2 : 1;
-    static_assert(SETS * ONE <= 160 * 1024 - 256, "workgroup exceeds the 160 KB of LDS");
+    static constexpr size_t ONE = (size_t)(CHUNK * DA + (PARTS + OUT) * CHUNK * CS + (OUT ? COLS * DA : 0)) * sizeof(T) +
+                                  (F16 && OUT ? KB * COLS : 0);
+    static constexpr int SETS = 2 * ONE <= 160 * 1024 ? 2 : 1;
+    static_assert(SETS * ONE <= 160 * 1024, "workgroup exceeds the 160 KB of LDS");
     // 16-row tiles of the state a wave keeps, and of its two 16-column ones: whole blocks of KF rows in 16 bits
     static constexpr int NW = DA == 64 ? 1 : 2, MT = DA == 64 ? 2 : DA / 64;
     static constexpr bool DEEP = DA * sizeof(T) <= 256;     // registers for the rows of two chunks ahead (else one)
@@ -224,11 +220,20 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
     const Walks &args;
     const Walk &wk;
     Lds &lds;
-    // f16: by how much the blocks of the state's copy are smaller (a workgroup without them has no place for it either)
-    static __device__ __forceinline__ float &range_of(int set, int block, int half)
+    // f16: by how much KF rows of a column of the state's copy are smaller, as an fp32 exponent (a workgroup without a copy has no
+    // place for it either).  Every column has its own, so that neither a neighbour 2^14 times larger nor one without finite values
+    // takes its bits.  (Two exchanges of lanes find it, six one for 16 columns: f16, 2 x 8192 rows of 32 heads of 128, forward 182 us
+    // and 188 with one for 16, backward 533 and 561.)
+    static __device__ __forceinline__ uint8_t *range_of(int set, int block)
     {
-        __shared__ float place[SETS][KB][2];
-        return place[set][block][half];
+        __shared__ __align__(8) uint8_t place[SETS][KB][COLS];
+        return place[set][block];
+    }
+    // columns 8 g4 + 4 nt .. + 3
+    static __device__ __forceinline__ f32x4 ranges(uint32_t w)
+    {
+        return f32x4{__uint_as_float(w << 23 & 0x7f800000u), __uint_as_float(w << 15 & 0x7f800000u), __uint_as_float(w << 7 & 0x7f800000u),
+                     __uint_as_float(w >> 1 & 0x7f800000u)};
     }
     int b, h, seg, job, da, dc, n0, lane, l16, g4, wave, tid;
     int length, from, rows;     // of the sequence; the segment's first row and its rows
@@ -448,9 +453,10 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                         float top = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(S[nw][2 * kb + i / 4][i & 3]));
-                        const Range r = range(wave_max(top));
+                        top = fmaxf(top, __shfl_xor(top, 16));
+                        const Range r = range(fmaxf(top, __shfl_xor(top, 32)));
                         by[kb] = r.down;
-                        if (lane == 0) range_of(set, m0 / KF + kb, c0 / 16 + nw) = r.up;
+                        if (g4 == 0) range_of(set, m0 / KF + kb)[c0 + 16 * nw + l16] = (uint8_t)(__float_as_uint(r.up) >> 23);
                     }
                 }
 #pragma unroll
@@ -658,11 +664,13 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
             if constexpr (DEEP) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < BLOCK; ++k) {
+                u32x2 up = {0, 0};
+                if constexpr (F16) up = *(const u32x2 *)(range_of(SET, kb + k) + 8 * g4);
 #pragma unroll
                 for (int st = 0; st <= W; ++st) P[st] = M::mul(xb[k][st], a.k[kb + k], P[st]);
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-                    if constexpr (F16) O[nt] += M::mul(xs[k][nt], a.k[kb + k], f32x4{0.f, 0.f, 0.f, 0.f}) * range_of(SET, kb + k, g4 >> 1);
+                    if constexpr (F16) O[nt] += M::mul(xs[k][nt], a.k[kb + k], f32x4{0.f, 0.f, 0.f, 0.f}) * ranges(up[nt]);
                     else O[nt] = M::mul(xs[k][nt], a.k[kb + k], O[nt]);
                 }
             }

@@ -7,6 +7,7 @@ rounded lose 2^-25 of the largest one beside them at most; the inputs here are s
 import pytest
 import torch
 
+from savanna_amd.operators.linear_attention import linear_attention
 from test_linear_attention_gpu import DEV, recurrence, step
 
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,29 @@ def test_operands_near_the_smallest(gcg_lib, which, states):
     initial, dfinal = (2.0 ** -10 * torch.randn(1, 3, 64, 48, generator=gen, device=DEV) if states else None for _ in range(2))
     got = step(*(t[n] for n in NAMES), ld, 0.125, initial, dfinal)
     check(got, reference(t, ld, 0.125, initial, dfinal), f"small {which}")
+
+
+@pytest.mark.parametrize("which", NAMES)
+@pytest.mark.parametrize("L,H,dk,dv", [(200, 2, 64, 64), (200, 1, 256, 40), (2049, 2, 128, 64)])
+def test_channels_of_different_size(gcg_lib, L, H, dk, dv, which):
+    """Neighbouring channels of one operand 2^8 and 2^-11, the other operands 2^-3: each column of the result keeps its own precision."""
+    t, gen = data(L, H, dk, dv, 3, 1.0)
+    by = torch.where(torch.arange(t[which].shape[-1], device=DEV) % 3 == 0, 2.0 ** 8, 2.0 ** -11)
+    for n in NAMES:
+        t[n] = (t[n].float() * (by if n == which else 2.0 ** -3)).half()
+    ld = torch.tensor([-0.01, -0.003], device=DEV)[:H].contiguous()
+    got = step(*(t[n] for n in NAMES), ld, 0.125)
+    check(got, reference(t, ld, 0.125, None, None), f"channels of {which}")
+
+
+def test_a_column_without_finite_values_leaves_its_neighbours_alone(gcg_lib):
+    """An infinity in one column of the given state, values beyond f16's largest in the others: those come out as without it."""
+    t, gen = data(100, 2, 64, 64, 4, 2.0 ** -8)
+    ld = torch.tensor([-0.01, -0.003], device=DEV)
+    initial = 1e5 * torch.randn(1, 2, 64, 64, generator=gen, device=DEV)
+    clean = linear_attention(t["q"], t["k"], t["v"], ld, initial_state=initial)
+    initial[0, 1, 5, 7] = float("inf")
+    o = linear_attention(t["q"], t["k"], t["v"], ld, initial_state=initial)
+    others = [j for j in range(64) if j != 7]
+    assert torch.isfinite(clean).all() and not torch.isfinite(o[0, :, 1, 7]).any()
+    assert torch.equal(o[..., others], clean[..., others])
