@@ -566,8 +566,7 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
  *
  * gcg_linear_attn_step takes one token: the state is moved on in place.
  *
- * A row of v that holds an infinity or a NaN also makes NaN of outputs up to 31 rows before it (forward; as of do
- * for dk and dv's rows after it): it meets them in one matrix instruction, times zero.
+ * An infinity or a NaN reaches the rows that the recurrence takes it to, and no others.
  *
  * dk, dv up to GCG_LINEAR_MAX_DIM, multiples of 8 (GCG_F32: of 4; the step takes any), bs * H up to GCG_LINEAR_MAX_HEADS, time strides up to GCG_LINEAR_MAX_TIME_STRIDE elements,
  * L up to GCG_LINEAR_MAX_ROWS, else GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, as is its inverse.  dtype:

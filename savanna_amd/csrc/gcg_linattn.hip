@@ -639,6 +639,48 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
             a.k[k] = load(c, FULL ? oa[0] + (uint32_t)(k * KF * sizeof(T)) : oa[FULL ? 0 : k]);
         __builtin_amdgcn_sched_barrier(0);
     }
+    // The last inner block's product again, where its result holds infinities or NaN.  The block's rows of c that the causal mask hides
+    // from a row are times a score of zero there, which is NaN for such an element.  So each of those counts as zero and a second
+    // product tells which results see one: only these keep theirs.  (The check before it: 1 % of the forward of 2 x 8192 rows of 32
+    // heads of 128, bf16 165 -> 167 us.)
+    template <int W> __device__ __forceinline__ void hide(int set, const u32x4 &x, const f32x4 (&before)[2], f32x4 (&near)[2]) const
+    {
+        constexpr uint32_t TOP = sizeof(T) == 4 ? 0x7f800000u : F16 ? 0x7c00u : 0x7f80u, ONE_ = sizeof(T) == 4 ? 0x3f800000u : F16 ? 0x3c00u : 0x3f80u;
+        const auto bit = [](uint32_t w, int j) { return (w >> 16 * j & TOP) == TOP; };
+        int row = l16;
+        uint32_t all = ONE_ | (sizeof(T) == 2 ? ONE_ << 16 : 0);
+        asm volatile("" : "+v"(row), "+v"(all));        // (or the masks are made before the walk and kept in registers all the way)
+        u32x4 seen;             // 1 where the score's row is at or before the result's
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                seen[j] = row >= score_row(g4, j) ? ONE_ : 0;
+            } else {
+                const int i = 2 * (j & 1);
+                const uint32_t own = (row >= score_row(g4, i) ? ONE_ : 0) | (row >= score_row(g4, i + 1) ? ONE_ << 16 : 0);
+                seen[j] = W & 1 ? j < 2 ? all : own : j < 2 ? own : 0;
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+            const u32x4 xc = inner_c(set, sizeof(T) == 2 ? W / 2 : W, nt);
+            u32x4 finite, rest;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = xc[j];
+                if constexpr (sizeof(T) == 4) {
+                    finite[j] = bit(w, 0) ? 0 : w;
+                    rest[j] = bit(w, 0) ? ONE_ : 0;
+                } else {
+                    finite[j] = (bit(w, 0) ? 0 : w & 0xffffu) | (bit(w, 1) ? 0 : w & 0xffff0000u);
+                    rest[j] = (bit(w, 0) ? ONE_ : 0) | (bit(w, 1) ? ONE_ << 16 : 0);
+                }
+            }
+            const f32x4 without = M::mul(finite, x, before[nt]), count = M::mul(rest, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) near[nt][i] = count[i] > 0.f ? near[nt][i] : without[i];
+        }
+    }
     template <int W, int PARITY> __device__ __forceinline__ void out_turn(int chunk, RowsA &a)
     {
         constexpr int SET = SETS == 2 ? PARITY : 0;
@@ -706,9 +748,10 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
             for (int st = 0; st <= W; ++st) P[st] *= r.down;
             near[0] = near[1] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        u32x4 x;
+        f32x4 before[2];
 #pragma unroll
         for (int p = 0; p < GROUPS; ++p) {
-            u32x4 x;
             if constexpr (sizeof(T) == 2) {
                 x[0] = M::pack(P[2 * p][0], P[2 * p][1]);
                 x[1] = M::pack(P[2 * p][2], P[2 * p][3]);
@@ -718,8 +761,15 @@ template <typename T, int DA, bool OUT, int PARTS, bool FULL> struct Walker {
                 x = __builtin_bit_cast(u32x4, P[p]);
             }
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) near[nt] = M::mul(xc[p][nt], x, near[nt]);
+            for (int nt = 0; nt < 2; ++nt) {
+                before[nt] = near[nt];
+                near[nt] = M::mul(xc[p][nt], x, near[nt]);
+            }
         }
+        float odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd = fmaf(near[i >> 2][i & 3], 0.f, odd);
+        if (__builtin_expect(__ballot(odd != 0.f) != 0, 0)) hide<W>(SET, x, before, near);
         const Chunk to_rows = so.next();
         const uint32_t off = oo + to_rows.shift;
         float v[8];
