@@ -943,7 +943,7 @@ struct Step {
 // bytes: 128 sequences of 64 heads of 128 x 128 in 204 us, 5.3 TB/s; one sequence of 32 heads in 5.2 us, hardly more than a launch.
 template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void step_kernel(Step a)
 {
-    __shared__ float lq[GCG_LINEAR_MAX_DIM], lk[GCG_LINEAR_MAX_DIM];
+    __shared__ float lq[GCG_LINEAR_MAX_DIM], lk[GCG_LINEAR_MAX_DIM], f[2];
     __shared__ __align__(16) float part[4 * THREADS];           // [thread of a column][column]
     const int slices = (a.dv + a.cols - 1) / a.cols;
     const int64_t bh = blockIdx.x / slices;
@@ -951,7 +951,6 @@ template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void s
     const int64_t b = bh / a.H;
     const T *q = (const T *)a.q + b * a.qb + h * a.qh, *k = (const T *)a.k + b * a.kb + h * a.kh, *v = (const T *)a.v + b * a.vb + h * a.vh;
     const int quads = a.cols / 4, R = THREADS / quads, col = slice * a.cols + tid % quads * 4, row0 = tid / quads;
-    const float f = expf(clamp_decay(a.log_decay[h]));
     float vv[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) vv[i] = col + i < a.dv ? Elem<T>::load(v + col + i) : 0.f;
@@ -959,9 +958,16 @@ template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void s
         lq[i] = Elem<T>::load(q + i);
         lk[i] = Elem<T>::load(k + i);
     }
+    // (as a sum of two floats, as in the walk: one float's rounding, the same for every token, would show after thousands of them)
+    if (tid < kWave) {
+        float hi, lo;
+        power(clamp_decay(a.log_decay[h]), 1, hi, lo);
+        if (tid == 0) { f[0] = hi; f[1] = lo; }
+    }
     float *const s = a.state + bh * a.dk * a.dv + col;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     __syncthreads();
+    const float hi = f[0], lo = f[1];
     if (row0 < R && col < a.dv) {
         constexpr int U = 8;
         for (int m = row0; m < a.dk; m += U * R) {
@@ -984,7 +990,7 @@ template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void s
                 if (r < a.dk) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[u][i] = fmaf(x[u][i], f, lk[r] * vv[i]);
+                        x[u][i] = fmaf(x[u][i], hi, fmaf(x[u][i], lo, lk[r] * vv[i]));
                         o[i] = fmaf(lq[r], x[u][i], o[i]);
                     }
                     if (ALIGNED) *(f32x4 *)(s + (int64_t)r * a.dv) = x[u];

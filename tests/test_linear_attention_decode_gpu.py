@@ -1,0 +1,28 @@
+"""Single tokens of linear attention where they are many, against the recurrence in 64 bits."""
+import pytest
+import torch
+
+from savanna_amd.operators.linear_attention import linear_attention_step
+from test_linear_attention_gpu import DEV
+
+pytestmark = pytest.mark.gpu
+
+
+def test_thousands_of_tokens(gcg_lib):
+    """The decay of every token is kept to more than fp32's 24 bits, as over the rows of a prompt: its rounding, the same way each time,
+    would add up.  A state is off by 2^-17 of its terms' magnitudes, an output by one rounding more."""
+    H, d, n = 3, 8, 8192
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = (0.5 + 0.5 * torch.rand(n, 1, H, d, generator=gen, device=DEV) for _ in range(3))        # (of one sign: nothing cancels)
+    ld = torch.tensor([-1.0 / 4096, -1.0 / 3000, -1e-5], device=DEV)
+    state = 4 * torch.randn(1, H, d, d, generator=gen, device=DEV)
+    f = torch.exp(ld.double())[:, None, None]
+    S, A = state.double(), state.double().abs()
+    with torch.no_grad():
+        for t in range(n):
+            o = linear_attention_step(q[t], k[t], v[t], ld, state, 0.5)
+            S = f * S + k[t].double()[..., None] * v[t].double()[..., None, :]
+            A = f * A + k[t].double().abs()[..., None] * v[t].double().abs()[..., None, :]
+    assert ((state.double() - S).abs() <= 2.0 ** -17 * A).all()
+    want, terms = ((x[..., None] * y).sum(-2) * 0.5 for x, y in ((q[-1].double(), S), (q[-1].double().abs(), A)))
+    assert ((o.double() - want).abs() <= 2.0 ** -16 * terms).all()
