@@ -568,13 +568,13 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
  *
  * An infinity or a NaN reaches the rows that the recurrence takes it to, and no others.
  *
- * dk, dv up to GCG_LINEAR_MAX_DIM, multiples of 8 (GCG_F32: of 4; the step takes any), bs * H up to GCG_LINEAR_MAX_HEADS, time strides up to GCG_LINEAR_MAX_TIME_STRIDE elements,
- * L up to GCG_LINEAR_MAX_ROWS, else GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, as is its inverse.  dtype:
- * GCG_F32, GCG_BF16, GCG_F16.  workspace: gcg_linear_attn_workspace_bytes (0: none), 256-byte aligned.  Results are the same on
- * every run.
+ * dk, dv up to GCG_LINEAR_MAX_DIM, multiples of 8 (GCG_F32: of 4; the step takes any), bs * H up to GCG_LINEAR_MAX_HEADS (the
+ * step: GCG_LINEAR_MAX_STEP_HEADS), time strides up to GCG_LINEAR_MAX_TIME_STRIDE elements, L up to GCG_LINEAR_MAX_ROWS, else
+ * GCG_ERR_UNSUPPORTED.  Strides are not negative.  scale: finite, as is its inverse.  dtype: GCG_F32, GCG_BF16, GCG_F16.
+ * workspace: gcg_linear_attn_workspace_bytes (0: none), 256-byte aligned.  Results are the same on every run.
  */
-enum { GCG_LINEAR_MAX_DIM = 256, GCG_LINEAR_MAX_HEADS = 65535, GCG_LINEAR_MAX_TIME_STRIDE = 1 << 22,
-       GCG_LINEAR_MAX_ROWS = 1 << 30 };
+enum { GCG_LINEAR_MAX_DIM = 256, GCG_LINEAR_MAX_HEADS = 65535, GCG_LINEAR_MAX_STEP_HEADS = (1 << 24) - 1,
+       GCG_LINEAR_MAX_TIME_STRIDE = 1 << 22, GCG_LINEAR_MAX_ROWS = 1 << 30 };
 GCG_API size_t gcg_linear_attn_workspace_bytes(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, int32_t backward);
 GCG_API int gcg_linear_attn_fwd(const void *q, const void *k, const void *v, const int64_t *strides, const float *log_decay,
             const float *initial, const int32_t *lengths, void *o, float *final, void *workspace, size_t workspace_bytes,

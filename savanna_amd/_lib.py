@@ -1145,6 +1145,7 @@ def layer_norm_bwd(dy, x, codes, scales, stats, w, b):
 # ---- linear attention with a decay for each head --------------------------------------------------------
 
 LINEAR_MAX_DIM = 256                # GCG_LINEAR_MAX_DIM
+LINEAR_MAX_HEADS = 65535            # GCG_LINEAR_MAX_HEADS
 
 
 def _check_linear(q, k, v, log_decay, dim) -> None:
@@ -1156,6 +1157,8 @@ def _check_linear(q, k, v, log_decay, dim) -> None:
     if log_decay.shape != (q.shape[-2],) or log_decay.dtype != torch.float32 or not log_decay.is_contiguous() \
             or log_decay.device != q.device:
         raise ValueError("log_decay must be a contiguous float32 tensor of one element a head on q's device")
+    if q.shape[-2] > 2 ** 31 - 1:
+        raise ValueError(f"{q.shape[-2]} heads; at most {2 ** 31 - 1} are supported")
     if not (0 < q.shape[-1] <= LINEAR_MAX_DIM and 0 < v.shape[-1] <= LINEAR_MAX_DIM):
         raise ValueError(f"head dimensions are 1 to {LINEAR_MAX_DIM}")
 
@@ -1211,6 +1214,13 @@ def _linear_workspace(lib, q, v, backward):
     return n, (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None)
 
 
+def _in_parts(into, q, *tensors) -> None:
+    """``into(part of every tensor)`` over the batch at once, or, with more heads in it than a launch takes, entry after entry."""
+    bs, n = q.shape[0], max(1, LINEAR_MAX_HEADS // q.shape[2])
+    for at in range(0, bs, n):
+        into(*(t if t is None or n >= bs else t[at:at + n] for t in (q, *tensors)))
+
+
 def linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale: float, final: bool):
     """(o, final state or None) of q, k (bs, L, H, dk), v (bs, L, H, dv); initial (bs, H, dk, dv) fp32 and lengths (bs) int32 may
     be None."""
@@ -1232,13 +1242,15 @@ def linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale: float, final: b
     if pk or pv:
         o, last = linear_attn_fwd(*_padded(pk, q, k), *_padded(pv, v), log_decay, _padded_state(initial, pk, pv), lengths, scale, final)
         return o[..., :dv].contiguous(), _cut_state(last, dk, dv)
-    with _on_device(q.device):
+    def into(q, k, v, initial, lengths, o, last):
         q, k, v = _rows(q), _rows(k), _rows(v)
         n, ws = _linear_workspace(lib, q, v, False)
         rc = lib.gcg_linear_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, q, k, v, o), log_decay.data_ptr(),
-                                     _ptr(initial), _ptr(lengths), o.data_ptr(), _ptr(last), _ptr(ws), n, bs, L, H, dk, dv, scale,
+                                     _ptr(initial), _ptr(lengths), o.data_ptr(), _ptr(last), _ptr(ws), n, *q.shape, dv, scale,
                                      dtype_code(q.dtype), torch.cuda.current_stream().cuda_stream)
-    check(rc, "gcg_linear_attn_fwd")
+        check(rc, "gcg_linear_attn_fwd")
+    with _on_device(q.device):
+        _in_parts(into, q, k, v, initial, lengths, o, last)
     return o, last
 
 
@@ -1246,14 +1258,17 @@ def _linear_bwd_into(do, q, k, v, log_decay, initial, lengths, dfinal, scale, dq
     lib = load()
     if do.shape != v.shape or do.dtype != v.dtype or do.device != v.device:
         raise ValueError("do must have the shape, dtype and device of v")
-    with _on_device(q.device):
+
+    def into(q, do, k, v, initial, lengths, dfinal, dq, dk, dv, dinitial):
         do, q, k, v = _rows(do), _rows(q), _rows(k), _rows(v)
         n, ws = _linear_workspace(lib, q, v, True)
         rc = lib.gcg_linear_attn_bwd(do.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(3, do, q, k, v, dq, dk, dv),
                                      log_decay.data_ptr(), _ptr(initial), _ptr(lengths), _ptr(dfinal), dq.data_ptr(), dk.data_ptr(),
                                      dv.data_ptr(), _ptr(dinitial), _ptr(ws), n, *q.shape, v.shape[-1], scale, dtype_code(q.dtype),
                                      torch.cuda.current_stream().cuda_stream)
-    check(rc, "gcg_linear_attn_bwd")
+        check(rc, "gcg_linear_attn_bwd")
+    with _on_device(q.device):
+        _in_parts(into, q, do, k, v, initial, lengths, dfinal, dq, dk, dv, dinitial)
 
 
 def linear_attn_bwd(do, q, k, v, log_decay, initial, lengths, dfinal, scale: float, need_dinitial: bool):

@@ -951,7 +951,8 @@ int linear_check(int64_t bs, int64_t L, int32_t H, int32_t dk, int32_t dv, float
     // rows are read in vectors (the step reads by elements); heads and batch index the grid together
     const int vec = dtype == GCG_F32 ? 4 : 8;
     if (L != 0 && (dk % vec || dv % vec)) return GCG_ERR_UNSUPPORTED;
-    return L > GCG_LINEAR_MAX_ROWS || dk > GCG_LINEAR_MAX_DIM || dv > GCG_LINEAR_MAX_DIM || bs > GCG_LINEAR_MAX_HEADS || bs * H > GCG_LINEAR_MAX_HEADS ? GCG_ERR_UNSUPPORTED : GCG_OK;
+    const int64_t heads = L == 0 ? GCG_LINEAR_MAX_STEP_HEADS : GCG_LINEAR_MAX_HEADS;
+    return L > GCG_LINEAR_MAX_ROWS || dk > GCG_LINEAR_MAX_DIM || dv > GCG_LINEAR_MAX_DIM || bs > heads || bs * H > heads ? GCG_ERR_UNSUPPORTED : GCG_OK;
 }
 // a chunk's rows are addressed by 32-bit offsets
 int strides_check(const int64_t *s, int tensors, int dims)

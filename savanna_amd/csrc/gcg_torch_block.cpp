@@ -274,6 +274,7 @@ void check_heads(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor
     TORCH_CHECK(log_decay.dim() == 1 && log_decay.size(0) == q.size(dim - 2) && log_decay.scalar_type() == at::kFloat &&
                     log_decay.is_contiguous() && log_decay.device() == q.device(),
                 "gcg: log_decay must be a contiguous float32 tensor of one element a head on q's device");
+    TORCH_CHECK(q.size(dim - 2) <= INT32_MAX, "gcg: ", q.size(dim - 2), " heads; at most ", INT32_MAX, " are supported");
     TORCH_CHECK(q.size(-1) <= GCG_LINEAR_MAX_DIM && v.size(-1) <= GCG_LINEAR_MAX_DIM && q.size(-1) > 0 && v.size(-1) > 0,
                 "gcg: head dimensions are 1 to ", (int)GCG_LINEAR_MAX_DIM);
 }
@@ -317,6 +318,31 @@ OptTensor padded_state(const OptTensor &t, int64_t dk, int64_t dv) { return give
 Tensor cut(const Tensor &t, int64_t d) { return t.size(-1) == d ? t : t.slice(-1, 0, d).contiguous(); }
 Tensor cut_state(const Tensor &t, int64_t dk, int64_t dv) { return t.numel() ? t.slice(2, 0, dk).slice(3, 0, dv).contiguous() : t; }
 
+// The batch at once, or, with more heads in it than a launch takes, some entries after the others.
+template <typename Part, typename Whole> void for_entries(const Tensor &q, Part part, Whole whole)
+{
+    const int64_t bs = q.size(0), H = q.size(2), n = std::max<int64_t>(1, GCG_LINEAR_MAX_HEADS / H);
+    if (bs <= n) return whole();
+    for (int64_t at = 0; at < bs; at += n) part(at, std::min(n, bs - at));
+}
+OptTensor entries(const OptTensor &t, int64_t at, int64_t n) { return given(t) ? OptTensor(t->narrow(0, at, n)) : t; }
+
+void linear_fwd_launch(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const OptTensor &initial,
+                       const OptTensor &lengths, double scale, const Tensor &o, const Tensor &last)
+{
+    const Tensor a = rows_of(q), b = rows_of(k), c = rows_of(v);
+    std::vector<int64_t> s;
+    for (const Tensor *t : {&a, &b, &c, &o}) add_strides(s, *t);
+    size_t bytes;
+    Tensor ws = linear_workspace(q, v, false, &bytes);
+    check_rc(gcg_linear_attn_fwd(a.data_ptr(), b.data_ptr(), c.data_ptr(), s.data(), (const float *)log_decay.data_ptr(),
+                                 (const float *)ptr(initial), (const int32_t *)ptr(lengths), o.data_ptr(),
+                                 last.defined() ? (float *)last.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, q.size(0),
+                                 q.size(1), (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), (float)scale,
+                                 dtype_code(q.scalar_type()), stream_of(q)),
+             "gcg_linear_attn_fwd");
+}
+
 std::tuple<Tensor, Tensor> linear_attn_fwd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                            const OptTensor &initial, const OptTensor &lengths, double scale, bool final)
 {
@@ -334,23 +360,16 @@ std::tuple<Tensor, Tensor> linear_attn_fwd(const Tensor &q, const Tensor &k, con
                                               scale, final);
         return {cut(po, dv), cut_state(pl, dk, dv)};
     }
-    const Tensor a = rows_of(q), b = rows_of(k), c = rows_of(v);
-    std::vector<int64_t> s;
-    for (const Tensor *t : {&a, &b, &c, (const Tensor *)&o}) add_strides(s, *t);
-    size_t bytes;
-    Tensor ws = linear_workspace(q, v, false, &bytes);
-    check_rc(gcg_linear_attn_fwd(a.data_ptr(), b.data_ptr(), c.data_ptr(), s.data(), (const float *)log_decay.data_ptr(),
-                                 (const float *)ptr(initial), (const int32_t *)ptr(lengths), o.data_ptr(),
-                                 final ? (float *)last.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, q.size(0), q.size(1),
-                                 (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), (float)scale, dtype_code(q.scalar_type()),
-                                 stream_of(q)),
-             "gcg_linear_attn_fwd");
+    for_entries(q, [&](int64_t at, int64_t n) {
+        linear_fwd_launch(q.narrow(0, at, n), k.narrow(0, at, n), v.narrow(0, at, n), log_decay, entries(initial, at, n),
+                          entries(lengths, at, n), scale, o.narrow(0, at, n), final ? last.narrow(0, at, n) : Tensor());
+    }, [&] { linear_fwd_launch(q, k, v, log_decay, initial, lengths, scale, o, final ? last : Tensor()); });
     return {o, last};
 }
 
 void linear_bwd_launch(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                        const OptTensor &initial, const OptTensor &lengths, const OptTensor &dfinal, double scale, const Tensor &dq,
-                       const Tensor &d_k, const Tensor &d_v, float *dinitial)
+                       const Tensor &d_k, const Tensor &d_v, const Tensor &dinitial)
 {
     const Tensor g = rows_of(d_o), a = rows_of(q), b = rows_of(k), c = rows_of(v);
     std::vector<int64_t> s;
@@ -359,10 +378,21 @@ void linear_bwd_launch(const Tensor &d_o, const Tensor &q, const Tensor &k, cons
     Tensor ws = linear_workspace(q, v, true, &bytes);
     check_rc(gcg_linear_attn_bwd(g.data_ptr(), a.data_ptr(), b.data_ptr(), c.data_ptr(), s.data(), (const float *)log_decay.data_ptr(),
                                  (const float *)ptr(initial), (const int32_t *)ptr(lengths), (const float *)ptr(dfinal), dq.data_ptr(),
-                                 d_k.data_ptr(), d_v.data_ptr(), dinitial, bytes ? ws.data_ptr() : nullptr, bytes, q.size(0), q.size(1),
-                                 (int32_t)q.size(2), (int32_t)q.size(3), (int32_t)v.size(3), (float)scale, dtype_code(q.scalar_type()),
-                                 stream_of(q)),
+                                 d_k.data_ptr(), d_v.data_ptr(), dinitial.defined() ? (float *)dinitial.data_ptr() : nullptr,
+                                 bytes ? ws.data_ptr() : nullptr, bytes, q.size(0), q.size(1), (int32_t)q.size(2), (int32_t)q.size(3),
+                                 (int32_t)v.size(3), (float)scale, dtype_code(q.scalar_type()), stream_of(q)),
              "gcg_linear_attn_bwd");
+}
+
+void linear_bwd_all(const Tensor &d_o, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const OptTensor &initial,
+                    const OptTensor &lengths, const OptTensor &dfinal, double scale, const Tensor &dq, const Tensor &d_k, const Tensor &d_v,
+                    const Tensor &dinitial)
+{
+    for_entries(q, [&](int64_t at, int64_t n) {
+        const auto of = [&](const Tensor &t) { return t.narrow(0, at, n); };
+        linear_bwd_launch(of(d_o), of(q), of(k), of(v), log_decay, entries(initial, at, n), entries(lengths, at, n), entries(dfinal, at, n),
+                          scale, of(dq), of(d_k), of(d_v), dinitial.defined() ? of(dinitial) : Tensor());
+    }, [&] { linear_bwd_launch(d_o, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, d_k, d_v, dinitial); });
 }
 
 void check_do(const Tensor &d_o, const Tensor &v)
@@ -392,8 +422,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attn_bwd(const Tensor &d_o, co
                                                         need_dinitial);
         return {cut(pq, dk), cut(pkk, dk), cut(pvv, dv), cut_state(pi, dk, dv)};
     }
-    linear_bwd_launch(d_o, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, d_k, d_v,
-                      need_dinitial ? (float *)dinitial.data_ptr() : nullptr);
+    linear_bwd_all(d_o, q, k, v, log_decay, initial, lengths, dfinal, scale, dq, d_k, d_v, need_dinitial ? dinitial : Tensor());
     return {dq, d_k, d_v, dinitial};
 }
 
@@ -429,7 +458,7 @@ Tensor linear_attn_packed_bwd(const Tensor &d_o, const Tensor &features, int64_t
         d_v.copy_(pv);
         return df;
     }
-    linear_bwd_launch(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, dq, d_k, d_v, nullptr);
+    linear_bwd_all(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, dq, d_k, d_v, Tensor());
     return df;
 }
 
