@@ -1343,4 +1343,6 @@ def linear_attn_step(q, k, v, log_decay, state, scale: float):
                                       log_decay.data_ptr(), state.data_ptr(), *q.shape, v.shape[-1], scale, dtype_code(q.dtype),
                                       torch.cuda.current_stream().cuda_stream)
     check(rc, "gcg_linear_attn_step")
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return o

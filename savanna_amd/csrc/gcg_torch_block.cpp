@@ -479,6 +479,20 @@ Tensor linear_attn_step(const Tensor &q, const Tensor &k, const Tensor &v, const
     return o;
 }
 
+// The step as in-place operators of torch are: whatever saved the state for a backward pass finds it modified.  (An inference tensor
+// has no such count, and nothing can have saved it.)
+Tensor linear_attn_step_in_place(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, Tensor &state, double scale)
+{
+    static const auto f = op<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, Tensor &, double)>("gcg::linear_attn_step");
+    Tensor o;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        o = f.call(q, k, v, log_decay, state, scale);
+    }
+    if (!state.is_inference()) torch::autograd::impl::bump_version(state);
+    return o;
+}
+
 std::tuple<Tensor, Tensor> linear_attn_fwd_meta(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay,
                                                 const OptTensor &initial, const OptTensor &lengths, double, bool final)
 {
@@ -614,6 +628,11 @@ TORCH_LIBRARY_IMPL(gcg, CUDA, m)
     m.impl("linear_attn_packed_fwd", &linear_attn_packed_fwd);
     m.impl("linear_attn_packed_bwd", &linear_attn_packed_bwd);
     m.impl("linear_attn_step", &linear_attn_step);
+}
+
+TORCH_LIBRARY_IMPL(gcg, ADInplaceOrView, m)
+{
+    m.impl("linear_attn_step", &linear_attn_step_in_place);
 }
 
 TORCH_LIBRARY_IMPL(gcg, Meta, m)

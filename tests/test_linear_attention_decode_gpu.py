@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from savanna_amd.operators.linear_attention import linear_attention_step
+from savanna_amd.operators.linear_attention import linear_attention, linear_attention_step
 from test_linear_attention_gpu import DEV
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +26,24 @@ def test_thousands_of_tokens(gcg_lib):
     assert ((state.double() - S).abs() <= 2.0 ** -17 * A).all()
     want, terms = ((x[..., None] * y).sum(-2) * 0.5 for x, y in ((q[-1].double(), S), (q[-1].double().abs(), A)))
     assert ((o.double() - want).abs() <= 2.0 ** -16 * terms).all()
+
+
+def test_a_state_kept_for_a_backward_is_not_moved_on_unseen(gcg_lib):
+    """A recorded sequence that began from a state, the state then moved on: its backward would form dq from another state, and raises."""
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    q, k, v = (torch.randn(2, 5, 3, 16, generator=gen, device=DEV) for _ in range(3))
+    ld = torch.tensor([-0.1, -0.01, 0.0], device=DEV)
+    state = torch.randn(2, 3, 16, 16, generator=gen, device=DEV)
+    o = linear_attention(q.requires_grad_(True), k, v, ld, initial_state=state)
+    with torch.no_grad():
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state.clone())
+    torch.autograd.grad(o.sum(), q, retain_graph=True)
+    with torch.no_grad():
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o.sum(), q)
+    with torch.inference_mode():
+        prompt, state = linear_attention(q, k, v, ld, output_final_state=True)
+        linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
+    with torch.no_grad():
+        assert linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state).shape == (2, 3, 16)
