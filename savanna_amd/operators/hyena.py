@@ -396,23 +396,44 @@ def _featurized(entry, function, tensors, *rest, save_8bit=False):
 
 
 class _Recomputed8(torch.autograd.Function):
-    """``run(features)`` of which only the features' 8-bit checkpoint is kept: the backward runs it again on that."""
+    """``chain(features)`` of whose input only the 8-bit checkpoint is kept: the backward runs the module again on that, with the
+    parameters and buffers (``tensors``, by their ``names``) and the autocast state that the forward saw."""
 
     @staticmethod
-    def forward(ctx, run, features, *params):
-        ctx.run, ctx.dtype = run, features.dtype
-        ctx.save_for_backward(*_lib.pack8(features.contiguous()), *params)
-        return run(features)
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, chain, names, features, *tensors):
+        ctx.chain, ctx.names, ctx.dtype = chain, names, features.dtype
+        ctx.save_for_backward(*_lib.pack8(features.contiguous()), *tensors)
+        return chain(features)
 
     @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
     def backward(ctx, dz):
-        codes, scales, *params = ctx.saved_tensors
+        codes, scales, *tensors = ctx.saved_tensors
         features = _lib.unpack8(codes, scales, ctx.dtype).requires_grad_(True)
+        tensors = [t.detach().requires_grad_(need) for t, need in zip(tensors, ctx.needs_input_grad[3:])]
         with torch.enable_grad():
-            z = ctx.run(features)
-        inputs = [features] + [p for p in params if p.requires_grad]
-        grads = iter(torch.autograd.grad(z, inputs, dz, allow_unused=True))
-        return None, next(grads), *(next(grads) if p.requires_grad else None for p in params)
+            z = torch.func.functional_call(ctx.chain, dict(zip(ctx.names, tensors)), (features,))
+        grads = iter(torch.autograd.grad(z, [features] + [t for t in tensors if t.requires_grad], dz, allow_unused=True))
+        return None, None, next(grads), *(next(grads) if t.requires_grad else None for t in tensors)
+
+
+def _recomputed8(chain: nn.Module, features: torch.Tensor) -> torch.Tensor:
+    named = dict(chain.named_parameters())
+    named.update(chain.named_buffers())
+    return _Recomputed8.apply(chain, tuple(named), features, *named.values())
+
+
+class _Chain(nn.Module):
+    """A mixer's featurizer, then its operator on the result where it lies: two kernels each way."""
+
+    def __init__(self, conv: CausalDepthwiseConv1d, operator: _CgcgOperatorBase, interleaved: bool):
+        super().__init__()
+        self.conv, self.operator, self.interleaved = conv, operator, interleaved
+
+    def forward(self, features: torch.Tensor) -> torch.Tensor:
+        return self.operator.forward_features(self.conv.forward_bld(features, feeds_operator=True), from_featurizer=True,
+                                              interleaved=self.interleaved)
 
 
 class HyenaMixer(nn.Module):
@@ -519,6 +540,6 @@ class HyenaMixer(nn.Module):
         if self._fusable(features, h.shape[-1]):
             return self._fused_short(features, h, planar)
         # otherwise the featurizer kernel, then the operator on its output where it lies (two kernels each way)
-        run = lambda f: op.forward_features(conv.forward_bld(f, feeds_operator=True), from_featurizer=True,  # noqa: E731
-                                            interleaved=not planar)
-        return _Recomputed8.apply(run, features, *self.parameters()) if save_8bit else run(features)
+        if save_8bit:
+            return _recomputed8(_Chain(conv, op, not planar), features)
+        return op.forward_features(conv.forward_bld(features, feeds_operator=True), from_featurizer=True, interleaved=not planar)

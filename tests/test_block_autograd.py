@@ -36,3 +36,73 @@ def test_a_step_on_inference_tensors(gcg_lib):
         assert token(state).is_inference()
     with torch.no_grad():
         assert token(state).shape == (2, 3, 8)
+
+
+# ---- a module run again in the backward on its input's checkpoint -------------------------------------------
+
+class Scaled(torch.nn.Module):
+    """y = x w s, with a parameter that nothing uses."""
+
+    def __init__(self):
+        super().__init__()
+        self.w = torch.nn.Parameter(torch.tensor([1.0, 2.0]))
+        self.idle = torch.nn.Parameter(torch.zeros(2))
+        self.register_buffer("s", torch.tensor([3.0, 3.0]))
+
+    def forward(self, x):
+        return x * self.w * self.s
+
+
+class Holder(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.inner = Scaled()
+
+    def forward(self, x):
+        from savanna_amd.operators import hyena
+        return hyena._recomputed8(self.inner, x)
+
+
+@pytest.fixture
+def exact_checkpoint(monkeypatch):
+    """The checkpoint as a copy, so that gradients have values to compare with."""
+    from savanna_amd import _lib
+    monkeypatch.setattr(_lib, "pack8", lambda x: (x.clone(), torch.ones(1)))
+    monkeypatch.setattr(_lib, "unpack8", lambda codes, scales, dtype: codes.clone())
+
+
+def test_recomputation_sees_the_parameters_of_its_forward(exact_checkpoint):
+    """Substituted by functional_call, parameters and buffers alike: gradients are theirs, at their values."""
+    m = Holder()
+    x = torch.tensor([10.0, 20.0], requires_grad=True)
+    w = torch.tensor([5.0, 7.0], requires_grad=True)
+    y = torch.func.functional_call(m, {"inner.w": w, "inner.s": torch.tensor([1.0, 2.0])}, (x,))
+    dx, dw = torch.autograd.grad(y.sum(), [x, w])
+    assert torch.equal(dx, torch.tensor([5.0, 14.0])) and torch.equal(dw, torch.tensor([10.0, 40.0]))
+    y = m(x)
+    dx, dw, idle = torch.autograd.grad(y.sum(), [x, m.inner.w, m.inner.idle], allow_unused=True)
+    assert torch.equal(dx, torch.tensor([3.0, 6.0])) and torch.equal(dw, torch.tensor([30.0, 60.0])) and idle is None
+    m.inner.w.requires_grad_(False)
+    m(x).sum().backward()
+    assert torch.equal(x.grad, torch.tensor([3.0, 6.0])) and m.inner.w.grad is None
+
+
+def test_recomputation_under_saved_tensor_hooks(exact_checkpoint):
+    """Hooks hand back other tensors than were saved (offloading, checkpointing): the gradients are the same."""
+    m, x = Holder(), torch.tensor([10.0, 20.0], requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t):
+        y = m(x)
+    dx, dw = torch.autograd.grad(y.sum(), [x, m.inner.w])
+    assert torch.equal(dx, torch.tensor([3.0, 6.0])) and torch.equal(dw, torch.tensor([30.0, 60.0]))
+    y = torch.utils.checkpoint.checkpoint(m, x, use_reentrant=False)
+    dx, dw = torch.autograd.grad(y.sum(), [x, m.inner.w])
+    assert torch.equal(dx, torch.tensor([3.0, 6.0])) and torch.equal(dw, torch.tensor([30.0, 60.0]))
+
+
+def test_recomputation_notices_changed_parameters(exact_checkpoint):
+    m, x = Holder(), torch.tensor([10.0, 20.0], requires_grad=True)
+    y = m(x)
+    with torch.no_grad():
+        m.inner.w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
