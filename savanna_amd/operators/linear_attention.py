@@ -106,7 +106,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
 class LinearAttention(nn.Module):
     """The mixer on projected features (bs, L, 3 * hidden_size), laid out "(p h d)" with p = q, k, v -> (bs, L, hidden_size).
 
-    ``log_decay``: a buffer, rates spaced over the heads' logarithm from a memory of ``shortest`` tokens to one of ``longest``.
+    ``log_decay``: a buffer, rates spaced over the heads' logarithm from a memory of ``shortest`` tokens to one of ``longest``; it stays
+    float32 when the module is cast.
     ``prefill`` also returns the state after a prompt (of ``lengths``, if its entries differ), ``step`` takes one token's
     features (bs, 3 * hidden_size) and moves that state on in place."""
 
@@ -116,8 +117,16 @@ class LinearAttention(nn.Module):
         assert hidden_size % num_heads == 0
         self.hidden_size, self.num_heads, self.head_dim = hidden_size, num_heads, hidden_size // num_heads
         self.save_8bit = save_8bit
-        spread = torch.linspace(0, 1, num_heads, device=device)
+        spread = torch.linspace(0, 1, num_heads, dtype=torch.float32, device=device)
         self.register_buffer("log_decay", -1.0 / (shortest * (longest / shortest) ** spread))
+
+    def _apply(self, fn, recurse=True):
+        """Moves the decays with the module and leaves them in fp32 when it is cast: rounded to 16 bits they would be others."""
+        decay = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != decay.dtype:
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
 
     def _split(self, features: torch.Tensor):
         return features.unflatten(-1, (3, self.num_heads, self.head_dim)).unbind(-3)
