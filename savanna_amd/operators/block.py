@@ -18,13 +18,14 @@ from .norm import LayerNorm
 
 
 class MixerBlock(nn.Module):
-    """x: (b, l, hidden_size).  ``mixer``: a HyenaMixer or a LinearAttention of that width; ``save_8bit`` sets the mixer's too."""
+    """x: (b, l, hidden_size).  ``mixer``: a HyenaMixer or a LinearAttention of that width; ``save_8bit`` sets the mixer's too
+    (a mixer that keeps its features in 8 bits by itself goes on doing so without)."""
 
     def __init__(self, hidden_size: int, mixer: Union[HyenaMixer, LinearAttention], eps: float = 1e-5, save_8bit: bool = False,
                  dtype=torch.float32, device=None):
         super().__init__()
         self.mixer = mixer
-        mixer.save_8bit = save_8bit
+        mixer.save_8bit = mixer.save_8bit or save_8bit
         self.norm = LayerNorm(hidden_size, eps, save_8bit=save_8bit, dtype=dtype, device=device)
         self.projection = nn.Linear(hidden_size, 3 * hidden_size, bias=False, dtype=dtype, device=device)
         self.out = nn.Linear(hidden_size, hidden_size, bias=False, dtype=dtype, device=device)

@@ -32,3 +32,12 @@ def test_decays_of_a_model_made_in_another_default_type(gcg_lib):
             assert LinearAttention(128, 4).log_decay.dtype == torch.float32
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+@pytest.mark.parametrize("mixers,block", [(False, False), (False, True), (True, False), (True, True)])
+def test_a_block_does_not_switch_a_mixers_checkpoint_off(gcg_lib, mixers, block):
+    from savanna_amd.operators.hyena import HyenaMixer, HyenaSEOperator
+
+    for mixer in (LinearAttention(128, 4, save_8bit=mixers), HyenaMixer(HyenaSEOperator(128, 8), save_8bit=mixers)):
+        layer = MixerBlock(128, mixer, save_8bit=block)
+        assert layer.mixer.save_8bit == (mixers or block) and layer.norm.save_8bit == block
