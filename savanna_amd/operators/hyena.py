@@ -454,6 +454,8 @@ class HyenaMixer(nn.Module):
     gradients are those at its values.  The one-kernel routes read it as they read the features; the others run their
     forward again on it, and so keep no featurized tensor either."""
 
+    save_8bit = False           # of modules pickled before there was one
+
     def __init__(self, operator: _CgcgOperatorBase, short_conv_L: int = 3, dtype=torch.float32, device=None,
                  fuse_short: bool = True, fuse_medium: bool = True, interleave_projections: bool = True, save_8bit: bool = False):
         super().__init__()

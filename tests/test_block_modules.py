@@ -41,3 +41,14 @@ def test_a_block_does_not_switch_a_mixers_checkpoint_off(gcg_lib, mixers, block)
     for mixer in (LinearAttention(128, 4, save_8bit=mixers), HyenaMixer(HyenaSEOperator(128, 8), save_8bit=mixers)):
         layer = MixerBlock(128, mixer, save_8bit=block)
         assert layer.mixer.save_8bit == (mixers or block) and layer.norm.save_8bit == block
+
+
+def test_mixers_pickled_before_there_was_a_checkpoint(gcg_lib):
+    """Such a module lacks the switch and goes on as it did."""
+    from savanna_amd.operators.hyena import HyenaMixer, HyenaSEOperator
+
+    mixer = HyenaMixer(HyenaSEOperator(128, 8))
+    del mixer.__dict__["save_8bit"]
+    assert not mixer._save_8bit()
+    mixer.save_8bit = True
+    assert mixer._save_8bit()
