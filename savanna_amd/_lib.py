@@ -227,13 +227,29 @@ class _on_device:
         return False
 
 
+def forward_mode() -> bool:
+    """Whether forward-mode differentiation is on: inputs may carry tangents, which the Python autograd functions refuse."""
+    return forward_ad._current_level >= 0
+
+
+def refuse_tangents(what: str, *args) -> None:
+    """For calls that pass the autograd functions by: a tangent would be lost there without a word.  (Inside such a function's forward
+    torch has switched forward mode off and refuses by itself.)"""
+    if forward_mode() and torch._C._is_fwd_grad_enabled() and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
+
+
 def _run(op, *args):
     """A torch.ops.gcg forward operator that writes none of its arguments.  With gradient recording off -- inference,
     and inside the autograd functions of the layers above -- the autograd formula these operators have, a Python
     function each (_ops.py), would only hand the call on; it is passed by then.  1 x 2048 x 256 fp32 forward of 7 taps,
     a call whose kernel takes 4.5 us: 19.0 us with it, 15.4 without.  Not under torch.compile or a function transform,
     which have layers of their own; the backward operators have no formula and gain nothing (9.8 -> 10.5 us)."""
-    if torch.is_grad_enabled() or torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active():
+    if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active():
+        return op(*args)
+    refuse_tangents(str(op), *args)
+    if torch.is_grad_enabled():
         return op(*args)
     with torch._C._AutoDispatchBelowAutograd():
         return op(*args)
@@ -1329,6 +1345,8 @@ def linear_attn_packed_bwd(do, features, heads: int, log_decay, scale: float):
 def linear_attn_step(q, k, v, log_decay, state, scale: float):
     """o (bs, H, dv) of one token, q, k (bs, H, dk), v (bs, H, dv); state (bs, H, dk, dv) fp32 moves on in place."""
     _require_gpu(q)
+    if not torch.compiler.is_compiling():
+        refuse_tangents("linear_attn_step", q, k, v, log_decay, state)
     if TORCH_OPS:
         return torch.ops.gcg.linear_attn_step(q, k, v, log_decay, state, scale)
     lib = load()

@@ -70,7 +70,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     the one after its last row."""
     _constant(log_decay)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() and not _lib.forward_mode():
         o, final = _lib.linear_attn_fwd(q, k, v, log_decay, initial_state, lengths, scale, output_final_state)
         return (o, final) if output_final_state else o
     if _lib.native_nodes(q) and v.numel() > 0:
@@ -87,7 +87,7 @@ def linear_attention_features(features: torch.Tensor, num_heads: int, log_decay:
     _constant(log_decay)
     features = features if features.is_contiguous() else features.contiguous()
     scale = (features.shape[-1] // (3 * num_heads)) ** -0.5 if scale is None else scale
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() and not _lib.forward_mode():
         return _lib.linear_attn_packed_fwd(features, num_heads, log_decay, scale)
     if _lib.native_nodes(features):
         return torch.ops.gcg.linear_attn_packed(features, num_heads, log_decay, scale, save_8bit)

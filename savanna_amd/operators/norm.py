@@ -35,7 +35,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     x: float32, bfloat16 or float16; weight and bias: of x's dtype, or float32 with 16-bit x.  ``save_8bit``: the backward
     pass works on x's 8-bit checkpoint, which is all that is kept of x (1.03 bytes an element)."""
     x = x if x.is_contiguous() else x.contiguous()
-    if not torch.is_grad_enabled():
+    if not torch.is_grad_enabled() and not _lib.forward_mode():
         return _lib.layer_norm_fwd(x, weight, bias, eps, stats=False)[0]
     if _lib.native_nodes(x):
         return torch.ops.gcg.layer_norm(x, weight, bias, eps, save_8bit)

@@ -106,3 +106,31 @@ def test_recomputation_notices_changed_parameters(exact_checkpoint):
         m.inner.w.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+# ---- forward mode ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused_not_dropped(gcg_lib, grad):
+    """None of the operators has a forward-mode derivative: inputs with tangents raise, with gradients recorded or not, and inputs without
+    pass inside a level too."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad
+
+    from savanna_amd import _lib
+    from savanna_amd.operators.linear_attention import linear_attention, linear_attention_features, linear_attention_step
+    from savanna_amd.operators.norm import layer_norm
+
+    with FakeTensorMode(), torch.set_grad_enabled(grad), forward_ad.dual_level():
+        x, q, f = (torch.empty(*s, device="cuda") for s in ((4, 64), (1, 5, 2, 8), (1, 5, 48)))
+        ld, state = torch.empty(2, device="cuda"), torch.empty(1, 2, 8, 8, device="cuda")
+        t = q[:, 0]
+        calls = [(lambda x: layer_norm(x), x), (lambda x: layer_norm(x, save_8bit=True), x), (lambda w: layer_norm(x, w), x[0]),
+                 (lambda q: linear_attention(q, q, q, ld), q), (lambda s: linear_attention(q, q, q, ld, initial_state=s), state),
+                 (lambda f: linear_attention_features(f, 2, ld), f), (lambda t: linear_attention_step(t, t, t, ld, state), t),
+                 (lambda s: linear_attention_step(t, t, t, ld, s), state), (lambda x: _lib.layer_norm_fwd(x, None, None, 1e-5), x),
+                 (lambda q: _lib.linear_attn_fwd(q, q, q, ld, None, None, 1.0, False), q)]
+        for call, at in calls:
+            call(at)
+            with pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(at, torch.empty_like(at)))
