@@ -140,7 +140,12 @@ def _register_autograd():
         return dx, dw if w is not None else None, db if b is not None else None, None, None
     reg("gcg::layer_norm_fwd", norm, setup_context=norm_setup)
 
+    def constant(log_decay):                 # as the C++ nodes and the Python layer have it
+        if log_decay.requires_grad:
+            raise RuntimeError("gcg: log_decay is a constant of the heads and has no gradient; pass log_decay.detach()")
+
     def linear_setup(ctx, inputs, output):   # linear_attn_fwd(q, k, v, log_decay, initial, lengths, scale, final) -> o, state
+        constant(inputs[3])
         ctx.save_for_backward(*inputs[:6])
         ctx.scale, ctx.final = inputs[6:]
         ctx.set_materialize_grads(False)
@@ -157,7 +162,11 @@ def _register_autograd():
     def linear_packed(ctx, do):              # linear_attn_packed_fwd(features, H, log_decay, scale)
         features, log_decay = ctx.saved_tensors
         return ops.linear_attn_packed_bwd(do, features, ctx.rest[1], log_decay, ctx.rest[3]), None, None, None
-    reg("gcg::linear_attn_packed_fwd", linear_packed, setup_context=save(0, 2))
+
+    def packed_setup(ctx, inputs, output):
+        constant(inputs[2])
+        save(0, 2)(ctx, inputs, output)
+    reg("gcg::linear_attn_packed_fwd", linear_packed, setup_context=packed_setup)
 
     def refuse(name, hint):
         def backward(ctx, *grads):

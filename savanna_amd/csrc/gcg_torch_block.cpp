@@ -583,13 +583,22 @@ struct PackedLinearAttnNode : torch::autograd::Function<PackedLinearAttnNode> {
     }
 };
 
+// the decays' gradient is none of the operator's: asked for, it is refused rather than left out
+void check_constant(const Tensor &log_decay)
+{
+    TORCH_CHECK(!(at::GradMode::is_enabled() && log_decay.requires_grad()),
+                "gcg: log_decay is a constant of the heads and has no gradient; pass log_decay.detach()");
+}
+
 std::vector<Tensor> linear_attn(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, const OptTensor &initial,
                                 const OptTensor &lengths, double scale, bool final)
 {
+    check_constant(log_decay);
     return LinearAttnNode::apply(q, k, v, log_decay, initial, lengths, scale, final);
 }
 Tensor linear_attn_packed(const Tensor &features, int64_t H, const Tensor &log_decay, double scale, bool save_8bit)
 {
+    check_constant(log_decay);
     return PackedLinearAttnNode::apply(features, H, log_decay, scale, save_8bit);
 }
 

@@ -134,3 +134,23 @@ def test_tangents_are_refused_not_dropped(gcg_lib, grad):
             call(at)
             with pytest.raises(NotImplementedError):
                 call(forward_ad.make_dual(at, torch.empty_like(at)))
+
+
+# ---- the decays -------------------------------------------------------------------------------------------------
+
+def test_operators_refuse_a_gradient_of_the_decays(gcg_lib):
+    """The registered operators as the Python layer does, and only where gradients are recorded."""
+    ops = torch.ops.gcg
+    ld = meta(3, dtype=torch.float32).requires_grad_(True)
+    q, v, features = meta(2, 50, 3, 16), meta(2, 50, 3, 8), meta(2, 50, 144)
+    calls = [lambda ld: ops.linear_attn(q, q, v, ld, None, None, 0.5, True)[0], lambda ld: ops.linear_attn_fwd(q, q, v, ld, None, None, 0.5, False)[0],
+             lambda ld: ops.linear_attn_packed(features, 3, ld, 0.5, False), lambda ld: ops.linear_attn_packed_fwd(features, 3, ld, 0.5)]
+    for q_grad in (False, True):
+        q.requires_grad_(q_grad)
+        features.requires_grad_(q_grad)
+        for call in calls:
+            with pytest.raises(RuntimeError, match="constant of the heads"):
+                call(ld)
+            assert call(ld.detach()).requires_grad == q_grad
+            with torch.no_grad():
+                assert not call(ld).requires_grad
