@@ -1125,11 +1125,11 @@ def layer_norm_fwd(x, w, b, eps: float, save_8bit: bool = False, stats: bool = T
     return y, kept, codes, scales
 
 
-def layer_norm_bwd(dy, x, codes, scales, stats, w, b):
-    """(dx, dw, db); x, or its 8-bit checkpoint and None in x's place.  w and b say which gradients are wanted."""
+def layer_norm_bwd(dy, x, codes, scales, stats, w, b, need_dw: bool = True, need_db: bool = True):
+    """(dx, dw, db); x, or its 8-bit checkpoint and None in x's place.  No dw without w or ``need_dw``, and db alike."""
     _require_gpu(dy)
     if TORCH_OPS:
-        return torch.ops.gcg.layer_norm_bwd(dy, x, codes, scales, stats, w, b)
+        return torch.ops.gcg.layer_norm_bwd(dy, x, codes, scales, stats, w, b, need_dw, need_db)
     lib = load()
     code = _norm_code(dy, w, b)
     if (codes is None) != (scales is None) or (x is None) == (codes is None):
@@ -1144,15 +1144,15 @@ def layer_norm_bwd(dy, x, codes, scales, stats, w, b):
     D = dy.shape[-1]
     rows = dy.numel() // D
     dx = torch.empty_like(dy)
-    dw = torch.empty_like(w) if w is not None else None
-    db = torch.empty_like(b) if b is not None else None
+    dw = torch.empty_like(w) if w is not None and need_dw else None
+    db = torch.empty_like(b) if b is not None and need_db else None
     if rows == 0:
         return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
-    nbytes = lib.gcg_layer_norm_bwd_workspace_bytes(rows, D, code)
+    nbytes = lib.gcg_layer_norm_bwd_workspace_bytes(rows, D, code) if dw is not None or db is not None else 0
     with _on_device(dy.device):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
         rc = lib.gcg_layer_norm_bwd(dy.data_ptr(), _ptr(x), _ptr(codes), _ptr(scales), stats.data_ptr(), _ptr(w), dx.data_ptr(),
-                                    _ptr(dw), _ptr(db), ws.data_ptr(), nbytes, rows, D, code,
+                                    _ptr(dw), _ptr(db), _ptr(ws), nbytes, rows, D, code,
                                     torch.cuda.current_stream().cuda_stream)
     check(rc, "gcg_layer_norm_bwd")
     return dx, dw, db

@@ -135,9 +135,9 @@ def _register_autograd():
         ctx.save_for_backward(*((None, codes, scales) if ctx.save_8bit else (x, None, None)), stats, w, b)
 
     def norm(ctx, dy, *_):
-        w, b = ctx.saved_tensors[4:]
-        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), *ctx.saved_tensors)
-        return dx, dw if w is not None else None, db if b is not None else None, None, None
+        _, need_dw, need_db = ctx.needs_input_grad[:3]
+        dx, dw, db = ops.layer_norm_bwd(dy.contiguous(), *ctx.saved_tensors, need_dw, need_db)
+        return dx, dw if need_dw else None, db if need_db else None, None, None
     reg("gcg::layer_norm_fwd", norm, setup_context=norm_setup)
 
     def constant(log_decay):                 # as the C++ nodes and the Python layer have it

@@ -173,9 +173,11 @@ void check_norm_bwd(const Tensor &dy, const OptTensor &x, const OptTensor &codes
                 "gcg: stats must be the forward's");
 }
 
-// (dx, dw, db); dw and db are empty without w and b
+Tensor norm_gradient(const OptTensor &p, bool need, const Tensor &dy) { return given(p) && need ? at::empty_like(*p) : at::empty({0}, dy.options()); }
+
+// (dx, dw, db); dw and db are empty without w and b, or where they are not needed
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor &dy, const OptTensor &x, const OptTensor &codes, const OptTensor &scales,
-                                                  const Tensor &stats, const OptTensor &w, const OptTensor &b)
+                                                  const Tensor &stats, const OptTensor &w, const OptTensor &b, bool need_dw, bool need_db)
 {
     require_gpu(dy, "dy");
     check_norm_bwd(dy, x, codes, scales, stats);
@@ -183,18 +185,19 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor &dy, const OptTen
     DeviceGuard guard(dy.device());
     const int64_t D = dy.size(-1), rows = dy.numel() / D;
     Tensor dx = at::empty_like(dy);
-    Tensor dw = given(w) ? at::empty_like(*w) : at::empty({0}, dy.options());
-    Tensor db = given(b) ? at::empty_like(*b) : at::empty({0}, dy.options());
+    need_dw = need_dw && given(w);
+    need_db = need_db && given(b);
+    Tensor dw = norm_gradient(w, need_dw, dy), db = norm_gradient(b, need_db, dy);
     if (rows == 0) return {dx, dw.zero_(), db.zero_()};
     Tensor ws;
     size_t bytes = 0;
-    if (given(w) || given(b)) {
+    if (need_dw || need_db) {
         bytes = gcg_layer_norm_bwd_workspace_bytes(rows, (int32_t)std::min<int64_t>(D, INT32_MAX), code);
         ws = workspace(bytes, dy, "gcg_layer_norm_bwd_workspace_bytes");
     }
     check_rc(gcg_layer_norm_bwd(dy.data_ptr(), ptr(x), (const int8_t *)ptr(codes), (const float *)ptr(scales),
-                                (const float *)stats.data_ptr(), ptr(w), dx.data_ptr(), given(w) ? dw.data_ptr() : nullptr,
-                                given(b) ? db.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, rows, (int32_t)D, code,
+                                (const float *)stats.data_ptr(), ptr(w), dx.data_ptr(), need_dw ? dw.data_ptr() : nullptr,
+                                need_db ? db.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, rows, (int32_t)D, code,
                                 stream_of(dy)),
              "gcg_layer_norm_bwd");
     return {dx, dw, db};
@@ -213,12 +216,11 @@ Tensor layer_norm_infer_meta(const Tensor &x, const OptTensor &w, const OptTenso
 }
 std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd_meta(const Tensor &dy, const OptTensor &x, const OptTensor &codes,
                                                        const OptTensor &scales, const Tensor &stats, const OptTensor &w,
-                                                       const OptTensor &b)
+                                                       const OptTensor &b, bool need_dw, bool need_db)
 {
     check_norm_bwd(dy, x, codes, scales, stats);
     (void)norm_code(dy, w, b);
-    return {at::empty_like(dy), given(w) ? at::empty_like(*w) : at::empty({0}, dy.options()),
-            given(b) ? at::empty_like(*b) : at::empty({0}, dy.options())};
+    return {at::empty_like(dy), norm_gradient(w, need_dw, dy), norm_gradient(b, need_db, dy)};
 }
 
 Tensor or_empty(const OptTensor &t) { return given(t) ? *t : Tensor(); }
@@ -233,16 +235,19 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
         auto [y, stats, codes, scales] = f.call(x, w, b, eps, save_8bit);
         if (save_8bit) ctx->save_for_backward({Tensor(), codes, scales, stats, or_empty(w), or_empty(b)});
         else ctx->save_for_backward({x, Tensor(), Tensor(), stats, or_empty(w), or_empty(b)});
+        ctx->saved_data["dw"] = given(w) && w->requires_grad();
+        ctx->saved_data["db"] = given(b) && b->requires_grad();
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list dy)
     {
         static const auto f = op<std::tuple<Tensor, Tensor, Tensor>(const Tensor &, const OptTensor &, const OptTensor &,
                                                                    const OptTensor &, const Tensor &, const OptTensor &,
-                                                                   const OptTensor &)>("gcg::layer_norm_bwd");
+                                                                   const OptTensor &, bool, bool)>("gcg::layer_norm_bwd");
         const variable_list s = ctx->get_saved_variables();
-        auto [dx, dw, db] = f.call(dy[0].contiguous(), opt(s[0]), opt(s[1]), opt(s[2]), s[3], opt(s[4]), opt(s[5]));
-        return {dx, s[4].defined() ? dw : Tensor(), s[5].defined() ? db : Tensor(), Tensor(), Tensor()};
+        const bool need_dw = ctx->saved_data["dw"].toBool(), need_db = ctx->saved_data["db"].toBool();
+        auto [dx, dw, db] = f.call(dy[0].contiguous(), opt(s[0]), opt(s[1]), opt(s[2]), s[3], opt(s[4]), opt(s[5]), need_dw, need_db);
+        return {dx, need_dw ? dw : Tensor(), need_db ? db : Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -610,8 +615,8 @@ TORCH_LIBRARY_FRAGMENT(gcg, m)
     m.def("unpack8(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
     m.def("layer_norm_fwd(Tensor x, Tensor? w, Tensor? b, float eps, bool save_8bit) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("layer_norm_infer(Tensor x, Tensor? w, Tensor? b, float eps) -> Tensor");
-    m.def("layer_norm_bwd(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor stats, Tensor? w, Tensor? b)"
-          " -> (Tensor, Tensor, Tensor)");
+    m.def("layer_norm_bwd(Tensor dy, Tensor? x, Tensor? codes, Tensor? scales, Tensor stats, Tensor? w, Tensor? b,"
+          " bool need_dw=True, bool need_db=True) -> (Tensor, Tensor, Tensor)");
     m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, bool save_8bit) -> Tensor", &layer_norm);
     m.def("linear_attn_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? initial, Tensor? lengths, float scale, bool final)"
           " -> (Tensor, Tensor)");

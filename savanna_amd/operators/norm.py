@@ -23,9 +23,9 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        w, b = ctx.saved_tensors[4:]
-        dx, dw, db = _lib.layer_norm_bwd(dy if dy.is_contiguous() else dy.contiguous(), *ctx.saved_tensors)
-        return dx, dw if w is not None else None, db if b is not None else None, None, None
+        _, need_dw, need_db = ctx.needs_input_grad[:3]
+        dx, dw, db = _lib.layer_norm_bwd(dy if dy.is_contiguous() else dy.contiguous(), *ctx.saved_tensors, need_dw, need_db)
+        return dx, dw if need_dw else None, db if need_db else None, None, None
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,

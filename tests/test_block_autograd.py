@@ -154,3 +154,12 @@ def test_operators_refuse_a_gradient_of_the_decays(gcg_lib):
             assert call(ld.detach()).requires_grad == q_grad
             with torch.no_grad():
                 assert not call(ld).requires_grad
+
+
+# ---- the norm's gradients ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("need_dw,need_db", [(True, True), (True, False), (False, True), (False, False)])
+def test_the_norms_backward_forms_what_is_needed(gcg_lib, need_dw, need_db):
+    x, w, stats = meta(5, 96), meta(96), meta(5, 2, dtype=torch.float32)
+    dx, dw, db = torch.ops.gcg.layer_norm_bwd(x, x, None, None, stats, w, w, need_dw, need_db)
+    assert dx.shape == x.shape and dw.numel() == 96 * need_dw and db.numel() == 96 * need_db
