@@ -90,6 +90,8 @@ int norm_code(const Tensor &x, const OptTensor &w, const OptTensor &b)
 {
     check_rows(x);
     TORCH_CHECK(x.size(-1) > 0, "gcg: layer norm over an empty dimension");
+    TORCH_CHECK(x.size(-1) <= GCG_NORM_MAX_WIDTH, "gcg: layer norm over ", x.size(-1), " elements; at most ", (int)GCG_NORM_MAX_WIDTH,
+                " are supported");
     const int code = dtype_code(x.scalar_type());
     bool wide = false;
     for (const OptTensor *p : {&w, &b}) {
@@ -127,7 +129,6 @@ void norm_fwd_launch(const Tensor &x, const OptTensor &w, const OptTensor &b, do
 {
     if (x.numel() == 0) return;
     const int64_t D = x.size(-1);
-    TORCH_CHECK(D <= GCG_NORM_MAX_WIDTH, "gcg: layer norm over ", D, " elements; at most ", (int)GCG_NORM_MAX_WIDTH, " are supported");
     check_rc(gcg_layer_norm_fwd(x.data_ptr(), ptr(w), ptr(b), y.data_ptr(), stats, codes, scales, x.numel() / D, (int32_t)D, (float)eps,
                                 code, stream_of(x)),
              "gcg_layer_norm_fwd");
@@ -192,7 +193,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor &dy, const OptTen
     Tensor ws;
     size_t bytes = 0;
     if (need_dw || need_db) {
-        bytes = gcg_layer_norm_bwd_workspace_bytes(rows, (int32_t)std::min<int64_t>(D, INT32_MAX), code);
+        bytes = gcg_layer_norm_bwd_workspace_bytes(rows, (int32_t)D, code);
         ws = workspace(bytes, dy, "gcg_layer_norm_bwd_workspace_bytes");
     }
     check_rc(gcg_layer_norm_bwd(dy.data_ptr(), ptr(x), (const int8_t *)ptr(codes), (const float *)ptr(scales),

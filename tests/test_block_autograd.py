@@ -163,3 +163,13 @@ def test_the_norms_backward_forms_what_is_needed(gcg_lib, need_dw, need_db):
     x, w, stats = meta(5, 96), meta(96), meta(5, 2, dtype=torch.float32)
     dx, dw, db = torch.ops.gcg.layer_norm_bwd(x, x, None, None, stats, w, w, need_dw, need_db)
     assert dx.shape == x.shape and dw.numel() == 96 * need_dw and db.numel() == 96 * need_db
+
+
+@pytest.mark.parametrize("D", [16385, 2 ** 32 + 64])
+def test_rows_wider_than_the_norm_takes(gcg_lib, D):
+    """Refused by every form, traced ones too; a width is not taken modulo 2^32."""
+    x, w, stats = meta(2, D), meta(D), meta(2, 2, dtype=torch.float32)
+    for call in (lambda: torch.ops.gcg.layer_norm_fwd(x, w, None, 1e-5, False), lambda: torch.ops.gcg.layer_norm_infer(x, None, None, 1e-5),
+                 lambda: torch.ops.gcg.layer_norm_bwd(x, x, None, None, stats, None, None)):
+        with pytest.raises(RuntimeError, match="at most 16384"):
+            call()
