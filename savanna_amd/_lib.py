@@ -1334,7 +1334,8 @@ def linear_attn_packed_bwd(do, features, heads: int, log_decay, scale: float):
     q, k, v = _split_features(features, heads)
     _check_linear(q, k, v, log_decay, 4)
     df = torch.empty_like(features)
-    if df.numel() and _to_whole(q, q.shape[-1]):
+    # (the kernels write no rows further apart than this; the forward copies such an input)
+    if df.numel() and (_to_whole(q, q.shape[-1]) or features.shape[2] > LINEAR_MAX_TIME_STRIDE):
         for part, g in zip(_split_features(df, heads), linear_attn_bwd(do, q, k, v, log_decay, None, None, None, scale, False)):
             part.copy_(g)
     elif df.numel():

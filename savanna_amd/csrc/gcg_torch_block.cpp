@@ -457,7 +457,8 @@ Tensor linear_attn_packed_bwd(const Tensor &d_o, const Tensor &features, int64_t
     Tensor df = at::empty_like(features);
     if (df.numel() == 0) return df;
     const auto [dq, d_k, d_v] = split_features(df, H);
-    if (odd_heads(q, v)) {
+    // (the kernels write no rows further apart; the forward copies such an input)
+    if (odd_heads(q, v) || features.size(2) > GCG_LINEAR_MAX_TIME_STRIDE) {
         const auto [pq, pk, pv, pi] = linear_attn_bwd(d_o, q, k, v, log_decay, OptTensor(), OptTensor(), OptTensor(), scale, false);
         dq.copy_(pq);
         d_k.copy_(pk);

@@ -173,3 +173,11 @@ def test_rows_wider_than_the_norm_takes(gcg_lib, D):
                  lambda: torch.ops.gcg.layer_norm_bwd(x, x, None, None, stats, None, None)):
         with pytest.raises(RuntimeError, match="at most 16384"):
             call()
+
+
+def test_more_heads_than_an_int_holds(gcg_lib):
+    """Refused with its number, not taken modulo 2^32."""
+    H = 2 ** 32 + 1
+    q, ld = torch.empty(1, 1, H, 8, device="meta"), torch.empty(H, device="meta")
+    with pytest.raises(RuntimeError, match="heads; at most"):
+        torch.ops.gcg.linear_attn_fwd(q, q, q, ld, None, None, 1.0, False)

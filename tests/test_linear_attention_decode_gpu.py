@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from savanna_amd import _lib
 from savanna_amd.operators.linear_attention import linear_attention, linear_attention_step
 from test_linear_attention_gpu import DEV
 
@@ -47,3 +48,19 @@ def test_a_state_kept_for_a_backward_is_not_moved_on_unseen(gcg_lib):
         linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state)
     with torch.no_grad():
         assert linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, state).shape == (2, 3, 16)
+
+
+@pytest.mark.skipif(not _lib.TORCH_OPS, reason="the ctypes binding is not traced")
+def test_a_step_traced(gcg_lib):
+    """Through torch.compile the step gives the same bits and moves the same state on, and counts as a change of it."""
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    q, k, v = (torch.randn(2, 3, 16, generator=gen, device=DEV) for _ in range(3))
+    ld = torch.tensor([-0.1, -0.01, 0.0], device=DEV)
+    state = torch.randn(2, 3, 16, 16, generator=gen, device=DEV)
+    traced = torch.compile(lambda q, k, v, s: linear_attention_step(q, k, v, ld, s) * 2, fullgraph=True, backend="aot_eager")
+    ours = state.clone()
+    with torch.no_grad():
+        for _ in range(3):
+            version = state._version
+            assert torch.equal(traced(q, k, v, state), linear_attention_step(q, k, v, ld, ours) * 2) and torch.equal(state, ours)
+            assert state._version > version

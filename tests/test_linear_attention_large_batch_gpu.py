@@ -52,3 +52,15 @@ def test_refusals(gcg_lib):
     st = (__import__("ctypes").c_int64 * 8)(*([0] * 8))
     assert gcg_lib.gcg_linear_attn_step(p, p, p, p, st, p, p, 1 << 20, 16, 8, 8, 1.0, 1, None) == -2
     assert gcg_lib.gcg_linear_attn_step(p, p, p, p, st, p, p, 1 << 32, 1, 8, 8, 1.0, 1, None) == -2
+
+
+def test_rows_of_features_further_apart_than_the_walk_takes(gcg_lib):
+    """Features of 6000 heads of 256: the forward takes them by a copy, and so does the backward."""
+    features = torch.randn(1, 3, 3 * 6000 * 256, device=DEV).to(torch.bfloat16).requires_grad_(True)
+    do = torch.randn(1, 3, 6000, 256, device=DEV).to(torch.bfloat16)
+    ld = decays(6000)
+    o = linear_attention_features(features, 6000, ld)
+    (df,) = torch.autograd.grad(o, features, do)
+    q, k, v = features.detach().view(1, 3, 3, 6000, 256).unbind(2)
+    want = step(q, k, v, do, ld)
+    assert torch.equal(o, want[0]) and torch.equal(df.view(1, 3, 3, 6000, 256), torch.stack(want[2:5], 2))
