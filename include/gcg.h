@@ -561,6 +561,7 @@ GCG_API int gcg_layer_norm_bwd(const void *dy, const void *x, const int8_t *code
  * batch, time and head, of q, k, v, o in this order (of do, q, k, v, dq, dk, dv in the backward; batch and head of q, k, v, o in
  * the step).  log_decay (H) fp32, a constant, at most 0 in use (-inf: no memory).  initial, final, dfinal, dinitial and state are
  * contiguous (bs, H, dk, dv) fp32.  initial and dfinal may be null (zeros), final and dinitial too (not wanted).
+ * dfinal / scale has to be finite.
  * lengths (bs) int32, or null: an entry's rows from its length on (clamped to 0 .. L) are not read, their outputs and gradients
  * are zero, and final is the state after the last row inside.
  *

@@ -20,8 +20,8 @@
 // on both sides.  Narrow slices fill the card from few heads (2 sequences of 32 heads of 128: 256 workgroups) and keep the
 // state small; a and b, which a head's slices share, come from the XCD's L2, where they are put side by side.
 //
-// Measured, bf16, 2 x 8192 rows of 32 heads of 128: forward 150 us, backward (three walks in one launch) 474 us, 3.6 and 3.4
-// TB/s of what it has to move (170 and 465 when launched back to back).  Neither LDS (busy for 35 % of a chunk's time) nor the
+// Measured, bf16, 2 x 8192 rows of 32 heads of 128: forward 152 us, backward (three walks in one launch) 467 us, 3.5 and 3.4
+// TB/s of what it has to move (167 and 456 when launched back to back).  Neither LDS (busy for 35 % of a chunk's time) nor the
 // matrix units (24 %) bound it, but a chunk's chain: LDS reads, two dependent products, rounding, the next state's copy, the
 // barrier; and HBM's latency, which shows through: back to back the forward takes 149 us where a head's rows follow each other
 // in memory and 117 where every head reads the same ones from L2.  Tried, within 5 % or slower: two workgroups of 128 registers a
@@ -29,10 +29,11 @@
 // the state and the rows, 8 a workgroup, 165 and 510 us.
 //
 // Few heads, long sequences: the rows are cut into segments whose states are made first, each from nothing, and joined by a scan
-// over segments; then all segments run at once (8 heads, 131072 rows: 486 us in three launches; in one segment 2.0 ms).
+// over segments; then all segments run at once (8 heads, 131072 rows: 488 us in three launches; in one segment 2.0 ms).
 //
 // Rounding of 16-bit walks: the matrix instructions take 16-bit operands, so P and the state's copy are rounded to the type once,
-// as the output is; the weighted c is given as a sum of two 16-bit parts (three where the state itself is a result), whose
+// as the output is (against 64 bits that makes 0.0023 of the 0.0017 that rounding the output alone gives in bf16, 0.00029 of 0.00021 in
+// f16); the weighted c is given as a sum of two 16-bit parts (three where the state itself is a result), whose
 // remainder, 2^-16 (2^-24), does not show in the fp32 state.  f16 has no range to spare: rows of P and the
 // columns of the state's copy, 32 rows at a time, are scaled by powers of two, and the later parts of the weighted c too, so that neither
 // large states nor small gradients leave it.  fp32 walks run on the fp32 matrix instructions, with nothing rounded.
@@ -940,7 +941,7 @@ struct Step {
 
 // A workgroup takes some columns of one head's state: each thread four columns of every R-th row, read, moved on, written back and
 // multiplied with q on the way; the threads of a column add up through LDS.  ALIGNED: dv is a multiple of 4.  Bound by the state's
-// bytes: 128 sequences of 64 heads of 128 x 128 in 204 us, 5.3 TB/s; one sequence of 32 heads in 5.2 us, hardly more than a launch.
+// bytes: 128 sequences of 64 heads of 128 x 128 in 207 us, 5.2 TB/s; one sequence of 32 heads in 5.4 us, hardly more than a launch.
 template <typename T, bool ALIGNED> __global__ __launch_bounds__(THREADS) void step_kernel(Step a)
 {
     __shared__ float lq[GCG_LINEAR_MAX_DIM], lk[GCG_LINEAR_MAX_DIM], f[2];
@@ -1057,9 +1058,10 @@ template <typename T> int run_walks(const Walks &w, bool states, hipStream_t st)
 
 int64_t seg_rows_of(int64_t L, int segments) { return ((L + segments - 1) / segments + CHUNK - 1) / CHUNK * CHUNK; }
 
-// Segments of a walk.  A CU takes one workgroup of a walk at a time, so a launch costs (rounds of 256 workgroups) * (chunks of a
-// segment), half as much again where the segments' states are made first, and two more launches and the join, about 10 chunks.
-// Segments are taken where that is below 3/4 of the walk in one piece, the fewest within 3 % of the best, four chunks at least.
+// Segments of a walk.  A CU takes one workgroup of a walk with an output at a time, so a launch costs (rounds of 256 workgroups) *
+// (chunks of a segment), half as much again where the segments' states are made first (two of whose workgroups would fit a CU, which
+// this count leaves out), and two more launches and the join, about 10 chunks.  Segments, four chunks at least, are taken where that is
+// 3 % below 3/4 of the walk in one piece, and a larger number of them wherever it gains 3 % on the last one taken.
 // Measured in us (bf16, 1 sequence, heads of 128): 8 heads of 131072 rows, forward, 1 segment 1961, 8 538, 16 525; backward, 1
 // segment 1890, 3 1841, 6 1429, 8 1289; 16 heads of 8192 rows, forward, 1 segment 103, 4 60, 8 71; backward, 1 segment 115, 2
 // 171; 8 heads of 1024 rows, forward, 1 segment 19, 2 26.

@@ -316,7 +316,8 @@ template <typename P> __global__ __launch_bounds__(1024) void layer_norm_reduce_
     }
 }
 
-// Lanes of a row and vectors of a lane: forward up to 32 (fp32: 16) columns a lane, backward 16, whose sums dw and db it keeps too.
+// Lanes of a row and vectors of a lane: forward up to 32 (fp32: 16) columns a lane, backward 8 (32 above 8192
+// columns), whose sums dw and db it keeps too.
 template <typename T, int TPR, int K, bool BITS8> int fwd_launch(const NormFwd &a, hipStream_t st)
 {
     constexpr int THREADS = TPR > 256 ? TPR : 256;

@@ -125,7 +125,7 @@ template <int N> __device__ __forceinline__ uint32_t lanes_max(uint32_t x)
 // ---- the 8-bit checkpoint format ----------------------------------------------------------------------------
 // Blocks of 128 elements along a row share an fp32 scale; the last block of a row may be shorter.  top = the largest
 // magnitude; scale = top * fp32(1 / 127), code = rint(x * (127 / top)), value = code * scale: one step is 1 / 127 of the
-// block's largest, so a value is at most half of that off (0.3 % of the largest).  Magnitudes are compared as integers,
+// block's largest, so a value is at most half of that off (0.4 % of the largest).  Magnitudes are compared as integers,
 // which orders infinities and NaN above everything: a block that holds one gets the scale NaN and comes back as NaN
 // throughout, so that an overflow is still seen in the gradients.  Below 2^-100 the quotient would leave fp32: zeros.
 constexpr int kBlock8 = 128;

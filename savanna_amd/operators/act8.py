@@ -4,8 +4,8 @@
 ``pack8`` and ``unpack8`` are the kernels by themselves.  The layers that use them: ``layer_norm(..., save_8bit=True)``
 (norm.py) writes the checkpoint in the forward's own pass and reads it in the backward's; ``HyenaMixer(..., save_8bit=True)``
 (hyena.py) and ``LinearAttention(..., save_8bit=True)`` (linear_attention.py) keep the projected features as one.  Forward
-results do not change; gradients are those at the activations' 8-bit values, half a step (0.4 % of the largest magnitude
-of 128 neighbours) at most from the exact ones.
+results do not change; a mixer's gradients are those at its features' 8-bit values, half a step (0.4 % of the largest magnitude
+of 128 neighbours) at most from the exact ones, and the norm's are its formula's with those values about the exact row's mean and rstd.
 """
 from __future__ import annotations
 

@@ -67,7 +67,11 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     their last dimension is contiguous (views of one projection are not copied).  log_decay: (H,) float32, at most 0.
     scale: dk ** -0.5 unless given.  initial_state and the final state: contiguous (bs, H, dk, dv) float32.  lengths: (bs,)
     int32; rows of an entry from its length on are not read, their outputs and gradients are zero, and its final state is
-    the one after its last row."""
+    the one after its last row.
+
+    States and sums are float32.  With 16-bit tensors the matrix instructions take 16-bit operands, so scores and the state's
+    read-out copy are rounded to the type once before the output is; where a state is a result, the rows it adds up are kept
+    to more bits, and ``o`` may then round differently.  Infinities and NaN reach later rows only."""
     _constant(log_decay)
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     if not torch.is_grad_enabled() and not _lib.forward_mode():
