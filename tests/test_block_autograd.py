@@ -181,3 +181,23 @@ def test_more_heads_than_an_int_holds(gcg_lib):
     q, ld = torch.empty(1, 1, H, 8, device="meta"), torch.empty(H, device="meta")
     with pytest.raises(RuntimeError, match="heads; at most"):
         torch.ops.gcg.linear_attn_fwd(q, q, q, ld, None, None, 1.0, False)
+
+
+# ---- tensors that are not on the GPU ----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("call", ["pack8", "unpack8", "layer_norm", "LayerNorm", "linear_attention", "linear_attention_features",
+                                  "linear_attention_step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_cpu_tensors_are_refused_by_name(gcg_lib, call, grad):
+    from savanna_amd.operators.act8 import Packed8, pack8, unpack8
+    from savanna_amd.operators.linear_attention import linear_attention, linear_attention_features, linear_attention_step
+    from savanna_amd.operators.norm import LayerNorm, layer_norm
+
+    x, q, ld = torch.randn(4, 64), torch.randn(1, 5, 2, 8), torch.zeros(2)
+    calls = {"pack8": lambda: pack8(x), "unpack8": lambda: unpack8(Packed8(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 1), x.dtype)),
+             "layer_norm": lambda: layer_norm(x, torch.ones(64)), "LayerNorm": lambda: LayerNorm(64)(x),
+             "linear_attention": lambda: linear_attention(q, q, q, ld),
+             "linear_attention_features": lambda: linear_attention_features(torch.randn(1, 5, 48), 2, ld),
+             "linear_attention_step": lambda: linear_attention_step(q[:, 0], q[:, 0], q[:, 0], ld, torch.zeros(1, 2, 8, 8))}
+    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no CPU path"):
+        calls[call]()
