@@ -233,9 +233,9 @@ def forward_mode() -> bool:
 
 
 def refuse_tangents(what: str, *args) -> None:
-    """For calls that pass the autograd functions by: a tangent would be lost there without a word.  (Inside such a function's forward
-    torch has switched forward mode off and refuses by itself.)"""
-    if forward_mode() and torch._C._is_fwd_grad_enabled() and any(
+    """For calls inside a forward-mode level that pass the autograd functions by: a tangent would be lost there without a word.  (Inside
+    such a function's forward torch has switched forward mode off and refuses by itself.)"""
+    if torch._C._is_fwd_grad_enabled() and any(
             isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in args):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
@@ -248,7 +248,8 @@ def _run(op, *args):
     which have layers of their own; the backward operators have no formula and gain nothing (9.8 -> 10.5 us)."""
     if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active():
         return op(*args)
-    refuse_tangents(str(op), *args)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(str(op), *args)
     if torch.is_grad_enabled():
         return op(*args)
     with torch._C._AutoDispatchBelowAutograd():
@@ -1346,7 +1347,7 @@ def linear_attn_packed_bwd(do, features, heads: int, log_decay, scale: float):
 def linear_attn_step(q, k, v, log_decay, state, scale: float):
     """o (bs, H, dv) of one token, q, k (bs, H, dk), v (bs, H, dv); state (bs, H, dk, dv) fp32 moves on in place."""
     _require_gpu(q)
-    if not torch.compiler.is_compiling():
+    if not torch.compiler.is_compiling() and forward_mode():
         refuse_tangents("linear_attn_step", q, k, v, log_decay, state)
     if TORCH_OPS:
         return torch.ops.gcg.linear_attn_step(q, k, v, log_decay, state, scale)
