@@ -587,6 +587,81 @@ GCG_API int gcg_linear_attn_bwd(const void *d_o, const void *q, const void *k, c
 GCG_API int gcg_linear_attn_step(const void *q, const void *k, const void *v, void *o, const int64_t *strides, const float *log_decay,
             float *state, int64_t bs, int32_t H, int32_t dk, int32_t dv, float scale, int32_t dtype, void *stream);
 
+/*
+ * Root-mean-square norm over the last dimension of a residual sum, contiguous (rows, D) tensors, and its backward:
+ *
+ *     r = x + residual (rounded to the type);  y = r * rstd * w,  rstd = (sum r^2 / D + eps)^-1/2
+ *     g = dy * w;  dx = rstd * (g - xh * mean(g * xh)) + dr,  xh = r * rstd;  dw = sum dy * xh
+ *
+ * residual and r: both or neither (r = x then, and the backward takes x in r's place).  dr, the gradient that reaches r by itself,
+ * may be null; dx is x's gradient and residual's.  codes, scales: both or neither; with them the forward writes y in 8-bit
+ * floating point (below; GCG_E4M3) and not y.  w (D) may be null (1); it and dw have the tensors' type, or are fp32 with 16-bit tensors
+ * (GCG_BF16_F32, GCG_F16_F32).  rstd: (rows) fp32, which the backward needs; may be null in the forward.  Sums are fp32, outputs
+ * rounded once.  dw may be null; it is overwritten and bit-reproducible.  workspace: gcg_rms_norm_bwd_workspace_bytes, 256-byte
+ * aligned; not needed without dw.  D up to GCG_NORM_MAX_WIDTH, else GCG_ERR_UNSUPPORTED.
+ */
+GCG_API int gcg_rms_norm_fwd(const void *x, const void *residual, const void *w, void *y, void *r, uint8_t *codes, uint8_t *scales,
+            float *rstd, int64_t rows, int32_t D, float eps, int32_t dtype, void *stream);
+GCG_API size_t gcg_rms_norm_bwd_workspace_bytes(int64_t rows, int32_t D, int32_t dtype);
+GCG_API int gcg_rms_norm_bwd(const void *dy, const void *r, const void *dr, const float *rstd, const void *w, void *dx, void *dw,
+            void *workspace, size_t workspace_bytes, int64_t rows, int32_t D, int32_t dtype, void *stream);
+
+/*
+ * Tensors in 8-bit floating point with a scale for each block of 128 elements along a row.  (rows, D) is kept as codes
+ * (rows, 128 ceil(D / 128)), zero beyond D, and scales (rows, 4 ceil(D / 512)), 127 beyond the last block.  A scale is a byte b and
+ * stands for 2^(b - 127), the smallest power of two, 2^-127 at least, that brings the block's largest magnitude to at most the format's
+ * largest number (GCG_E4M3: 448, no infinities; GCG_E5M2: 57344); a block of zeros has 127.  A code is the element times 2^(127 - b),
+ * rounded to nearest even.  A block that holds an infinity or a NaN has b = 247; they become NaN (GCG_E5M2: an infinity stays one).
+ *
+ * gcg_to_float8 quantises a contiguous tensor along its rows, gcg_from_float8 makes a tensor of it again (one rounding at most).
+ * gcg_to_float8_columns quantises along the columns and writes the result transposed: codes_t (D, 128 ceil(rows / 128)), scales_t
+ * (D, 4 ceil(rows / 512)); with codes and scales (both or neither) along the rows as well, from the same reading.  Its
+ * operand is of type `dtype`, or, with x_scales, in 8 bits itself, of the format `dtype`; codes and scales are null then.
+ *
+ * gcg_product8: y (M, N) = a b^T, contiguous, GCG_BF16 or GCG_F16, of a (M, K) and b (N, K) in 8 bits, accumulated in fp32.  workspace:
+ * gcg_product8_workspace_bytes (0: none), 256-byte aligned.  K up to GCG_PRODUCT8_MAX_K.
+ *
+ * codes are 16-byte aligned, scales 4-byte.  Results are the same on every run.
+ */
+enum { GCG_E4M3 = 16, GCG_E5M2 = 17 };
+enum { GCG_PRODUCT8_MAX_K = 1 << 22 };
+GCG_API int gcg_to_float8(const void *x, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t D, int32_t dtype, int32_t format, void *stream);
+GCG_API int gcg_from_float8(const uint8_t *codes, const uint8_t *scales, void *x, int64_t rows, int64_t D, int32_t dtype, int32_t format,
+            void *stream);
+GCG_API int gcg_to_float8_columns(const void *x, const uint8_t *x_scales, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+            int64_t rows, int64_t D, int32_t dtype, int32_t format, void *stream);
+GCG_API size_t gcg_product8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+GCG_API int gcg_product8(const uint8_t *a, const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, void *y, void *workspace,
+            size_t workspace_bytes, int64_t M, int64_t N, int64_t K, int32_t a_format, int32_t b_format, int32_t dtype, void *stream);
+
+/*
+ * Gated linear recurrence, channel by channel, with a state h (fp32) of D numbers a batch entry:
+ *
+ *     a_t = sigmoid(f_t + bias),   h_t = a_t h_{t-1} + (1 - a_t) x_t,   y_t = gate_t h_t
+ *
+ * x, f, gate, y (bs, L, D), the last dimension contiguous; `strides` holds batch and time strides in elements of x, f, gate, y (of
+ * dy, x, f, gate, dx, df, dgate in the backward; of the rows of x, f, gate in the step, whose y is contiguous).  gate may be null
+ * (y = h; dgate is null then), and so may bias (D), dbias, initial, final, dfinal, dinitial (bs, D), all fp32 and contiguous.
+ * lengths (bs) int32, or null: an entry's rows from its length on (clamped to 0 .. L) are not read, their outputs and gradients
+ * are zero, and final is the state after the last row inside.
+ *
+ * states: (bs, gcg_scan_states(L), D) fp32, which the backward needs of the forward; null otherwise.  gcg_scan_step takes one token: the
+ * state is moved on in place.  workspace: gcg_scan_workspace_bytes (0: none), 256-byte aligned; concurrent calls need their own.
+ * Time strides up to GCG_SCAN_MAX_TIME_STRIDE elements, D up to GCG_SCAN_MAX_WIDTH, L up to GCG_SCAN_MAX_ROWS, else GCG_ERR_UNSUPPORTED.
+ * dtype: GCG_F32, GCG_BF16, GCG_F16.  Results are the same on every run.
+ */
+enum { GCG_SCAN_MAX_TIME_STRIDE = 1 << 21, GCG_SCAN_MAX_WIDTH = 1 << 19, GCG_SCAN_MAX_ROWS = 1 << 30 };
+GCG_API size_t gcg_scan_workspace_bytes(int64_t bs, int64_t L, int32_t D, int32_t backward);
+GCG_API int64_t gcg_scan_states(int64_t L);
+GCG_API int gcg_scan_fwd(const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, const float *initial,
+            const int32_t *lengths, void *y, float *final, float *states, void *workspace, size_t workspace_bytes,
+            int64_t bs, int64_t L, int32_t D, int32_t dtype, void *stream);
+GCG_API int gcg_scan_bwd(const void *dy, const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias,
+            const float *states, const int32_t *lengths, const float *dfinal, void *dx, void *df, void *dgate, float *dbias,
+            float *dinitial, void *workspace, size_t workspace_bytes, int64_t bs, int64_t L, int32_t D, int32_t dtype, void *stream);
+GCG_API int gcg_scan_step(const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, float *state, void *y,
+            int64_t bs, int32_t D, int32_t dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

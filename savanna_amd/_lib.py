@@ -42,6 +42,9 @@ EXPORTS = (
     "gcg_fwd_decay", "gcg_bwd_decay", "gcg_fwd_interleaved_decay", "gcg_bwd_interleaved_decay",
     "gcg_pack8", "gcg_unpack8", "gcg_layer_norm_fwd", "gcg_layer_norm_bwd_workspace_bytes", "gcg_layer_norm_bwd",
     "gcg_linear_attn_workspace_bytes", "gcg_linear_attn_fwd", "gcg_linear_attn_bwd", "gcg_linear_attn_step",
+    "gcg_rms_norm_fwd", "gcg_rms_norm_bwd_workspace_bytes", "gcg_rms_norm_bwd",
+    "gcg_to_float8", "gcg_from_float8", "gcg_to_float8_columns", "gcg_product8_workspace_bytes", "gcg_product8",
+    "gcg_scan_workspace_bytes", "gcg_scan_states", "gcg_scan_fwd", "gcg_scan_bwd", "gcg_scan_step",
 )
 
 _lock = threading.Lock()
@@ -167,6 +170,22 @@ def load() -> ctypes.CDLL:
         lib.gcg_linear_attn_bwd.restype = ctypes.c_int
         lib.gcg_linear_attn_step.argtypes = [vp] * 7 + [i64, i32, i32, i32, ctypes.c_float, i32, vp]
         lib.gcg_linear_attn_step.restype = ctypes.c_int
+        for name, result, args in (
+                ("rms_norm_fwd", ctypes.c_int, [vp] * 8 + [i64, i32, ctypes.c_float, i32, vp]),
+                ("rms_norm_bwd_workspace_bytes", sz, [i64, i32, i32]),
+                ("rms_norm_bwd", ctypes.c_int, [vp] * 8 + [sz, i64, i32, i32, vp]),
+                ("to_float8", ctypes.c_int, [vp] * 3 + [i64, i64, i32, i32, vp]),
+                ("from_float8", ctypes.c_int, [vp] * 3 + [i64, i64, i32, i32, vp]),
+                ("to_float8_columns", ctypes.c_int, [vp] * 6 + [i64, i64, i32, i32, vp]),
+                ("product8_workspace_bytes", sz, [i64, i64, i64]),
+                ("product8", ctypes.c_int, [vp] * 6 + [sz, i64, i64, i64, i32, i32, i32, vp]),
+                ("scan_workspace_bytes", sz, [i64, i64, i32, i32]),
+                ("scan_states", i64, [i64]),
+                ("scan_fwd", ctypes.c_int, [vp] * 11 + [sz, i64, i64, i32, i32, vp]),
+                ("scan_bwd", ctypes.c_int, [vp] * 15 + [sz, i64, i64, i32, i32, vp]),
+                ("scan_step", ctypes.c_int, [vp] * 7 + [i64, i32, i32, vp])):
+            entry = getattr(lib, "gcg_" + name)
+            entry.restype, entry.argtypes = result, args
         _lib = lib
         return lib
 
@@ -1366,3 +1385,419 @@ def linear_attn_step(q, k, v, log_decay, state, scale: float):
     if not state.is_inference():
         torch.autograd.graph.increment_version(state)
     return o
+
+
+# ---- root-mean-square norm --------------------------------------------------------------------------------
+
+def _rms_code(x, residual, w) -> int:
+    code = dtype_code(x.dtype)
+    _check_rows(x)
+    if not 0 < x.shape[-1] <= NORM_MAX_WIDTH:
+        raise ValueError(f"norm over {x.shape[-1]} elements; 1 to {NORM_MAX_WIDTH} are supported")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device
+                                 or not residual.is_contiguous()):
+        raise ValueError("the residual must be a contiguous tensor with the shape, dtype and device of x")
+    if w is None:
+        return code
+    if w.dim() != 1 or w.shape[0] != x.shape[-1] or w.device != x.device or not w.is_contiguous():
+        raise ValueError("the weight must be contiguous, on x's device and of the size of x's last dimension")
+    if w.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"the weight must have x's dtype or be float32; got {w.dtype} with {x.dtype}")
+    return code if w.dtype == x.dtype else GCG_BF16_F32 if code == GCG_BF16 else GCG_F16_F32
+
+
+def _rms_launch(x, residual, w, eps, code, y, r, codes, scales, rstd) -> None:
+    if x.numel() == 0:
+        return
+    D = x.shape[-1]
+    with _on_device(x.device):
+        rc = load().gcg_rms_norm_fwd(x.data_ptr(), _ptr(residual), _ptr(w), _ptr(y), _ptr(r), _ptr(codes), _ptr(scales), _ptr(rstd),
+                                     x.numel() // D, D, eps, code, torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_rms_norm_fwd")
+
+
+def rms_norm_fwd(x, residual, w, eps: float, stats: bool = True):
+    """(y, r, rstd) over the last dimension of r = x + residual; residual and w may be None.  r is empty (x itself is normed) without a
+    residual, rstd None without ``stats``, which the backward needs."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        if not stats:
+            return *_run(torch.ops.gcg.rms_norm_infer, x, residual, w, eps), None
+        return _run(torch.ops.gcg.rms_norm_fwd, x, residual, w, eps)
+    code = _rms_code(x, residual, w)
+    y, r = torch.empty_like(x), torch.empty_like(x) if residual is not None else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if stats else None
+    _rms_launch(x, residual, w, eps, code, y, r, None, None, rstd)
+    return y, r if r is not None else x.new_empty(0), rstd
+
+
+def rms_norm_float8(x, residual, w, eps: float):
+    """(codes, scales, r, rstd): y in 8 bits, blocks of 128 along its last dimension."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.rms_norm_float8, x, residual, w, eps)
+    code = _rms_code(x, residual, w)
+    codes, scales = _empty_float8(x.shape, torch.float8_e4m3fn, x.device)
+    r = torch.empty_like(x) if residual is not None else None
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _rms_launch(x, residual, w, eps, code, None, r, codes, scales, rstd)
+    return codes, scales, r if r is not None else x.new_empty(0), rstd
+
+
+def rms_norm_bwd(dy, r, dr, rstd, w, need_dw: bool = True):
+    """(dx, dw): the gradient of x and of the residual, and the weight's (empty without w or ``need_dw``)."""
+    _require_gpu(dy)
+    if TORCH_OPS:
+        return torch.ops.gcg.rms_norm_bwd(dy, r, dr, rstd, w, need_dw)
+    code = _rms_code(dy, None, w)
+    for t in (r, dr):
+        if t is not None and (t.shape != dy.shape or t.dtype != dy.dtype or t.device != dy.device or not t.is_contiguous()):
+            raise ValueError("dy and dr must be contiguous tensors with the shape, dtype and device of r")
+    if rstd.shape != dy.shape[:-1] or rstd.dtype != torch.float32 or not rstd.is_contiguous() or rstd.device != dy.device:
+        raise ValueError("rstd must be the forward's")
+    D = dy.shape[-1]
+    rows, need_dw = dy.numel() // D, need_dw and w is not None
+    dx, dw = torch.empty_like(dy), torch.empty_like(w) if need_dw else dy.new_empty(0)
+    if rows == 0:
+        return dx, dw.zero_()
+    lib = load()
+    n = lib.gcg_rms_norm_bwd_workspace_bytes(rows, D, code) if need_dw else 0
+    with _on_device(dy.device):
+        ws = torch.empty(n, dtype=torch.uint8, device=dy.device) if n else None
+        rc = lib.gcg_rms_norm_bwd(dy.data_ptr(), r.data_ptr(), _ptr(dr), rstd.data_ptr(), _ptr(w), dx.data_ptr(), dw.data_ptr() if need_dw else None,
+                                  _ptr(ws), n, rows, D, code, torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_rms_norm_bwd")
+    return dx, dw
+
+
+# ---- 8-bit floating point -----------------------------------------------------------------------------------
+
+GCG_E4M3, GCG_E5M2 = 16, 17
+PRODUCT8_MAX_K = 1 << 22            # GCG_PRODUCT8_MAX_K
+_FORMATS = {torch.float8_e4m3fn: GCG_E4M3, torch.float8_e5m2: GCG_E5M2}
+
+
+def format_code(dtype: torch.dtype) -> int:
+    if dtype not in _FORMATS:
+        raise TypeError(f"8-bit tensors are float8_e4m3fn or float8_e5m2; got {dtype}")
+    return _FORMATS[dtype]
+
+
+def code_columns(D: int) -> int:
+    """Codes of a row of D elements: whole blocks."""
+    return (D + 127) // 128 * 128
+
+
+def scale_columns(D: int) -> int:
+    """Scales of a row of D elements: one for every 128, and whole words of four."""
+    return (D + 511) // 512 * 4
+
+
+def _empty_float8(shape, format, device):
+    *lead, D = shape
+    return (torch.empty((*lead, code_columns(D)), dtype=format, device=device),
+            torch.empty((*lead, scale_columns(D)), dtype=torch.float8_e8m0fnu, device=device))
+
+
+def _check_float8(codes, scales, columns: int) -> None:
+    format_code(codes.dtype)
+    if columns < 0 or codes.dim() < 1 or not codes.is_contiguous() or codes.shape[-1] != code_columns(columns):
+        raise ValueError(f"the codes of {columns} columns must be contiguous rows of {code_columns(columns)}")
+    if scales.dtype != torch.float8_e8m0fnu or not scales.is_contiguous() or scales.device != codes.device \
+            or tuple(scales.shape) != (*codes.shape[:-1], scale_columns(columns)):
+        raise ValueError(f"the scales of {columns} columns must be contiguous float8_e8m0fnu rows of {scale_columns(columns)}")
+
+
+def _product_dtype(dtype: torch.dtype) -> int:
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"products of 8-bit tensors are bfloat16 or float16; got {dtype} (the matrix instructions' own sums do not hold "
+                        "float32's bits)")
+    return dtype_code(dtype)
+
+
+def to_float8(x, format: torch.dtype):
+    """(codes, scales) of a contiguous tensor; blocks of 128 along the last dimension."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.to_float8, x, format)
+    _check_rows(x)
+    f, code = format_code(format), dtype_code(x.dtype)
+    codes, scales = _empty_float8(x.shape, format, x.device)
+    if x.numel():
+        D = x.shape[-1]
+        with _on_device(x.device):
+            rc = load().gcg_to_float8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), x.numel() // D, D, code, f,
+                                      torch.cuda.current_stream().cuda_stream)
+        check(rc, "gcg_to_float8")
+    return codes, scales
+
+
+def from_float8(codes, scales, columns: int, dtype: torch.dtype):
+    """The tensor of ``dtype`` that codes and scales stand for."""
+    _require_gpu(codes)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.from_float8, codes, scales, columns, dtype)
+    _check_float8(codes, scales, columns)
+    code = dtype_code(dtype)
+    x = torch.empty((*codes.shape[:-1], columns), dtype=dtype, device=codes.device)
+    if x.numel():
+        with _on_device(codes.device):
+            rc = load().gcg_from_float8(codes.data_ptr(), scales.data_ptr(), x.data_ptr(), x.numel() // columns, columns, code,
+                                        format_code(codes.dtype), torch.cuda.current_stream().cuda_stream)
+        check(rc, "gcg_from_float8")
+    return x
+
+
+def _columns_launch(x, x_scales, rows, D, code, codes, scales, codes_t, scales_t) -> None:
+    if rows and D:
+        with _on_device(x.device):
+            rc = load().gcg_to_float8_columns(x.data_ptr(), _ptr(x_scales), _ptr(codes), _ptr(scales), codes_t.data_ptr(), scales_t.data_ptr(),
+                                              rows, D, code, format_code(codes_t.dtype), torch.cuda.current_stream().cuda_stream)
+        check(rc, "gcg_to_float8_columns")
+
+
+def _check_matrix(x) -> None:
+    _check_rows(x)
+    if x.dim() != 2:
+        raise ValueError("x must be a matrix")
+
+
+def to_float8_both(x, format: torch.dtype):
+    """(codes, scales) of a matrix along its rows, and those of its transpose, from one reading."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.to_float8_both, x, format)
+    _check_matrix(x)
+    format_code(format)
+    R, D = x.shape
+    out = *_empty_float8((R, D), format, x.device), *_empty_float8((D, R), format, x.device)
+    _columns_launch(x, None, R, D, dtype_code(x.dtype), *out)
+    return out
+
+
+def to_float8_columns(x, format: torch.dtype):
+    """(codes, scales) of a matrix's transpose."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.to_float8_columns, x, format)
+    _check_matrix(x)
+    format_code(format)
+    R, D = x.shape
+    out = _empty_float8((D, R), format, x.device)
+    _columns_launch(x, None, R, D, dtype_code(x.dtype), None, None, *out)
+    return out
+
+
+def float8_columns(codes, scales, columns: int, format: torch.dtype):
+    """(codes, scales) of the transpose of a matrix in 8 bits."""
+    _require_gpu(codes)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.float8_columns, codes, scales, columns, format)
+    _check_float8(codes, scales, columns)
+    if codes.dim() != 2:
+        raise ValueError("codes must be a matrix")
+    out = _empty_float8((columns, codes.shape[0]), format, codes.device)
+    _columns_launch(codes, scales, codes.shape[0], columns, format_code(codes.dtype), None, None, *out)
+    return out
+
+
+def matmul_float8(a, a_scales, b, b_scales, columns: int, dtype: torch.dtype):
+    """a b^T of a (..., columns) and a matrix b (N, columns), both in 8 bits."""
+    _require_gpu(a)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.matmul_float8, a, a_scales, b, b_scales, columns, dtype)
+    _check_float8(a, a_scales, columns)
+    _check_float8(b, b_scales, columns)
+    if b.dim() != 2 or b.device != a.device:
+        raise ValueError("b must be a matrix on a's device")
+    if columns > PRODUCT8_MAX_K:
+        raise ValueError(f"a product over {columns} columns; at most {PRODUCT8_MAX_K} are supported")
+    code, N = _product_dtype(dtype), b.shape[0]
+    y = torch.empty((*a.shape[:-1], N), dtype=dtype, device=a.device)
+    if y.numel() == 0 or columns == 0:
+        return y.zero_()
+    lib, M = load(), y.numel() // N
+    n = lib.gcg_product8_workspace_bytes(M, N, columns)
+    with _on_device(a.device):
+        ws = torch.empty(n, dtype=torch.uint8, device=a.device) if n else None
+        rc = lib.gcg_product8(a.data_ptr(), a_scales.data_ptr(), b.data_ptr(), b_scales.data_ptr(), y.data_ptr(), _ptr(ws), n, M, N, columns,
+                              format_code(a.dtype), format_code(b.dtype), code, torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_product8")
+    return y
+
+
+def linear_float8_infer(x, codes, scales, columns: int):
+    """x w^T of a contiguous x, which is quantised in the call, and a weight in 8 bits."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.linear_float8_infer, x, codes, scales, columns)
+    _check_rows(x)
+    _product_dtype(x.dtype)
+    _check_float8(codes, scales, columns)
+    if codes.dim() != 2 or codes.device != x.device or x.shape[-1] != columns:
+        raise ValueError("the weight must be a matrix on x's device with as many columns as x")
+    return matmul_float8(*to_float8(x, torch.float8_e4m3fn), codes, scales, columns, x.dtype)
+
+
+# ---- gated linear recurrence -----------------------------------------------------------------------------------
+
+SCAN_MAX_TIME_STRIDE = 1 << 21      # GCG_SCAN_MAX_TIME_STRIDE
+SCAN_MAX_WIDTH = 1 << 19            # GCG_SCAN_MAX_WIDTH
+SCAN_MAX_ROWS = 1 << 30             # GCG_SCAN_MAX_ROWS
+
+
+def _scan_rows(t):
+    """The tensor with a contiguous last dimension and rows near enough to each other, as the kernels read it."""
+    if t is None or (t.shape[-1] == 1 or t.stride(-1) == 1) and (t.dim() < 3 or t.stride(1) <= SCAN_MAX_TIME_STRIDE):
+        return t
+    return t.contiguous()
+
+
+def _scan_strides(n: int, *tensors):
+    s = [t.stride(i) if t is not None else 0 for t in tensors for i in range(n)]
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def _check_scan(x, f, gate, bias, dim) -> None:
+    if x.dim() != dim or f.shape != x.shape or (gate is not None and gate.shape != x.shape):
+        raise ValueError("x, f and gate must be (bs, L, D)" if dim == 3 else "x, f and gate must be (bs, D)")
+    if any(t is not None and (t.dtype != x.dtype or t.device != x.device) for t in (f, gate)):
+        raise ValueError("x, f and gate must share dtype and device")
+    dtype_code(x.dtype)
+    if bias is not None and (bias.shape != x.shape[-1:] or bias.dtype != torch.float32 or not bias.is_contiguous() or bias.device != x.device):
+        raise ValueError("bias must be a contiguous float32 tensor of one element a channel on x's device")
+    if not 0 < x.shape[-1] <= SCAN_MAX_WIDTH:
+        raise ValueError(f"{x.shape[-1]} channels; 1 to {SCAN_MAX_WIDTH} are supported")
+    if dim == 3 and x.shape[1] > SCAN_MAX_ROWS:
+        raise ValueError(f"{x.shape[1]} rows; at most {SCAN_MAX_ROWS} are supported")
+
+
+def _check_scan_state(t, x, name) -> None:
+    if t is not None and (t.shape != (x.shape[0], x.shape[-1]) or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device):
+        raise ValueError(f"{name} must be a contiguous (bs, D) float32 tensor on x's device")
+
+
+def _scan_workspace(lib, x, backward):
+    n = lib.gcg_scan_workspace_bytes(x.shape[0], x.shape[1], x.shape[2], int(backward))
+    return n, (torch.empty(n, dtype=torch.uint8, device=x.device) if n else None)
+
+
+def scan_fwd(x, f, gate, bias, initial, lengths, final: bool, keep: bool):
+    """(y, final state, kept states); what is not asked for is empty."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.scan_fwd, x, f, gate, bias, initial, lengths, final, keep)
+    lib = load()
+    _check_scan(x, f, gate, bias, 3)
+    _check_scan_state(initial, x, "initial_state")
+    _check_lengths(lengths, x)
+    bs, L, D = x.shape
+    f32 = dict(dtype=torch.float32, device=x.device)
+    y, last = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty((bs, D) if final else (0,), **f32)
+    states = torch.empty((bs, lib.gcg_scan_states(L), D) if keep else (0,), **f32)
+    if y.numel() == 0:
+        if final:
+            _passed_on(initial, last)
+        return y, last, states
+    a, b, c = _scan_rows(x), _scan_rows(f), _scan_rows(gate)
+    with _on_device(x.device):
+        n, ws = _scan_workspace(lib, x, False)
+        rc = lib.gcg_scan_fwd(a.data_ptr(), b.data_ptr(), _ptr(c), _scan_strides(2, a, b, c, y), _ptr(bias), _ptr(initial), _ptr(lengths),
+                              y.data_ptr(), last.data_ptr() if final else None, states.data_ptr() if keep else None, _ptr(ws), n, bs, L, D,
+                              dtype_code(x.dtype), torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_scan_fwd")
+    return y, last, states
+
+
+def _scan_bwd_into(dy, x, f, gate, bias, states, lengths, dfinal, dx, df, dgate, dbias, dinitial) -> None:
+    lib = load()
+    bs, L, D = x.shape
+    d, a, b, c = _scan_rows(dy), _scan_rows(x), _scan_rows(f), _scan_rows(gate)
+    with _on_device(x.device):
+        n, ws = _scan_workspace(lib, x, True)
+        rc = lib.gcg_scan_bwd(d.data_ptr(), a.data_ptr(), b.data_ptr(), _ptr(c), _scan_strides(2, d, a, b, c, dx, df, dgate), _ptr(bias),
+                              states.data_ptr(), _ptr(lengths), _ptr(dfinal), dx.data_ptr(), df.data_ptr(), _ptr(dgate), _ptr(dbias),
+                              _ptr(dinitial), _ptr(ws), n, bs, L, D, dtype_code(x.dtype), torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_scan_bwd")
+
+
+def _check_scan_bwd(dy, x, states, lengths, dfinal) -> None:
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("dy must have the shape, dtype and device of x")
+    if tuple(states.shape) != (x.shape[0], load().gcg_scan_states(x.shape[1]), x.shape[2]) or states.dtype != torch.float32 \
+            or not states.is_contiguous() or states.device != x.device:
+        raise ValueError("states must be the forward's")
+    _check_scan_state(dfinal, x, "the final state's gradient")
+    _check_lengths(lengths, x)
+
+
+def scan_bwd(dy, x, f, gate, bias, states, lengths, dfinal, need_dbias: bool, need_dinitial: bool):
+    """(dx, df, dgate, dbias, dinitial); what is not asked for is empty."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return torch.ops.gcg.scan_bwd(dy, x, f, gate, bias, states, lengths, dfinal, need_dbias, need_dinitial)
+    _check_scan(x, f, gate, bias, 3)
+    _check_scan_bwd(dy, x, states, lengths, dfinal)
+    bs, _, D = x.shape
+    new = lambda: torch.empty(x.shape, dtype=x.dtype, device=x.device)               # noqa: E731
+    dx, df, dg = new(), new(), new() if gate is not None else None
+    f32 = dict(dtype=torch.float32, device=x.device)
+    db, di = torch.empty((D,) if need_dbias else (0,), **f32), torch.empty((bs, D) if need_dinitial else (0,), **f32)
+    if x.numel() == 0:
+        db.zero_()
+        if need_dinitial:
+            _passed_on(dfinal, di)
+    else:
+        _scan_bwd_into(dy, x, f, gate, bias, states, lengths, dfinal, dx, df, dg, db if need_dbias else None, di if need_dinitial else None)
+    return dx, df, dg if dg is not None else x.new_empty(0), db, di
+
+
+def _split_scan(features):
+    if features.dim() != 3 or not features.is_contiguous() or features.shape[2] % 3:
+        raise ValueError("features must be a contiguous (bs, L, 3 * D) tensor")
+    return features.unflatten(2, (3, -1)).unbind(2) if features.shape[2] else (features,) * 3
+
+
+def scan_packed_fwd(features, bias, keep: bool):
+    """(y, kept states) of the projected features (bs, L, 3 * D), "(p d)" with p = x, f, gate."""
+    _require_gpu(features)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.scan_packed_fwd, features, bias, keep)
+    y, _, states = scan_fwd(*_split_scan(features), bias, None, None, False, keep)
+    return y, states
+
+
+def scan_packed_bwd(dy, features, bias, states, need_dbias: bool):
+    """(the features' gradient in their layout, dbias)."""
+    _require_gpu(features)
+    if TORCH_OPS:
+        return torch.ops.gcg.scan_packed_bwd(dy, features, bias, states, need_dbias)
+    x, f, gate = _split_scan(features)
+    _check_scan(x, f, gate, bias, 3)
+    _check_scan_bwd(dy, x, states, None, None)
+    d = torch.empty_like(features)
+    db = torch.empty(x.shape[2] if need_dbias else 0, dtype=torch.float32, device=features.device)
+    if d.numel() == 0:
+        return d, db.zero_()
+    _scan_bwd_into(dy, x, f, gate, bias, states, None, None, *_split_scan(d), db if need_dbias else None, None)
+    return d, db
+
+
+def scan_step(x, f, gate, bias, state):
+    """y (bs, D) of one token; ``state`` (bs, D) float32 is moved on in place."""
+    _require_gpu(x)
+    if not torch.compiler.is_compiling() and forward_mode():
+        refuse_tangents("scan_step", x, f, gate, bias, state)
+    if TORCH_OPS:
+        return torch.ops.gcg.scan_step(x, f, gate, bias, state)
+    _check_scan(x, f, gate, bias, 2)
+    _check_scan_state(state, x, "state")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel() == 0:
+        return y
+    a, b, c = _scan_rows(x), _scan_rows(f), _scan_rows(gate)
+    with _on_device(x.device):
+        rc = load().gcg_scan_step(a.data_ptr(), b.data_ptr(), _ptr(c), _scan_strides(1, a, b, c), _ptr(bias), state.data_ptr(), y.data_ptr(),
+                                  x.shape[0], x.shape[1], dtype_code(x.dtype), torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_scan_step")
+    return y

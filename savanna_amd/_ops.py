@@ -43,10 +43,17 @@ BLOCK_OP_NAMES = (
     "pack8", "unpack8", "layer_norm_fwd", "layer_norm_infer", "layer_norm_bwd",
     "linear_attn_fwd", "linear_attn_bwd", "linear_attn_packed_fwd", "linear_attn_packed_bwd", "linear_attn_step",
 )
+# those of a layer in 8-bit floating point around a recurrent mixer
+LAYER8_OP_NAMES = (
+    "rms_norm_fwd", "rms_norm_infer", "rms_norm_float8", "rms_norm_bwd",
+    "to_float8", "to_float8_both", "to_float8_columns", "float8_columns", "from_float8", "matmul_float8", "linear_float8_infer",
+    "scan_fwd", "scan_bwd", "scan_packed_fwd", "scan_packed_bwd", "scan_step",
+)
 
 # differentiable as they are: C++ autograd nodes around operators above, which a trace sees in their place
 NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay")
 BLOCK_NODE_NAMES = ("layer_norm", "linear_attn", "linear_attn_packed")
+LAYER8_NODE_NAMES = ("rms_norm", "linear_float8", "norm_linear_float8", "scan", "scan_packed")
 
 
 # ---- autograd --------------------------------------------------------------------------------------------
@@ -168,12 +175,61 @@ def _register_autograd():
         save(0, 2)(ctx, inputs, output)
     reg("gcg::linear_attn_packed_fwd", linear_packed, setup_context=packed_setup)
 
+    def rms_setup(ctx, inputs, output):      # rms_norm_fwd(x, residual, w, eps) -> y, r, rstd
+        x, residual, w, _ = inputs
+        _, r, rstd = output
+        ctx.added = residual is not None
+        ctx.save_for_backward(r if ctx.added else x, rstd, w)
+        ctx.set_materialize_grads(False)
+
+    def rms(ctx, dy, dr, _):
+        r, rstd, w = ctx.saved_tensors
+        dy = dy.contiguous() if dy is not None else torch.zeros_like(r)
+        need = w is not None and ctx.needs_input_grad[2]
+        dx, dw = ops.rms_norm_bwd(dy, r, dr.contiguous() if ctx.added and dr is not None else None, rstd, w, need)
+        return dx, dx if ctx.added else None, dw if need else None, None
+    reg("gcg::rms_norm_fwd", rms, setup_context=rms_setup)
+
+    def scan_setup(ctx, inputs, output):     # scan_fwd(x, f, gate, bias, initial, lengths, final, keep) -> y, state, kept states
+        x, f, gate, bias, initial, lengths, ctx.final, keep = inputs
+        if not keep:
+            raise RuntimeError("torch.ops.gcg.scan_fwd is differentiable with keep=True only")
+        ctx.save_for_backward(x, f, gate, bias, output[2], lengths)
+        ctx.set_materialize_grads(False)
+
+    def scan(ctx, dy, dfinal, _):
+        x, f, gate, bias, states, lengths = ctx.saved_tensors
+        nb, ni = ctx.needs_input_grad[3:5]
+        dy = dy if dy is not None else torch.zeros_like(x)
+        dfinal = dfinal.contiguous() if ctx.final and dfinal is not None else None
+        dx, df, dg, db, di = ops.scan_bwd(dy, x, f, gate, bias, states, lengths, dfinal, nb, ni)
+        return dx, df, dg if gate is not None else None, db if nb else None, di if ni else None, None, None, None
+    reg("gcg::scan_fwd", scan, setup_context=scan_setup)
+
+    def packed_scan_setup(ctx, inputs, output):     # scan_packed_fwd(features, bias, keep) -> y, kept states
+        features, bias, keep = inputs
+        if not keep:
+            raise RuntimeError("torch.ops.gcg.scan_packed_fwd is differentiable with keep=True only")
+        ctx.save_for_backward(features, bias, output[1])
+        ctx.set_materialize_grads(False)
+
+    def packed_scan(ctx, dy, _):
+        if dy is None:
+            return None, None, None
+        need = ctx.needs_input_grad[1]
+        df, db = ops.scan_packed_bwd(dy, *ctx.saved_tensors, need)
+        return df, db if need else None, None
+    reg("gcg::scan_packed_fwd", packed_scan, setup_context=packed_scan_setup)
+
     def refuse(name, hint):
         def backward(ctx, *grads):
             raise RuntimeError(f"torch.ops.gcg.{name} is not differentiable; {hint}")
         return backward
     nothing = lambda ctx, inputs, output: None                                       # noqa: E731
     reg("gcg::layer_norm_infer", refuse("layer_norm_infer", "use torch.ops.gcg.layer_norm"), setup_context=nothing)
+    reg("gcg::rms_norm_infer", refuse("rms_norm_infer", "use torch.ops.gcg.rms_norm"), setup_context=nothing)
+    for name in ("rms_norm_float8", "to_float8", "to_float8_both", "to_float8_columns", "linear_float8_infer"):
+        reg(f"gcg::{name}", refuse(name, "use torch.ops.gcg.linear_float8 or norm_linear_float8"), setup_context=nothing)
     reg("gcg::pack8", refuse("pack8", "a checkpoint is what a backward pass reads"), setup_context=nothing)
     reg("gcg::fwd_full", refuse("fwd_full", "use torch.ops.gcg.fwd for a differentiable y"), setup_context=lambda ctx, inputs, output: None)
 

@@ -1019,4 +1019,173 @@ GCG_API int gcg_linear_attn_step(const void *q, const void *k, const void *v, vo
     return finish(gcg::linear_attn_step_launch(dtype, q, k, v, o, strides, log_decay, state, bs, H, dk, dv, scale, (hipStream_t)stream));
 }
 
+// ---- root-mean-square norm ------------------------------------------------------------------------------
+
+GCG_API int gcg_rms_norm_fwd(const void *x, const void *residual, const void *w, void *y, void *r, uint8_t *codes, uint8_t *scales,
+                             float *rstd, int64_t rows, int32_t D, float eps, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || (residual == nullptr) != (r == nullptr) || (codes == nullptr) != (scales == nullptr) || (y == nullptr) == (codes == nullptr) ||
+        !(eps >= 0.f))
+        return GCG_ERR_BAD_ARG;
+    if ((uintptr_t)codes & 15) return GCG_ERR_BAD_ARG;
+    int rc = norm_check(rows, D, dtype);
+    if (rc) return rc;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::rms_norm_fwd_launch(dtype, x, residual, w, y, r, codes, scales, rstd, rows, D, eps, (hipStream_t)stream));
+}
+
+GCG_API size_t gcg_rms_norm_bwd_workspace_bytes(int64_t rows, int32_t D, int32_t dtype)
+{
+    if (norm_check(rows, D, dtype)) return 0;
+    return (gcg::rms_norm_bwd_workspace(rows, D) + 255) & ~(size_t)255;
+}
+
+GCG_API int gcg_rms_norm_bwd(const void *dy, const void *r, const void *dr, const float *rstd, const void *w, void *dx, void *dw,
+                             void *workspace, size_t workspace_bytes, int64_t rows, int32_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!dy || !r || !rstd || !dx) return GCG_ERR_BAD_ARG;
+    int rc = norm_check(rows, D, dtype);
+    if (rc) return rc;
+    if (dw && missing(workspace, workspace_bytes, gcg_rms_norm_bwd_workspace_bytes(rows, D, dtype))) return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::rms_norm_bwd_launch(dtype, dy, r, dr, rstd, w, dx, dw, workspace, rows, D, (hipStream_t)stream));
+}
+
+// ---- 8-bit floating point -----------------------------------------------------------------------------------
+
+namespace {
+bool is_format(int32_t f) { return f == GCG_E4M3 || f == GCG_E5M2; }
+bool is_type(int32_t dtype) { return dtype == GCG_F32 || dtype == GCG_BF16 || dtype == GCG_F16; }
+bool placed(const void *codes, const void *scales) { return codes && scales && !((uintptr_t)codes & 15) && !((uintptr_t)scales & 3); }
+} // namespace
+
+GCG_API int gcg_to_float8(const void *x, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t D, int32_t dtype, int32_t format, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !placed(codes, scales) || rows <= 0 || D <= 0 || !is_type(dtype) || !is_format(format)) return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::to_float8_launch(dtype, format == GCG_E5M2, x, codes, scales, rows, D, (hipStream_t)stream));
+}
+
+GCG_API int gcg_from_float8(const uint8_t *codes, const uint8_t *scales, void *x, int64_t rows, int64_t D, int32_t dtype, int32_t format,
+                            void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !placed(codes, scales) || rows <= 0 || D <= 0 || !is_type(dtype) || !is_format(format)) return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::from_float8_launch(dtype, format == GCG_E5M2, codes, scales, x, rows, D, (hipStream_t)stream));
+}
+
+GCG_API int gcg_to_float8_columns(const void *x, const uint8_t *x_scales, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+                                  int64_t rows, int64_t D, int32_t dtype, int32_t format, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !placed(codes_t, scales_t) || (codes == nullptr) != (scales == nullptr) || (codes && !placed(codes, scales)) || rows <= 0 || D <= 0 ||
+        !is_format(format) || !(x_scales ? is_format(dtype) && placed(x, x_scales) && !codes : is_type(dtype)))
+        return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::to_float8_columns_launch(dtype, format == GCG_E5M2, dtype == GCG_E5M2, x, x_scales, codes, scales, codes_t, scales_t, rows, D,
+                                                (hipStream_t)stream));
+}
+
+GCG_API size_t gcg_product8_workspace_bytes(int64_t M, int64_t N, int64_t K)
+{
+    if (M <= 0 || N <= 0 || K <= 0 || K > GCG_PRODUCT8_MAX_K) return 0;
+    return (gcg::product8_workspace(M, N, K) + 255) & ~(size_t)255;
+}
+
+GCG_API int gcg_product8(const uint8_t *a, const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, void *y, void *workspace,
+                         size_t workspace_bytes, int64_t M, int64_t N, int64_t K, int32_t a_format, int32_t b_format, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!placed(a, a_scales) || !placed(b, b_scales) || !y || M <= 0 || N <= 0 || K <= 0 || !is_format(a_format) || !is_format(b_format) ||
+        (dtype != GCG_BF16 && dtype != GCG_F16))
+        return GCG_ERR_BAD_ARG;
+    if (K > GCG_PRODUCT8_MAX_K) return GCG_ERR_UNSUPPORTED;
+    if (missing(workspace, workspace_bytes, gcg_product8_workspace_bytes(M, N, K))) return GCG_ERR_WORKSPACE;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::product8_launch(dtype, a_format == GCG_E5M2, b_format == GCG_E5M2, a, a_scales, b, b_scales, y, workspace, M, N, K,
+                                       (hipStream_t)stream));
+}
+
+// ---- gated linear recurrence -----------------------------------------------------------------------------------
+
+namespace {
+int scan_check(int64_t bs, int64_t L, int32_t D, int32_t dtype)
+{
+    if (bs <= 0 || L <= 0 || D <= 0 || !is_type(dtype)) return GCG_ERR_BAD_ARG;
+    return bs > INT32_MAX || L > GCG_SCAN_MAX_ROWS || D > GCG_SCAN_MAX_WIDTH ? GCG_ERR_UNSUPPORTED : GCG_OK;
+}
+int scan_strides(const int64_t *s, int tensors)
+{
+    for (int i = 0; i < tensors; ++i) {
+        if (s[2 * i] < 0 || s[2 * i + 1] < 0) return GCG_ERR_BAD_ARG;
+        if (s[2 * i + 1] > GCG_SCAN_MAX_TIME_STRIDE) return GCG_ERR_UNSUPPORTED;
+    }
+    return GCG_OK;
+}
+} // namespace
+
+GCG_API size_t gcg_scan_workspace_bytes(int64_t bs, int64_t L, int32_t D, int32_t backward)
+{
+    if (scan_check(bs, L, D, GCG_F32)) return 0;
+    return (gcg::scan_workspace(bs, L, D, backward != 0) + 255) & ~(size_t)255;
+}
+
+GCG_API int64_t gcg_scan_states(int64_t L) { return L > 0 ? gcg::scan_states(L) : 0; }
+
+GCG_API int gcg_scan_fwd(const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, const float *initial,
+                         const int32_t *lengths, void *y, float *final, float *states, void *workspace, size_t workspace_bytes,
+                         int64_t bs, int64_t L, int32_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !f || !strides || !y) return GCG_ERR_BAD_ARG;
+    int rc = scan_check(bs, L, D, dtype);
+    if (!rc) rc = scan_strides(strides, 4);
+    if (rc) return rc;
+    if (missing(workspace, workspace_bytes, gcg_scan_workspace_bytes(bs, L, D, 0))) return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::scan_fwd_launch(dtype, x, f, gate, strides, bias, initial, lengths, y, final, states, workspace, bs, L, D,
+                                       (hipStream_t)stream));
+}
+
+GCG_API int gcg_scan_bwd(const void *dy, const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias,
+                         const float *states, const int32_t *lengths, const float *dfinal, void *dx, void *df, void *dgate, float *dbias,
+                         float *dinitial, void *workspace, size_t workspace_bytes, int64_t bs, int64_t L, int32_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!dy || !x || !f || !strides || !states || !dx || !df || (gate == nullptr) != (dgate == nullptr)) return GCG_ERR_BAD_ARG;
+    int rc = scan_check(bs, L, D, dtype);
+    if (!rc) rc = scan_strides(strides, 7);
+    if (rc) return rc;
+    if (missing(workspace, workspace_bytes, gcg_scan_workspace_bytes(bs, L, D, 1))) return GCG_ERR_WORKSPACE;
+    rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::scan_bwd_launch(dtype, dy, x, f, gate, strides, bias, states, lengths, dfinal, dx, df, dgate, dbias, dinitial, workspace,
+                                       bs, L, D, (hipStream_t)stream));
+}
+
+GCG_API int gcg_scan_step(const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, float *state, void *y,
+                          int64_t bs, int32_t D, int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !f || !strides || !state || !y) return GCG_ERR_BAD_ARG;
+    const int rc0 = scan_check(bs, 1, D, dtype);
+    if (rc0) return rc0;
+    for (int i = 0; i < 3; ++i)
+        if (strides[i] < 0) return GCG_ERR_BAD_ARG;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::scan_step_launch(dtype, x, f, gate, strides, bias, state, y, bs, D, (hipStream_t)stream));
+}
+
 } // extern "C"

@@ -436,4 +436,31 @@ int linear_attn_bwd_launch(int dtype, const void *d_o, const void *q, const void
 int linear_attn_step_launch(int dtype, const void *q, const void *k, const void *v, void *o, const int64_t *strides, const float *log_decay,
                             float *state, int64_t bs, int H, int dk, int dv, float scale, hipStream_t st);
 
+// root-mean-square norm of a residual sum; r (and dr) null without a residual, codes and scales in y's place
+int rms_norm_fwd_launch(int dtype, const void *x, const void *residual, const void *w, void *y, void *r, uint8_t *codes, uint8_t *scales,
+                        float *rstd, int64_t rows, int D, float eps, hipStream_t st);
+size_t rms_norm_bwd_workspace(int64_t rows, int D);
+int rms_norm_bwd_launch(int dtype, const void *dy, const void *r, const void *dr, const float *rstd, const void *w, void *dx, void *dw,
+                        void *ws, int64_t rows, int D, hipStream_t st);
+
+// 8-bit floating point with a scale for each block of 128: along the rows and back, along the columns, products
+int to_float8_launch(int dtype, int e5m2, const void *x, uint8_t *codes, uint8_t *scales, int64_t rows, int64_t D, hipStream_t st);
+int from_float8_launch(int dtype, int e5m2, const uint8_t *codes, const uint8_t *scales, void *x, int64_t rows, int64_t D, hipStream_t st);
+int to_float8_columns_launch(int dtype, int e5m2, int from5, const void *x, const uint8_t *x_scales, uint8_t *codes, uint8_t *scales,
+                             uint8_t *codes_t, uint8_t *scales_t, int64_t rows, int64_t D, hipStream_t st);
+size_t product8_workspace(int64_t M, int64_t N, int64_t K);
+int product8_launch(int dtype, int a5, int b5, const uint8_t *a, const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, void *y,
+                    void *ws, int64_t M, int64_t N, int64_t K, hipStream_t st);
+
+// gated linear recurrence; strides: batch and time of x, f, gate, y (dy, x, f, gate, dx, df, dgate; the step: rows of x, f, gate), in elements
+size_t scan_workspace(int64_t bs, int64_t L, int D, bool backward);
+int64_t scan_states(int64_t L);
+int scan_fwd_launch(int dtype, const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, const float *initial,
+                    const int32_t *lengths, void *y, float *final, float *states, void *ws, int64_t bs, int64_t L, int D, hipStream_t st);
+int scan_bwd_launch(int dtype, const void *dy, const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias,
+                    const float *states, const int32_t *lengths, const float *dfinal, void *dx, void *df, void *dgate, float *dbias,
+                    float *dinitial, void *ws, int64_t bs, int64_t L, int D, hipStream_t st);
+int scan_step_launch(int dtype, const void *x, const void *f, const void *gate, const int64_t *strides, const float *bias, float *state, void *y,
+                     int64_t bs, int D, hipStream_t st);
+
 } // namespace gcg

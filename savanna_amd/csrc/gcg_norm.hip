@@ -15,46 +15,6 @@
 namespace gcg {
 namespace {
 
-// weight or bias elements c .. c + V - 1: of the tensors' type, or fp32
-template <typename T, bool TAIL>
-__device__ __forceinline__ void load_param(const void *p, bool f32, int c, int D, float absent, float (&v)[kVec<T>])
-{
-    constexpr int V = kVec<T>;
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = absent;
-    if (!p || c >= D) return;
-    if (f32 && sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (!TAIL || c + i < D) v[i] = ((const float *)p)[c + i];
-    } else {
-        unpack_vec(load_row_vec<T, TAIL, false>((const T *)p, c, D), v, T{});
-    }
-}
-
-// sums of N numbers over the TPR lanes of a row.  More than one wave: through `slots`, of which the caller gives another set
-// every time, so that one barrier is enough.
-template <int TPR, int N> __device__ __forceinline__ void row_sum(float (&s)[N], float *slots)
-{
-#pragma unroll
-    for (int n = 0; n < N; ++n) s[n] = wave_sum(s[n]);
-    if constexpr (TPR > kWave) {
-        constexpr int W = TPR / kWave;
-        const int wave = threadIdx.x / kWave, first = threadIdx.x / TPR * W;
-        if (threadIdx.x % kWave == 0) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) slots[wave * N + n] = s[n];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            s[n] = slots[first * N + n];
-#pragma unroll
-            for (int i = 1; i < W; ++i) s[n] += slots[(first + i) * N + n];
-        }
-    }
-}
-
 struct NormFwd {
     const void *x, *w, *b;
     void *y;
