@@ -133,7 +133,9 @@ __global__ __launch_bounds__(WM * WN * 64) void product8_kernel(Product8 p)
     request(k0, 0);
     for (int k = k0; k < k1; ++k) {
         const int s = (k - k0) & 1;
-        __syncthreads();        // the stage is there, and nobody reads the other one any more
+        // the stage is there (a barrier alone does not wait for loads into shared memory), and nobody reads the other one any more
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
         if (((k - k0) & 3) == 0) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) ca[i] = na[i];
@@ -198,8 +200,27 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
     return p;
 }
 
+template <int BM, int BN, int WM, int WN, typename T, bool A5, bool B5> int tile_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
+{
+    p.tiles_m = (uint32_t)((p.M + BM - 1) / BM);
+    p.tiles_n = (uint32_t)((p.N + BN - 1) / BN);
+    return launch_main(product8_kernel<BM, BN, WM, WN, T, A5, B5>, dim3(p.tiles_m * p.tiles_n, (unsigned)plan.splits), dim3(WM * WN * 64), st, p);
+}
 template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
 {
+#ifdef GCG_TUNING
+    if constexpr (!A5 && !B5) {
+    const char *e = tuning_env("GCG_P8");
+    switch (e ? atoi(e) : 0) {
+    case 1: return tile_launch<256, 256, 2, 2, T, A5, B5>(p, plan, st);
+    case 2: return tile_launch<256, 256, 2, 4, T, A5, B5>(p, plan, st);
+    case 3: return tile_launch<256, 128, 2, 2, T, A5, B5>(p, plan, st);
+    case 4: return tile_launch<128, 256, 2, 2, T, A5, B5>(p, plan, st);
+    case 5: return tile_launch<256, 256, 4, 2, T, A5, B5>(p, plan, st);
+    case 6: return tile_launch<256, 128, 4, 2, T, A5, B5>(p, plan, st);
+    }
+    }
+#endif
     p.tiles_m = (uint32_t)((p.M + 127) / 128);
     p.tiles_n = (uint32_t)((p.N + 127) / 128);
     return launch_main(product8_kernel<128, 128, 2, 2, T, A5, B5>, dim3(p.tiles_m * p.tiles_n, (unsigned)plan.splits), dim3(256), st, p);
