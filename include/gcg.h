@@ -621,6 +621,10 @@ GCG_API int gcg_rms_norm_bwd(const void *dy, const void *r, const void *dr, cons
  * gcg_product8: y (M, N) = a b^T, contiguous, GCG_BF16 or GCG_F16, of a (M, K) and b (N, K) in 8 bits, accumulated in fp32.  workspace:
  * gcg_product8_workspace_bytes (0: none), 256-byte aligned.  K up to GCG_PRODUCT8_MAX_K.
  *
+ * gcg_linear8: y (M, N) = x b^T of a contiguous x (M, K) of type `dtype`, GCG_BF16 or GCG_F16, which the kernel quantises itself
+ * (GCG_E4M3; the same numbers as through gcg_to_float8), and b in 8 bits: for the few tokens of a decoding step.  Sizes for which
+ * gcg_linear8_supported returns 1 (x in 8 bits takes 16 KB at most, and M is 16 at most), else GCG_ERR_UNSUPPORTED.
+ *
  * codes are 16-byte aligned, scales 4-byte.  Results are the same on every run.
  */
 enum { GCG_E4M3 = 16, GCG_E5M2 = 17 };
@@ -633,6 +637,9 @@ GCG_API int gcg_to_float8_columns(const void *x, const uint8_t *x_scales, uint8_
 GCG_API size_t gcg_product8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 GCG_API int gcg_product8(const uint8_t *a, const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, void *y, void *workspace,
             size_t workspace_bytes, int64_t M, int64_t N, int64_t K, int32_t a_format, int32_t b_format, int32_t dtype, void *stream);
+GCG_API int gcg_linear8_supported(int64_t M, int64_t N, int64_t K);
+GCG_API int gcg_linear8(const void *x, const uint8_t *b, const uint8_t *b_scales, void *y, int64_t M, int64_t N, int64_t K, int32_t b_format,
+            int32_t dtype, void *stream);
 
 /*
  * Gated linear recurrence, channel by channel, with a state h (fp32) of D numbers a batch entry:

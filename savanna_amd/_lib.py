@@ -43,7 +43,7 @@ EXPORTS = (
     "gcg_pack8", "gcg_unpack8", "gcg_layer_norm_fwd", "gcg_layer_norm_bwd_workspace_bytes", "gcg_layer_norm_bwd",
     "gcg_linear_attn_workspace_bytes", "gcg_linear_attn_fwd", "gcg_linear_attn_bwd", "gcg_linear_attn_step",
     "gcg_rms_norm_fwd", "gcg_rms_norm_bwd_workspace_bytes", "gcg_rms_norm_bwd",
-    "gcg_to_float8", "gcg_from_float8", "gcg_to_float8_columns", "gcg_product8_workspace_bytes", "gcg_product8",
+    "gcg_to_float8", "gcg_from_float8", "gcg_to_float8_columns", "gcg_product8_workspace_bytes", "gcg_product8", "gcg_linear8_supported", "gcg_linear8",
     "gcg_scan_workspace_bytes", "gcg_scan_states", "gcg_scan_fwd", "gcg_scan_bwd", "gcg_scan_step",
 )
 
@@ -179,6 +179,8 @@ def load() -> ctypes.CDLL:
                 ("to_float8_columns", ctypes.c_int, [vp] * 6 + [i64, i64, i32, i32, vp]),
                 ("product8_workspace_bytes", sz, [i64, i64, i64]),
                 ("product8", ctypes.c_int, [vp] * 6 + [sz, i64, i64, i64, i32, i32, i32, vp]),
+                ("linear8_supported", ctypes.c_int, [i64, i64, i64]),
+                ("linear8", ctypes.c_int, [vp] * 4 + [i64, i64, i64, i32, i32, vp]),
                 ("scan_workspace_bytes", sz, [i64, i64, i32, i32]),
                 ("scan_states", i64, [i64]),
                 ("scan_fwd", ctypes.c_int, [vp] * 11 + [sz, i64, i64, i32, i32, vp]),
@@ -1636,7 +1638,16 @@ def linear_float8_infer(x, codes, scales, columns: int):
     _check_float8(codes, scales, columns)
     if codes.dim() != 2 or codes.device != x.device or x.shape[-1] != columns:
         raise ValueError("the weight must be a matrix on x's device with as many columns as x")
-    return matmul_float8(*to_float8(x, torch.float8_e4m3fn), codes, scales, columns, x.dtype)
+    N = codes.shape[0]
+    M = x.numel() // columns if columns else 0
+    if not load().gcg_linear8_supported(M, N, columns):
+        return matmul_float8(*to_float8(x, torch.float8_e4m3fn), codes, scales, columns, x.dtype)
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    with _on_device(x.device):
+        rc = load().gcg_linear8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), y.data_ptr(), M, N, columns, format_code(codes.dtype),
+                                dtype_code(x.dtype), torch.cuda.current_stream().cuda_stream)
+    check(rc, "gcg_linear8")
+    return y
 
 
 # ---- gated linear recurrence -----------------------------------------------------------------------------------

@@ -1116,6 +1116,23 @@ GCG_API int gcg_product8(const uint8_t *a, const uint8_t *a_scales, const uint8_
                                        (hipStream_t)stream));
 }
 
+GCG_API int gcg_linear8_supported(int64_t M, int64_t N, int64_t K)
+{
+    return M > 0 && N > 0 && K > 0 && K <= GCG_PRODUCT8_MAX_K && gcg::linear8_fits(M, K);
+}
+
+GCG_API int gcg_linear8(const void *x, const uint8_t *b, const uint8_t *b_scales, void *y, int64_t M, int64_t N, int64_t K, int32_t b_format,
+                        int32_t dtype, void *stream)
+{
+    TimerScope timer_scope;
+    if (!x || !placed(b, b_scales) || !y || M <= 0 || N <= 0 || K <= 0 || !is_format(b_format) || (dtype != GCG_BF16 && dtype != GCG_F16))
+        return GCG_ERR_BAD_ARG;
+    if (!gcg_linear8_supported(M, N, K)) return GCG_ERR_UNSUPPORTED;
+    const int rc = check_device();
+    if (rc) return rc;
+    return finish(gcg::linear8_launch(dtype, b_format == GCG_E5M2, x, b, b_scales, y, M, N, K, (hipStream_t)stream));
+}
+
 // ---- gated linear recurrence -----------------------------------------------------------------------------------
 
 namespace {

@@ -451,6 +451,10 @@ int to_float8_columns_launch(int dtype, int e5m2, int from5, const void *x, cons
 size_t product8_workspace(int64_t M, int64_t N, int64_t K);
 int product8_launch(int dtype, int a5, int b5, const uint8_t *a, const uint8_t *a_scales, const uint8_t *b, const uint8_t *b_scales, void *y,
                     void *ws, int64_t M, int64_t N, int64_t K, hipStream_t st);
+// x (M, K) b^T with x quantised in the kernel, of sizes that linear8_fits
+bool linear8_fits(int64_t M, int64_t K);
+int linear8_launch(int dtype, int b5, const void *x, const uint8_t *b, const uint8_t *b_scales, void *y, int64_t M, int64_t N, int64_t K,
+                   hipStream_t st);
 
 // gated linear recurrence; strides: batch and time of x, f, gate, y (dy, x, f, gate, dx, df, dgate; the step: rows of x, f, gate), in elements
 size_t scan_workspace(int64_t bs, int64_t L, int D, bool backward);

@@ -34,6 +34,7 @@ struct Product8 {
     int32_t S;                  // scales of a row
     int32_t steps;              // blocks of a row
     int32_t split_steps;        // blocks of a part, a multiple of four
+    int32_t splits;
     uint32_t tiles_m, tiles_n;
 };
 
@@ -176,6 +177,306 @@ __global__ __launch_bounds__(WM * WN * 64) void product8_kernel(Product8 p)
     }
 }
 
+// The same by four waves, one a SIMD, of 128 x 128 each.  A fragment is then read from shared memory for eight products, twice as many as in
+// the other kernel, and a block takes as long as 64 products; to keep those fed without a second wave, a block goes in four phases of 16, each of
+// one half of the wave's rows and one half of its columns, and each reads the half that is needed next where the one that is no longer needed was:
+//
+//   (A0 B0) reads B1,  (A0 B1) reads A1,  barrier,  (A1 B1) reads the next block's A0,  (A1 B0) reads its B1;  the next block starts with (A0 B1)
+//
+// At the barrier a stage has been read and the next one has arrived; the one after that is requested into it.  Four blocks, whose scales are a word
+// of each row, are one turn of the loop, without a branch in it: past the end the last block is requested again, and not used.  One to
+// three blocks that are left go one after the other.
+//
+// The requests are written out because the compiler makes every read of shared memory wait for all requests under way, whichever stage they go to.
+// They have no register to write, and the wait for them stands before the barrier.
+template <int BYTES> __device__ __forceinline__ void request_to_lds(win_t w, uint32_t to, uint32_t off, int at)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory");
+#endif
+}
+// The instruction with its accumulator where the compiler would not leave it by itself, in the 256 registers that only matrix instructions use.
+// An operand that a vector instruction has just written has to be two wait states old.
+template <bool A5, bool B5, int BYTE> __device__ __forceinline__ void mfma8_acc(const i32x8 &a, const i32x8 &b, f32x4 &c, uint32_t sa, uint32_t sb)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+#define GCG_MFMA8(SEL) \
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " SEL " cbsz:%5 blgp:%6" \
+                 : "+a"(c) : "v"(a), "v"(b), "v"(sa), "v"(sb), "n"(A5 ? 1 : 0), "n"(B5 ? 1 : 0))
+    if constexpr (BYTE == 0) GCG_MFMA8("op_sel_hi:[0,0,0]");
+    else if constexpr (BYTE == 1) GCG_MFMA8("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+    else if constexpr (BYTE == 2) GCG_MFMA8("op_sel_hi:[1,1,0]");
+    else GCG_MFMA8("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#undef GCG_MFMA8
+#endif
+}
+
+template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) void product8_wide_kernel(Product8 p)
+{
+    constexpr int BM = 256, BN = 256, LOADS = 8, STAGE = (BM + BN) * 128;
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[2][STAGE];
+    __shared__ uint32_t words[2][BM + BN];
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64;
+    const uint32_t tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
+    int64_t m0, n0;
+    int k0, k1, split;
+    win_t wa, wb, wsa, wsb;
+    const auto take = [&](uint32_t item) {
+        split = (int)(item / tiles);
+        const uint32_t tile = xcd_contiguous_u32(item - split * tiles, tiles);
+        const uint32_t group = tile / (8 * p.tiles_n), first = group * 8, high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
+        const uint32_t in = tile - group * 8 * p.tiles_n;
+        // tiles that would reach beyond the tensor start earlier and make some of their neighbours' results again, the same bits (M, N >= 256)
+        m0 = (int64_t)(first + in % high) * BM;
+        n0 = (int64_t)(in / high) * BN;
+        m0 = m0 < p.M - BM ? m0 : p.M - BM;
+        n0 = n0 < p.N - BN ? n0 : p.N - BN;
+        k0 = split * p.split_steps;
+        k1 = p.steps - k0 < p.split_steps ? p.steps : k0 + p.split_steps;
+        wa = make_window(p.a + m0 * p.Kp, 0x7fffffff);
+        wb = make_window(p.b + n0 * p.Kp, 0x7fffffff);
+        wsa = make_window(p.a_scales + m0 * p.S, 0x7fffffff);
+        wsb = make_window(p.b_scales + n0 * p.S, 0x7fffffff);
+    };
+
+    // a thread's pieces: row t / 8 + 32 i of the tile, the piece that belongs to place t % 8
+    const uint32_t piece = (uint32_t)(t / 8 * p.Kp) + ((t % 8) ^ ((t >> 4) & 7)) * 16;
+    const int rows32 = __builtin_amdgcn_readfirstlane((int)(32 * p.Kp));
+    const uint32_t lds = (uint32_t)(uintptr_t)(lds_t)stage[0] + wave * 1024, lds_words = (uint32_t)(uintptr_t)(lds_t)words[0] + wave * 256;
+    const auto request_piece = [&](int at, int s, int i) {
+        request_to_lds<16>(wa, lds + s * STAGE + i * 4096, piece, at + i * rows32);
+        request_to_lds<16>(wb, lds + s * STAGE + BM * 128 + i * 4096, piece, at + i * rows32);
+    };
+    const auto place_of = [&](int k) { return __builtin_amdgcn_readfirstlane((k < k1 ? k : k1 - 1) * 128); };
+    const auto request = [&](int k, int s) {
+        const int at = place_of(k);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) request_piece(at, s, i);
+    };
+    // the scales of the tile's rows for four blocks from k on, a word a row
+    const uint32_t row_scales = (uint32_t)(t * p.S);
+    const auto request_words = [&](int k, int s) {
+        const int at = __builtin_amdgcn_readfirstlane((k < k1 ? k : k1 - 1) / 4 * 4);
+        request_to_lds<4>(wsa, lds_words + s * ((BM + BN) * 4), row_scales, at);
+        request_to_lds<4>(wsb, lds_words + s * ((BM + BN) * 4) + BM * 4, row_scales, at);
+    };
+
+    const int wm = wave & 1, wn = wave >> 1, r16 = lane % 16, quarter = lane / 16, swap = (r16 >> 1) & 7;
+    const int fa = (wm * 128 + r16) * 128, fb = BM * 128 + (wn * 128 + r16) * 128;
+    const int p0 = (quarter ^ swap) * 16, p1 = ((quarter + 4) ^ swap) * 16;
+    const auto fragment = [&](int s, int at) {
+        const u32x4 lo = *(const u32x4 *)(stage[s] + at + p0), hi = *(const u32x4 *)(stage[s] + at + p1);
+        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
+    uint32_t ca[8], cb[8];
+    const auto take_words = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            ca[i] = words[s][wm * 128 + i * 16 + r16];
+            cb[i] = words[s][BM + wn * 128 + i * 16 + r16];
+        }
+    };
+    f32x4 acc[8][8];
+    i32x8 A[2][4], B[2][4];
+    // 16 products of half I of the rows and half J of the columns, and between them the four fragments at `from` of stage s into `to`, and with
+    // `more` the requests for block k into the other stage.  (These statements stay in the order they are written in.)
+    const auto phase = [&](auto i_, auto j_, auto byte_, i32x8(&to)[4], int s, int from, auto more_, int at) {
+        constexpr int i = decltype(i_)::value, j = decltype(j_)::value, byte = decltype(byte_)::value;
+        constexpr bool more = decltype(more_)::value;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const u32x4 part = *(const u32x4 *)(stage[s] + from + q / 2 * 16 * 128 + (q % 2 ? p1 : p0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[q / 2][q % 2 * 4 + e] = (int)part[e];
+            if constexpr (more) {
+                request_piece(at, s ^ 1, q);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int x = q / 2, y = q % 2 * 2 + h;
+                mfma8_acc<B5, A5, byte>(B[j][y], A[i][x], acc[i * 4 + x][j * 4 + y], cb[j * 4 + y], ca[i * 4 + x]);
+            }
+        }
+    };
+    constexpr std::integral_constant<int, 0> zero;
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 3> three;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    const auto hand_over = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    // one block, whose first half of columns is J (whose fragments, and those of A's first half, are there)
+    const auto block = [&](int k, auto s_, auto byte_) {
+        constexpr int s = decltype(s_)::value, J = s, notJ = 1 - s;
+        constexpr std::integral_constant<int, J> j;
+        constexpr std::integral_constant<int, notJ> not_j;
+        phase(zero, j, byte_, B[notJ], s, fb + notJ * 64 * 128, no, 0);
+        phase(zero, not_j, byte_, A[1], s, fa + 64 * 128, no, 0);
+        hand_over();
+        phase(one, not_j, byte_, A[0], s ^ 1, fa, yes, place_of(k + 2));
+        phase(one, j, byte_, B[notJ], s ^ 1, fb + notJ * 64 * 128, no, 0);
+    };
+
+    take(blockIdx.x);
+    request_words(k0, 0);
+    request(k0, 0);
+    request(k0 + 1, 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (uint32_t item = blockIdx.x;;) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { A[0][q] = fragment(0, fa + q * 16 * 128); B[0][q] = fragment(0, fb + q * 16 * 128); }
+    int k = k0, w = 0;
+    for (; k + 4 <= k1; k += 4, w ^= 1) {
+        take_words(w);
+        request_words(k + 4, w ^ 1);
+        block(k, zero, zero);
+        block(k + 1, one, one);
+        block(k + 2, zero, two);
+        block(k + 3, one, three);
+    }
+    if (k < k1) take_words(w);
+    for (; k < k1; ++k) {
+        const int s = (k - k0) & 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                A[h][q] = fragment(s, fa + (h * 4 + q) * 16 * 128);
+                B[h][q] = fragment(s, fb + (h * 4 + q) * 16 * 128);
+            }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mfma8_acc<B5, A5, 0>(B[j / 4][j % 4], A[i / 4][i % 4], acc[i][j], cb[j], ca[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { ca[i] >>= 8; cb[i] >>= 8; }
+        hand_over();
+        request(k + 2, s);
+    }
+    // A wave's results leave in whole rows of 128 columns, which lie together in shared memory first: a pass of 64 rows (fp32: 32) in its quarter of
+    // the second stage, the 16-byte pieces of a row at exchanged places.  The next tile's first block is on its way to the first stage by then.
+    constexpr int ROWS = 16384 / (128 * (int)sizeof(T)), PIECES = 128 * (int)sizeof(T) / 16;
+    uint8_t *y = (uint8_t *)((p.partial ? (T *)(p.partial + (int64_t)split * p.M * p.N) : (T *)p.y) + (m0 + wm * 128) * p.N + n0 + wn * 128);
+    hand_over();                                                                // nobody reads a stage any more, and nothing arrives
+    item += gridDim.x;
+    const bool more = item < items;
+    if (more) {
+        take(item);
+        request_words(k0, 0);
+        request(k0, 0);
+    }
+    asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");             // the last products have written their accumulators
+    int l = lane;
+    asm volatile("" : "+v"(l));                                                 // (addresses are formed here, not kept over the products)
+    uint8_t *mine = stage[1] + wave * 16384;
+    const int64_t down = 64 / PIECES * p.N * (int64_t)sizeof(T);                // from one store's rows to the next one's
+    const uint32_t off = (uint32_t)(l / PIECES * p.N * (int64_t)sizeof(T)) + l % PIECES * 16;
+#pragma unroll
+    for (int r = 0; r < 128; r += ROWS) {
+#pragma unroll
+        for (int i = r / 16; i < (r + ROWS) / 16; ++i) {
+            const int row = i * 16 - r + l % 16;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                asm volatile("" : "+a"(acc[i][j]));         // (read after that wait)
+                const int at = (j * 16 + l / 16 * 4) * (int)sizeof(T);
+                store4((T *)(mine + row * (PIECES * 16) + (((at / 16) ^ (row & 15)) * 16) + at % 16), acc[i][j], 4, true);
+            }
+        }
+        // (a wave reads what it has written itself)
+#pragma unroll
+        for (int q = 0; q < ROWS * PIECES / 64; ++q) {
+            const int row = (q * 64 + l) / PIECES, piece = l % PIECES;
+            const u32x4 v = *(const u32x4 *)(mine + row * (PIECES * 16) + ((piece ^ (row & 15)) * 16));
+            *(u32x4_any *)(y + off) = v;
+            y += down;
+        }
+    }
+    if (!more) return;
+    __syncthreads();
+    request(k0 + 1, 1);
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");           // all but the second block
+    }
+}
+
+// Few rows of a (tokens, 16 at most): what counts is how fast b's rows arrive.  A workgroup takes 16 of them, its W waves each a part of the blocks;
+// fragments come straight from memory into registers, UNROLL blocks' at a time, each row's 128 bytes by two instructions of 64.  With FUSED, a is
+// a tensor of type T, and the workgroup quantises it into shared memory while b's first rows are on their way: kTokenBytes of codes at most, since
+// every workgroup does.  The waves' sums join in shared memory, in their order.
+constexpr int kTokenBytes = 16384;
+struct Tokens8 {
+    Product8 p;
+    const void *x;              // FUSED: a in its own type
+    int64_t K;
+};
+template <typename T, int W, bool FUSED, bool A5, bool B5> __global__ __launch_bounds__(W * 64) void product8_tokens_kernel(Tokens8 s)
+{
+    constexpr int UNROLL = 8;
+    const Product8 &p = s.p;
+    __shared__ f32x4 sums[W - 1][64];
+    __shared__ __attribute__((aligned(16))) uint8_t own[FUSED ? kTokenBytes : 16];
+    __shared__ uint8_t own_scales[FUSED ? kTokenBytes / 128 : 1];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, quarter = lane / 16;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1, m = r16 < p.M ? r16 : p.M - 1;
+    const int per = (p.steps + W - 1) / W, k0 = wave * per, k1 = k0 + per < p.steps ? k0 + per : p.steps;
+    const uint8_t *b = p.b + n * p.Kp + quarter * 16, *sb = p.b_scales + n * p.S;
+    const uint8_t *a = (FUSED ? own : p.a) + m * p.Kp + quarter * 16, *sa = FUSED ? own_scales + m * p.steps : p.a_scales + m * p.S;
+    const auto fragment = [](const uint8_t *from) {
+        const u32x4 lo = *(const u32x4 *)from, hi = *(const u32x4 *)(from + 64);
+        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
+    i32x8 fb[UNROLL];
+    uint32_t cb[UNROLL];
+    const auto request = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t at = k + u < k1 ? k + u : p.steps - 1;
+            fb[u] = fragment(b + at * 128);
+            cb[u] = sb[at];
+        }
+    };
+    request(k0);
+    if constexpr (FUSED) {
+        // sixteen lanes a block, whole waves at a time
+        const int blocks = (int)p.M * p.steps, c = threadIdx.x % 16 * 8;
+        for (int i = threadIdx.x / 16; i < (blocks + 3) / 4 * 4; i += W * 4) {
+            const int row = i / p.steps, k = i - row * p.steps;
+            const int64_t left = s.K - (k * 128 + c);
+            u32x4 raw = {0, 0, 0, 0};
+            if (i < blocks && left > 0) raw = load_row_vec<T, true, false>((const T *)s.x + row * s.K + k * 128 + c, 0, (int)(left < 8 ? left : 8));
+            float v[8];
+            unpack_vec(raw, v, T{});
+            store_f8<8, A5, false>(own + i * 128, own_scales + i, c, i < blocks ? 128 : 0, v);
+        }
+        __syncthreads();
+    }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = k0; k < k1; k += UNROLL) {
+        if (k > k0) request(k);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (k + u < k1) acc = mfma8<B5, A5>(fb[u], fragment(a + (k + u) * 128), acc, cb[u], sa[k + u]);
+    }
+    if (wave > 0) sums[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0 || r16 >= p.M) return;
+#pragma unroll
+    for (int w = 0; w < W - 1; ++w) acc += sums[w][lane];
+    T *y = (T *)p.y + m * p.N + n0 + quarter * 4;
+    store4(y, acc, p.N - n0 - quarter * 4, p.N % 4 == 0 && ((uintptr_t)p.y & (4 * sizeof(T) - 1)) == 0);
+}
+
 // the parts of a product that was split over its blocks, added in their order
 template <typename T> __global__ __launch_bounds__(256) void product8_join_kernel(const float *partial, T *y, int64_t n, int splits)
 {
@@ -186,18 +487,44 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
     }
 }
 
-struct Plan8 { int tile; int splits; int split_steps; };
+// Which kernel, and in how many parts of the blocks (each a sum in fp32, joined by another kernel): what would take the least time.
+// Few rows go by product8_tokens_kernel: 12288 x 4096 with 1 row 12.3 us (tiles of 128 in four parts 14.5), with 16 rows 17.8 (14.8).
+// Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.3 a block and 6 around them; 512 tiles of 128 x 128 (two
+// a CU) take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice at 4 TB/s, and 3 for its launch.  So
+// 4096 x 4096 x 4096 goes wide (53.6; 88.1), 2048 x 4096 x 4096 either way (47.0; 46.9), 1024 x 4096 x 4096 in small tiles (36.1; 43.6),
+// 7680 x 2561 x 5003 wide although its second round is short (118.9; 143.6), 512 x 512 x 16384 in small tiles and parts (121.7 in one, 37.0 in four).
+enum { TOKENS = 0, TILE = 128, WIDE = 256 };
+constexpr int kTokens = 8;
+struct Plan8 { int kernel, splits, split_steps; };
+float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
+{
+    const int64_t items = ((M + kernel - 1) / kernel) * ((N + kernel - 1) / kernel) * splits;
+    const float join = splits > 1 ? 3.f + (float)M * (float)N * (float)splits * 8.f / 4e6f : 0.f;
+    if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.3f + 6.f) + join;
+    return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + join;
+}
 Plan8 plan_of(int64_t M, int64_t N, int64_t K)
 {
     const int steps = (int)(f8_cols(K) / 128);
-    const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128);
-    Plan8 p = {128, 1, (steps + 3) / 4 * 4};
-    while (tiles * p.splits < 256 && p.split_steps >= 8) {
-        p.splits *= 2;
-        p.split_steps = ((steps + p.splits - 1) / p.splits + 3) / 4 * 4;
+    if (const char *e = tuning_env("GCG_P8")) {
+        const char *s = tuning_env("GCG_P8S");
+        const int n = s ? atoi(s) : 1, per = ((steps + n - 1) / n + 3) / 4 * 4, kernel = atoi(e);
+        if ((kernel == WIDE && (M < 256 || N < 256)) || (kernel == TOKENS && M > 16)) return {TILE, 1, (steps + 3) / 4 * 4};
+        return {kernel, (steps + per - 1) / per, per};
     }
-    p.splits = (steps + p.split_steps - 1) / p.split_steps;
-    return p;
+    if (M <= kTokens) return {TOKENS, 1, steps};
+    Plan8 best = {TILE, 1, (steps + 3) / 4 * 4};
+    float least = 0.f;
+    for (int kernel = TILE; kernel <= (M >= 256 && N >= 256 ? WIDE : TILE); kernel *= 2)
+        for (int n = 1; n == 1 || (n <= 32 && steps >= 4 * n); n *= 2) {
+            const int per = ((steps + n - 1) / n + 3) / 4 * 4, splits = (steps + per - 1) / per;
+            const float time = estimate(kernel, M, N, splits > 1 ? per : steps, splits);
+            if (least == 0.f || time < least) {
+                least = time;
+                best = {kernel, splits, per};
+            }
+        }
+    return best;
 }
 
 template <int BM, int BN, int WM, int WN, typename T, bool A5, bool B5> int tile_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
@@ -206,24 +533,26 @@ template <int BM, int BN, int WM, int WN, typename T, bool A5, bool B5> int tile
     p.tiles_n = (uint32_t)((p.N + BN - 1) / BN);
     return launch_main(product8_kernel<BM, BN, WM, WN, T, A5, B5>, dim3(p.tiles_m * p.tiles_n, (unsigned)plan.splits), dim3(WM * WN * 64), st, p);
 }
+template <typename T, bool FUSED, bool A5, bool B5> int tokens_launch(const Tokens8 &s, hipStream_t st)
+{
+    const dim3 grid((unsigned)((s.p.N + 15) / 16));
+    // eight waves where four a workgroup would leave the card half empty
+    return grid.x < 512 && s.p.steps >= 16 ? launch_main(product8_tokens_kernel<T, 8, FUSED, A5, B5>, grid, dim3(512), st, s)
+                                           : launch_main(product8_tokens_kernel<T, 4, FUSED, A5, B5>, grid, dim3(256), st, s);
+}
 template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
 {
-#ifdef GCG_TUNING
-    if constexpr (!A5 && !B5) {
-    const char *e = tuning_env("GCG_P8");
-    switch (e ? atoi(e) : 0) {
-    case 1: return tile_launch<256, 256, 2, 2, T, A5, B5>(p, plan, st);
-    case 2: return tile_launch<256, 256, 2, 4, T, A5, B5>(p, plan, st);
-    case 3: return tile_launch<256, 128, 2, 2, T, A5, B5>(p, plan, st);
-    case 4: return tile_launch<128, 256, 2, 2, T, A5, B5>(p, plan, st);
-    case 5: return tile_launch<256, 256, 4, 2, T, A5, B5>(p, plan, st);
-    case 6: return tile_launch<256, 128, 4, 2, T, A5, B5>(p, plan, st);
+    if constexpr (sizeof(T) == 2) {
+        if (plan.kernel == TOKENS) {
+            const Tokens8 s = {p, nullptr, 0};
+            return tokens_launch<T, false, A5, B5>(s, st);
+        }
     }
-    }
-#endif
-    p.tiles_m = (uint32_t)((p.M + 127) / 128);
-    p.tiles_n = (uint32_t)((p.N + 127) / 128);
-    return launch_main(product8_kernel<128, 128, 2, 2, T, A5, B5>, dim3(p.tiles_m * p.tiles_n, (unsigned)plan.splits), dim3(256), st, p);
+    if (plan.kernel == TILE) return tile_launch<128, 128, 2, 2, T, A5, B5>(p, plan, st);
+    p.tiles_m = (uint32_t)((p.M + 255) / 256);
+    p.tiles_n = (uint32_t)((p.N + 255) / 256);
+    const int64_t items = (int64_t)p.tiles_m * p.tiles_n * plan.splits;
+    return launch_main(product8_wide_kernel<T, A5, B5>, dim3((unsigned)(items < 256 ? items : 256)), dim3(256), st, p);
 }
 template <typename T> int product_format(Product8 &p, int a5, int b5, const Plan8 &plan, hipStream_t st)
 {
@@ -253,8 +582,19 @@ int product8_launch(int dtype, int a5, int b5, const uint8_t *a, const uint8_t *
 {
     const Plan8 plan = plan_of(M, N, K);
     Product8 p = {a, a_scales, b, b_scales, y, plan.splits > 1 ? (float *)ws : nullptr, M, N, f8_cols(K), (int32_t)f8_scales(K),
-                  (int32_t)(f8_cols(K) / 128), plan.split_steps, 0, 0};
+                  (int32_t)(f8_cols(K) / 128), plan.split_steps, plan.splits, 0, 0};
     return dtype == GCG_BF16 ? product_type<bf16_t>(p, a5, b5, plan, st) : product_type<f16_t>(p, a5, b5, plan, st);
+}
+
+bool linear8_fits(int64_t M, int64_t K) { return M <= 16 && M * f8_cols(K) <= kTokenBytes; }
+
+int linear8_launch(int dtype, int b5, const void *x, const uint8_t *b, const uint8_t *b_scales, void *y, int64_t M, int64_t N, int64_t K,
+                   hipStream_t st)
+{
+    const Product8 p = {nullptr, nullptr, b, b_scales, y, nullptr, M, N, f8_cols(K), (int32_t)f8_scales(K), (int32_t)(f8_cols(K) / 128), 0, 1, 0, 0};
+    const Tokens8 s = {p, x, K};
+    if (dtype == GCG_BF16) return b5 ? tokens_launch<bf16_t, true, false, true>(s, st) : tokens_launch<bf16_t, true, false, false>(s, st);
+    return b5 ? tokens_launch<f16_t, true, false, true>(s, st) : tokens_launch<f16_t, true, false, false>(s, st);
 }
 
 } // namespace gcg

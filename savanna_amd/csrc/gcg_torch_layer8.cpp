@@ -184,8 +184,17 @@ Tensor linear_float8_infer(const Tensor &x, const Tensor &codes, const Tensor &s
 {
     require_gpu(x, "x");
     check_linear(x, codes, scales, columns);
-    auto [c, s] = to_float8(x, at::kFloat8_e4m3fn);
-    return matmul_float8(c, s, codes, scales, columns, x.scalar_type());
+    const int64_t M = rows_of(x), N = codes.size(0);
+    if (!gcg_linear8_supported(M, N, columns)) {
+        auto [c, s] = to_float8(x, at::kFloat8_e4m3fn);
+        return matmul_float8(c, s, codes, scales, columns, x.scalar_type());
+    }
+    DeviceGuard guard(x.device());
+    Tensor y = at::empty(with_last(x, N), x.options());
+    check_rc(gcg_linear8(x.data_ptr(), bytes(codes), bytes(scales), y.data_ptr(), M, N, columns, format_code(codes.scalar_type()),
+                         dtype_code(x.scalar_type()), stream_of(x)),
+             "gcg_linear8");
+    return y;
 }
 
 Two to_float8_meta(const Tensor &x, at::ScalarType format)
