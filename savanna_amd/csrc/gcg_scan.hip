@@ -63,22 +63,17 @@ template <int C> __device__ __forceinline__ void store_channels(win_t w, uint32_
     }
 }
 
-// a = sigmoid(z) and b = 1 - a = sigmoid(-z), each to its own last bits: e = exp(-|z|), 1 / (1 + e) and e / (1 + e).  With EXACT (fp32
-// tensors) the rounding of z log2(e) is put back and the reciprocal refined; for 16-bit tensors they are far below the output's own.
+// a = sigmoid(z) and b = 1 - a = sigmoid(-z): with e = exp(-|z|) the smaller is e / (1 + e), the larger 1 less it, to half a unit of its last bit.  (As
+// a reciprocal of its own, a whole unit off, it takes 1e-6 from a state in some hundred rows: the decays multiply.)  EXACT (fp32 tensors): what
+// the rounding of |z| log2(e) takes from e is put back.
 template <bool EXACT> __device__ __forceinline__ void sigmoids(float z, float &a, float &b)
 {
-    const float m = -fabsf(z), t = m * 1.44269504f;
+    const float m = fmaxf(-fabsf(z), -200.f), t = m * 1.44269504f;
     float e = __builtin_amdgcn_exp2f(t);
-    if constexpr (EXACT) {
-        const float lost = fmaf(m, 1.44269504f, -t) + m * 1.92596299e-8f;
-        if (t > -126.f) e = fmaf(e * 0.693147181f, lost, e);
-    }
-    const float d = 1.f + e;
-    float r = __builtin_amdgcn_rcpf(d);
-    if constexpr (EXACT) r = fmaf(r, fmaf(-d, r, 1.f), r);
-    const float s = e * r;
-    a = z < 0.f ? s : r;
-    b = z < 0.f ? r : s;
+    if constexpr (EXACT) e = fmaf(e * 0.693147181f, fmaf(m, 1.44269504f, -t), e);
+    const float s = e * __builtin_amdgcn_rcpf(1.f + e), l = 1.f - s;
+    a = z < 0.f ? s : l;
+    b = z < 0.f ? l : s;
     if (z != z) a = b = z;
 }
 
@@ -133,10 +128,13 @@ template <typename T> __device__ __forceinline__ win_t window_of(const ScanTenso
     return make_window((const T *)t.p + b * t.batch + row * t.time, rows > 0 ? ((int64_t)(rows - 1) * t.time + D) * (int64_t)sizeof(T) : 0);
 }
 
-// The state that enters a chunk: `from` (of the group's start, given or waited for) through the pairs at first, first + step, ..., n of them.
-template <int C> __device__ __forceinline__ void through(const uint64_t *first, int64_t step, int n, bool here, float (&h)[C])
+// The pair (A, H) of the n pairs at first, first + step, ...: what a chunk's predecessors in its group do to the state.  (Put together before the
+// state of the group's start is waited for, so that a state passes a group in the time of one word's way.)
+template <int C> __device__ __forceinline__ void together(const uint64_t *first, int64_t step, int n, bool here, float (&A)[C], float (&H)[C])
 {
-    constexpr int B = 4;
+    constexpr int B = 4 / C;
+#pragma unroll
+    for (int c = 0; c < C; ++c) { A[c] = 1.f; H[c] = 0.f; }
     for (int i = 0; i < n; i += B) {
         uint64_t w[B][C];
 #pragma unroll
@@ -149,14 +147,16 @@ template <int C> __device__ __forceinline__ void through(const uint64_t *first, 
             for (int c = 0; c < C; ++c) {
                 if (i + k < n) {
                     w[k][c] = wait_for(first + (i + k) * step + c, w[k][c]);
-                    h[c] = fmaf(word_A(w[k][c]), h[c], word_H(w[k][c]));
+                    const float Ak = word_A(w[k][c]);
+                    H[c] = fmaf(Ak, H[c], word_H(w[k][c]));
+                    A[c] = kept_decay(A[c] * Ak, fminf(A[c], Ak));
                 }
             }
     }
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
-template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds__(W * 64) void scan_fwd_kernel(Scan p)
+template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds__(W * 64, 4) void scan_fwd_kernel(Scan p)
 {
     constexpr int ROWS = R * W, E = (int)sizeof(T);
     __shared__ float pairA[W][64 * C], pairH[W][64 * C], enter[64 * C];
@@ -244,12 +244,15 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
 #pragma unroll
                 for (int c = 0; c < C; ++c) publish(mine + c, word_of(TA[c], TH[c]));
             }
+            float GA[C], GH[C];
+            together<C>(mine - (int64_t)j * p.D, p.D, j, here, GA, GH);
             if (g > 0 && here) {
                 const uint64_t *from = p.carries + ((int64_t)at.b * ((p.chunks + p.group - 1) / p.group) + g) * p.D + ch;
 #pragma unroll
                 for (int c = 0; c < C; ++c) h[c] = word_H(wait_for(from + c, look(from + c)));
             }
-            through<C>(mine - (int64_t)j * p.D, p.D, j, here, h);
+#pragma unroll
+            for (int c = 0; c < C; ++c) h[c] = fmaf(GA[c], h[c], GH[c]);
             if (here && j + 1 == p.group && at.c + 1 < p.chunks) {
                 uint64_t *to = p.carries + ((int64_t)at.b * ((p.chunks + p.group - 1) / p.group) + g + 1) * p.D + ch;
 #pragma unroll
@@ -288,7 +291,7 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------------
-template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(Scan p)
+template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds__(W * 64, 4) void scan_bwd_kernel(Scan p)
 {
     constexpr int ROWS = R * W, E = (int)sizeof(T);
     static_assert(ROWS == kChunk, "a chunk starts at a kept state");
@@ -327,32 +330,42 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
         h0[c] = here ? p.states[((int64_t)at.b * p.kept + at.c) * p.D + ch + c] : 0.f;
     }
 
-    float a[R][C], b[R][C], gd[R][C], A[C], H[C], K[C], least[C];
+    float a[R][C], b[R][C], A[C], H[C], K[C], least[C];
+    // gate dy of row i
+    const auto weighted = [&](int i, float (&v)[C]) {
+        channels(rd[i], v, T{});
+        if constexpr (GATE) {
+            float g[C];
+            channels(rg[i], g, T{});
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[c] *= g[c];
+        }
+    };
 #pragma unroll
     for (int c = 0; c < C; ++c) { A[c] = 1.f; H[c] = 0.f; K[c] = 0.f; least[c] = 1.f; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        float x[C], f[C], d[C], g[C];
+        float x[C], f[C];
         channels(rx[i], x, T{});
         channels(rf[i], f, T{});
-        channels(rd[i], d, T{});
-        if constexpr (GATE) channels(rg[i], g, T{});
         const bool inside = slot * R + i < rows;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             sigmoids<E == 4>(f[c] + bias[c], a[i][c], b[i][c]);
             a[i][c] = inside ? a[i][c] : 1.f;
             b[i][c] = inside ? b[i][c] : 0.f;
-            gd[i][c] = GATE ? g[c] * d[c] : d[c];
             A[c] *= a[i][c];
             H[c] = fmaf(a[i][c], H[c], b[i][c] * x[c]);
             least[c] = fminf(least[c], a[i][c]);
         }
     }
 #pragma unroll
-    for (int i = R - 1; i >= 0; --i)
+    for (int i = R - 1; i >= 0; --i) {
+        float gd[C];
+        weighted(i, gd);
 #pragma unroll
-        for (int c = 0; c < C; ++c) K[c] = a[i][c] * (gd[i][c] + K[c]);
+        for (int c = 0; c < C; ++c) K[c] = a[i][c] * (gd[c] + K[c]);
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         A[c] = kept_decay(A[c], least[c]);
@@ -392,13 +405,16 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
 #pragma unroll
                 for (int c = 0; c < C; ++c) publish(mine + c, word_of(TA[c], TK[c]));
             }
+            const int behind = end < last ? end : last;
+            float GA[C], GK[C];
+            together<C>(mine + (int64_t)(behind - at.c) * p.D, -(int64_t)p.D, behind - at.c, here, GA, GK);
             if (end < last && here) {
                 const uint64_t *from = p.carries + ((int64_t)at.b * ((p.chunks + p.group - 1) / p.group) + g) * p.D + ch;
 #pragma unroll
                 for (int c = 0; c < C; ++c) k[c] = word_H(wait_for(from + c, look(from + c)));
             }
-            const int behind = end < last ? end : last;
-            through<C>(mine + (int64_t)(behind - at.c) * p.D, -(int64_t)p.D, behind - at.c, here, k);
+#pragma unroll
+            for (int c = 0; c < C; ++c) k[c] = fmaf(GA[c], k[c], GK[c]);
             if (here && at.c == g * p.group && g > 0) {
                 uint64_t *to = p.carries + ((int64_t)at.b * ((p.chunks + p.group - 1) / p.group) + g - 1) * p.D + ch;
 #pragma unroll
@@ -412,8 +428,13 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
             for (int c = 0; c < C; ++c) p.dinitial[(int64_t)at.b * p.D + ch + c] = rows > 0 ? fmaf(TA[c], k[c], TK[c]) : k[c];
         }
     }
-    // dgate, and what df is times G, while the first slot waits
+    // dgate, and what df is times G, while the first slot waits.  (The raw rows are converted again, not kept in fp32 over the barrier.)
     float q[R][C];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        asm volatile("" : "+v"(rd[i]), "+v"(rx[i]));
+        if constexpr (GATE) asm volatile("" : "+v"(rg[i]));
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         float x[C], d[C], dg[C];
@@ -433,11 +454,12 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
     for (int c = 0; c < C; ++c) { k[c] = fmaf(PA[c], enter[lane * C + c], PK[c]); sum[c] = 0.f; }
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
-        float dx[C], df[C];
+        float dx[C], df[C], gd[C];
+        weighted(i, gd);
         const bool inside = slot * R + i < rows;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const float G = gd[i][c] + k[c];
+            const float G = gd[c] + k[c];
             dx[c] = inside ? b[i][c] * G : 0.f;
             df[c] = inside ? q[i][c] * G : 0.f;
             sum[c] += df[c];
@@ -512,14 +534,15 @@ template <typename T, bool GATE> __global__ __launch_bounds__(256) void scan_ste
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
 constexpr int kFwdRows = 128;       // rows of a chunk of the forward
-int group_of(int64_t chunks) { return chunks <= 256 ? 8 : 32; }
+// Chunks of a group: 131072 x 512 fp32 193 us with 8, 196 with 16, 223 with 32; 2 x 8192 x 4096 bf16 113, 118 and 131.
+constexpr int kGroup = 8;
 
 struct Layout { int64_t chunks, groups, pairs, carries, total; };
 Layout layout_of(int64_t bs, int64_t L, int64_t D, bool backward)
 {
     Layout l;
     l.chunks = (L + (backward ? kChunk : kFwdRows) - 1) / (backward ? kChunk : kFwdRows);
-    l.groups = (l.chunks + group_of(l.chunks) - 1) / group_of(l.chunks);
+    l.groups = (l.chunks + kGroup - 1) / kGroup;
     l.pairs = 256;
     l.carries = l.pairs + bs * l.chunks * D * 8;
     l.total = l.chunks > 1 ? (l.carries + bs * l.groups * D * 8 + 255) / 256 * 256 : 0;
@@ -530,7 +553,7 @@ Layout layout_of(int64_t bs, int64_t L, int64_t D, bool backward)
 int set_up(Scan &p, const Layout &l, void *ws, hipStream_t st)
 {
     p.chunks = (int32_t)l.chunks;
-    p.group = group_of(l.chunks);
+    p.group = kGroup;
     p.pairs = p.carries = nullptr;
     p.ticket = nullptr;
     if (l.chunks == 1) return 0;
