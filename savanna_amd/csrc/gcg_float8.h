@@ -8,8 +8,8 @@
 //
 // Powers of two make scaling exact: a code is its element rounded once, to 4 (3) significant bits, the matrix instructions apply the
 // bytes by themselves, and what is already in 8 bits is quantised again along its other dimension without another rounding (only
-// numbers 2^15 times smaller than the largest of the new block lose bits).  A block that holds an infinity or a NaN takes the largest
-// scale, 2^120: these become NaN (an infinity stays one with 5 bits of exponent) and numbers below 2^110 zero.
+// numbers 2^15 times smaller than the largest of the new block lose bits).  A block that holds an infinity or a NaN takes the scale of fp32's
+// largest numbers, 2^120 (5 bits of exponent: 2^113): these become NaN (an infinity stays one with 5 bits) and numbers below 2^110 (2^96) zero.
 #pragma once
 #include "gcg_row.h"
 

@@ -32,8 +32,8 @@ class Float8(NamedTuple):
 def to_float8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Float8:
     """x (float32, bfloat16 or float16) in 8 bits: of each block of 128 along the last dimension the scale is the smallest power of two, 2^-127
     at least, that brings the largest magnitude to at most 448 (``float8_e5m2``: 57344), and a code the element over it, rounded to nearest even.  A block
-    that holds an infinity or a NaN has the scale 2^120; they become NaN (in ``float8_e5m2`` an infinity stays one) and smaller numbers than 2^110
-    zero.  Not differentiable: x's own graph is left alone."""
+    that holds an infinity or a NaN has the scale 2^120 (``float8_e5m2``: 2^113); they become NaN (in ``float8_e5m2`` an infinity stays one) and
+    numbers below 2^110 (2^96) zero.  Not differentiable: x's own graph is left alone."""
     x = x.detach()
     return Float8(*_lib.to_float8(x if x.is_contiguous() else x.contiguous(), dtype), x.shape[-1])
 

@@ -1,0 +1,242 @@
+"""Products of 8-bit tensors.
+
+Whole numbers: with elements that 8 bits hold, scales of small powers of two and sums below 2^24 every product and sum is exact (what an
+instruction cuts off lies 2^-14 below the largest of eight products, and these hold less than that), so results are the exact ones rounded once.
+
+Normal numbers, tolerance: an instruction aligns groups of eight products to their largest and cuts at 2^-14 of it: at most 7 * 2^-14 of the
+largest magnitude of each eight along k (of either half of 64, where a lane's pieces lie).  Sums in fp32: a rounding for each group
+and each join, of the sum of magnitudes.  Then one rounding U to the type."""
+import pytest
+import torch
+
+from layer8 import TINY, U, check, float8, values
+from savanna_amd import _lib
+from savanna_amd.operators.float8 import (E4M3, E5M2, Float8, LinearFloat8, from_float8, linear_float8, matmul_float8, norm_linear_float8,
+                                          to_float8)
+from savanna_amd.operators.norm import rms_norm, rms_norm_float8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def whole(rows, D, fmt, seed, most=8):
+    """Whole numbers that 8 bits hold exactly, rows and blocks at different powers of two."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    held = torch.tensor([v for v in range(-most, most + 1) if fmt is E4M3 or abs(v) in (0, 1, 2, 3, 4, 5, 6, 7, 8, 10)], device=DEV).float()
+    x = held[torch.randint(0, len(held), (rows, D), generator=gen, device=DEV)]
+    power = torch.randint(0, 3, (rows, (D + 127) // 128), generator=gen, device=DEV).float()
+    return (x * torch.exp2(power).repeat_interleave(128, -1)[:, :D]).to(torch.bfloat16)
+
+
+SIZES = [(1, 1, 1), (1, 64, 128), (3, 70, 300), (8, 130, 4096), (9, 130, 640), (16, 33, 129), (17, 300, 513), (64, 129, 2048), (65, 64, 100),
+         (128, 128, 128), (129, 257, 640), (200, 1000, 1500), (256, 256, 128), (256, 256, 384), (257, 300, 512), (300, 520, 1100),
+         (511, 513, 640), (1000, 700, 900), (64, 64, 16384), (300, 300, 8200), (4096, 4097, 300)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("fa,fb", [(E4M3, E4M3), (E5M2, E4M3), (E4M3, E5M2), (E5M2, E5M2)])
+def test_whole_numbers(M, N, K, fa, fb):
+    most = 8 if K < 2000 else 4                                     # |sums| < 16384 * 4 * 4 * 16 < 2^24
+    a, b = whole(M, K, fa, M + K, most), whole(N, K, fb, N + K + 1, most)
+    qa, qb = to_float8(a, fa), to_float8(b, fb)
+    assert torch.equal(values(qa), a.double()) and torch.equal(values(qb), b.double())
+    want = (a.float().double() @ b.float().double().t())
+    for dtype in (torch.bfloat16, torch.float16):
+        got = matmul_float8(qa, qb, dtype)
+        assert torch.equal(got, want.to(dtype)), f"{M} x {N} x {K}: {(got != want.to(dtype)).sum().item()} differ"
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4095, 3841, 256), (3850, 4001, 300), (4096, 3900, 512), (3841, 4096, 640), (4001, 4001, 700),
+                                   (4090, 4094, 1000), (8200, 6000, 1300), (2040, 2048, 16384)])
+def test_wide_tiles(M, N, K):
+    """Sizes that take least time in tiles of 256 x 256, at rows and columns that the tiles do not divide, in every length of the loop's rest, in
+    several rounds, and in parts."""
+    most = 8 if K < 2000 else 4
+    a, b = whole(M, K, E4M3, K, most), whole(N, K, E4M3, K + 1, most)
+    want = (a.float() @ b.float().t()).to(torch.bfloat16)                               # (fp32 holds these sums)
+    qa, qb = to_float8(a), to_float8(b)
+    for _ in range(3):
+        assert torch.equal(matmul_float8(qa, qb), want)
+
+
+def bound(A, B):
+    """Rounding of the sums, as above, on 64-bit values (M, K) and (N, K)."""
+    K = A.shape[1]
+    pad = torch.nn.functional.pad
+    p = pad(A, (0, -K % 128))[:, None] * pad(B, (0, -K % 128))[None]
+    p = p.abs().unflatten(-1, (-1, 8))
+    return 7 * 2.0 ** -14 * p.amax(-1).sum(-1) + (K / 8 + 40) * 2.0 ** -24 * p.sum((-1, -2))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 100, 4096), (5, 70, 300), (16, 64, 1000), (33, 65, 700), (130, 129, 513), (300, 256, 260)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_normal_numbers(M, N, K, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(M)
+    x = torch.randn(M, K, generator=gen, device=DEV) * torch.exp(0.7 * torch.randn(K, generator=gen, device=DEV))
+    w = torch.randn(N, K, generator=gen, device=DEV) * K ** -0.5
+    x, w = x.to(dtype), w.to(dtype)
+    for fa in (E4M3, E5M2):
+        qa, qb = to_float8(x, fa), to_float8(w)
+        A, B = values(qa), values(qb)
+        ref = A @ B.t()
+        got = matmul_float8(qa, qb, dtype)
+        check(got, ref, U[dtype] * ref.abs() + bound(A, B) * (1 + U[dtype]) + TINY[dtype], f"{M} x {N} x {K}")
+        assert torch.equal(got, matmul_float8(qa, qb, dtype))
+    # the weight's 8 bits given: the call quantises x by itself, in the product's kernel or before it
+    with torch.no_grad():
+        a, b = linear_float8(x, to_float8(w)), matmul_float8(to_float8(x), to_float8(w), dtype)
+        assert torch.equal(a, b)
+        assert torch.equal(linear_float8(x, w), a)
+        deep = linear_float8(x.reshape(1, M, K), to_float8(w))
+        assert deep.shape == (1, M, N) and torch.equal(deep[0], a)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 16, 1), (1, 17, 127), (1, 3000, 4096), (2, 640, 8192), (3, 64, 5000), (4, 130, 4096), (7, 40, 2047), (8, 100, 2048),
+                                   (16, 256, 1024), (16, 9000, 1000)])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+def test_tokens_quantised_in_the_kernel(M, N, K, fmt):
+    assert _lib.load().gcg_linear8_supported(M, N, K)
+    x, w = whole(M, K, E4M3, M, 4), to_float8(whole(N, K, fmt, N, 4), fmt)
+    want = x.double() @ values(w).t()
+    with torch.no_grad():
+        for dtype in (torch.bfloat16, torch.float16):
+            assert torch.equal(linear_float8(x.to(dtype), w), want.to(dtype))
+
+
+def test_infinities_and_nan():
+    for M in (2, 20, 300):
+        a, b = torch.ones(M, 300, device=DEV).bfloat16(), torch.ones(260, 300, device=DEV).bfloat16()
+        a[1, 200], b[7, 5] = float("nan"), float("inf")
+        y = matmul_float8(to_float8(a), to_float8(b))
+        bad = torch.zeros(M, 260, dtype=torch.bool, device=DEV)
+        bad[1], bad[:, 7] = True, True
+        assert torch.equal(torch.isnan(y), bad) and (y[~bad] == 300).all()
+        with torch.no_grad():
+            z = linear_float8(a, to_float8(b))
+        assert torch.equal(torch.isnan(z), bad) and (z[~bad] == 300).all()
+        y = matmul_float8(to_float8(a), to_float8(b, E5M2))
+        assert torch.isnan(y[1]).all() and (y[0, 7] == float("inf") or torch.isnan(y[0, 7])) and (y[0, :7] == 300).all()
+
+
+def gradients(x8, dy, w, fmt=E4M3):
+    """((dx, bound), (dw, bound)) in 64 bits; x8: the values that the forward kept"""
+    d, wt = float8(dy, fmt)[0], float8(w.t())[0]
+    dt, xt = float8(dy.t(), fmt)[0], float8(x8.t())[0]
+    return (d @ wt.t(), bound(d, wt)), (dt @ xt.t(), bound(dt, xt))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", [E4M3, E5M2])
+@pytest.mark.parametrize("shape,N", [((1, 130), 70), ((3, 50, 200), 90), ((257, 129), 300)])
+def test_linear_step(shape, N, dtype, fmt):
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    K = shape[-1]
+    x = torch.randn(*shape, generator=gen, device=DEV).to(dtype).requires_grad_(True)
+    w = (torch.randn(N, K, generator=gen, device=DEV) * K ** -0.5).to(dtype).requires_grad_(True)
+    dy = torch.randn(*shape[:-1], N, generator=gen, device=DEV).to(dtype)
+    y = linear_float8(x, w, fmt)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x8, w8 = float8(x.detach().reshape(-1, K))[0], float8(w.detach())[0]
+    ref = x8 @ w8.t()
+    check(y.detach().reshape(-1, N), ref, U[dtype] * ref.abs() + 1.01 * bound(x8, w8) + TINY[dtype], "y")
+    for name, got, (ref, tol) in zip(("dx", "dw"), (dx.reshape(-1, K), dw), gradients(x8, dy.reshape(-1, N), w.detach(), fmt)):
+        check(got, ref, U[dtype] * ref.abs() + 1.01 * tol + TINY[dtype], name)
+    # one gradient alone is the same; a transposed weight and a strided x as well
+    gx, = torch.autograd.grad(linear_float8(x, w.detach(), fmt), x, dy)
+    gw, = torch.autograd.grad(linear_float8(x.detach(), w, fmt), w, dy)
+    assert torch.equal(gx, dx) and torch.equal(gw, dw)
+    wt = w.detach().t().contiguous().t().requires_grad_(True)
+    gx, gw = torch.autograd.grad(linear_float8(x, wt, fmt), (x, wt), dy)
+    assert torch.equal(gx, dx) and torch.equal(gw, dw)
+
+
+def test_gradient_against_differences():
+    """On whole numbers the layer is exactly linear, and a difference of one is exact."""
+    x, w = whole(150, 200, E4M3, 1, 3), whole(60, 200, E4M3, 2, 3)
+    dy = whole(150, 60, E4M3, 3, 2)
+    x.requires_grad_(True), w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(linear_float8(x, w), (x, w), dy)
+    f = lambda x, w: (x.double() @ w.double().t() * dy.double()).sum()                           # noqa: E731
+    with torch.no_grad():
+        for i, j in ((0, 0), (149, 199), (77, 130)):
+            e = torch.zeros_like(x)
+            e[i, j] = 1
+            assert dx[i, j] == (f(x.double() + e.double(), w) - f(x, w)).to(torch.bfloat16)
+        for i, j in ((0, 0), (59, 199), (30, 130)):
+            e = torch.zeros_like(w)
+            e[i, j] = 1
+            assert dw[i, j] == (f(x, w.double() + e.double()) - f(x, w)).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("added", [False, True])
+@pytest.mark.parametrize("rows,K,N", [(5, 300, 70), (130, 513, 200)])
+def test_norm_and_product(rows, K, N, added, dtype):
+    """Each part is what the operators by themselves give, bit for bit."""
+    gen = torch.Generator(device=DEV).manual_seed(K)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(dtype)                       # noqa: E731
+    x, res, gain, w, dy, dr = rand(rows, K), rand(rows, K), rand(K), rand(N, K) / 16, rand(rows, N), rand(rows, K)
+    leaves = [t.requires_grad_(True) for t in ([x, res, gain, w] if added else [x, gain, w])]
+    out = norm_linear_float8(x, gain, w, 1e-5, residual=res if added else None)
+    with torch.no_grad():
+        q = rms_norm_float8(x, gain, 1e-5, residual=res if added else None)
+        q, r = q if added else (q, x)
+        y = matmul_float8(q, to_float8(w), dtype)
+        ready = norm_linear_float8(x, gain, to_float8(w), 1e-5, residual=res if added else None)
+        d = _lib.to_float8_both(dy, E4M3)
+        dn = _lib.matmul_float8(*d[:2], *_lib.to_float8_columns(w, E4M3), N, dtype)
+        dw = _lib.matmul_float8(*d[2:], *_lib.float8_columns(q.codes, q.scales, K, E4M3), rows, dtype)
+    assert torch.equal(out[0] if added else out, y) and torch.equal(ready[0] if added else ready, y)
+    if added:
+        assert torch.equal(out[1], r) and torch.equal(ready[1], r)
+    grads = torch.autograd.grad(out, leaves, [dy, dr] if added else dy)
+    n = r.detach().requires_grad_(True)
+    g = gain.detach().requires_grad_(True)
+    dx, dg = torch.autograd.grad(rms_norm(n, g, 1e-5), (n, g), dn)
+    if added:                                               # (the norm's own node adds dr before its one rounding)
+        z = torch.zeros_like(n).requires_grad_(True)
+        dx, dg = torch.autograd.grad(rms_norm(n, g, 1e-5, residual=z), (n, g), [dn, dr])
+        assert torch.equal(grads[1], dx)
+    assert torch.equal(grads[0], dx) and torch.equal(grads[-2], dg) and torch.equal(grads[-1], dw)
+
+
+def test_module():
+    torch.manual_seed(0)
+    m = LinearFloat8(300, 130, device=DEV)
+    x = torch.randn(20, 300, device=DEV).bfloat16()
+    y = m(x)
+    y.float().square().sum().backward()
+    assert m.weight.grad.shape == (130, 300) and torch.isfinite(m.weight.grad).all()
+    m.lay_out()
+    assert isinstance(m.operand(), torch.Tensor)                                                # with gradients: the weight
+    with torch.no_grad():
+        assert isinstance(m.operand(), Float8) and torch.equal(m(x), y)
+        state = {k: v * 2 for k, v in m.state_dict().items()}
+        m.load_state_dict(state)
+        assert isinstance(m.operand(), torch.Tensor) and not torch.equal(m(x), y)
+        m.lay_out().train()
+        assert isinstance(m.operand(), torch.Tensor)
+        m.lay_out().eval()
+        assert isinstance(m.operand(), Float8)
+        m.to(torch.float16)
+        assert isinstance(m.operand(), torch.Tensor)
+
+
+def test_refusals():
+    x, w = torch.randn(4, 300, device=DEV).bfloat16(), torch.randn(20, 300, device=DEV).bfloat16()
+    q = to_float8(w)
+    for bad in (lambda: linear_float8(x.float(), w.float()), lambda: linear_float8(x, w.half()), lambda: linear_float8(x, w[:, :200]),
+                lambda: linear_float8(x[:, :200], q), lambda: linear_float8(x.float(), q), lambda: matmul_float8(q, q, torch.float32),
+                lambda: matmul_float8(q, to_float8(x[:, :200])), lambda: matmul_float8(q, Float8(q.codes[None], q.scales[None], 300)),
+                lambda: linear_float8(x, w, torch.bfloat16), lambda: linear_float8(x.requires_grad_(True), q),
+                lambda: norm_linear_float8(x, None, q), lambda: norm_linear_float8(x, None, w.float()), lambda: linear_float8(x.cpu(), w.cpu())):
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            bad()
+    x = x.detach()
+    with torch.no_grad():
+        assert linear_float8(x[:0], q).shape == (0, 20) and linear_float8(x[:, :0], to_float8(w[:, :0])).eq(0).all()
+        assert linear_float8(x, to_float8(w[:0])).shape == (4, 0)
+    e, v = x[:0].clone().requires_grad_(True), w.clone().requires_grad_(True)
+    linear_float8(e, v).sum().backward()
+    assert e.grad.shape == (0, 300) and not v.grad.any()
+    assert from_float8(q, torch.float32).shape == (20, 300)
