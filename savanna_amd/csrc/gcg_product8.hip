@@ -177,9 +177,10 @@ __global__ __launch_bounds__(WM * WN * 64) void product8_kernel(Product8 p)
     }
 }
 
-// The same by four waves, one a SIMD, of 128 x 128 each.  A fragment is then read from shared memory for eight products, twice as many as in
-// the other kernel, and a block takes as long as 64 products; to keep those fed without a second wave, a block goes in four phases of 16, each of
-// one half of the wave's rows and one half of its columns, and each reads the half that is needed next where the one that is no longer needed was:
+// The same by four waves, one a SIMD, of 128 x 128 (BN = 256) or 128 x 64 (BN = 128) each.  A fragment is then read from shared memory for eight
+// products, twice as many as in the other kernel (four and eight), and a block takes as long as 64 (32) products; to keep those fed without a second
+// wave, a block goes in four phases, each of one half of the wave's rows and one half of its columns, and each reads the half that is needed next
+// where the one that is no longer needed was:
 //
 //   (A0 B0) reads B1,  (A0 B1) reads A1,  barrier,  (A1 B1) reads the next block's A0,  (A1 B0) reads its B1;  the next block starts with (A0 B1)
 //
@@ -193,9 +194,9 @@ template <int BYTES> __device__ __forceinline__ void request_to_lds(win_t w, uin
 {
 #ifdef __HIP_DEVICE_COMPILE__
     if constexpr (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(w), "s"(at) : "memory", "m0");
 #endif
 }
 // The instruction with its accumulator where the compiler would not leave it by itself, in the 256 registers that only matrix instructions use.
@@ -214,9 +215,10 @@ template <bool A5, bool B5, int BYTE> __device__ __forceinline__ void mfma8_acc(
 #endif
 }
 
-template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) void product8_wide_kernel(Product8 p)
+template <int BN, typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) void product8_wide_kernel(Product8 p)
 {
-    constexpr int BM = 256, BN = 256, LOADS = 8, STAGE = (BM + BN) * 128;
+    constexpr int BM = 256, LA = 8, LB = BN / 32, STAGE = (BM + BN) * 128;
+    constexpr int COLS = BN / 2, HALF = COLS / 32;              // a wave's columns, and fragments of half of them
     __shared__ __attribute__((aligned(1024))) uint8_t stage[2][STAGE];
     __shared__ uint32_t words[2][BM + BN];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64;
@@ -229,7 +231,7 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
         const uint32_t tile = xcd_contiguous_u32(item - split * tiles, tiles);
         const uint32_t group = tile / (8 * p.tiles_n), first = group * 8, high = p.tiles_m - first < 8 ? p.tiles_m - first : 8;
         const uint32_t in = tile - group * 8 * p.tiles_n;
-        // tiles that would reach beyond the tensor start earlier and make some of their neighbours' results again, the same bits (M, N >= 256)
+        // tiles that would reach beyond the tensor start earlier and make some of their neighbours' results again, the same bits (M >= 256, N >= BN)
         m0 = (int64_t)(first + in % high) * BM;
         n0 = (int64_t)(in / high) * BN;
         m0 = m0 < p.M - BM ? m0 : p.M - BM;
@@ -246,58 +248,64 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
     const uint32_t piece = (uint32_t)(t / 8 * p.Kp) + ((t % 8) ^ ((t >> 4) & 7)) * 16;
     const int rows32 = __builtin_amdgcn_readfirstlane((int)(32 * p.Kp));
     const uint32_t lds = (uint32_t)(uintptr_t)(lds_t)stage[0] + wave * 1024, lds_words = (uint32_t)(uintptr_t)(lds_t)words[0] + wave * 256;
-    const auto request_piece = [&](int at, int s, int i) {
-        request_to_lds<16>(wa, lds + s * STAGE + i * 4096, piece, at + i * rows32);
-        request_to_lds<16>(wb, lds + s * STAGE + BM * 128 + i * 4096, piece, at + i * rows32);
-    };
+    const auto request_a = [&](int at, int s, int i) { request_to_lds<16>(wa, lds + s * STAGE + i * 4096, piece, at + i * rows32); };
+    const auto request_b = [&](int at, int s, int i) { request_to_lds<16>(wb, lds + s * STAGE + BM * 128 + i * 4096, piece, at + i * rows32); };
     const auto place_of = [&](int k) { return __builtin_amdgcn_readfirstlane((k < k1 ? k : k1 - 1) * 128); };
     const auto request = [&](int k, int s) {
         const int at = place_of(k);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) request_piece(at, s, i);
+        for (int i = 0; i < LA; ++i) request_a(at, s, i);
+#pragma unroll
+        for (int i = 0; i < LB; ++i) request_b(at, s, i);
     };
     // the scales of the tile's rows for four blocks from k on, a word a row
     const uint32_t row_scales = (uint32_t)(t * p.S);
     const auto request_words = [&](int k, int s) {
         const int at = __builtin_amdgcn_readfirstlane((k < k1 ? k : k1 - 1) / 4 * 4);
         request_to_lds<4>(wsa, lds_words + s * ((BM + BN) * 4), row_scales, at);
-        request_to_lds<4>(wsb, lds_words + s * ((BM + BN) * 4) + BM * 4, row_scales, at);
+        if (BN == 256 || wave < BN / 64) request_to_lds<4>(wsb, lds_words + s * ((BM + BN) * 4) + BM * 4, row_scales, at);
     };
 
     const int wm = wave & 1, wn = wave >> 1, r16 = lane % 16, quarter = lane / 16, swap = (r16 >> 1) & 7;
-    const int fa = (wm * 128 + r16) * 128, fb = BM * 128 + (wn * 128 + r16) * 128;
+    const int fa = (wm * 128 + r16) * 128, fb = BM * 128 + (wn * COLS + r16) * 128;
     const int p0 = (quarter ^ swap) * 16, p1 = ((quarter + 4) ^ swap) * 16;
     const auto fragment = [&](int s, int at) {
         const u32x4 lo = *(const u32x4 *)(stage[s] + at + p0), hi = *(const u32x4 *)(stage[s] + at + p1);
         return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
     };
-    uint32_t ca[8], cb[8];
+    uint32_t ca[8], cb[2 * HALF];
     const auto take_words = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            ca[i] = words[s][wm * 128 + i * 16 + r16];
-            cb[i] = words[s][BM + wn * 128 + i * 16 + r16];
-        }
+        for (int i = 0; i < 8; ++i) ca[i] = words[s][wm * 128 + i * 16 + r16];
+#pragma unroll
+        for (int j = 0; j < 2 * HALF; ++j) cb[j] = words[s][BM + wn * COLS + j * 16 + r16];
     };
-    f32x4 acc[8][8];
-    i32x8 A[2][4], B[2][4];
-    // 16 products of half I of the rows and half J of the columns, and between them the four fragments at `from` of stage s into `to`, and with
+    f32x4 acc[8][2 * HALF];
+    i32x8 A[2][4], B[2][HALF];
+    // The products of half I of the rows and half J of the columns, and between them the FRAGMENTS fragments at `from` of stage s into `to`, and with
     // `more` the requests for block k into the other stage.  (These statements stay in the order they are written in.)
-    const auto phase = [&](auto i_, auto j_, auto byte_, i32x8(&to)[4], int s, int from, auto more_, int at) {
+    const auto phase = [&](auto i_, auto j_, auto byte_, auto &to, int s, int from, auto more_, int at) {
         constexpr int i = decltype(i_)::value, j = decltype(j_)::value, byte = decltype(byte_)::value;
         constexpr bool more = decltype(more_)::value;
+        constexpr int FRAGMENTS = (int)(sizeof(to) / sizeof(i32x8)), TURNS = 2 * HALF, READS = 2 * FRAGMENTS;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const u32x4 part = *(const u32x4 *)(stage[s] + from + q / 2 * 16 * 128 + (q % 2 ? p1 : p0));
+        for (int q = 0; q < TURNS; ++q) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[q / 2][q % 2 * 4 + e] = (int)part[e];
+            for (int f = q * READS / TURNS; f < (q + 1) * READS / TURNS; ++f) {
+                const u32x4 part = *(const u32x4 *)(stage[s] + from + f / 2 * 16 * 128 + (f % 2 ? p1 : p0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[f / 2][f % 2 * 4 + e] = (int)part[e];
+            }
             if constexpr (more) {
-                request_piece(at, s ^ 1, q);
+#pragma unroll
+                for (int f = q * LA / TURNS; f < (q + 1) * LA / TURNS; ++f) request_a(at, s ^ 1, f);
+#pragma unroll
+                for (int f = q * LB / TURNS; f < (q + 1) * LB / TURNS; ++f) request_b(at, s ^ 1, f);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int x = q / 2, y = q % 2 * 2 + h;
-                mfma8_acc<B5, A5, byte>(B[j][y], A[i][x], acc[i * 4 + x][j * 4 + y], cb[j * 4 + y], ca[i * 4 + x]);
+                const int x = (q * 2 + h) / HALF, y = (q * 2 + h) % HALF;
+                mfma8_acc<B5, A5, byte>(B[j][y], A[i][x], acc[i * 4 + x][j * HALF + y], cb[j * HALF + y], ca[i * 4 + x]);
             }
         }
     };
@@ -316,11 +324,11 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
         constexpr int s = decltype(s_)::value, J = s, notJ = 1 - s;
         constexpr std::integral_constant<int, J> j;
         constexpr std::integral_constant<int, notJ> not_j;
-        phase(zero, j, byte_, B[notJ], s, fb + notJ * 64 * 128, no, 0);
+        phase(zero, j, byte_, B[notJ], s, fb + notJ * HALF * 16 * 128, no, 0);
         phase(zero, not_j, byte_, A[1], s, fa + 64 * 128, no, 0);
         hand_over();
         phase(one, not_j, byte_, A[0], s ^ 1, fa, yes, place_of(k + 2));
-        phase(one, j, byte_, B[notJ], s ^ 1, fb + notJ * 64 * 128, no, 0);
+        phase(one, j, byte_, B[notJ], s ^ 1, fb + notJ * HALF * 16 * 128, no, 0);
     };
 
     take(blockIdx.x);
@@ -333,9 +341,11 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 2 * HALF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) { A[0][q] = fragment(0, fa + q * 16 * 128); B[0][q] = fragment(0, fb + q * 16 * 128); }
+    for (int q = 0; q < 4; ++q) A[0][q] = fragment(0, fa + q * 16 * 128);
+#pragma unroll
+    for (int q = 0; q < HALF; ++q) B[0][q] = fragment(0, fb + q * 16 * 128);
     int k = k0, w = 0;
     for (; k + 4 <= k1; k += 4, w ^= 1) {
         take_words(w);
@@ -349,25 +359,29 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
     for (; k < k1; ++k) {
         const int s = (k - k0) & 1;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                A[h][q] = fragment(s, fa + (h * 4 + q) * 16 * 128);
-                B[h][q] = fragment(s, fb + (h * 4 + q) * 16 * 128);
-            }
+            for (int q = 0; q < 4; ++q) A[h][q] = fragment(s, fa + (h * 4 + q) * 16 * 128);
+#pragma unroll
+            for (int q = 0; q < HALF; ++q) B[h][q] = fragment(s, fb + (h * HALF + q) * 16 * 128);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mfma8_acc<B5, A5, 0>(B[j / 4][j % 4], A[i / 4][i % 4], acc[i][j], cb[j], ca[i]);
+            for (int j = 0; j < 2 * HALF; ++j) mfma8_acc<B5, A5, 0>(B[j / HALF][j % HALF], A[i / 4][i % 4], acc[i][j], cb[j], ca[i]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { ca[i] >>= 8; cb[i] >>= 8; }
+        for (int i = 0; i < 8; ++i) ca[i] >>= 8;
+#pragma unroll
+        for (int j = 0; j < 2 * HALF; ++j) cb[j] >>= 8;
         hand_over();
         request(k + 2, s);
     }
-    // A wave's results leave in whole rows of 128 columns, which lie together in shared memory first: a pass of 64 rows (fp32: 32) in its quarter of
+    // A wave's results leave in whole rows of its columns, which lie together in shared memory first: a pass of 64 rows (fp32: 32) in its quarter of
     // the second stage, the 16-byte pieces of a row at exchanged places.  The next tile's first block is on its way to the first stage by then.
-    constexpr int ROWS = 16384 / (128 * (int)sizeof(T)), PIECES = 128 * (int)sizeof(T) / 16;
-    uint8_t *y = (uint8_t *)((p.partial ? (T *)(p.partial + (int64_t)split * p.M * p.N) : (T *)p.y) + (m0 + wm * 128) * p.N + n0 + wn * 128);
+    constexpr int ROWS = 128 / (int)sizeof(T), PIECES = COLS * (int)sizeof(T) / 16;
+    static_assert(4 * ROWS * PIECES * 16 <= STAGE, "in the second stage");
+    const auto exchanged = [](int piece, int row) { return piece ^ (PIECES >= 16 ? row & 15 : (row >> 1) & 7); };
+    uint8_t *y = (uint8_t *)((p.partial ? (T *)(p.partial + (int64_t)split * p.M * p.N) : (T *)p.y) + (m0 + wm * 128) * p.N + n0 + wn * COLS);
     hand_over();                                                                // nobody reads a stage any more, and nothing arrives
     item += gridDim.x;
     const bool more = item < items;
@@ -379,26 +393,26 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");             // the last products have written their accumulators
     int l = lane;
     asm volatile("" : "+v"(l));                                                 // (addresses are formed here, not kept over the products)
-    uint8_t *mine = stage[1] + wave * 16384;
+    uint8_t *mine = stage[1] + wave * (ROWS * PIECES * 16);
     const int64_t down = 64 / PIECES * p.N * (int64_t)sizeof(T);                // from one store's rows to the next one's
-    const uint32_t off = (uint32_t)(l / PIECES * p.N * (int64_t)sizeof(T)) + l % PIECES * 16;
+    const int64_t off = l / PIECES * p.N * (int64_t)sizeof(T) + l % PIECES * 16;
 #pragma unroll
     for (int r = 0; r < 128; r += ROWS) {
 #pragma unroll
         for (int i = r / 16; i < (r + ROWS) / 16; ++i) {
             const int row = i * 16 - r + l % 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 2 * HALF; ++j) {
                 asm volatile("" : "+a"(acc[i][j]));         // (read after that wait)
                 const int at = (j * 16 + l / 16 * 4) * (int)sizeof(T);
-                store4((T *)(mine + row * (PIECES * 16) + (((at / 16) ^ (row & 15)) * 16) + at % 16), acc[i][j], 4, true);
+                store4((T *)(mine + row * (PIECES * 16) + exchanged(at / 16, row) * 16 + at % 16), acc[i][j], 4, true);
             }
         }
         // (a wave reads what it has written itself)
 #pragma unroll
         for (int q = 0; q < ROWS * PIECES / 64; ++q) {
             const int row = (q * 64 + l) / PIECES, piece = l % PIECES;
-            const u32x4 v = *(const u32x4 *)(mine + row * (PIECES * 16) + ((piece ^ (row & 15)) * 16));
+            const u32x4 v = *(const u32x4 *)(mine + row * (PIECES * 16) + exchanged(piece, row) * 16);
             *(u32x4_any *)(y + off) = v;
             y += down;
         }
@@ -406,7 +420,7 @@ template <typename T, bool A5, bool B5> __global__ __launch_bounds__(256, 1) voi
     if (!more) return;
     __syncthreads();
     request(k0 + 1, 1);
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");           // all but the second block
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");           // all but the second block
     }
 }
 
@@ -489,34 +503,38 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 
 // Which kernel, and in how many parts of the blocks (each a sum in fp32, joined by another kernel): what would take the least time.
 // Few rows go by product8_tokens_kernel: 12288 x 4096 with 1 row 12.3 us (tiles of 128 in four parts 14.5), with 16 rows 17.8 (14.8).
-// Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.3 a block and 6 around them; 512 tiles of 128 x 128 (two
-// a CU) take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice at 4 TB/s, and 3 for its launch.  So
-// 4096 x 4096 x 4096 goes wide (53.6; 88.1), 2048 x 4096 x 4096 either way (47.0; 46.9), 1024 x 4096 x 4096 in small tiles (36.1; 43.6),
-// 7680 x 2561 x 5003 wide although its second round is short (118.9; 143.6), 512 x 512 x 16384 in small tiles and parts (121.7 in one, 37.0 in four).
-enum { TOKENS = 0, TILE = 128, WIDE = 256 };
+// Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.65 if half the
+// card is idle); 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice
+// at 4 TB/s, and 3 for its launch.  So (tiles of 128 x 128, 256 x 128, 256 x 256) 4096 x 4096 x 4096 goes by the last (88, 63, 55), 2048 x 4096 x 4096
+// by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115), 701 x 7683 x 2560 by the second (35, 23, 34), and
+// 512 x 512 x 16384 in parts (119, 98, 147; the first in four parts 37, the second 33).
+enum { TOKENS, TILE, TALL, WIDE };       // tiles of 128 x 128, 256 x 128, 256 x 256
 constexpr int kTokens = 8;
 struct Plan8 { int kernel, splits, split_steps; };
 float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
 {
-    const int64_t items = ((M + kernel - 1) / kernel) * ((N + kernel - 1) / kernel) * splits;
+    const int bm = kernel == TILE ? 128 : 256, bn = kernel == WIDE ? 256 : 128;
+    const int64_t items = ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits;
     const float join = splits > 1 ? 3.f + (float)M * (float)N * (float)splits * 8.f / 4e6f : 0.f;
-    if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.3f + 6.f) + join;
+    if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.35f + 6.f) + join;
+    if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.65f : 0.85f) + 5.f) + join;
     return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + join;
 }
+bool takes(int kernel, int64_t M, int64_t N) { return kernel == TILE || (M >= 256 && N >= (kernel == WIDE ? 256 : 128)); }
 Plan8 plan_of(int64_t M, int64_t N, int64_t K)
 {
     const int steps = (int)(f8_cols(K) / 128);
     if (const char *e = tuning_env("GCG_P8")) {
         const char *s = tuning_env("GCG_P8S");
         const int n = s ? atoi(s) : 1, per = ((steps + n - 1) / n + 3) / 4 * 4, kernel = atoi(e);
-        if ((kernel == WIDE && (M < 256 || N < 256)) || (kernel == TOKENS && M > 16)) return {TILE, 1, (steps + 3) / 4 * 4};
+        if (kernel == TOKENS ? M > 16 : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4};
         return {kernel, (steps + per - 1) / per, per};
     }
     if (M <= kTokens) return {TOKENS, 1, steps};
     Plan8 best = {TILE, 1, (steps + 3) / 4 * 4};
     float least = 0.f;
-    for (int kernel = TILE; kernel <= (M >= 256 && N >= 256 ? WIDE : TILE); kernel *= 2)
-        for (int n = 1; n == 1 || (n <= 32 && steps >= 4 * n); n *= 2) {
+    for (int kernel = TILE; kernel <= WIDE; ++kernel)
+        for (int n = 1; takes(kernel, M, N) && (n == 1 || (n <= 32 && steps >= 4 * n)); n *= 2) {
             const int per = ((steps + n - 1) / n + 3) / 4 * 4, splits = (steps + per - 1) / per;
             const float time = estimate(kernel, M, N, splits > 1 ? per : steps, splits);
             if (least == 0.f || time < least) {
@@ -549,10 +567,13 @@ template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Pl
         }
     }
     if (plan.kernel == TILE) return tile_launch<128, 128, 2, 2, T, A5, B5>(p, plan, st);
+    const int bn = plan.kernel == WIDE ? 256 : 128;
     p.tiles_m = (uint32_t)((p.M + 255) / 256);
-    p.tiles_n = (uint32_t)((p.N + 255) / 256);
+    p.tiles_n = (uint32_t)((p.N + bn - 1) / bn);
     const int64_t items = (int64_t)p.tiles_m * p.tiles_n * plan.splits;
-    return launch_main(product8_wide_kernel<T, A5, B5>, dim3((unsigned)(items < 256 ? items : 256)), dim3(256), st, p);
+    const dim3 grid((unsigned)(items < 256 ? items : 256)), block(256);
+    return plan.kernel == WIDE ? launch_main(product8_wide_kernel<256, T, A5, B5>, grid, block, st, p)
+                               : launch_main(product8_wide_kernel<128, T, A5, B5>, grid, block, st, p);
 }
 template <typename T> int product_format(Product8 &p, int a5, int b5, const Plan8 &plan, hipStream_t st)
 {
