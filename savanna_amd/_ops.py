@@ -230,6 +230,8 @@ def _register_autograd():
     reg("gcg::rms_norm_infer", refuse("rms_norm_infer", "use torch.ops.gcg.rms_norm"), setup_context=nothing)
     for name in ("rms_norm_float8", "to_float8", "to_float8_both", "to_float8_columns", "linear_float8_infer"):
         reg(f"gcg::{name}", refuse(name, "use torch.ops.gcg.linear_float8 or norm_linear_float8"), setup_context=nothing)
+    for name in ("rms_norm_bwd", "float8_columns", "from_float8", "matmul_float8", "scan_bwd", "scan_packed_bwd"):
+        reg(f"gcg::{name}", refuse(name, "its operator is differentiated once"), setup_context=nothing)
     reg("gcg::pack8", refuse("pack8", "a checkpoint is what a backward pass reads"), setup_context=nothing)
     reg("gcg::fwd_full", refuse("fwd_full", "use torch.ops.gcg.fwd for a differentiable y"), setup_context=lambda ctx, inputs, output: None)
 

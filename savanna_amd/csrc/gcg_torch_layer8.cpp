@@ -582,7 +582,26 @@ Tensor scan_step_meta(const Tensor &x, const Tensor &f, const OptTensor &gate, c
 }
 
 // ---- autograd nodes ------------------------------------------------------------------------------------------
-// Each calls the operators above through the dispatcher, below autograd.
+// Each calls the operators above through the dispatcher, below autograd; a backward pass that is recorded itself (create_graph) calls them above it,
+// where those without a derivative say so.
+struct BelowAutograd {
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+    BelowAutograd() { if (!at::GradMode::is_enabled()) below.emplace(); }
+};
+
+// A leaf whose gradient is still the business of a graph that was recorded on the default stream takes a captured backward pass there, which ends
+// the capture, and with it the process: such a call is refused.
+void check_leaves(std::initializer_list<const Tensor *> tensors)
+{
+    if (!(*tensors.begin())->is_cuda() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor *t : tensors) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() != 0, "gcg: the stream is being captured into a graph, and an argument is a leaf of a graph that was "
+                    "recorded on the default stream and still lives; let that graph go before the capture");
+    }
+}
 
 struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const OptTensor &residual, const OptTensor &w, double eps)
@@ -598,6 +617,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g)
     {
+        const BelowAutograd below;
         static const auto f = op<Two(const Tensor &, const Tensor &, const OptTensor &, const Tensor &, const OptTensor &, bool)>("gcg::rms_norm_bwd");
         const variable_list s = ctx->get_saved_variables();
         const bool need = ctx->saved_data["dw"].toBool(), added = g.size() > 1;
@@ -608,6 +628,13 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     }
 };
 
+// (the rows counted from x's sizes: a matrix of no columns has some)
+Tensor as_matrix(const Tensor &t)
+{
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+    return t.reshape({rows, t.size(-1)});
+}
 // dx and dw of y = x w^T from x in 8 bits, each operand in 8 bits along what it is summed over; dy: (rows, out)
 Two linear_gradients(const Tensor &dy, const Tensor &codes, const Tensor &scales, int64_t columns, const Tensor &w, at::ScalarType format,
                      bool need_dx, bool need_dw)
@@ -657,11 +684,12 @@ struct LinearFloat8Node : torch::autograd::Function<LinearFloat8Node> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g)
     {
+        const BelowAutograd below;
         const variable_list s = ctx->get_saved_variables();
         const bool need_dx = ctx->saved_data["dx"].toBool(), need_dw = ctx->saved_data["dw"].toBool();
         const Tensor &w = s[2], dy = g[0].contiguous();
-        const Tensor flat = need_dw ? s[0].reshape({-1, s[0].size(-1)}) : Tensor(), scales = need_dw ? s[1].reshape({-1, s[1].size(-1)}) : Tensor();
-        auto [dx, dw] = linear_gradients(dy.reshape({-1, w.size(0)}), flat, scales, w.size(1), w,
+        const Tensor flat = need_dw ? as_matrix(s[0]) : Tensor(), scales = need_dw ? as_matrix(s[1]) : Tensor();
+        auto [dx, dw] = linear_gradients(as_matrix(dy), flat, scales, w.size(1), w,
                                          (at::ScalarType)ctx->saved_data["format"].toInt(), need_dx, need_dw);
         if (need_dx) {
             std::vector<int64_t> sizes = dy.sizes().vec();
@@ -696,6 +724,7 @@ struct NormLinearFloat8Node : torch::autograd::Function<NormLinearFloat8Node> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g)
     {
+        const BelowAutograd below;
         static const auto norm = op<Two(const Tensor &, const Tensor &, const OptTensor &, const Tensor &, const OptTensor &, bool)>("gcg::rms_norm_bwd");
         const variable_list s = ctx->get_saved_variables();
         const Tensor &w = s[2], &r = s[3];
@@ -704,8 +733,8 @@ struct NormLinearFloat8Node : torch::autograd::Function<NormLinearFloat8Node> {
         std::vector<int64_t> sizes = r.sizes().vec();
         sizes.back() = w.size(0);
         const Tensor dy = g[0].defined() ? g[0].contiguous() : at::zeros(sizes, r.options());
-        const Tensor flat = need_dw ? s[0].reshape({-1, s[0].size(-1)}) : Tensor(), scales = need_dw ? s[1].reshape({-1, s[1].size(-1)}) : Tensor();
-        auto [dn, dw] = linear_gradients(dy.reshape({-1, w.size(0)}), flat, scales, w.size(1), w,
+        const Tensor flat = need_dw ? as_matrix(s[0]) : Tensor(), scales = need_dw ? as_matrix(s[1]) : Tensor();
+        auto [dn, dw] = linear_gradients(as_matrix(dy), flat, scales, w.size(1), w,
                                          (at::ScalarType)ctx->saved_data["format"].toInt(), need_dx, need_dw);
         Tensor dx, dgain;
         if (need_dx) {
@@ -733,6 +762,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g)
     {
+        const BelowAutograd below;
         static const auto bwd = op<Five(const Tensor &, const Tensor &, const Tensor &, const OptTensor &, const OptTensor &, const Tensor &,
                                         const OptTensor &, const OptTensor &, bool, bool)>("gcg::scan_bwd");
         const variable_list s = ctx->get_saved_variables();
@@ -756,6 +786,7 @@ struct PackedScanNode : torch::autograd::Function<PackedScanNode> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list g)
     {
+        const BelowAutograd below;
         static const auto bwd = op<Two(const Tensor &, const Tensor &, const OptTensor &, const Tensor &, bool)>("gcg::scan_packed_bwd");
         const variable_list s = ctx->get_saved_variables();
         const bool need = ctx->saved_data["dbias"].toBool();
@@ -766,25 +797,37 @@ struct PackedScanNode : torch::autograd::Function<PackedScanNode> {
 
 std::vector<Tensor> rms_norm(const Tensor &x, const OptTensor &residual, const OptTensor &w, double eps)
 {
+    const Tensor a = or_empty(residual), b = or_empty(w);
+    check_leaves({&x, &a, &b});
     return RmsNormNode::apply(x, residual, w, eps);
 }
 Tensor linear_float8(const Tensor &x, const Tensor &w, at::ScalarType format)
 {
     check_weight(x, w);
+    check_leaves({&x, &w});
     return LinearFloat8Node::apply(x, w, format);
 }
 std::vector<Tensor> norm_linear_float8(const Tensor &x, const OptTensor &residual, const OptTensor &gain, const Tensor &w, double eps,
                                        at::ScalarType format)
 {
     check_weight(x, w);
+    const Tensor a = or_empty(residual), b = or_empty(gain);
+    check_leaves({&x, &a, &b, &w});
     return NormLinearFloat8Node::apply(x, residual, gain, w, eps, format);
 }
 std::vector<Tensor> scan(const Tensor &x, const Tensor &f, const OptTensor &gate, const OptTensor &bias, const OptTensor &initial,
                          const OptTensor &lengths, bool final)
 {
+    const Tensor a = or_empty(gate), b = or_empty(bias), c = or_empty(initial);
+    check_leaves({&x, &f, &a, &b, &c});
     return ScanNode::apply(x, f, gate, bias, initial, lengths, final);
 }
-Tensor scan_packed(const Tensor &features, const OptTensor &bias) { return PackedScanNode::apply(features, bias); }
+Tensor scan_packed(const Tensor &features, const OptTensor &bias)
+{
+    const Tensor b = or_empty(bias);
+    check_leaves({&features, &b});
+    return PackedScanNode::apply(features, bias);
+}
 
 } // namespace
 

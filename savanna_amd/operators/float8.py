@@ -15,6 +15,7 @@ from typing import NamedTuple, Optional, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -59,7 +60,7 @@ def _check_weight(x: torch.Tensor, w: torch.Tensor) -> None:
 
 def _gradients(dy, x8, w, grad_dtype, need_dx, need_dw):
     """(dx, dw) of y = x w^T from x in 8 bits; dy contiguous (..., out)."""
-    flat = dy.reshape(-1, w.shape[0])
+    flat = dy.reshape(dy.shape[:-1].numel(), w.shape[0])
     dx = dw = rows = cols = None
     if need_dx and need_dw:
         *rows, codes, scales = _lib.to_float8_both(flat, grad_dtype)
@@ -71,7 +72,7 @@ def _gradients(dy, x8, w, grad_dtype, need_dx, need_dw):
     if need_dx:
         dx = _lib.matmul_float8(*rows, *_lib.to_float8_columns(w, E4M3), w.shape[0], dy.dtype).reshape(*dy.shape[:-1], w.shape[1])
     if need_dw:
-        codes, scales = (t.reshape(-1, t.shape[-1]) for t in x8)
+        codes, scales = (t.reshape(flat.shape[0], t.shape[-1]) for t in x8)
         dw = _lib.matmul_float8(*cols, *_lib.float8_columns(codes, scales, w.shape[1], E4M3), flat.shape[0], dy.dtype)
     return dx, dw
 
@@ -86,6 +87,7 @@ class _LinearFloat8(torch.autograd.Function):
         return _lib.matmul_float8(codes, scales, *_lib.to_float8(w, E4M3), w.shape[1], x.dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         codes, scales, w = ctx.saved_tensors
         return *_gradients(dy.contiguous(), (codes, scales), w, ctx.grad_dtype, *ctx.needs_input_grad[:2]), None
@@ -103,6 +105,7 @@ class _NormLinearFloat8(torch.autograd.Function):
         return (y, r) if ctx.added else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dr=None):
         codes, scales, w, r, rstd, gain = ctx.saved_tensors
         need_x, need_residual, need_gain, need_w = ctx.needs_input_grad[:4]

@@ -13,6 +13,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -26,6 +27,7 @@ class _GatedRecurrence(torch.autograd.Function):
         return (y, last) if final else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dfinal=None):
         x, f, gate, bias, states, lengths = ctx.saved_tensors
         need_bias, need_initial = ctx.needs_input_grad[3:5]
@@ -43,6 +45,7 @@ class _PackedRecurrence(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         features, bias, states = ctx.saved_tensors
         need = ctx.needs_input_grad[1]

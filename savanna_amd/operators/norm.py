@@ -13,6 +13,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .float8 import Float8
@@ -71,6 +72,7 @@ class _RMSNorm(torch.autograd.Function):
         return (y, r) if ctx.added else y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dr=None):
         r, rstd, w = ctx.saved_tensors
         need = ctx.needs_input_grad[2]

@@ -152,6 +152,72 @@ def test_two_captured_graphs_and_eager_work_between_their_replays():
     assert all(torch.equal(a, b) for a, b in zip(outs[0], everything(*new)))
 
 
+@pytest.mark.skipif(not _lib.TORCH_OPS, reason="the check is the torch binding's")
+def test_a_capture_with_leaves_of_a_living_graph_is_refused():
+    i = inputs(11)
+    x, res, gain, w, _, features, bias = i[:7]
+    lives = [(x * 1).sum(), (gain * 1).sum(), (w * 1).sum(), (features * 1).sum(), (bias * 1).sum()]
+    calls = [lambda: rms_norm(x, gain, residual=res), lambda: linear_float8(res.detach(), w), lambda: norm_linear_float8(res.detach(), gain, w.detach()),
+             lambda: gated_recurrence_features(features.detach(), bias), lambda: gated_recurrence_features(features)]
+    for call in calls:
+        call()                                                                      # (not captured: allowed)
+        g = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="still lives"), torch.cuda.graph(g):
+            res.detach() + 1
+            call()
+        del g
+    del lives
+    torch.cuda.synchronize()
+    want = everything(*i)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = everything(*i)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("nodes", [True, False])
+def test_no_second_derivative(nodes, monkeypatch):
+    """A gradient that is recorded itself is the same, and its own gradient an error rather than zero."""
+    x, res, gain, w, _, features, bias = inputs(12)[:7]
+    if not nodes:
+        monkeypatch.setattr(_lib, "native_nodes", lambda t: False)
+    for f, leaf in ((lambda: rms_norm(x, gain), x), (lambda: linear_float8(x, w), w), (lambda: norm_linear_float8(x, gain, w), x),
+                    (lambda: gated_recurrence_features(features, bias), features)):
+        once = torch.autograd.grad(f().float().square().sum(), leaf)[0]
+        kept = torch.autograd.grad(f().float().square().sum(), leaf, create_graph=True)[0]
+        assert torch.equal(once, kept)
+        with pytest.raises(RuntimeError, match="differentia"):
+            torch.autograd.grad(kept.float().square().sum(), leaf)
+
+
+def test_gradients_of_one_tensor_in_two_places():
+    """x and the residual are one leaf, or two whose gradients are then written to."""
+    x, _, gain = inputs(13)[:3]
+    dy, dr = torch.randn_like(x), torch.randn_like(x)
+    a, b = x.detach().clone().requires_grad_(True), x.detach().clone().requires_grad_(True)
+    torch.autograd.backward(rms_norm(a, gain, residual=b), [dy, dr])
+    torch.autograd.backward(rms_norm(x, gain, residual=x), [dy, dr])
+    assert torch.equal(a.grad, b.grad) and torch.equal(x.grad, a.grad + b.grad)
+    before = b.grad.clone()
+    a.grad.zero_()
+    assert torch.equal(b.grad, before)
+
+
+@pytest.mark.parametrize("rows,K,N", [(0, 40, 30), (5, 40, 0), (5, 0, 30), (0, 0, 30)])
+def test_products_of_nothing(rows, K, N):
+    x = torch.randn(rows, K, device=DEV).bfloat16().requires_grad_(True)
+    w = torch.randn(N, K, device=DEV).bfloat16().requires_grad_(True)
+    for nograd in (False, True):
+        with torch.set_grad_enabled(not nograd):
+            y = linear_float8(x, w)
+        assert y.shape == (rows, N) and not y.any()
+    y = linear_float8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert dx.shape == x.shape and dw.shape == w.shape and not dw.any() and (K == 0 or N == 0 or rows == 0) and not (N == 0 and dx.any())
+
+
 def test_two_streams_at_once():
     ins = [inputs(s, L=3000, D=130) for s in (4, 5)]
     want = [everything(*i) for i in ins]
