@@ -508,9 +508,11 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 // at 4 TB/s, and 3 for its launch.  So (tiles of 128 x 128, 256 x 128, 256 x 256) 4096 x 4096 x 4096 goes by the last (88, 63, 55), 2048 x 4096 x 4096
 // by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115), 701 x 7683 x 2560 by the second (35, 23, 34), and
 // 512 x 512 x 16384 in parts (119, 98, 147; the first in four parts 37, the second 33).
+// Where the last round of 256 x 256 tiles would leave the card half empty, the rows of the rounds before it go by those, the rest by
+// 256 x 128: 7683 x 2561 x 5003 by either alone 116 and 114 us, 105 so; 5040 x 7680 x 2560 97 and 101, 91 so.
 enum { TOKENS, TILE, TALL, WIDE };       // tiles of 128 x 128, 256 x 128, 256 x 256
 constexpr int kTokens = 8;
-struct Plan8 { int kernel, splits, split_steps; };
+struct Plan8 { int kernel, splits, split_steps; int64_t rest; };        // rest (WIDE): rows at the end that go by TALL
 float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
 {
     const int bm = kernel == TILE ? 128 : 256, bn = kernel == WIDE ? 256 : 128;
@@ -527,11 +529,11 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
     if (const char *e = tuning_env("GCG_P8")) {
         const char *s = tuning_env("GCG_P8S");
         const int n = s ? atoi(s) : 1, per = ((steps + n - 1) / n + 3) / 4 * 4, kernel = atoi(e);
-        if (kernel == TOKENS ? M > 16 : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4};
-        return {kernel, (steps + per - 1) / per, per};
+        if (kernel == TOKENS ? M > 16 : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4, 0};
+        return {kernel, (steps + per - 1) / per, per, 0};
     }
-    if (M <= kTokens) return {TOKENS, 1, steps};
-    Plan8 best = {TILE, 1, (steps + 3) / 4 * 4};
+    if (M <= kTokens) return {TOKENS, 1, steps, 0};
+    Plan8 best = {TILE, 1, (steps + 3) / 4 * 4, 0};
     float least = 0.f;
     for (int kernel = TILE; kernel <= WIDE; ++kernel)
         for (int n = 1; takes(kernel, M, N) && (n == 1 || (n <= 32 && steps >= 4 * n)); n *= 2) {
@@ -539,9 +541,20 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
             const float time = estimate(kernel, M, N, splits > 1 ? per : steps, splits);
             if (least == 0.f || time < least) {
                 least = time;
-                best = {kernel, splits, per};
+                best = {kernel, splits, per, 0};
             }
         }
+    if (best.kernel == TILE || best.splits > 1 || !takes(WIDE, M, N)) return best;
+    const int64_t across = (N + 255) / 256, items = (M + 255) / 256 * across;
+    for (int64_t rounds = 1; rounds * 256 < items; ++rounds) {
+        const int64_t rows = rounds * 256 / across * 256;
+        if (rows == 0 || M - rows < 256) continue;
+        const float time = estimate(WIDE, rows, N, steps, 1) + estimate(TALL, M - rows, N, steps, 1) + 2.f;
+        if (time < least) {
+            least = time;
+            best = {WIDE, 1, best.split_steps, M - rows};
+        }
+    }
     return best;
 }
 
@@ -567,17 +580,27 @@ template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Pl
         }
     }
     if (plan.kernel == TILE) return tile_launch<128, 128, 2, 2, T, A5, B5>(p, plan, st);
-    const int bn = plan.kernel == WIDE ? 256 : 128;
-    p.tiles_m = (uint32_t)((p.M + 255) / 256);
-    p.tiles_n = (uint32_t)((p.N + bn - 1) / bn);
-    const int64_t items = (int64_t)p.tiles_m * p.tiles_n * plan.splits;
-    const dim3 grid((unsigned)(items < 256 ? items : 256)), block(256);
     // Results that the last-level cache does not hold go past it: 16384 x 12288 x 4096, 402 MB, with the kernel that quantises its operand before it
     // 830 us without the hint, 790 with it.
     const bool stream = sizeof(T) == 2 && p.M * p.N * (int64_t)sizeof(T) > kStreamBytes;
-    if (plan.kernel == TALL) return launch_main(product8_wide_kernel<128, T, A5, B5, false>, grid, block, st, p);
-    return stream ? launch_main(product8_wide_kernel<256, T, A5, B5, sizeof(T) == 2>, grid, block, st, p)
-                  : launch_main(product8_wide_kernel<256, T, A5, B5, false>, grid, block, st, p);
+    const auto go = [&](auto launch, auto kernel, int64_t m0, int64_t M, int bn) {
+        Product8 q = p;
+        q.a += m0 * p.Kp;
+        q.a_scales += m0 * p.S;
+        q.y = (T *)p.y + m0 * p.N;
+        q.M = M;
+        q.tiles_m = (uint32_t)((M + 255) / 256);
+        q.tiles_n = (uint32_t)((p.N + bn - 1) / bn);
+        const int64_t items = (int64_t)q.tiles_m * q.tiles_n * plan.splits;
+        return launch(kernel, dim3((unsigned)(items < 256 ? items : 256)), dim3(256), st, q);
+    };
+    const auto main_one = [](auto... a) { return launch_main(a...); };
+    const auto plain_one = [](auto... a) { return launch_plain(a...); };
+    if (plan.kernel == TALL) return go(main_one, product8_wide_kernel<128, T, A5, B5, false>, 0, p.M, 128);
+    const int64_t M = p.M - plan.rest;
+    const int rc = stream ? go(main_one, product8_wide_kernel<256, T, A5, B5, sizeof(T) == 2>, 0, M, 256)
+                          : go(main_one, product8_wide_kernel<256, T, A5, B5, false>, 0, M, 256);
+    return rc || plan.rest == 0 ? rc : go(plain_one, product8_wide_kernel<128, T, A5, B5, false>, M, plan.rest, 128);
 }
 template <typename T> int product_format(Product8 &p, int a5, int b5, const Plan8 &plan, hipStream_t st)
 {

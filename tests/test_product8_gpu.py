@@ -49,9 +49,29 @@ def test_whole_numbers(M, N, K, fa, fb):
 @pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4095, 3841, 256), (3850, 4001, 300), (4096, 3900, 512), (3841, 4096, 640), (4001, 4001, 700),
                                    (4090, 4094, 1000), (8200, 6000, 1300), (12000, 11500, 1300),
                                    (2048, 4096, 128), (2047, 4000, 256), (1793, 3999, 300), (2000, 4095, 512), (2040, 4001, 640), (701, 7683, 1000),
-                                   (1900, 3970, 1101), (300, 200, 5000), (1000, 1000, 8200), (2040, 2048, 16384)])
+                                   (1900, 3970, 1101), (300, 200, 5000), (1000, 1000, 8200), (2040, 2048, 16384),
+                                   (5003, 7683, 1301), (4700, 4201, 1300), (9000, 2000, 1100), (70000, 257, 1300), (16700, 1025, 900)])
 def test_wide_tiles(M, N, K):
-    """Sizes that take least time in tiles of 256 x 256 (the first nine and the last) and of 256 x 128, at rows and columns that the tiles do not divide, in every
+    """Sizes that take least time in tiles of 256 x 256 (the first nine and the nineteenth), of 256 x 128, and (the last five) of both, at rows
+    and columns that the tiles do not divide, in every length of the loop's rest, in several rounds, in parts, and with more results than
+    the last-level cache holds."""
+    most = 8 if K < 2000 else 4                                     # |sums| < 16384 * 4 * 4 * 16 < 2^24
+    a, b = whole(M, K, fa, M + K, most), whole(N, K, fb, N + K + 1, most)
+    qa, qb = to_float8(a, fa), to_float8(b, fb)
+    assert torch.equal(values(qa), a.double()) and torch.equal(values(qb), b.double())
+    want = (a.float().double() @ b.float().double().t())
+    for dtype in (torch.bfloat16, torch.float16):
+        got = matmul_float8(qa, qb, dtype)
+        assert torch.equal(got, want.to(dtype)), f"{M} x {N} x {K}: {(got != want.to(dtype)).sum().item()} differ"
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4095, 3841, 256), (3850, 4001, 300), (4096, 3900, 512), (3841, 4096, 640), (4001, 4001, 700),
+                                   (4090, 4094, 1000), (8200, 6000, 1300), (12000, 11500, 1300),
+                                   (2048, 4096, 128), (2047, 4000, 256), (1793, 3999, 300), (2000, 4095, 512), (2040, 4001, 640), (701, 7683, 1000),
+                                   (1900, 3970, 1101), (300, 200, 5000), (1000, 1000, 8200), (2040, 2048, 16384),
+                                   (5003, 7683, 1301), (4700, 4201, 1300), (9000, 2000, 1100), (70000, 257, 1300), (16700, 1025, 900)])
+def test_wide_tiles(M, N, K):
+    """Sizes that take least time in tiles of 256 x 256 (the first nine and the twentieth), of 256 x 128 and (the last five) of both, at rows and columns that the tiles do not divide, in every
     length of the loop's rest, in several rounds, in parts, and with more results than the last-level cache holds."""
     most = 8 if K < 2000 else 4
     a, b = whole(M, K, E4M3, K, most), whole(N, K, E4M3, K + 1, most)
