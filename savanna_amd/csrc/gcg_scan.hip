@@ -533,7 +533,15 @@ template <typename T, bool GATE> __global__ __launch_bounds__(256) void scan_ste
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
-constexpr int kFwdRows = 128;       // rows of a chunk of the forward
+// Rows of a chunk of the forward: 128, two workgroups a CU, which overlap one's loads with the other's sums.  256, one workgroup a CU, where the card
+// holds all of those at once and either they are whole sequences or those of 128 are more than a CU's one: what counts then is the chain of waits.
+// In chunks of 128 and 256: 4 x 701 x 2560 f16 17.8 and 15.9 us, 1 x 8192 x 1024 bf16 28.6 and 23.4, 16 x 256 x 1024 fp32 22.7 and 11.9; but
+// 1 x 512 x 4096 14.1 and 16.1, 64 x 256 x 4096 112 and 122, 2 x 8192 x 4096 118 and 131.
+int fwd_rows(int64_t bs, int64_t L, int64_t D)
+{
+    const int64_t cols = (D + 127) / 128, high = bs * ((L + 255) / 256) * cols, low = bs * ((L + 127) / 128) * cols;
+    return L > 128 && high <= 256 && (L <= 256 || low > 256) ? 256 : 128;
+}
 // Chunks of a group: 131072 x 512 fp32 193 us with 8, 196 with 16, 223 with 32; 2 x 8192 x 4096 bf16 113, 118 and 131.
 constexpr int kGroup = 8;
 
@@ -541,7 +549,8 @@ struct Layout { int64_t chunks, groups, pairs, carries, total; };
 Layout layout_of(int64_t bs, int64_t L, int64_t D, bool backward)
 {
     Layout l;
-    l.chunks = (L + (backward ? kChunk : kFwdRows) - 1) / (backward ? kChunk : kFwdRows);
+    const int rows = backward ? kChunk : fwd_rows(bs, L, D);
+    l.chunks = (L + rows - 1) / rows;
     l.groups = (l.chunks + kGroup - 1) / kGroup;
     l.pairs = 256;
     l.carries = l.pairs + bs * l.chunks * D * 8;
@@ -566,13 +575,17 @@ int set_up(Scan &p, const Layout &l, void *ws, hipStream_t st)
 
 bool even(const ScanTensor &t, bool given) { return !given || (((uintptr_t)t.p & 3) == 0 && t.batch % 2 == 0 && t.time % 2 == 0); }
 
+template <typename T, int C, int W> int fwd_w(const Scan &p, int64_t n, hipStream_t st)
+{
+    if (!launch_holds(n, W * 64)) return (int)hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)n), block(W * 64);
+    return p.gate.p ? launch_main(scan_fwd_kernel<T, C, 16, W, true>, grid, block, st, p) : launch_main(scan_fwd_kernel<T, C, 16, W, false>, grid, block, st, p);
+}
 template <typename T, int C> int fwd_c(Scan &p, hipStream_t st)
 {
     p.cols = (p.D + 64 * C - 1) / (64 * C);
     const int64_t n = (int64_t)p.chunks * p.bs * p.cols;
-    if (!launch_holds(n, 512)) return (int)hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)n), block(512);
-    return p.gate.p ? launch_main(scan_fwd_kernel<T, C, 16, 8, true>, grid, block, st, p) : launch_main(scan_fwd_kernel<T, C, 16, 8, false>, grid, block, st, p);
+    return fwd_rows(p.bs, p.L, p.D) == 256 ? fwd_w<T, C, 16>(p, n, st) : fwd_w<T, C, 8>(p, n, st);
 }
 template <typename T, int C> int bwd_c(Scan &p, hipStream_t st)
 {

@@ -115,6 +115,19 @@ def test_forward_and_backward(bs, L, D, dtype):
     assert all(torch.equal(again[n], v) for n, v in got.items())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bs,L,D,lengths", [(2, 256, 129, None), (2, 255, 70, [255, 130]), (6, 700, 1601, [700, 0, 1, 256, 257, 513]), (1, 3000, 1300, None),
+                                            (2, 2300, 896, [2300, 2049])])
+def test_sizes_whose_chunks_are_long(bs, L, D, lengths, dtype):
+    """Those that the card holds at once in chunks of 256 rows: a sequence in one chunk, in several, in more than a group of them."""
+    d = data(bs, L, D, dtype, seed=L + D)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    got = run(d, lengths=n)
+    compare(got, reference(d, lengths=n), f"{bs} x {L} x {D}")
+    again = run(d, lengths=n)
+    assert all(torch.equal(again[n], v) for n, v in got.items())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("gate,bias,initial,final", [(False, False, False, False), (True, False, False, False), (False, True, True, False), (True, True, False, True),
                                                      (False, False, True, True)])
