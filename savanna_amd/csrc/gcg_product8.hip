@@ -424,71 +424,153 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
     }
 }
 
-// Few rows of a (tokens, 16 at most): what counts is how fast b's rows arrive.  A workgroup takes 16 of them, its W waves each a part of the blocks;
-// fragments come straight from memory into registers, UNROLL blocks' at a time, each row's 128 bytes by two instructions of 64.  With FUSED, a is
+// Few rows of a (tokens, 64 at most): what counts is how fast b's rows arrive.  A workgroup takes 16 NT of them and all of a's, its W waves each a
+// part of the blocks; a wave keeps R blocks on their way into its own ring in shared memory, and waits for nobody.  (Straight into registers a
+// fragment's load takes a line a lane, since neighbouring lanes hold neighbouring rows: four times the cycles of one that goes along the rows, and
+// more than the memory's time from some rows of a on: 12288 x 4096 with 1 row 13.3, with 64 rows 43 us.)  With FUSED, a is
 // a tensor of type T, and the workgroup quantises it into shared memory while b's first rows are on their way: kTokenBytes of codes at most, since
 // every workgroup does.  The waves' sums join in shared memory, in their order.
 constexpr int kTokenBytes = 16384;
+constexpr int kTokenBlocks = 32;    // of a wave, at most
 struct Tokens8 {
     Product8 p;
     const void *x;              // FUSED: a in its own type
     int64_t K;
 };
-template <typename T, int W, bool FUSED, bool A5, bool B5> __global__ __launch_bounds__(W * 64) void product8_tokens_kernel(Tokens8 s)
+template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> __global__ __launch_bounds__(W * 64) void product8_tokens_kernel(Tokens8 s)
 {
-    constexpr int UNROLL = 8;
+    static_assert(!FUSED || MT == 1, "tokens that are quantised here are 16 at most");
+    constexpr int AT = FUSED ? 0 : MT, TILES = AT + NT, STAGE = TILES * 2048;
+    constexpr int FIT = 32768 / (W * STAGE), R = FIT < 2 ? 2 : FIT;
+    constexpr int WORDS = (kTokenBlocks + 3) / 4 + 1, ROWS = (TILES + 3) / 4 * 64;
+    constexpr int SUMS = W * MT * NT * 1024;
     const Product8 &p = s.p;
-    __shared__ f32x4 sums[W - 1][64];
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[W * R * STAGE > SUMS ? W * R * STAGE : SUMS];
+    __shared__ uint32_t words[W][WORDS][ROWS];
     __shared__ __attribute__((aligned(16))) uint8_t own[FUSED ? kTokenBytes : 16];
     __shared__ uint8_t own_scales[FUSED ? kTokenBytes / 128 : 1];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, r16 = lane % 16, quarter = lane / 16;
-    const int64_t n0 = (int64_t)blockIdx.x * 16, n = n0 + r16 < p.N ? n0 + r16 : p.N - 1, m = r16 < p.M ? r16 : p.M - 1;
-    const int per = (p.steps + W - 1) / W, k0 = wave * per, k1 = k0 + per < p.steps ? k0 + per : p.steps;
-    const uint8_t *b = p.b + n * p.Kp + quarter * 16, *sb = p.b_scales + n * p.S;
-    const uint8_t *a = (FUSED ? own : p.a) + m * p.Kp + quarter * 16, *sa = FUSED ? own_scales + m * p.steps : p.a_scales + m * p.S;
-    const auto fragment = [](const uint8_t *from) {
-        const u32x4 lo = *(const u32x4 *)from, hi = *(const u32x4 *)(from + 64);
-        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    };
-    i32x8 fb[UNROLL];
-    uint32_t cb[UNROLL];
-    const auto request = [&](int k) {
+    // (the wave's number in a scalar register: a product ignores the lanes' mask, so its conditions have to be branches)
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r16 = lane % 16, quarter = lane / 16;
+    const int64_t n0 = (int64_t)blockIdx.x * (NT * 16);
+    const int per = (p.steps + W - 1) / W, k0 = wave * per, n = p.steps - k0 < per ? p.steps - k0 : per;
+    const win_t wa = make_window(p.a, 0x7fffffff), wb = make_window(p.b + n0 * p.Kp, 0x7fffffff);
+    // a load's eight rows of 128 bytes, their pieces at exchanged places
+    uint32_t off[TILES][2];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int64_t at = k + u < k1 ? k + u : p.steps - 1;
-            fb[u] = fragment(b + at * 128);
-            cb[u] = sb[at];
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = h * 8 + lane / 8, row = (i < AT ? i : i - AT) * 16 + r;
+            const int64_t last = i < AT ? p.M - 1 : p.N - 1 - n0;
+            off[i][h] = (uint32_t)((row < last ? row : last) * p.Kp) + ((lane % 8) ^ ((r >> 1) & 7)) * 16;
         }
+    const uint32_t to = (uint32_t)(uintptr_t)(lds_t)ring + wave * (R * STAGE);
+    const auto request = [&](int i, int slot) {
+        const int at = (k0 + i) * 128;
+        const uint32_t q = to + slot * STAGE;
+#pragma unroll
+        for (int f = 0; f < TILES; ++f)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) request_to_lds<16>(f < AT ? wa : wb, q + f * 2048 + h * 1024, off[f][h], at);
     };
-    request(k0);
+    if (n > 0) {
+        // the rows' scales, a word of four at a time, one row a lane
+        const win_t wsa = make_window(p.a_scales, 0x7fffffff), wsb = make_window(p.b_scales + n0 * p.S, 0x7fffffff);
+        const uint32_t first = (uint32_t)(uintptr_t)(lds_t)words[wave][0];
+#pragma unroll
+        for (int c = 0; c < ROWS; c += 64) {
+            const int f = (c + lane) / 16, row = (f < AT ? f : f - AT) * 16 + r16;
+            const int64_t last = f < AT ? p.M - 1 : p.N - 1 - n0;
+            const uint32_t at = (uint32_t)((row < last ? row : last) * p.S);
+            for (int w = 0; w <= (k0 + n - 1) / 4 - k0 / 4; ++w) {
+                if (f < AT) request_to_lds<4>(wsa, first + (w * ROWS + c) * 4, at, (k0 / 4 + w) * 4);
+                else if (f < TILES) request_to_lds<4>(wsb, first + (w * ROWS + c) * 4, at, (k0 / 4 + w) * 4);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (i < n) request(i, i);
+    }
     if constexpr (FUSED) {
-        // sixteen lanes a block, whole waves at a time
+        // sixteen lanes a block, whole waves at a time; everything is requested before the first is waited for
+        constexpr int TURNS = kTokenBytes / 128 / (W * 4);
         const int blocks = (int)p.M * p.steps, c = threadIdx.x % 16 * 8;
-        for (int i = threadIdx.x / 16; i < (blocks + 3) / 4 * 4; i += W * 4) {
-            const int row = i / p.steps, k = i - row * p.steps;
+        u32x4 raw[TURNS];
+#pragma unroll
+        for (int q = 0; q < TURNS; ++q) {
+            const int i = q * (W * 4) + threadIdx.x / 16, row = i / p.steps, k = i - row * p.steps;
             const int64_t left = s.K - (k * 128 + c);
-            u32x4 raw = {0, 0, 0, 0};
-            if (i < blocks && left > 0) raw = load_row_vec<T, true, false>((const T *)s.x + row * s.K + k * 128 + c, 0, (int)(left < 8 ? left : 8));
+            raw[q] = u32x4{0, 0, 0, 0};
+            if (i < blocks && left > 0) raw[q] = load_row_vec<T, true, false>((const T *)s.x + row * s.K + k * 128 + c, 0, (int)(left < 8 ? left : 8));
+        }
+#pragma unroll
+        for (int q = 0; q < TURNS; ++q) {
+            const int i = q * (W * 4) + threadIdx.x / 16;
+            if (q * (W * 4) + wave * 4 >= blocks) break;
             float v[8];
-            unpack_vec(raw, v, T{});
+            unpack_vec(raw[q], v, T{});
             store_f8<8, A5, false>(own + i * 128, own_scales + i, c, i < blocks ? 128 : 0, v);
         }
         __syncthreads();
     }
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = k0; k < k1; k += UNROLL) {
-        if (k > k0) request(k);
+    const int swap = (r16 >> 1) & 7, p0 = r16 * 128 + (quarter ^ swap) * 16, p1 = r16 * 128 + ((quarter + 4) ^ swap) * 16;
+    const int64_t m_own = r16 < p.M ? r16 : p.M - 1;
+    const auto fragment = [](const uint8_t *lo_at, const uint8_t *hi_at) {
+        const u32x4 lo = *(const u32x4 *)lo_at, hi = *(const u32x4 *)hi_at;
+        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
+    f32x4 acc[MT][NT];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (k + u < k1) acc = mfma8<B5, A5>(fb[u], fragment(a + (k + u) * 128), acc, cb[u], sa[k + u]);
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0, slot = 0; i < n; ++i, slot = slot + 1 < R ? slot + 1 : 0) {
+        // the block is there: all but the R - 1 after it have arrived
+        if (n - i >= R) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R - 1) * TILES * 2) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint8_t *from = ring + wave * (R * STAGE) + slot * STAGE;
+        const int k = k0 + i, shift = k % 4 * 8;
+        const uint32_t *w = words[wave][k / 4 - k0 / 4];
+        i32x8 A[MT], B[NT];
+        uint32_t ca[MT], cb[NT];
+#pragma unroll
+        for (int f = 0; f < MT; ++f) {
+            const uint8_t *mine = own + m_own * p.Kp + k * 128 + quarter * 16;
+            A[f] = FUSED ? fragment(mine, mine + 64) : fragment(from + f * 2048 + p0, from + f * 2048 + p1);
+            ca[f] = FUSED ? own_scales[m_own * p.steps + k] : w[f * 16 + r16] >> shift;
+        }
+#pragma unroll
+        for (int f = 0; f < NT; ++f) {
+            B[f] = fragment(from + (AT + f) * 2048 + p0, from + (AT + f) * 2048 + p1);
+            cb[f] = w[(AT + f) * 16 + r16] >> shift;
+        }
+        if (i + R < n) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");              // read, before it is written over
+            request(i + R, slot);
+        }
+#pragma unroll
+        for (int x = 0; x < MT; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y) acc[x][y] = mfma8<B5, A5>(B[y], A[x], acc[x][y], cb[y], ca[x]);
     }
-    if (wave > 0) sums[wave - 1][lane] = acc;
     __syncthreads();
-    if (wave > 0 || r16 >= p.M) return;
+    f32x4 *sums = (f32x4 *)ring;
 #pragma unroll
-    for (int w = 0; w < W - 1; ++w) acc += sums[w][lane];
-    T *y = (T *)p.y + m * p.N + n0 + quarter * 4;
-    store4(y, acc, p.N - n0 - quarter * 4, p.N % 4 == 0 && ((uintptr_t)p.y & (4 * sizeof(T) - 1)) == 0);
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sums[(wave * (MT * NT) + i * NT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int f0 = 0; f0 < MT * NT; f0 += W) {
+        const int f = f0 + wave;
+        if (f < MT * NT) {
+            f32x4 v = sums[f * 64 + lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v += sums[(w * (MT * NT) + f) * 64 + lane];
+            const int64_t m = f / NT * 16 + r16, col = n0 + f % NT * 16 + quarter * 4;
+            if (m < p.M) store4((T *)p.y + m * p.N + col, v, p.N - col, p.N % 4 == 0 && ((uintptr_t)p.y & (4 * sizeof(T) - 1)) == 0);
+        }
+    }
 }
 
 // the parts of a product that was split over its blocks, added in their order
@@ -502,8 +584,8 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 }
 
 // Which kernel, and in how many parts of the blocks (each a sum in fp32, joined by another kernel): what would take the least time.
-// Few rows go by product8_tokens_kernel: 12288 x 4096 with 1 row 12.3 us (tiles of 128 in four parts 14.5), with 16 rows 17.8 (14.8).
-// Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.65 if half the
+// Up to 64 rows go by product8_tokens_kernel (from 12288 x 4096 with 1, 16, 64 rows 11.6, 12.7, 16.3 us, tiles of 128 in parts 14.5, 18.5, 23.2;
+// 2560 x 2560 4.2, 4.4, 5.6 and 11.4 to 12.6; 4096 x 16384 15, 15, 27 and 22 to 27).  Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.65 if half the
 // card is idle); 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice
 // at 4 TB/s, and 3 for its launch.  So (tiles of 128 x 128, 256 x 128, 256 x 256) 4096 x 4096 x 4096 goes by the last (88, 63, 55), 2048 x 4096 x 4096
 // by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115), 701 x 7683 x 2560 by the second (35, 23, 34), and
@@ -511,7 +593,6 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 // Where the last round of 256 x 256 tiles would leave the card half empty, the rows of the rounds before it go by those, the rest by
 // 256 x 128: 7683 x 2561 x 5003 by either alone 116 and 114 us, 105 so; 5040 x 7680 x 2560 97 and 101, 91 so.
 enum { TOKENS, TILE, TALL, WIDE };       // tiles of 128 x 128, 256 x 128, 256 x 256
-constexpr int kTokens = 8;
 struct Plan8 { int kernel, splits, split_steps; int64_t rest; };        // rest (WIDE): rows at the end that go by TALL
 float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
 {
@@ -522,6 +603,8 @@ float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
     if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.65f : 0.85f) + 5.f) + join;
     return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + join;
 }
+// whether product8_tokens_kernel takes it: its waves have kTokenBlocks each at most
+bool tokens(int64_t M, int steps) { return M <= 32 ? steps <= 8 * kTokenBlocks : M <= 64 && steps <= 4 * kTokenBlocks; }
 bool takes(int kernel, int64_t M, int64_t N) { return kernel == TILE || (M >= 256 && N >= (kernel == WIDE ? 256 : 128)); }
 Plan8 plan_of(int64_t M, int64_t N, int64_t K)
 {
@@ -529,10 +612,10 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
     if (const char *e = tuning_env("GCG_P8")) {
         const char *s = tuning_env("GCG_P8S");
         const int n = s ? atoi(s) : 1, per = ((steps + n - 1) / n + 3) / 4 * 4, kernel = atoi(e);
-        if (kernel == TOKENS ? M > 16 : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4, 0};
+        if (kernel == TOKENS ? !tokens(M, steps) : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4, 0};
         return {kernel, (steps + per - 1) / per, per, 0};
     }
-    if (M <= kTokens) return {TOKENS, 1, steps, 0};
+    if (tokens(M, steps)) return {TOKENS, 1, steps, 0};
     Plan8 best = {TILE, 1, (steps + 3) / 4 * 4, 0};
     float least = 0.f;
     for (int kernel = TILE; kernel <= WIDE; ++kernel)
@@ -564,19 +647,29 @@ template <int BM, int BN, int WM, int WN, typename T, bool A5, bool B5> int tile
     p.tiles_n = (uint32_t)((p.N + BN - 1) / BN);
     return launch_main(product8_kernel<BM, BN, WM, WN, T, A5, B5>, dim3(p.tiles_m * p.tiles_n, (unsigned)plan.splits), dim3(WM * WN * 64), st, p);
 }
-template <typename T, bool FUSED, bool A5, bool B5> int tokens_launch(const Tokens8 &s, hipStream_t st)
+template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> int tokens_go(const Tokens8 &s, hipStream_t st)
 {
-    const dim3 grid((unsigned)((s.p.N + 15) / 16));
-    // eight waves where four a workgroup would leave the card half empty
-    return grid.x < 512 && s.p.steps >= 16 ? launch_main(product8_tokens_kernel<T, 8, FUSED, A5, B5>, grid, dim3(512), st, s)
-                                           : launch_main(product8_tokens_kernel<T, 4, FUSED, A5, B5>, grid, dim3(256), st, s);
+    const dim3 grid((unsigned)((s.p.N + NT * 16 - 1) / (NT * 16)));
+    return launch_main(product8_tokens_kernel<T, MT, NT, W, FUSED, A5, B5>, grid, dim3(W * 64), st, s);
+}
+// Rows of b for a workgroup: 16 while the card's CUs have one workgroup each, else more, which share a's fragments.  Eight waves where a wave of
+// four would have sixteen blocks and the CU no other workgroup.  (FUSED changes nothing in it, so that sums are in the same order.)
+template <typename T, int MT, bool FUSED, bool A5, bool B5> int tokens_tiles(const Tokens8 &s, hipStream_t st)
+{
+    const int64_t sixteens = (s.p.N + 15) / 16;
+    if constexpr (MT <= 2)
+        if (s.p.steps > 4 * kTokenBlocks || (s.p.steps >= 64 && sixteens <= 256)) return tokens_go<T, MT, 1, 8, FUSED, A5, B5>(s, st);
+    if (sixteens <= 256) return tokens_go<T, MT, 1, 4, FUSED, A5, B5>(s, st);
+    if constexpr (MT == 4)
+        if (sixteens > 512) return tokens_go<T, MT, 4, 4, FUSED, A5, B5>(s, st);
+    return tokens_go<T, MT, 2, 4, FUSED, A5, B5>(s, st);
 }
 template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
 {
     if constexpr (sizeof(T) == 2) {
         if (plan.kernel == TOKENS) {
             const Tokens8 s = {p, nullptr, 0};
-            return tokens_launch<T, false, A5, B5>(s, st);
+            return p.M <= 16 ? tokens_tiles<T, 1, false, A5, B5>(s, st) : p.M <= 32 ? tokens_tiles<T, 2, false, A5, B5>(s, st) : tokens_tiles<T, 4, false, A5, B5>(s, st);
         }
     }
     if (plan.kernel == TILE) return tile_launch<128, 128, 2, 2, T, A5, B5>(p, plan, st);
@@ -641,8 +734,8 @@ int linear8_launch(int dtype, int b5, const void *x, const uint8_t *b, const uin
 {
     const Product8 p = {nullptr, nullptr, b, b_scales, y, nullptr, M, N, f8_cols(K), (int32_t)f8_scales(K), (int32_t)(f8_cols(K) / 128), 0, 1, 0, 0};
     const Tokens8 s = {p, x, K};
-    if (dtype == GCG_BF16) return b5 ? tokens_launch<bf16_t, true, false, true>(s, st) : tokens_launch<bf16_t, true, false, false>(s, st);
-    return b5 ? tokens_launch<f16_t, true, false, true>(s, st) : tokens_launch<f16_t, true, false, false>(s, st);
+    if (dtype == GCG_BF16) return b5 ? tokens_tiles<bf16_t, 1, true, false, true>(s, st) : tokens_tiles<bf16_t, 1, true, false, false>(s, st);
+    return b5 ? tokens_tiles<f16_t, 1, true, false, true>(s, st) : tokens_tiles<f16_t, 1, true, false, false>(s, st);
 }
 
 } // namespace gcg

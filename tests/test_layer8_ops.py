@@ -145,8 +145,8 @@ def test_c_entries_of_float8_refuse(gcg_lib):
     ok = [p] * 5
     assert mul(*ok, M=0) == mul(*ok, N=-1) == mul(*ok, K=0) == mul(*ok, fa=0) == mul(*ok, fb=18) == mul(*ok, dtype=0) == mul(odd, *ok[1:]) == BAD_ARG
     assert mul(*ok, K=(1 << 22) + 1) == UNSUPPORTED
-    need = gcg_lib.gcg_product8_workspace_bytes(64, 64, 16384)
-    assert need > 0 and need % 256 == 0 and mul(*ok, M=64, N=64, K=16384) == WORKSPACE and gcg_lib.gcg_product8_workspace_bytes(4096, 4096, 4096) == 0
+    need = gcg_lib.gcg_product8_workspace_bytes(65, 64, 16384)
+    assert need > 0 and need % 256 == 0 and mul(*ok, M=65, N=64, K=16384) == WORKSPACE and gcg_lib.gcg_product8_workspace_bytes(4096, 4096, 4096) == 0
     assert gcg_lib.gcg_product8_workspace_bytes(1, 1, (1 << 22) + 1) == 0
     few = lambda *a, M=1, N=64, K=4096, fb=16, dtype=1: gcg_lib.gcg_linear8(*a, M, N, K, fb, dtype, none)                      # noqa: E731
     for i in range(4):
@@ -164,9 +164,9 @@ def test_c_entries_of_the_recurrence_refuse(gcg_lib):
     assert fwd(x=none) == fwd(f=none) == fwd(y=none) == BAD_ARG
     assert fwd(bs=0) == fwd(L=0) == fwd(D=0) == fwd(dtype=3) == fwd(s=strides(4, time=-1)) == fwd(s=strides(4, batch=-1)) == BAD_ARG
     assert fwd(D=(1 << 19) + 1) == fwd(s=strides(4, time=(1 << 21) + 1)) == fwd(L=(1 << 30) + 1) == fwd(bs=1 << 31) == UNSUPPORTED
-    assert gcg_lib.gcg_scan_workspace_bytes(2, 128, 64, 0) == 0 and fwd(L=129) == WORKSPACE
-    need = gcg_lib.gcg_scan_workspace_bytes(2, 129, 64, 0)
-    assert need % 256 == 0 and fwd(L=129, ws=ptr((1 << 20) + 64), n=need) == WORKSPACE and fwd(L=129, ws=p, n=need - 1) == WORKSPACE
+    assert gcg_lib.gcg_scan_workspace_bytes(2, 256, 64, 0) == 0 and fwd(L=257) == WORKSPACE
+    need = gcg_lib.gcg_scan_workspace_bytes(2, 257, 64, 0)
+    assert need % 256 == 0 and fwd(L=257, ws=ptr((1 << 20) + 64), n=need) == WORKSPACE and fwd(L=257, ws=p, n=need - 1) == WORKSPACE
     bwd = lambda *a, s=None, gate=none, dgate=none, L=10, D=64: gcg_lib.gcg_scan_bwd(                                          # noqa: E731
         a[0], a[1], a[2], gate, s if s is not None else strides(7), none, a[3], none, none, a[4], a[5], dgate, none, none, none, 0, 2, L, D, 0, none)
     for i in range(6):

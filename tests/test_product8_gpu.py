@@ -125,6 +125,18 @@ def test_tokens_quantised_in_the_kernel(M, N, K, fmt):
             assert torch.equal(linear_float8(x.to(dtype), w), want.to(dtype))
 
 
+@pytest.mark.parametrize("N", [40, 300, 4097, 9000])
+@pytest.mark.parametrize("M", [1, 15, 16, 17, 31, 33, 50, 64])
+def test_tokens(M, N):
+    """Rows that go by one workgroup's tokens: every number of them, of b's rows for a workgroup, and of blocks for a wave, none and many."""
+    for K in (1, 128, 390, 512, 1150, 4224, 8192 + 100, 16384, 16500, 32768):
+        most = 8 if K < 2000 else 3                                 # |sums| < 32768 * 3 * 3 * 16 < 2^23
+        a, b = whole(M, K, E4M3, K, most), whole(N, K, E4M3, K + 1, most)
+        got = matmul_float8(to_float8(a), to_float8(b))
+        want = (a.float() @ b.float().t()).to(torch.bfloat16)       # (fp32 holds these sums)
+        assert torch.equal(got, want), f"{M} x {N} x {K}: {(got != want).sum().item()} differ"
+
+
 def test_infinities_and_nan():
     for M in (2, 20, 300):
         a, b = torch.ones(M, 300, device=DEV).bfloat16(), torch.ones(260, 300, device=DEV).bfloat16()
