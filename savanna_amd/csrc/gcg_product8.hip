@@ -451,9 +451,11 @@ template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> __glo
     __shared__ uint8_t own_scales[FUSED ? kTokenBytes / 128 : 1];
     // (the wave's number in a scalar register: a product ignores the lanes' mask, so its conditions have to be branches)
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r16 = lane % 16, quarter = lane / 16;
-    const int64_t n0 = (int64_t)blockIdx.x * (NT * 16);
+    // groups of a's rows that read the same rows of b follow each other
+    const uint32_t item = xcd_contiguous_u32(blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)(item % p.tiles_m) * (MT * 16), n0 = (int64_t)(item / p.tiles_m) * (NT * 16);
     const int per = (p.steps + W - 1) / W, k0 = wave * per, n = p.steps - k0 < per ? p.steps - k0 : per;
-    const win_t wa = make_window(p.a, 0x7fffffff), wb = make_window(p.b + n0 * p.Kp, 0x7fffffff);
+    const win_t wa = make_window(p.a + m0 * p.Kp, 0x7fffffff), wb = make_window(p.b + n0 * p.Kp, 0x7fffffff);
     // a load's eight rows of 128 bytes, their pieces at exchanged places
     uint32_t off[TILES][2];
 #pragma unroll
@@ -461,7 +463,7 @@ template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> __glo
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = h * 8 + lane / 8, row = (i < AT ? i : i - AT) * 16 + r;
-            const int64_t last = i < AT ? p.M - 1 : p.N - 1 - n0;
+            const int64_t last = i < AT ? p.M - 1 - m0 : p.N - 1 - n0;
             off[i][h] = (uint32_t)((row < last ? row : last) * p.Kp) + ((lane % 8) ^ ((r >> 1) & 7)) * 16;
         }
     const uint32_t to = (uint32_t)(uintptr_t)(lds_t)ring + wave * (R * STAGE);
@@ -475,12 +477,12 @@ template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> __glo
     };
     if (n > 0) {
         // the rows' scales, a word of four at a time, one row a lane
-        const win_t wsa = make_window(p.a_scales, 0x7fffffff), wsb = make_window(p.b_scales + n0 * p.S, 0x7fffffff);
+        const win_t wsa = make_window(p.a_scales + m0 * p.S, 0x7fffffff), wsb = make_window(p.b_scales + n0 * p.S, 0x7fffffff);
         const uint32_t first = (uint32_t)(uintptr_t)(lds_t)words[wave][0];
 #pragma unroll
         for (int c = 0; c < ROWS; c += 64) {
             const int f = (c + lane) / 16, row = (f < AT ? f : f - AT) * 16 + r16;
-            const int64_t last = f < AT ? p.M - 1 : p.N - 1 - n0;
+            const int64_t last = f < AT ? p.M - 1 - m0 : p.N - 1 - n0;
             const uint32_t at = (uint32_t)((row < last ? row : last) * p.S);
             for (int w = 0; w <= (k0 + n - 1) / 4 - k0 / 4; ++w) {
                 if (f < AT) request_to_lds<4>(wsa, first + (w * ROWS + c) * 4, at, (k0 / 4 + w) * 4);
@@ -567,7 +569,7 @@ template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> __glo
             f32x4 v = sums[f * 64 + lane];
 #pragma unroll
             for (int w = 1; w < W; ++w) v += sums[(w * (MT * NT) + f) * 64 + lane];
-            const int64_t m = f / NT * 16 + r16, col = n0 + f % NT * 16 + quarter * 4;
+            const int64_t m = m0 + f / NT * 16 + r16, col = n0 + f % NT * 16 + quarter * 4;
             if (m < p.M) store4((T *)p.y + m * p.N + col, v, p.N - col, p.N % 4 == 0 && ((uintptr_t)p.y & (4 * sizeof(T) - 1)) == 0);
         }
     }
@@ -584,12 +586,13 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 }
 
 // Which kernel, and in how many parts of the blocks (each a sum in fp32, joined by another kernel): what would take the least time.
-// Up to 64 rows go by product8_tokens_kernel (from 12288 x 4096 with 1, 16, 64 rows 11.6, 12.7, 16.3 us, tiles of 128 in parts 14.5, 18.5, 23.2;
-// 2560 x 2560 4.2, 4.4, 5.6 and 11.4 to 12.6; 4096 x 16384 15, 15, 27 and 22 to 27).  Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.65 if half the
-// card is idle); 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice
+// Up to 64 rows go by product8_tokens_kernel (from 12288 x 4096 with 1, 16, 64 rows 11.8, 12.7, 15.7 us, tiles of 128 in parts 14.5, 18.5, 23.2;
+// 2560 x 2560 4.2, 4.4, 5.7 and 11.4 to 12.6; 4096 x 16384 15, 15, 27 and 22 to 27), and more in groups of 64 where that takes least time (256 rows
+// from 4096 x 4096 10, by tiles of 128 in parts 21; 512 rows 18 and 30; 1000 x 1000 x 1000 5.7 and 9.5; 400 rows from 12288 x 4096 53, tiles of 256 x 128
+// 46).  Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.9 if half
+// the card is idle); 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice
 // at 4 TB/s, and 3 for its launch.  So (tiles of 128 x 128, 256 x 128, 256 x 256) 4096 x 4096 x 4096 goes by the last (88, 63, 55), 2048 x 4096 x 4096
-// by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115), 701 x 7683 x 2560 by the second (35, 23, 34), and
-// 512 x 512 x 16384 in parts (119, 98, 147; the first in four parts 37, the second 33).
+// by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115) and 701 x 7683 x 2560 by the second (35, 23, 34).
 // Where the last round of 256 x 256 tiles would leave the card half empty, the rows of the rounds before it go by those, the rest by
 // 256 x 128: 7683 x 2561 x 5003 by either alone 116 and 114 us, 105 so; 5040 x 7680 x 2560 97 and 101, 91 so.
 enum { TOKENS, TILE, TALL, WIDE };       // tiles of 128 x 128, 256 x 128, 256 x 256
@@ -600,8 +603,23 @@ float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
     const int64_t items = ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits;
     const float join = splits > 1 ? 3.f + (float)M * (float)N * (float)splits * 8.f / 4e6f : 0.f;
     if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.35f + 6.f) + join;
-    if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.65f : 0.85f) + 5.f) + join;
+    if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.9f : 0.85f) + 5.f) + join;
     return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + join;
+}
+// Groups of 64 rows by product8_tokens_kernel: the rows of b for a workgroup (in sixteens) that take least time, and that time; as measured, a round
+// of 256 workgroups takes 1.9 us and 0.55, 0.85, 0.95 for each block of a wave, the first one as long as b takes to arrive at 4.3 TB/s at least.
+struct TokensTime { int tiles; float time; };
+TokensTime tokens_estimate(int64_t M, int64_t N, int steps)
+{
+    TokensTime best = {0, 0.f};
+    const float arrive = 1.8f + (float)N * (float)steps * (128.f / 4.3e6f);
+    for (int tiles = 1; tiles <= 4; tiles *= 2) {
+        const int64_t items = ((M + 63) / 64) * ((N + tiles * 16 - 1) / (tiles * 16));
+        const float round = 1.9f + (float)((steps + 3) / 4) * (tiles == 1 ? 0.55f : tiles == 2 ? 0.85f : 0.95f);
+        const float time = 0.8f + (round > arrive ? round : arrive) + (float)((items - 1) / 256) * round;
+        if (best.tiles == 0 || time < best.time) best = {tiles, time};
+    }
+    return best;
 }
 // whether product8_tokens_kernel takes it: its waves have kTokenBlocks each at most
 bool tokens(int64_t M, int steps) { return M <= 32 ? steps <= 8 * kTokenBlocks : M <= 64 && steps <= 4 * kTokenBlocks; }
@@ -612,7 +630,7 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
     if (const char *e = tuning_env("GCG_P8")) {
         const char *s = tuning_env("GCG_P8S");
         const int n = s ? atoi(s) : 1, per = ((steps + n - 1) / n + 3) / 4 * 4, kernel = atoi(e);
-        if (kernel == TOKENS ? !tokens(M, steps) : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4, 0};
+        if (kernel == TOKENS ? (M <= 32 ? !tokens(M, steps) : steps > 4 * kTokenBlocks) : !takes(kernel, M, N)) return {TILE, 1, (steps + 3) / 4 * 4, 0};
         return {kernel, (steps + per - 1) / per, per, 0};
     }
     if (tokens(M, steps)) return {TOKENS, 1, steps, 0};
@@ -627,6 +645,7 @@ Plan8 plan_of(int64_t M, int64_t N, int64_t K)
                 best = {kernel, splits, per, 0};
             }
         }
+    if (steps <= 4 * kTokenBlocks && tokens_estimate(M, N, steps).time < least) return {TOKENS, 1, steps, 0};
     if (best.kernel == TILE || best.splits > 1 || !takes(WIDE, M, N)) return best;
     const int64_t across = (N + 255) / 256, items = (M + 255) / 256 * across;
     for (int64_t rounds = 1; rounds * 256 < items; ++rounds) {
@@ -649,27 +668,29 @@ template <int BM, int BN, int WM, int WN, typename T, bool A5, bool B5> int tile
 }
 template <typename T, int MT, int NT, int W, bool FUSED, bool A5, bool B5> int tokens_go(const Tokens8 &s, hipStream_t st)
 {
-    const dim3 grid((unsigned)((s.p.N + NT * 16 - 1) / (NT * 16)));
-    return launch_main(product8_tokens_kernel<T, MT, NT, W, FUSED, A5, B5>, grid, dim3(W * 64), st, s);
+    Tokens8 q = s;
+    q.p.tiles_m = (uint32_t)((s.p.M + MT * 16 - 1) / (MT * 16));
+    const dim3 grid((unsigned)((s.p.N + NT * 16 - 1) / (NT * 16) * q.p.tiles_m));
+    return launch_main(product8_tokens_kernel<T, MT, NT, W, FUSED, A5, B5>, grid, dim3(W * 64), st, q);
 }
-// Rows of b for a workgroup: 16 while the card's CUs have one workgroup each, else more, which share a's fragments.  Eight waves where a wave of
-// four would have sixteen blocks and the CU no other workgroup.  (FUSED changes nothing in it, so that sums are in the same order.)
+// Rows of b for a workgroup, of up to 32 rows of a: 16 while the card's CUs have one workgroup each, else 32, which share a's fragments.  Eight waves where
+// a wave of four would have sixteen blocks and the CU no other workgroup.  (FUSED changes nothing in it, so that sums are in the same order.)
 template <typename T, int MT, bool FUSED, bool A5, bool B5> int tokens_tiles(const Tokens8 &s, hipStream_t st)
 {
     const int64_t sixteens = (s.p.N + 15) / 16;
-    if constexpr (MT <= 2)
-        if (s.p.steps > 4 * kTokenBlocks || (s.p.steps >= 64 && sixteens <= 256)) return tokens_go<T, MT, 1, 8, FUSED, A5, B5>(s, st);
-    if (sixteens <= 256) return tokens_go<T, MT, 1, 4, FUSED, A5, B5>(s, st);
-    if constexpr (MT == 4)
-        if (sixteens > 512) return tokens_go<T, MT, 4, 4, FUSED, A5, B5>(s, st);
-    return tokens_go<T, MT, 2, 4, FUSED, A5, B5>(s, st);
+    if (s.p.steps > 4 * kTokenBlocks || (s.p.steps >= 64 && sixteens <= 256)) return tokens_go<T, MT, 1, 8, FUSED, A5, B5>(s, st);
+    return sixteens <= 256 ? tokens_go<T, MT, 1, 4, FUSED, A5, B5>(s, st) : tokens_go<T, MT, 2, 4, FUSED, A5, B5>(s, st);
 }
 template <typename T, bool A5, bool B5> int product_launch(Product8 &p, const Plan8 &plan, hipStream_t st)
 {
     if constexpr (sizeof(T) == 2) {
         if (plan.kernel == TOKENS) {
             const Tokens8 s = {p, nullptr, 0};
-            return p.M <= 16 ? tokens_tiles<T, 1, false, A5, B5>(s, st) : p.M <= 32 ? tokens_tiles<T, 2, false, A5, B5>(s, st) : tokens_tiles<T, 4, false, A5, B5>(s, st);
+            if (p.M <= 16) return tokens_tiles<T, 1, false, A5, B5>(s, st);
+            if (p.M <= 32) return tokens_tiles<T, 2, false, A5, B5>(s, st);
+            const int tiles = tokens_estimate(p.M, p.N, p.steps).tiles;
+            return tiles == 1 ? tokens_go<T, 4, 1, 4, false, A5, B5>(s, st) : tiles == 2 ? tokens_go<T, 4, 2, 4, false, A5, B5>(s, st)
+                                                                                         : tokens_go<T, 4, 4, 4, false, A5, B5>(s, st);
         }
     }
     if (plan.kernel == TILE) return tile_launch<128, 128, 2, 2, T, A5, B5>(p, plan, st);

@@ -30,7 +30,8 @@ def whole(rows, D, fmt, seed, most=8):
 
 SIZES = [(1, 1, 1), (1, 64, 128), (3, 70, 300), (8, 130, 4096), (9, 130, 640), (16, 33, 129), (17, 300, 513), (64, 129, 2048), (65, 64, 100),
          (128, 128, 128), (129, 257, 640), (200, 1000, 1500), (256, 256, 128), (256, 256, 384), (257, 300, 512), (300, 520, 1100),
-         (511, 513, 640), (1000, 700, 900), (64, 64, 16384), (300, 300, 8200), (4096, 4097, 300)]
+         (511, 513, 640), (1000, 700, 900), (64, 64, 16384), (300, 300, 8200), (4096, 4097, 300),
+         (65, 130, 16500), (2047, 4000, 256), (4001, 4001, 700), (600, 600, 17000)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
@@ -51,28 +52,10 @@ def test_whole_numbers(M, N, K, fa, fb):
                                    (2048, 4096, 128), (2047, 4000, 256), (1793, 3999, 300), (2000, 4095, 512), (2040, 4001, 640), (701, 7683, 1000),
                                    (1900, 3970, 1101), (300, 200, 5000), (1000, 1000, 8200), (2040, 2048, 16384),
                                    (5003, 7683, 1301), (4700, 4201, 1300), (9000, 2000, 1100), (70000, 257, 1300), (16700, 1025, 900)])
-def test_wide_tiles(M, N, K):
-    """Sizes that take least time in tiles of 256 x 256 (the first nine and the nineteenth), of 256 x 128, and (the last five) of both, at rows
+def test_large_tiles(M, N, K):
+    """Sizes that take least time in tiles of 256 x 256 (the first nine), of 256 x 128, or (the last five) of both, at rows
     and columns that the tiles do not divide, in every length of the loop's rest, in several rounds, in parts, and with more results than
     the last-level cache holds."""
-    most = 8 if K < 2000 else 4                                     # |sums| < 16384 * 4 * 4 * 16 < 2^24
-    a, b = whole(M, K, fa, M + K, most), whole(N, K, fb, N + K + 1, most)
-    qa, qb = to_float8(a, fa), to_float8(b, fb)
-    assert torch.equal(values(qa), a.double()) and torch.equal(values(qb), b.double())
-    want = (a.float().double() @ b.float().double().t())
-    for dtype in (torch.bfloat16, torch.float16):
-        got = matmul_float8(qa, qb, dtype)
-        assert torch.equal(got, want.to(dtype)), f"{M} x {N} x {K}: {(got != want.to(dtype)).sum().item()} differ"
-
-
-@pytest.mark.parametrize("M,N,K", [(4096, 4096, 128), (4095, 3841, 256), (3850, 4001, 300), (4096, 3900, 512), (3841, 4096, 640), (4001, 4001, 700),
-                                   (4090, 4094, 1000), (8200, 6000, 1300), (12000, 11500, 1300),
-                                   (2048, 4096, 128), (2047, 4000, 256), (1793, 3999, 300), (2000, 4095, 512), (2040, 4001, 640), (701, 7683, 1000),
-                                   (1900, 3970, 1101), (300, 200, 5000), (1000, 1000, 8200), (2040, 2048, 16384),
-                                   (5003, 7683, 1301), (4700, 4201, 1300), (9000, 2000, 1100), (70000, 257, 1300), (16700, 1025, 900)])
-def test_wide_tiles(M, N, K):
-    """Sizes that take least time in tiles of 256 x 256 (the first nine and the twentieth), of 256 x 128 and (the last five) of both, at rows and columns that the tiles do not divide, in every
-    length of the loop's rest, in several rounds, in parts, and with more results than the last-level cache holds."""
     most = 8 if K < 2000 else 4
     a, b = whole(M, K, E4M3, K, most), whole(N, K, E4M3, K + 1, most)
     want = (a.float() @ b.float().t()).to(torch.bfloat16)                               # (fp32 holds these sums)
@@ -123,6 +106,16 @@ def test_tokens_quantised_in_the_kernel(M, N, K, fmt):
     with torch.no_grad():
         for dtype in (torch.bfloat16, torch.float16):
             assert torch.equal(linear_float8(x.to(dtype), w), want.to(dtype))
+
+
+@pytest.mark.parametrize("M,N,K", [(2357, 3272, 242), (143, 11372, 1634), (14673, 2327, 124), (67, 14005, 6507), (65, 130, 16500), (200, 300, 20000),
+                                   (150, 15000, 10000), (100, 129, 16385),
+                                   (129, 8000, 9000), (256, 12288, 4096), (1000, 1000, 8200), (450, 4096, 4096), (700, 900, 130), (1100, 33, 2000),
+                                   (300, 6797, 9893), (1300, 2000, 7001), (600, 600, 17000)])
+def test_other_tiles(M, N, K):
+    """Sizes that take least time in tiles of 128 x 128 (the first eight: alone, in rounds, in parts), in groups of 64 rows, and in parts of
+    tiles of 256 x 128 (the last three)."""
+    test_large_tiles(M, N, K)
 
 
 @pytest.mark.parametrize("N", [40, 300, 4097, 9000])
