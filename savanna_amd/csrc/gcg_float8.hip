@@ -2,6 +2,9 @@
 // (the result transposed, as a product over the rows reads it) or both from one reading, and back.
 //
 // Bound by memory: s + 1 bytes an element for one direction (s the element's size), s + 2 for both, against a dozen vector instructions.
+//
+// Measured, bf16: 16384 x 4096 along the rows 34 us (5.9 TB/s), 16384 x 8192 back 69 (5.8); 8192 x 4096 along both from one reading 29 (4.6; a pass each
+// way 22 + 29), 4096 x 4096 along the columns 14 (3.5: a tile's two barriers, four workgroups a CU), 8192 x 4096 from 8 bits along the columns 17 (4.0).
 #include "gcg_float8.h"
 
 namespace gcg {
