@@ -189,7 +189,9 @@ __global__ __launch_bounds__(WM * WN * 64) void product8_kernel(Product8 p)
 //
 //   (A0 B0) reads B1,  (A0 B1) reads A1,  barrier,  (A1 B1) reads the next block's A0,  (A1 B0) reads its B1;  the next block starts with (A0 B1)
 //
-// At the barrier a stage has been read and the next one has arrived; the one after that is requested into it.  Four blocks, whose scales are a word
+// At the barrier a stage has been read and the next one has arrived; the one after the last that is under way is requested into it: with tiles of 256 x
+// 256 the shared memory holds two stages, with 256 x 128 three, so that operands have two blocks' time to arrive (512 x 12288 x 4096 from HBM 46 us with
+// two, 36 with three, 4096 x 512 x 8192 85 and 65; operands from the cache 5 to 8 % less).  Four blocks, whose scales are a word
 // of each row, are one turn of the loop, without a branch in it: past the end the last block is requested again, and not used.  One to
 // three blocks that are left go one after the other.
 //
@@ -227,9 +229,9 @@ template <bool A5, bool B5, int BYTE> __device__ __forceinline__ void mfma8_acc(
 
 template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch_bounds__(256, 1) void product8_wide_kernel(Product8 p)
 {
-    constexpr int BM = 256, LA = 8, LB = BN / 32, STAGE = (BM + BN) * 128;
+    constexpr int BM = 256, LA = 8, LB = BN / 32, STAGE = (BM + BN) * 128, STAGES = BN == 128 ? 3 : 2;
     constexpr int COLS = BN / 2, HALF = COLS / 32;              // a wave's columns, and fragments of half of them
-    __shared__ __attribute__((aligned(1024))) uint8_t stage[2][STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[STAGES][STAGE];
     __shared__ uint32_t words[2][BM + BN];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64;
     const uint32_t tiles = p.tiles_m * p.tiles_n, items = tiles * p.splits;
@@ -293,8 +295,8 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
     f32x4 acc[8][2 * HALF];
     i32x8 A[2][4], B[2][HALF];
     // The products of half I of the rows and half J of the columns, and between them the FRAGMENTS fragments at `from` of stage s into `to`, and with
-    // `more` the requests for block k into the other stage.  (These statements stay in the order they are written in.)
-    const auto phase = [&](auto i_, auto j_, auto byte_, auto &to, int s, int from, auto more_, int at) {
+    // `more` the requests for the block at `at` into stage r.  (These statements stay in the order they are written in.)
+    const auto phase = [&](auto i_, auto j_, auto byte_, auto &to, int s, int from, auto more_, int at, int r) {
         constexpr int i = decltype(i_)::value, j = decltype(j_)::value, byte = decltype(byte_)::value;
         constexpr bool more = decltype(more_)::value;
         constexpr int FRAGMENTS = (int)(sizeof(to) / sizeof(i32x8)), TURNS = 2 * HALF, READS = 2 * FRAGMENTS;
@@ -308,9 +310,9 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
             }
             if constexpr (more) {
 #pragma unroll
-                for (int f = q * LA / TURNS; f < (q + 1) * LA / TURNS; ++f) request_a(at, s ^ 1, f);
+                for (int f = q * LA / TURNS; f < (q + 1) * LA / TURNS; ++f) request_a(at, r, f);
 #pragma unroll
-                for (int f = q * LB / TURNS; f < (q + 1) * LB / TURNS; ++f) request_b(at, s ^ 1, f);
+                for (int f = q * LB / TURNS; f < (q + 1) * LB / TURNS; ++f) request_b(at, r, f);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -325,27 +327,30 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
     constexpr std::integral_constant<int, 3> three;
     constexpr std::true_type yes;
     constexpr std::false_type no;
-    const auto hand_over = [&]() {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const auto hand_over = [&](auto under_way) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(under_way)::value) : "memory");
         __syncthreads();
     };
-    // one block, whose first half of columns is J (whose fragments, and those of A's first half, are there)
-    const auto block = [&](int k, auto s_, auto byte_) {
-        constexpr int s = decltype(s_)::value, J = s, notJ = 1 - s;
+    constexpr std::integral_constant<int, (STAGES - 2) * (LA + LB)> later;          // the requests behind the next block's
+    // one block, in stage s, whose first half of columns is J (whose fragments, and those of A's first half, are there)
+    const auto block = [&](int k, auto j_, auto byte_, int s) {
+        constexpr int J = decltype(j_)::value, notJ = 1 - J;
         constexpr std::integral_constant<int, J> j;
         constexpr std::integral_constant<int, notJ> not_j;
-        phase(zero, j, byte_, B[notJ], s, fb + notJ * HALF * 16 * 128, no, 0);
-        phase(zero, not_j, byte_, A[1], s, fa + 64 * 128, no, 0);
-        hand_over();
-        phase(one, not_j, byte_, A[0], s ^ 1, fa, yes, place_of(k + 2));
-        phase(one, j, byte_, B[notJ], s ^ 1, fb + notJ * HALF * 16 * 128, no, 0);
+        const int next = s + 1 < STAGES ? s + 1 : 0;
+        phase(zero, j, byte_, B[notJ], s, fb + notJ * HALF * 16 * 128, no, 0, 0);
+        phase(zero, not_j, byte_, A[1], s, fa + 64 * 128, no, 0, 0);
+        hand_over(later);
+        phase(one, not_j, byte_, A[0], next, fa, yes, place_of(k + STAGES), s);
+        phase(one, j, byte_, B[notJ], next, fb + notJ * HALF * 16 * 128, no, 0, 0);
+        return next;
     };
 
     take(blockIdx.x);
     request_words(k0, 0);
-    request(k0, 0);
-    request(k0 + 1, 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) request(k0 + s, s);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * (LA + LB)) : "memory");     // the scales and the first block
     for (uint32_t item = blockIdx.x;;) {
     __syncthreads();
 #pragma unroll
@@ -356,18 +361,17 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
     for (int q = 0; q < 4; ++q) A[0][q] = fragment(0, fa + q * 16 * 128);
 #pragma unroll
     for (int q = 0; q < HALF; ++q) B[0][q] = fragment(0, fb + q * 16 * 128);
-    int k = k0, w = 0;
+    int k = k0, w = 0, s = 0;
     for (; k + 4 <= k1; k += 4, w ^= 1) {
         take_words(w);
         request_words(k + 4, w ^ 1);
-        block(k, zero, zero);
-        block(k + 1, one, one);
-        block(k + 2, zero, two);
-        block(k + 3, one, three);
+        s = block(k, zero, zero, STAGES == 2 ? 0 : s);
+        s = block(k + 1, one, one, STAGES == 2 ? 1 : s);
+        s = block(k + 2, zero, two, STAGES == 2 ? 0 : s);
+        s = block(k + 3, one, three, STAGES == 2 ? 1 : s);
     }
     if (k < k1) take_words(w);
     for (; k < k1; ++k) {
-        const int s = (k - k0) & 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -383,27 +387,29 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
         for (int i = 0; i < 8; ++i) ca[i] >>= 8;
 #pragma unroll
         for (int j = 0; j < 2 * HALF; ++j) cb[j] >>= 8;
-        hand_over();
-        request(k + 2, s);
+        hand_over(later);
+        request(k + STAGES, s);
+        s = s + 1 < STAGES ? s + 1 : 0;
     }
     // A wave's results leave in whole rows of its columns, which lie together in shared memory first: a pass of 64 rows (fp32: 32) in its quarter of
-    // the second stage, the 16-byte pieces of a row at exchanged places.  The next tile's first block is on its way to the first stage by then.
+    // the last stage, the 16-byte pieces of a row at exchanged places.  The next tile's first blocks are on their way to the others by then.
     constexpr int ROWS = 128 / (int)sizeof(T), PIECES = COLS * (int)sizeof(T) / 16;
-    static_assert(4 * ROWS * PIECES * 16 <= STAGE, "in the second stage");
+    static_assert(4 * ROWS * PIECES * 16 <= STAGE, "in the last stage");
     const auto exchanged = [](int piece, int row) { return piece ^ (PIECES >= 16 ? row & 15 : (row >> 1) & 7); };
     uint8_t *y = (uint8_t *)((p.partial ? (T *)(p.partial + (int64_t)split * p.M * p.N) : (T *)p.y) + (m0 + wm * 128) * p.N + n0 + wn * COLS);
-    hand_over();                                                                // nobody reads a stage any more, and nothing arrives
+    hand_over(zero);                                                            // nobody reads a stage any more, and nothing arrives
     item += gridDim.x;
     const bool more = item < items;
     if (more) {
         take(item);
         request_words(k0, 0);
-        request(k0, 0);
+#pragma unroll
+        for (int i = 0; i + 1 < STAGES; ++i) request(k0 + i, i);
     }
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");             // the last products have written their accumulators
     int l = lane;
     asm volatile("" : "+v"(l));                                                 // (addresses are formed here, not kept over the products)
-    uint8_t *mine = stage[1] + wave * (ROWS * PIECES * 16);
+    uint8_t *mine = stage[STAGES - 1] + wave * (ROWS * PIECES * 16);
     const int64_t down = 64 / PIECES * p.N * (int64_t)sizeof(T);                // from one store's rows to the next one's
     const int64_t off = l / PIECES * p.N * (int64_t)sizeof(T) + l % PIECES * 16;
 #pragma unroll
@@ -429,8 +435,8 @@ template <int BN, typename T, bool A5, bool B5, bool STREAM> __global__ __launch
     }
     if (!more) return;
     __syncthreads();
-    request(k0 + 1, 1);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");           // all but the second block
+    request(k0 + STAGES - 1, STAGES - 1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LA + LB) : "memory");           // all but the last one
     }
 }
 
