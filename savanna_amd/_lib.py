@@ -1650,6 +1650,18 @@ def linear_float8_infer(x, codes, scales, columns: int):
     return y
 
 
+def norm_linear_float8_infer(x, residual, gain, codes, scales, columns: int, eps: float):
+    """(y, r): the root-mean-square norm of a contiguous x, or of r = x + residual, times a weight in 8 bits (r is empty without a residual)."""
+    _require_gpu(x)
+    if TORCH_OPS:
+        return _run(torch.ops.gcg.norm_linear_float8_infer, x, residual, gain, codes, scales, columns, eps)
+    _product_dtype(x.dtype)
+    a, a_scales, r, _ = rms_norm_float8(x, residual, gain, eps)
+    if x.shape[-1] != columns:
+        raise ValueError("the weight must be a matrix on x's device with as many columns as x")
+    return matmul_float8(a, a_scales, codes, scales, columns, x.dtype), r
+
+
 # ---- gated linear recurrence -----------------------------------------------------------------------------------
 
 SCAN_MAX_TIME_STRIDE = 1 << 21      # GCG_SCAN_MAX_TIME_STRIDE

@@ -47,6 +47,7 @@ BLOCK_OP_NAMES = (
 LAYER8_OP_NAMES = (
     "rms_norm_fwd", "rms_norm_infer", "rms_norm_float8", "rms_norm_bwd",
     "to_float8", "to_float8_both", "to_float8_columns", "float8_columns", "from_float8", "matmul_float8", "linear_float8_infer",
+    "norm_linear_float8_infer",
     "scan_fwd", "scan_bwd", "scan_packed_fwd", "scan_packed_bwd", "scan_step",
 )
 
@@ -228,7 +229,7 @@ def _register_autograd():
     nothing = lambda ctx, inputs, output: None                                       # noqa: E731
     reg("gcg::layer_norm_infer", refuse("layer_norm_infer", "use torch.ops.gcg.layer_norm"), setup_context=nothing)
     reg("gcg::rms_norm_infer", refuse("rms_norm_infer", "use torch.ops.gcg.rms_norm"), setup_context=nothing)
-    for name in ("rms_norm_float8", "to_float8", "to_float8_both", "to_float8_columns", "linear_float8_infer"):
+    for name in ("rms_norm_float8", "to_float8", "to_float8_both", "to_float8_columns", "linear_float8_infer", "norm_linear_float8_infer"):
         reg(f"gcg::{name}", refuse(name, "use torch.ops.gcg.linear_float8 or norm_linear_float8"), setup_context=nothing)
     for name in ("rms_norm_bwd", "float8_columns", "from_float8", "matmul_float8", "scan_bwd", "scan_packed_bwd"):
         reg(f"gcg::{name}", refuse(name, "its operator is differentiated once"), setup_context=nothing)

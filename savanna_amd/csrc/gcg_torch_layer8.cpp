@@ -303,6 +303,20 @@ Four rms_norm_float8(const Tensor &x, const OptTensor &residual, const OptTensor
     return {codes, scales, r, rstd};
 }
 
+// the norm and a product with a weight in 8 bits: (y, r)
+Two norm_linear_float8_infer(const Tensor &x, const OptTensor &residual, const OptTensor &gain, const Tensor &codes, const Tensor &scales,
+                             int64_t columns, double eps)
+{
+    require_gpu(x, "x");
+    const int code = rms_code(x, residual, gain);
+    check_linear(x, codes, scales, columns);
+    DeviceGuard guard(x.device());
+    auto [c, s] = empty_float8(x, x.sizes().vec(), at::kFloat8_e4m3fn);
+    Tensor r = new_sum(x, residual);
+    rms_launch(x, residual, gain, eps, code, nullptr, r, bytes(c), bytes(s), nullptr);
+    return {matmul_float8(c, s, codes, scales, columns, x.scalar_type()), r};
+}
+
 void check_rms_bwd(const Tensor &dy, const Tensor &r, const OptTensor &dr, const Tensor &rstd)
 {
     check_rows(dy, "dy");
@@ -348,6 +362,13 @@ Four rms_norm_float8_meta(const Tensor &x, const OptTensor &residual, const OptT
     (void)rms_code(x, residual, w);
     auto [codes, scales] = empty_float8(x, x.sizes().vec(), at::kFloat8_e4m3fn);
     return {codes, scales, new_sum(x, residual), at::empty(rstd_sizes(x), x.options().dtype(at::kFloat))};
+}
+Two norm_linear_float8_infer_meta(const Tensor &x, const OptTensor &residual, const OptTensor &gain, const Tensor &codes, const Tensor &scales,
+                                  int64_t columns, double)
+{
+    (void)rms_code(x, residual, gain);
+    check_linear(x, codes, scales, columns);
+    return {at::empty(with_last(x, codes.size(0)), x.options()), new_sum(x, residual)};
 }
 Two rms_norm_bwd_meta(const Tensor &dy, const Tensor &r, const OptTensor &dr, const Tensor &rstd, const OptTensor &w, bool need_dw)
 {
@@ -844,6 +865,8 @@ TORCH_LIBRARY_FRAGMENT(gcg, m)
     m.def("from_float8(Tensor codes, Tensor scales, int columns, ScalarType dtype) -> Tensor");
     m.def("matmul_float8(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, int columns, ScalarType dtype) -> Tensor");
     m.def("linear_float8_infer(Tensor x, Tensor codes, Tensor scales, int columns) -> Tensor");
+    m.def("norm_linear_float8_infer(Tensor x, Tensor? residual, Tensor? gain, Tensor codes, Tensor scales, int columns, float eps)"
+          " -> (Tensor, Tensor)");
     m.def("scan_fwd(Tensor x, Tensor f, Tensor? gate, Tensor? bias, Tensor? initial, Tensor? lengths, bool final, bool keep)"
           " -> (Tensor, Tensor, Tensor)");
     m.def("scan_bwd(Tensor dy, Tensor x, Tensor f, Tensor? gate, Tensor? bias, Tensor states, Tensor? lengths, Tensor? dfinal,"
@@ -871,6 +894,7 @@ TORCH_LIBRARY_IMPL(gcg, CUDA, m)
     m.impl("from_float8", &from_float8);
     m.impl("matmul_float8", &matmul_float8);
     m.impl("linear_float8_infer", &linear_float8_infer);
+    m.impl("norm_linear_float8_infer", &norm_linear_float8_infer);
     m.impl("scan_fwd", &scan_fwd);
     m.impl("scan_bwd", &scan_bwd);
     m.impl("scan_packed_fwd", &scan_packed_fwd);
@@ -896,6 +920,7 @@ TORCH_LIBRARY_IMPL(gcg, Meta, m)
     m.impl("from_float8", &from_float8_meta);
     m.impl("matmul_float8", &matmul_float8_meta);
     m.impl("linear_float8_infer", &linear_float8_infer_meta);
+    m.impl("norm_linear_float8_infer", &norm_linear_float8_infer_meta);
     m.impl("scan_fwd", &scan_fwd_meta);
     m.impl("scan_bwd", &scan_bwd_meta);
     m.impl("scan_packed_fwd", &scan_packed_fwd_meta);

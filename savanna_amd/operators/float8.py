@@ -154,9 +154,7 @@ def norm_linear_float8(x: torch.Tensor, gain: Optional[torch.Tensor], w: Union[t
         _check_weight(x, w)
         _lib.format_code(grad_dtype)
     if ready or (not torch.is_grad_enabled() and not _lib.forward_mode()):
-        w8 = w if ready else to_float8(w)
-        codes, scales, r, _ = _lib.rms_norm_float8(x, residual, gain, eps)
-        y = matmul_float8(Float8(codes, scales, x.shape[-1]), w8, x.dtype)
+        y, r = _lib.norm_linear_float8_infer(x, residual, gain, *(w if ready else to_float8(w)), eps)
         return y if residual is None else (y, r)
     if _lib.native_nodes(x):
         out = torch.ops.gcg.norm_linear_float8(x, residual, gain, w, eps, grad_dtype)

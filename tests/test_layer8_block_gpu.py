@@ -268,7 +268,7 @@ def test_schemas_and_meta_results(gcg_lib):
     entries = {"rms_norm_fwd": (x, x, g, 1e-6), "rms_norm_infer": (x, None, g, 1e-6), "rms_norm_float8": (x, x, g, 1e-6), "rms_norm_bwd": (x, x, x, rstd, g),
                "to_float8": (x, E5M2), "to_float8_both": (x, E4M3), "to_float8_columns": (x, E4M3), "float8_columns": (codes, scales, 300, E4M3),
                "from_float8": (codes, scales, 300, torch.float16), "matmul_float8": (codes, scales, wc, ws, 300, torch.bfloat16),
-               "linear_float8_infer": (x, wc, ws, 300), "scan_fwd": (s, s, s, bias, state, None, True, True),
+               "linear_float8_infer": (x, wc, ws, 300), "norm_linear_float8_infer": (x, x, g, wc, ws, 300, 1e-6), "scan_fwd": (s, s, s, bias, state, None, True, True),
                "scan_bwd": (s, s, s, s, bias, states, None, state, True, True), "scan_packed_fwd": (features, bias, True),
                "scan_packed_bwd": (s, features, bias, states, True), "scan_step": (s[:, 0], s[:, 0], None, bias, state)}
     assert set(nodes) == set(_ops.LAYER8_NODE_NAMES) and set(entries) == set(_ops.LAYER8_OP_NAMES)

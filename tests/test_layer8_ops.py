@@ -38,6 +38,7 @@ def test_meta_shapes(gcg_lib, dtype):
             assert ops.from_float8(codes, scales, 600, dtype).shape == (70, 600)
             if dtype != torch.float32:
                 y = ops.matmul_float8(codes, scales, codes, scales, 600, dtype)
+                assert [t.shape for t in ops.norm_linear_float8_infer(m, m, None, codes, scales, 600, 1e-6)] == [(70, 70), (70, 600)]
                 assert y.shape == (70, 70) and y.dtype == dtype and ops.linear_float8_infer(m, codes, scales, 600).shape == (70, 70)
         f = torch.empty(2, 200, 30, dtype=dtype, device="cuda")
         bias, state = torch.empty(10, device="cuda"), torch.empty(2, 10, device="cuda")
