@@ -606,7 +606,8 @@ template <typename T> __global__ __launch_bounds__(256) void product8_join_kerne
 // 2560 x 2560 4.2, 4.4, 5.7 and 11.4 to 12.6; 4096 x 16384 15, 15, 27 and 22 to 27), and more in groups of 64 where that takes least time (256 rows
 // from 4096 x 4096 10, by tiles of 128 in parts 21; 512 rows 18 and 30; 1000 x 1000 x 1000 5.7 and 9.5; 400 rows from 12288 x 4096 53, tiles of 256 x 128
 // 46).  Else, in microseconds as measured: a round of 256 tiles of 256 x 256 takes 1.35 a block and 6 around them, of 256 x 128 0.85 and 5 (0.9 if half
-// the card is idle); 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9; joining moves four bytes for every part of a result twice
+// the card is idle), 3 and 2 once; 512 tiles of 128 x 128, two a CU, take 1.22 a block, 256 of them 0.9, and their results, in four columns at a time or
+// one by one, leave at 4.2 or 1.3 TB/s (8000 x 8000 x 256 56 us, 8000 x 8001 x 256 118; tiles of 256 x 256 43 and 44); joining moves four bytes for every part of a result twice
 // at 4 TB/s, and 3 for its launch.  So (tiles of 128 x 128, 256 x 128, 256 x 256) 4096 x 4096 x 4096 goes by the last (88, 63, 55), 2048 x 4096 x 4096
 // by the second (48, 34, 46), 7680 x 2561 x 5003 by either of them (147, 116, 115) and 701 x 7683 x 2560 by the second (35, 23, 34).
 // Where the last round of 256 x 256 tiles would leave the card half empty, the rows of the rounds before it go by those, the rest by
@@ -618,9 +619,10 @@ float estimate(int kernel, int64_t M, int64_t N, int per, int splits)
     const int bm = kernel == TILE ? 128 : 256, bn = kernel == WIDE ? 256 : 128;
     const int64_t items = ((M + bm - 1) / bm) * ((N + bn - 1) / bn) * splits;
     const float join = splits > 1 ? 3.f + (float)M * (float)N * (float)splits * 8.f / 4e6f : 0.f;
-    if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.35f + 6.f) + join;
-    if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.9f : 0.85f) + 5.f) + join;
-    return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + join;
+    if (kernel == WIDE) return (float)((items + 255) / 256) * ((float)per * 1.35f + 6.f) + 3.f + join;
+    if (kernel == TALL) return (float)((items + 255) / 256) * ((float)per * (items <= 128 ? 0.9f : 0.85f) + 5.f) + 2.f + join;
+    const float leave = (float)M * (float)N / (N % 4 == 0 || splits > 1 ? 2.1e6f : 0.65e6f);
+    return (items <= 256 ? (float)per * 0.9f : (float)((items + 511) / 512) * (float)per * 1.22f) + 6.f + leave + join;
 }
 // Groups of 64 rows by product8_tokens_kernel: the rows of b for a workgroup (in sixteens) that take least time, and that time; as measured, a round
 // of 256 workgroups takes 1.9 us and 0.55, 0.85, 0.95 for each block of a wave, the first one as long as b takes to arrive at 4.3 TB/s at least.

@@ -9,8 +9,9 @@
 // worked on; a row of one wave needs no barrier.  All sums are fp32; r is rounded before it is normed, since it is what the
 // backward and the next layer read.  The 8-bit output is formed of y in fp32, each block's largest by lane exchanges.
 //
-// Measured: 16384 x 4096 bf16 with the residual forward 87 us (6.0 TB/s), backward 112 + 4 (4.7); 16384 x 8192 into 8 bits 169 (5.5); 5003 x 2561, whose
-// rows lie on 2 bytes, 28 into 8 bits (3.3) and 37 + 4; 8 x 4096 3.3, a launch.
+// Measured: 16384 x 4096 bf16 with the residual forward 87 us (6.0 TB/s), backward 112 + 4 (4.7); 16384 x 8192 into 8 bits 169 (5.5); 15325 x 2358, whose
+// rows end inside a vector, 56 (5.1) and 59 + 4 (4.9; with that vector loaded in a branch, which keeps the next row from being under way, 96 and 152);
+// 8 x 4096 3.3, a launch.
 #include "gcg_float8.h"
 
 namespace gcg {
@@ -40,8 +41,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Rms
     const auto request = [&](int64_t r) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            next[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.x + r * D, (k * TPR + t) * V, D);
-            if constexpr (RES) next_res[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.residual + r * D, (k * TPR + t) * V, D);
+            next[k] = request_row_vec<T, TAIL, STREAM>((const T *)a.x + r * D, (k * TPR + t) * V, D);
+            if constexpr (RES) next_res[k] = request_row_vec<T, TAIL, STREAM>((const T *)a.residual + r * D, (k * TPR + t) * V, D);
         }
     };
 #pragma unroll
@@ -58,10 +59,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_fwd_kernel(Rms
         float v[K][V], s[1] = {0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            unpack_vec(next[k], v[k], T{});
+            unpack_vec(in_place<T, TAIL>(next[k], (k * TPR + t) * V, D), v[k], T{});
             if constexpr (RES) {
                 float q[V];
-                unpack_vec(next_res[k], q, T{});
+                unpack_vec(in_place<T, TAIL>(next_res[k], (k * TPR + t) * V, D), q, T{});
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[k][i] += q[i];
                 if (row < a.rows) store_row_vec<T, TAIL, STREAM>((T *)a.r + row * D, (k * TPR + t) * V, D, v[k]);
@@ -116,6 +117,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Rms
     const int64_t step = (int64_t)gridDim.x * GROUPS;
     int64_t row = (int64_t)blockIdx.x * GROUPS + group;
 
+    // (without requests ahead a row is waited for anyway)
+    constexpr bool PLACE = TAIL && AHEAD;
+    const auto load = [&](const void *p, int64_t r, int c) {
+        if constexpr (PLACE) return request_row_vec<T, true, STREAM>((const T *)p + r * D, c, D);
+        else return load_row_vec<T, TAIL, STREAM>((const T *)p + r * D, c, D);
+    };
     u32x4 next_dy[K], next_r[K], next_dr[ADD && AHEAD ? K : 1];
     float next_rstd = 0.f;
     const auto request = [&](int64_t r) {
@@ -123,15 +130,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Rms
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * TPR + t) * V;
-            next_dy[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.dy + r * D, c, D);
-            next_r[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.r + r * D, c, D);
-            if constexpr (ADD && AHEAD) next_dr[k] = load_row_vec<T, TAIL, STREAM>((const T *)a.dr + r * D, c, D);
+            next_dy[k] = load(a.dy, r, c);
+            next_r[k] = load(a.r, r, c);
+            if constexpr (ADD && AHEAD) next_dr[k] = load(a.dr, r, c);
         }
     };
     // the row's dy and xh of vector k (absent columns: zeros, which count for nothing)
     const auto values = [&](int k, float (&dy)[V], float (&xh)[V], float rstd) {
-        unpack_vec(next_dy[k], dy, T{});
-        unpack_vec(next_r[k], xh, T{});
+        unpack_vec(in_place<T, PLACE>(next_dy[k], (k * TPR + t) * V, D), dy, T{});
+        unpack_vec(in_place<T, PLACE>(next_r[k], (k * TPR + t) * V, D), xh, T{});
 #pragma unroll
         for (int i = 0; i < V; ++i) xh[i] *= rstd;
     };
@@ -189,7 +196,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_norm_bwd_kernel(Rms
                     weights(k, w[0]);
                 }
                 float dx[V], more[V];
-                if constexpr (ADD && AHEAD) unpack_vec(dr[at], more, T{});
+                if constexpr (ADD && AHEAD) unpack_vec(in_place<T, PLACE>(dr[at], (k * TPR + t) * V, D), more, T{});
                 else if constexpr (ADD) unpack_vec(load_row_vec<T, TAIL, STREAM>((const T *)a.dr + row * D, (k * TPR + t) * V, D), more, T{});
 #pragma unroll
                 for (int i = 0; i < V; ++i) {

@@ -75,6 +75,35 @@ template <typename T, bool TAIL, bool STREAM> __device__ __forceinline__ u32x4 l
     }
     return r;
 }
+// The same for a lane that goes from row to row and requests the next one while it works: element by element in a branch, the vector that ends
+// inside the row would be waited for there.  So where a vector would reach beyond the row, its last kVec elements are loaded, and put
+// in their place (in_place) when they are needed.  Rows shorter than a vector take the branch.
+template <typename T, bool TAIL, bool STREAM> __device__ __forceinline__ u32x4 request_row_vec(const T *row, int c, int D)
+{
+    constexpr int V = kVec<T>;
+    if constexpr (TAIL) {
+        if (D < V) return load_row_vec<T, true, STREAM>(row, c, D);
+        return fetch<STREAM>((const u32x4_any *)(row + (c < D - V ? c : D - V)));
+    } else {
+        return load_row_vec<T, false, STREAM>(row, c, D);
+    }
+}
+template <typename T, bool TAIL> __device__ __forceinline__ u32x4 in_place(u32x4 r, int c, int D)
+{
+    constexpr int V = kVec<T>;
+    if constexpr (TAIL) {
+        const int left = D - c;
+        if (D >= V && __any(left < V)) {
+            const int s = (V - D % V) * (int)sizeof(T);                     // bytes
+            u32x4 t = r;
+            if (s & 8) t = u32x4{t[2], t[3], 0, 0};
+            if (s & 4) t = u32x4{t[1], t[2], t[3], 0};
+            if (s & 2) t = u32x4{t[0] >> 16 | t[1] << 16, t[1] >> 16 | t[2] << 16, t[2] >> 16 | t[3] << 16, t[3] >> 16};
+            if (left < V) r = left > 0 ? t : u32x4{0, 0, 0, 0};
+        }
+    }
+    return r;
+}
 template <typename T, bool TAIL, bool STREAM>
 __device__ __forceinline__ void store_row_vec(T *row, int c, int D, const float (&v)[kVec<T>])
 {

@@ -108,13 +108,13 @@ def test_tokens_quantised_in_the_kernel(M, N, K, fmt):
             assert torch.equal(linear_float8(x.to(dtype), w), want.to(dtype))
 
 
-@pytest.mark.parametrize("M,N,K", [(2357, 3272, 242), (143, 11372, 1634), (14673, 2327, 124), (67, 14005, 6507), (65, 130, 16500), (200, 300, 20000),
-                                   (150, 15000, 10000), (100, 129, 16385),
+@pytest.mark.parametrize("M,N,K", [(606, 11384, 1158), (220, 12400, 361), (3869, 4140, 597), (67, 14005, 6507), (65, 130, 16500), (200, 300, 20000),
+                                   (150, 15000, 10000), (100, 129, 16385), (2357, 3272, 242), (143, 11372, 1634), (14673, 2327, 124),
                                    (129, 8000, 9000), (256, 12288, 4096), (1000, 1000, 8200), (450, 4096, 4096), (700, 900, 130), (1100, 33, 2000),
                                    (7675, 2057, 766), (8252, 1863, 892), (4875, 3188, 939), (300, 6797, 9893), (1300, 2000, 7001), (600, 600, 17000)])
 def test_other_tiles(M, N, K):
-    """Sizes that take least time in tiles of 128 x 128 (the first eight: alone, in rounds, in parts), in groups of 64 rows, in several rounds
-    of tiles of 256 x 128, and in parts of them (three each at the end)."""
+    """Sizes that take least time in tiles of 128 x 128 (the first eight: alone, in rounds, in parts), in groups of 64 rows, in
+    wide tiles with one block or two, in several rounds of tiles of 256 x 128, and in parts of them (three each at the end)."""
     test_large_tiles(M, N, K)
 
 

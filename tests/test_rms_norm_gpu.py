@@ -69,6 +69,14 @@ def test_forward_and_backward(rows, D, dtype, wtype, added):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype,wtype", TYPES)
+@pytest.mark.parametrize("D", [9, 10, 130, 131, 132, 133, 134, 135, 1031, 2053, 2054, 4099, 8201, 8207, 9003])
+def test_rows_that_end_inside_a_vector(D, dtype, wtype):
+    """Every length of the last vector, at several widths of the kernels, with more rows than go at once in none of them and in some."""
+    test_forward_and_backward(23, D, dtype, wtype, True)
+    test_output_in_8_bits(5, D, dtype)
+
+
 def test_without_weight_more_dimensions_and_module():
     x, res, w, dy, _ = data((2, 5, 130), torch.bfloat16, torch.bfloat16)
     check(rms_norm(x), *reference(x, None, dy, None, 1e-6)[0], "no weight")
