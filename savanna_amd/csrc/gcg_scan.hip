@@ -537,24 +537,32 @@ template <typename T, bool GATE> __global__ __launch_bounds__(256) void scan_ste
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
 // Rows of a chunk of the forward: 128, two workgroups a CU, which overlap one's loads with the other's sums.  256, one workgroup a CU, where the card
-// holds all of those at once and either they are whole sequences or those of 128 are more than a CU's one: what counts then is the chain of waits.
+// holds all of those at once and they are whole sequences, or those of 128 more than a CU's one or very many: what counts then is the chain of waits.
 // In chunks of 128 and 256: 4 x 701 x 2560 f16 17.8 and 15.9 us, 1 x 8192 x 1024 bf16 28.6 and 23.4, 16 x 256 x 1024 fp32 22.7 and 11.9; but
-// 1 x 512 x 4096 14.1 and 16.1, 64 x 256 x 4096 112 and 122, 2 x 8192 x 4096 118 and 131.
+// 1 x 512 x 4096 14.1 and 16.1, 64 x 256 x 4096 112 and 122, 2 x 8192 x 4096 118 and 131.  So also with many chunks after each other: 32768 x 128 fp32 36
+// and 25, 16384 x 256 bf16 26 and 23, 8192 x 512 20 and 21.
 int fwd_rows(int64_t bs, int64_t L, int64_t D)
 {
     const int64_t cols = (D + 127) / 128, high = bs * ((L + 255) / 256) * cols, low = bs * ((L + 127) / 128) * cols;
-    return L > 128 && high <= 256 && (L <= 256 || low > 256) ? 256 : 128;
+    return L > 128 && high <= 256 && (L <= 256 || low > 256 || L > 12288) ? 256 : 128;
 }
-// Chunks of a group: 131072 x 512 fp32 193 us with 8, 196 with 16, 223 with 32; 2 x 8192 x 4096 bf16 113, 118 and 131.
-constexpr int kGroup = 8;
+// Chunks of a group: 8 where there is enough to do beside the words' way (131072 x 512 fp32 193 us with 8, 196 with 16, 223 with 32; 2 x 8192 x 4096 bf16 113,
+// 118 and 131; the backward of 27733 x 984 bf16 130 with 8, 148 with 32).  Where four workgroups at most have the same time, a
+// group's step is most of it: 65536 x 64 bf16 39 us with 8, 30 with 32, backward 113 and 57; 24531 x 109 fp32, backward, 57 and 39.
+int group_of(int64_t bs, int64_t chunks, int64_t D)
+{
+    if (chunks <= 64 || bs * ((D + 127) / 128) > 4) return 8;
+    return chunks <= 256 ? 16 : 32;
+}
 
-struct Layout { int64_t chunks, groups, pairs, carries, total; };
+struct Layout { int64_t chunks, group, groups, pairs, carries, total; };
 Layout layout_of(int64_t bs, int64_t L, int64_t D, bool backward)
 {
     Layout l;
     const int rows = backward ? kChunk : fwd_rows(bs, L, D);
     l.chunks = (L + rows - 1) / rows;
-    l.groups = (l.chunks + kGroup - 1) / kGroup;
+    l.group = group_of(bs, l.chunks, D);
+    l.groups = (l.chunks + l.group - 1) / l.group;
     l.pairs = 256;
     l.carries = l.pairs + bs * l.chunks * D * 8;
     l.total = l.chunks > 1 ? (l.carries + bs * l.groups * D * 8 + 255) / 256 * 256 : 0;
@@ -565,7 +573,7 @@ Layout layout_of(int64_t bs, int64_t L, int64_t D, bool backward)
 int set_up(Scan &p, const Layout &l, void *ws, hipStream_t st)
 {
     p.chunks = (int32_t)l.chunks;
-    p.group = kGroup;
+    p.group = (int32_t)l.group;
     p.pairs = p.carries = nullptr;
     p.ticket = nullptr;
     if (l.chunks == 1) return 0;
