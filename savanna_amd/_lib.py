@@ -277,6 +277,17 @@ def _run(op, *args):
         return op(*args)
 
 
+def _run_plain(op, *args):
+    """``_run`` of an operator whose results belong to no graph, whatever its arguments do: rms_norm_float8 of 64 x 256 11.7 us on the host with
+    recording on, 9.1 so."""
+    if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active():
+        return op(*args)
+    if forward_ad._current_level >= 0:
+        refuse_tangents(str(op), *args)
+    with torch._C._AutoDispatchBelowAutograd():
+        return op(*args)
+
+
 def native_nodes(t: torch.Tensor) -> bool:
     """Whether a layer's call on ``t`` may pass its Python autograd function by: the forward entry points below then hand a
     call whose gradients are recorded to the C++ form of that function (csrc/gcg_torch.cpp: same operators, same tensors
@@ -1437,7 +1448,7 @@ def rms_norm_float8(x, residual, w, eps: float):
     """(codes, scales, r, rstd): y in 8 bits, blocks of 128 along its last dimension."""
     _require_gpu(x)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.rms_norm_float8, x, residual, w, eps)
+        return _run_plain(torch.ops.gcg.rms_norm_float8, x, residual, w, eps)
     code = _rms_code(x, residual, w)
     codes, scales = _empty_float8(x.shape, torch.float8_e4m3fn, x.device)
     r = torch.empty_like(x) if residual is not None else None
@@ -1521,7 +1532,7 @@ def to_float8(x, format: torch.dtype):
     """(codes, scales) of a contiguous tensor; blocks of 128 along the last dimension."""
     _require_gpu(x)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.to_float8, x, format)
+        return _run_plain(torch.ops.gcg.to_float8, x, format)
     _check_rows(x)
     f, code = format_code(format), dtype_code(x.dtype)
     codes, scales = _empty_float8(x.shape, format, x.device)
@@ -1538,7 +1549,7 @@ def from_float8(codes, scales, columns: int, dtype: torch.dtype):
     """The tensor of ``dtype`` that codes and scales stand for."""
     _require_gpu(codes)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.from_float8, codes, scales, columns, dtype)
+        return _run_plain(torch.ops.gcg.from_float8, codes, scales, columns, dtype)
     _check_float8(codes, scales, columns)
     code = dtype_code(dtype)
     x = torch.empty((*codes.shape[:-1], columns), dtype=dtype, device=codes.device)
@@ -1607,7 +1618,7 @@ def matmul_float8(a, a_scales, b, b_scales, columns: int, dtype: torch.dtype):
     """a b^T of a (..., columns) and a matrix b (N, columns), both in 8 bits."""
     _require_gpu(a)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.matmul_float8, a, a_scales, b, b_scales, columns, dtype)
+        return _run_plain(torch.ops.gcg.matmul_float8, a, a_scales, b, b_scales, columns, dtype)
     _check_float8(a, a_scales, columns)
     _check_float8(b, b_scales, columns)
     if b.dim() != 2 or b.device != a.device:
@@ -1632,7 +1643,7 @@ def linear_float8_infer(x, codes, scales, columns: int):
     """x w^T of a contiguous x, which is quantised in the call, and a weight in 8 bits."""
     _require_gpu(x)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.linear_float8_infer, x, codes, scales, columns)
+        return _run_plain(torch.ops.gcg.linear_float8_infer, x, codes, scales, columns)
     _check_rows(x)
     _product_dtype(x.dtype)
     _check_float8(codes, scales, columns)
@@ -1654,7 +1665,7 @@ def norm_linear_float8_infer(x, residual, gain, codes, scales, columns: int, eps
     """(y, r): the root-mean-square norm of a contiguous x, or of r = x + residual, times a weight in 8 bits (r is empty without a residual)."""
     _require_gpu(x)
     if TORCH_OPS:
-        return _run(torch.ops.gcg.norm_linear_float8_infer, x, residual, gain, codes, scales, columns, eps)
+        return _run_plain(torch.ops.gcg.norm_linear_float8_infer, x, residual, gain, codes, scales, columns, eps)
     _product_dtype(x.dtype)
     a, a_scales, r, _ = rms_norm_float8(x, residual, gain, eps)
     if x.shape[-1] != columns:

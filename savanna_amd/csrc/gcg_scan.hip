@@ -547,11 +547,11 @@ int fwd_rows(int64_t bs, int64_t L, int64_t D)
     return L > 128 && high <= 256 && (L <= 256 || low > 256 || L > 12288) ? 256 : 128;
 }
 // Chunks of a group: 8 where there is enough to do beside the words' way (131072 x 512 fp32 193 us with 8, 196 with 16, 223 with 32; 2 x 8192 x 4096 bf16 113,
-// 118 and 131; the backward of 27733 x 984 bf16 130 with 8, 148 with 32).  Where four workgroups at most have the same time, a
+// 118 and 131; the backward of 27733 x 984 bf16 130 with 8, 148 with 32).  Where two workgroups (fp32: four) at most have the same time, a
 // group's step is most of it: 65536 x 64 bf16 39 us with 8, 30 with 32, backward 113 and 57; 24531 x 109 fp32, backward, 57 and 39.
 int group_of(int64_t bs, int64_t chunks, int64_t D)
 {
-    if (chunks <= 64 || bs * ((D + 127) / 128) > 4) return 8;
+    if (chunks <= 64 || bs * ((D + 127) / 128) > 2) return 8;
     return chunks <= 256 ? 16 : 32;
 }
 

@@ -100,7 +100,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
 def rms_norm_float8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
     """``rms_norm`` with y as a ``Float8`` (float8.py), formed of y in float32: y, or (y, r).  Not differentiable: the graphs of its arguments
     are left alone (``norm_linear_float8`` is the differentiable form, with the product)."""
-    x, residual, weight = (t.detach() if t is not None else None for t in (x, residual, weight))
+    x, residual, weight = (t.detach() if t is not None and t.requires_grad else t for t in (x, residual, weight))
     x = x if x.is_contiguous() else x.contiguous()
     residual = residual if residual is None or residual.is_contiguous() else residual.contiguous()
     codes, scales, r, _ = _lib.rms_norm_float8(x, residual, weight, eps)

@@ -117,7 +117,8 @@ def test_forward_and_backward(bs, L, D, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("bs,L,D,lengths", [(2, 256, 129, None), (2, 255, 70, [255, 130]), (6, 700, 1601, [700, 0, 1, 256, 257, 513]), (1, 3000, 1300, None),
-                                            (2, 2300, 896, [2300, 2049]), (1, 12500, 40, None), (1, 9000, 70, [8321]), (3, 17000, 20, [16999, 12345, 0])])
+                                            (2, 2300, 896, [2300, 2049]), (1, 12500, 40, None), (1, 9000, 70, [8321]), (3, 17000, 20, [16999, 12345, 0]),
+                                            (2, 17000, 20, [16999, 300])])
 def test_sizes_whose_chunks_are_long(bs, L, D, lengths, dtype):
     """Those that the card holds at once in chunks of 256 rows: a sequence in one chunk, in several, in more than a group of them."""
     d = data(bs, L, D, dtype, seed=L + D)
