@@ -323,8 +323,10 @@ template <typename T, int C, int R, int W, bool GATE> __global__ __launch_bounds
         const uint32_t row = slot * R + i;
         rf[i] = load_channels<T, C>(wf, lane_off + row * sf);
         rx[i] = load_channels<T, C>(wx, lane_off + row * sx);
-        rd[i] = load_channels<T, C>(wd, lane_off + row * sd);
-        if constexpr (GATE) rg[i] = load_channels<T, C>(wg, lane_off + row * sg);
+        // (a row that is not in the sequence may lie inside the window where rows share their elements: a sum's gradient is one row for all)
+        const bool inside = (int)row < rows;
+        rd[i] = load_channels<T, C>(wd, inside ? lane_off + row * sd : WIN_OFF);
+        if constexpr (GATE) rg[i] = load_channels<T, C>(wg, inside ? lane_off + row * sg : WIN_OFF);
     }
     float bias[C], h0[C];
 #pragma unroll

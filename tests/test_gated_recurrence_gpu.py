@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from layer8 import TINY, U, check
+from savanna_amd import _lib
 from savanna_amd.operators.gated_recurrence import (GatedRecurrence, gated_recurrence, gated_recurrence_features, gated_recurrence_step)
 
 pytestmark = pytest.mark.gpu
@@ -290,3 +291,41 @@ def test_refusals():
     last.sum().backward()
     assert (s.grad == 1).all() and not b.grad.any()
     assert gated_recurrence(x[:0], x[:0]).shape == (0, 5, 8)
+
+
+@pytest.mark.parametrize("nodes", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bs,L,D,lengths", [(1, 70, 3, None), (2, 70, 66, None), (3, 70, 33, [70, 0, 9]), (2, 300, 64, [300, 129]), (2, 70, 1, None),
+                                            (1, 1100, 70, None)])
+def test_rows_that_share_their_elements(bs, L, D, lengths, dtype, nodes, monkeypatch):
+    """What the rows behind a sequence's end hold in memory is no part of it: gradients of one row for all, as that of a sum over the
+    rows is, and rows that overlap, are those of the same numbers in rows of their own.  So also with such gates and inputs."""
+    if not nodes:
+        monkeypatch.setattr(_lib, "native_nodes", lambda t: False)
+    d = data(bs, L, D, dtype, seed=L + D)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    rows = lambda name: d[name][:, :1].expand(bs, L, D)                                             # noqa: E731
+    overlapping = lambda name: torch.cat([d[name][..., 0], d[name][:, :D - 1, 0]], 1).unfold(1, D, 1) if D <= L else rows(name)   # noqa: E731
+
+    def gradients(x, f, gate, dy):
+        t = [v.detach().requires_grad_(True) for v in (x, f, d["bias"], d["initial"])]
+        y, last = gated_recurrence(t[0], t[1], gate, t[2], initial_state=t[3], lengths=n, output_final_state=True)
+        return y, t, torch.autograd.grad([y, last], t, [dy, d["dstate"]], retain_graph=True)
+
+    for view in (rows, overlapping):
+        for x, f, gate in ((d["x"], d["f"], None), (d["x"], d["f"], view("gate")), (view("x"), view("f"), d["gate"]), (view("x"), view("f"), None)):
+            own = [v if v is None else v.contiguous() for v in (x, f, gate)]
+            y, t, got = gradients(x, f, gate, view("dy"))
+            _, _, want = gradients(*own, view("dy").contiguous())
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (view, gate is None, [(a - b).abs().max().item() for a, b in zip(got, want)])
+            if view is rows:
+                summed = torch.autograd.grad(y.sum(1), t, d["dy"][:, 0], retain_graph=True)
+                alone = torch.autograd.grad(y, t, view("dy").contiguous(), retain_graph=True)
+                assert all(torch.equal(a, b) for a, b in zip(summed, alone))
+                if D == 1:
+                    whole = torch.autograd.grad(y.sum(), t, retain_graph=True)
+                    assert all(torch.equal(a, b) for a, b in zip(whole, torch.autograd.grad(y, t, torch.ones_like(y))))
+    c = dict(d, dy=rows("dy").contiguous())
+    y, t, got = gradients(d["x"], d["f"], None, rows("dy"))
+    want = reference(c, gate=False, lengths=n)
+    compare(dict(zip(("dx", "df", "dbias", "dinitial"), got)), want, f"{bs} x {L} x {D}")
