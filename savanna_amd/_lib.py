@@ -1834,4 +1834,6 @@ def scan_step(x, f, gate, bias, state):
         rc = load().gcg_scan_step(a.data_ptr(), b.data_ptr(), _ptr(c), _scan_strides(1, a, b, c), _ptr(bias), state.data_ptr(), y.data_ptr(),
                                   x.shape[0], x.shape[1], dtype_code(x.dtype), torch.cuda.current_stream().cuda_stream)
     check(rc, "gcg_scan_step")
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     return y

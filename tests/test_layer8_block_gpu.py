@@ -342,3 +342,21 @@ def test_example():
     sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
     import recurrent_float8
     assert recurrent_float8.main(["--width", "192", "--length", "150", "--steps", "2"])
+
+
+def test_ctypes_binding_says_that_a_step_modifies_its_state(tmp_path):
+    """Whatever saved the state for a backward pass finds it modified, as through the other binding; an inference tensor has no count of it."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys, torch; sys.path[:0] = [%r]; from savanna_amd import _lib; from savanna_amd.operators.gated_recurrence import gated_recurrence_step as step\n"
+            "assert not _lib.TORCH_OPS\n"
+            "x, state = torch.randn(3, 70, device='cuda:0'), torch.zeros(3, 70, device='cuda:0')\n"
+            "w = torch.ones_like(state).requires_grad_(True)\n"
+            "loss = (w * state).sum()\n"
+            "for n in (1, 2, 3):\n"
+            "    with torch.no_grad(): step(x, x, state)\n"
+            "    assert state._version == n, state._version\n"
+            "try: loss.backward()\n"
+            "except RuntimeError as e: assert 'modified by an inplace operation' in str(e)\n"
+            "else: raise AssertionError('a gradient of what is no longer there')\n"
+            "with torch.inference_mode(): step(x, x, torch.zeros(3, 70, device='cuda:0'))\n") % os.path.dirname(here)
+    subprocess.run([sys.executable, "-c", code], check=True, env={**os.environ, "GCG_BINDING": "ctypes"}, timeout=100)
