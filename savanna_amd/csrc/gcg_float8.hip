@@ -170,7 +170,7 @@ template <typename T, bool TAIL> __device__ __forceinline__ void load8(const Col
 
 template <typename T, bool E5M2, bool ROWS, bool TAIL> __global__ __launch_bounds__(256) void to_float8_columns_kernel(ColumnsF8 a)
 {
-    __shared__ uint8_t tile[128 * 128];
+    __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     __shared__ uint32_t tops[4][128];
     const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, wave = threadIdx.x / kWave;
     const int64_t rt = blockIdx.x / a.col_tiles, ct = blockIdx.x % a.col_tiles;

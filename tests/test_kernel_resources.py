@@ -1,5 +1,6 @@
 """Registers of the built kernels, read from the code objects' own metadata: spills and waves per SIMD that a change to shared
 code can cost in kernels nobody timed."""
+import os
 import re
 import struct
 
@@ -85,3 +86,12 @@ def test_waves_per_simd(kernels, pattern, waves):
     for name, k in _select(kernels, pattern).items():
         vgpr = k[".vgpr_count"]                          # (with the accumulation registers)
         assert 512 // ((vgpr + 7) // 8 * 8) >= waves, (name, vgpr)
+
+
+@pytest.mark.parametrize("name", sorted(n for n in os.listdir(os.path.dirname(_lib.LIB_PATH)) if n.endswith((".hip", ".h"))))
+def test_bytes_in_shared_memory_that_are_read_in_vectors_say_their_alignment(name):
+    """The language gives an array of bytes an alignment of one."""
+    text = open(os.path.join(os.path.dirname(_lib.LIB_PATH), name)).read()
+    for declaration, buffer in re.findall(r"(__shared__[^;=]*?\buint8_t\s+(\w+)\s*\[)", text):
+        if re.search(r"u32x\d+ \*\)\(?" + buffer + r"\b", text):
+            assert "align" in declaration, declaration
