@@ -55,6 +55,7 @@ LAYER8_OP_NAMES = (
 NODE_NAMES = ("gate_conv_gate", "gate_conv_gate_decay", "short_hyena", "mixer_mr", "mixer_mr_decay")
 BLOCK_NODE_NAMES = ("layer_norm", "linear_attn", "linear_attn_packed")
 LAYER8_NODE_NAMES = ("rms_norm", "linear_float8", "norm_linear_float8", "scan", "scan_packed")
+STREAM_NODE_NAMES = ("rms_norm_float8_stream",)         # of its outputs the residual stream is differentiable, the 8 bits are not
 
 
 # ---- autograd --------------------------------------------------------------------------------------------

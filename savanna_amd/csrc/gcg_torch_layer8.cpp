@@ -649,6 +649,20 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     }
 };
 
+// The norm into 8 bits with a residual: (codes, scales, r), of which r, a sum, is differentiable.
+struct StreamNode : torch::autograd::Function<StreamNode> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &residual, const OptTensor &w, double eps)
+    {
+        static const auto f = op<Four(const Tensor &, const OptTensor &, const OptTensor &, double)>("gcg::rms_norm_float8");
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [codes, scales, r, rstd] = f.call(x, residual, w, eps);
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({codes, scales});
+        return {codes, scales, r};
+    }
+    static variable_list backward(AutogradContext *, variable_list g) { return {g[2], g[2], Tensor(), Tensor()}; }
+};
+
 // (the rows counted from x's sizes: a matrix of no columns has some)
 Tensor as_matrix(const Tensor &t)
 {
@@ -822,6 +836,11 @@ std::vector<Tensor> rms_norm(const Tensor &x, const OptTensor &residual, const O
     check_leaves({&x, &a, &b});
     return RmsNormNode::apply(x, residual, w, eps);
 }
+std::vector<Tensor> rms_norm_float8_stream(const Tensor &x, const Tensor &residual, const OptTensor &w, double eps)
+{
+    check_leaves({&x, &residual});
+    return StreamNode::apply(x, residual, w, eps);
+}
 Tensor linear_float8(const Tensor &x, const Tensor &w, at::ScalarType format)
 {
     check_weight(x, w);
@@ -875,6 +894,7 @@ TORCH_LIBRARY_FRAGMENT(gcg, m)
     m.def("scan_packed_bwd(Tensor dy, Tensor features, Tensor? bias, Tensor states, bool need_dbias) -> (Tensor, Tensor)");
     m.def("scan_step(Tensor x, Tensor f, Tensor? gate, Tensor? bias, Tensor(a!) state) -> Tensor");
     m.def("rms_norm(Tensor x, Tensor? residual, Tensor? w, float eps) -> Tensor[]", &rms_norm);
+    m.def("rms_norm_float8_stream(Tensor x, Tensor residual, Tensor? w, float eps) -> Tensor[]", &rms_norm_float8_stream);
     m.def("linear_float8(Tensor x, Tensor w, ScalarType format) -> Tensor", &linear_float8);
     m.def("norm_linear_float8(Tensor x, Tensor? residual, Tensor? gain, Tensor w, float eps, ScalarType format) -> Tensor[]", &norm_linear_float8);
     m.def("scan(Tensor x, Tensor f, Tensor? gate, Tensor? bias, Tensor? initial, Tensor? lengths, bool final) -> Tensor[]", &scan);

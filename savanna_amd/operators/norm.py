@@ -97,13 +97,34 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     return _RMSNorm.apply(x, residual, weight, eps)
 
 
+class _StreamBeside8Bits(torch.autograd.Function):
+    """rms_norm_float8 with a residual: r is a sum with a gradient, the 8 bits beside it have none."""
+
+    @staticmethod
+    def forward(ctx, x, residual, w, eps):
+        ctx.set_materialize_grads(False)
+        codes, scales, r, _ = _lib.rms_norm_float8(x, residual, w, eps)
+        ctx.mark_non_differentiable(codes, scales)
+        return codes, scales, r
+
+    @staticmethod
+    def backward(ctx, _codes, _scales, dr):
+        return dr, dr, None, None
+
+
 def rms_norm_float8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
-    """``rms_norm`` with y as a ``Float8`` (float8.py), formed of y in float32: y, or (y, r).  Not differentiable: the graphs of its arguments
-    are left alone (``norm_linear_float8`` is the differentiable form, with the product)."""
-    x, residual, weight = (t.detach() if t is not None and t.requires_grad else t for t in (x, residual, weight))
+    """``rms_norm`` with y as a ``Float8`` (float8.py), formed of y in float32: y, or (y, r).  y is not differentiable: no gradient reaches x, the
+    residual or the weight through it (``norm_linear_float8`` is the differentiable form, with the product).  r is, as the sum that it is."""
+    recorded = residual is not None and torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad)
+    if not recorded:
+        x, residual, weight = (t.detach() if t is not None and t.requires_grad else t for t in (x, residual, weight))
     x = x if x.is_contiguous() else x.contiguous()
     residual = residual if residual is None or residual.is_contiguous() else residual.contiguous()
-    codes, scales, r, _ = _lib.rms_norm_float8(x, residual, weight, eps)
+    if recorded:
+        node = torch.ops.gcg.rms_norm_float8_stream if _lib.native_nodes(x) else _StreamBeside8Bits.apply
+        codes, scales, r = node(x, residual, weight, eps)
+    else:
+        codes, scales, r, _ = _lib.rms_norm_float8(x, residual, weight, eps)
     y = Float8(codes, scales, x.shape[-1])
     return y if residual is None else (y, r)
 

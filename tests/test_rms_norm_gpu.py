@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from layer8 import TINY, U, check, float8, values
+from savanna_amd import _lib
 from savanna_amd.operators.norm import RMSNorm, rms_norm, rms_norm_float8
 
 pytestmark = pytest.mark.gpu
@@ -152,3 +153,65 @@ def test_refusals():
     w = torch.ones(64, device=DEV, requires_grad=True)
     rms_norm(e, w).sum().backward()
     assert not w.grad.any()
+
+
+@pytest.mark.parametrize("nodes", [True, False])
+@pytest.mark.parametrize("grads", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_stream_beside_8_bits_keeps_its_gradient(dtype, grads, nodes, monkeypatch):
+    """The 8 bits have none, the sum beside them is a sum: its gradient reaches both that were added."""
+    if not nodes:
+        monkeypatch.setattr(_lib, "native_nodes", lambda t: False)
+    x, res, w, dy, dr = data((37, 300), dtype, dtype)
+    want = rms_norm_float8(x, w, residual=res)
+    leaves = [t.requires_grad_(need) for t, need in zip((x, res), grads)]
+    q, r = rms_norm_float8(x * 1, w.requires_grad_(True), residual=res * 1)
+    assert torch.equal(r, want[1]) and torch.equal(q.codes.view(torch.uint8), want[0].codes.view(torch.uint8))
+    assert r.requires_grad and not q.codes.requires_grad and not q.scales.requires_grad
+    for g in torch.autograd.grad(r, [t for t in leaves if t.requires_grad], dr):
+        assert torch.equal(g, dr)
+    r.mul_(2)                                               # r belongs to the caller
+    with torch.no_grad():
+        assert not rms_norm_float8(x, w, residual=res)[1].requires_grad
+    assert not rms_norm_float8(x.detach(), w, residual=res.detach())[1].requires_grad
+    assert not rms_norm_float8(x, w).codes.requires_grad
+
+
+@pytest.mark.skipif(not _lib.TORCH_OPS, reason="the ctypes binding is not traced")
+def test_the_stream_beside_8_bits_is_traced():
+    x, res, w, dy, dr = data((37, 300), torch.bfloat16, torch.bfloat16)
+    x.requires_grad_(True), res.requires_grad_(True)
+
+    def f(x, res, w):
+        q, r = rms_norm_float8(x, w, residual=res)
+        return q.codes.view(torch.uint8), r * 2
+    (a, r), (b, s) = f(x, res, w), torch.compile(f, fullgraph=True, backend="aot_eager")(x, res, w)
+    assert torch.equal(a, b) and torch.equal(r, s)
+    for g, h in zip(torch.autograd.grad(r, (x, res), dr), torch.autograd.grad(s, (x, res), dr)):
+        assert torch.equal(g, h) and torch.equal(g, 2 * dr)
+
+
+@pytest.mark.skipif(not _lib.TORCH_OPS, reason="the nodes are the torch binding's")
+def test_the_stream_beside_8_bits_is_captured():
+    """Replayed like the other operators, and refused where a leaf belongs to a living graph of the default stream."""
+    x, res, w, _, dr = data((37, 300), torch.bfloat16, torch.bfloat16)
+    x.requires_grad_(True), res.requires_grad_(True)
+
+    def f():
+        q, r = rms_norm_float8(x, w, residual=res)
+        return [q.codes.view(torch.uint8), r.detach(), *torch.autograd.grad(r * 3, (x, res), dr)]
+    want = f()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = f()
+    for _ in range(3):
+        g.replay()
+        f()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    lives = (x * 1).sum()
+    refused = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="still lives"), torch.cuda.graph(refused):
+        res.detach() + 1
+        rms_norm_float8(x, w, residual=res)
+    del lives
