@@ -166,7 +166,10 @@ class LinearFloat8(nn.Module):
     """``linear_float8`` with its weight (out_features, in_features), initialised as ``nn.Linear``'s.
 
     ``lay_out()`` quantises the weight once for calls without gradients, as a serving program does after loading; until then, and after ``train()``,
-    a move or cast of the module or ``load_state_dict``, every call quantises it.  (Call it again if the weight is changed in another way.)"""
+    a move or cast of the module, ``load_state_dict`` or any change of the weight that torch counts, every call quantises it.  (It counts none that goes
+    by ``weight.data``, by a pointer, of a weight made in inference mode, or inside a traced program: call it again then.)"""
+
+    _laid_out_of = None             # the weight that was laid out, and torch's count of its modifications then
 
     def __init__(self, in_features: int, out_features: int, grad_dtype: torch.dtype = E4M3, dtype=torch.bfloat16, device=None):
         super().__init__()
@@ -177,7 +180,31 @@ class LinearFloat8(nn.Module):
 
     def lay_out(self) -> "LinearFloat8":
         self._laid_out = to_float8(self.weight)
+        self._note()
         return self
+
+    def _note(self) -> None:
+        # (in a tuple: an attribute of its own would be a second parameter)
+        self._laid_out_of = self.weight, None if self.weight.is_inference() else self.weight._version
+
+    def _current(self) -> bool:
+        if self._laid_out is None or self._laid_out_of is None:
+            return False
+        weight, count = self._laid_out_of
+        if self._parameters.get("weight") is not weight:
+            return False
+        return count is None or torch.compiler.is_compiling() or weight._version == count
+
+    def __getstate__(self):
+        """A copy's weight has a count of its own, so what a copy holds is either of its weight as it is, or not there."""
+        return {**self.__dict__, "_laid_out": self._laid_out if self._current() else None, "_laid_out_of": None}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_laid_out_of" not in state:             # (written before it was noted what was laid out)
+            self._laid_out = None
+        if self._laid_out is not None:
+            self._note()
 
     def _apply(self, fn, recurse=True):
         self._laid_out = None
@@ -194,7 +221,7 @@ class LinearFloat8(nn.Module):
 
     def operand(self) -> Union[torch.Tensor, Float8]:
         """The weight, or its 8 bits where they are laid out and no gradient is wanted."""
-        return self.weight if self._laid_out is None or torch.is_grad_enabled() else self._laid_out
+        return self._laid_out if not torch.is_grad_enabled() and self._current() else self.weight
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return linear_float8(x, self.operand(), self.grad_dtype)

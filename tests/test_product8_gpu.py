@@ -267,3 +267,66 @@ def test_refusals():
     linear_float8(e, v).sum().backward()
     assert e.grad.shape == (0, 300) and not v.grad.any()
     assert from_float8(q, torch.float32).shape == (20, 300)
+
+
+def test_a_laid_out_weight_that_has_changed_is_not_used():
+    """A weight updated in place, assigned anew or given by functional_call is the one that is multiplied by; copies of the module stay laid out."""
+    import copy
+    import io
+    torch.manual_seed(0)
+    x = torch.randn(20, 300, device=DEV).bfloat16()
+    other = (torch.randn(130, 300, device=DEV) / 17).bfloat16()
+
+    def change_in_place(m):
+        m.weight.mul_(2)
+
+    def assign(m):
+        m.weight = torch.nn.Parameter(other.clone())
+
+    def step(m):
+        m.weight.grad = other.clone()
+        torch.optim.SGD(m.parameters(), lr=1.0).step()
+
+    with torch.no_grad():
+        for change in (change_in_place, assign, step):
+            m = LinearFloat8(300, 130, device=DEV).eval().lay_out()
+            assert isinstance(m.operand(), Float8)
+            y = m(x)
+            change(m)
+            assert torch.equal(m(x), linear_float8(x, m.weight)) and not torch.equal(m(x), y)
+            m.lay_out()
+            assert isinstance(m.operand(), Float8) and torch.equal(m(x), linear_float8(x, m.weight))
+        m = LinearFloat8(300, 130, device=DEV).eval().lay_out()
+        y = m(x)
+        assert torch.equal(torch.func.functional_call(m, {"weight": other}, (x,)), linear_float8(x, other))
+        assert isinstance(m.operand(), Float8) and torch.equal(m(x), y)
+        copied = copy.deepcopy(m)
+        assert isinstance(copied.operand(), Float8) and torch.equal(copied(x), y)
+        copied.weight.mul_(2)
+        assert not torch.equal(copied(x), y) and torch.equal(m(x), y)
+        assert torch.equal(copy.deepcopy(copied)(x), linear_float8(x, copied.weight))
+        file = io.BytesIO()
+        torch.save(m, file)
+        file.seek(0)
+        loaded = torch.load(file, weights_only=False)
+        assert isinstance(loaded.operand(), Float8) and torch.equal(loaded(x), y)
+        loaded.weight.mul_(2)
+        assert torch.equal(loaded(x), linear_float8(x, loaded.weight))
+    with torch.inference_mode():                            # such weights have no count of their changes, and need lay_out() again
+        m = LinearFloat8(300, 130, device=DEV).lay_out()
+        assert isinstance(m.operand(), Float8) and torch.equal(m(x), linear_float8(x, m.weight))
+        assert torch.equal(copy.deepcopy(m)(x), m(x))
+
+
+@pytest.mark.skipif(not _lib.TORCH_OPS, reason="the ctypes binding is not traced")
+def test_a_laid_out_weight_is_traced():
+    m = LinearFloat8(300, 130, device=DEV).eval().lay_out()
+    x = torch.randn(20, 300, device=DEV).bfloat16()
+    with torch.no_grad():
+        f = torch.compile(m, fullgraph=True, backend="aot_eager")
+        assert torch.equal(f(x), m(x))
+        m.weight.mul_(2)
+        m.lay_out()
+        assert torch.equal(f(x), linear_float8(x, m.weight))
+        m.weight = torch.nn.Parameter(m.weight * 2)
+        assert torch.equal(f(x), linear_float8(x, m.weight))
