@@ -612,7 +612,7 @@ GCG_API int gcg_rms_norm_bwd(const void *dy, const void *r, const void *dr, cons
  * stands for 2^(b - 127), the smallest power of two, 2^-127 at least, that brings the block's largest magnitude to at most the format's
  * largest number (GCG_E4M3: 448, no infinities; GCG_E5M2: 57344); a block of zeros has 127.  A code is the element times 2^(127 - b),
  * rounded to nearest even.  A block that holds an infinity or a NaN has the largest b, 247 (GCG_E5M2: 240); they
- * become NaN (GCG_E5M2: an infinity stays one).
+ * become NaN (GCG_E5M2: an infinity stays one).  A byte of 255, which only tensors made elsewhere hold, makes its block NaN.
  *
  * gcg_to_float8 quantises a contiguous tensor along its rows, gcg_from_float8 makes a tensor of it again (one rounding at most).
  * gcg_to_float8_columns quantises along the columns and writes the result transposed: codes_t (D, 128 ceil(rows / 128)), scales_t

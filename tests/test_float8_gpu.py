@@ -110,3 +110,20 @@ def test_refusals():
         assert from_float8(e, torch.float32).shape == shape
     grad = to_float8(x.requires_grad_(True))
     assert not grad.codes.requires_grad
+
+
+def test_a_scale_that_is_no_number():
+    """The byte 255 of float8_e8m0fnu, which tensors made elsewhere may hold, makes its whole block NaN, whatever the codes."""
+    x = torch.randn(130, 300, device=DEV)
+    for fmt in (E4M3, E5M2):
+        q = to_float8(x, fmt)
+        q.codes.view(torch.uint8)[3, 130] = 0
+        clean = from_float8(q, torch.float32)
+        q.scales.view(torch.uint8)[3, 1] = 255
+        bad = torch.zeros(130, 300, dtype=torch.bool, device=DEV)
+        bad[3, 128:256] = True
+        for out in TYPES:
+            v = from_float8(q, out)
+            assert torch.equal(torch.isnan(v), bad) and torch.equal(v[~bad], clean[~bad].to(out))
+        t = Float8(*_lib.float8_columns(q.codes, q.scales, 300, E4M3), 130)
+        assert torch.equal(torch.isnan(from_float8(t, torch.float32)).t(), bad)

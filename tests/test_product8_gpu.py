@@ -330,3 +330,22 @@ def test_a_laid_out_weight_is_traced():
         assert torch.equal(f(x), linear_float8(x, m.weight))
         m.weight = torch.nn.Parameter(m.weight * 2)
         assert torch.equal(f(x), linear_float8(x, m.weight))
+
+
+def test_a_scale_that_is_no_number():
+    """The byte 255 in either operand makes the results of its row NaN and leaves the others alone, by every kernel."""
+    for M, N, K in ((2, 70, 300), (20, 70, 300), (60, 70, 300), (150, 129, 16385), (300, 128, 2000), (300, 260, 20000)):
+        a, b = whole(M, K, E4M3, 1, 3), whole(N, K, E4M3, 2, 3)
+        qa, qb = to_float8(a), to_float8(b)
+        clean = matmul_float8(qa, qb)
+        qa.codes.view(torch.uint8)[1, 128:256] = 0
+        qa.scales.view(torch.uint8)[1, 1] = qb.scales.view(torch.uint8)[5, 2] = 255
+        y = matmul_float8(qa, qb)
+        bad = torch.zeros(M, N, dtype=torch.bool, device=DEV)
+        bad[1], bad[:, 5] = True, True
+        assert torch.equal(torch.isnan(y), bad) and torch.equal(y[~bad], clean[~bad]), (M, N, K)
+        if M == 2:
+            with torch.no_grad():
+                z = linear_float8(a, qb)
+            bad[1], bad[:, 5] = False, True
+            assert torch.equal(torch.isnan(z), bad) and torch.equal(z[~bad], clean[~bad])
