@@ -58,3 +58,19 @@ def test_more_sequences_than_a_launch_holds(hl):
     h = torch.randn(1, 1, hl, device=DEV).to(torch.bfloat16)
     with pytest.raises(RuntimeError, match="hipError 9"):          # hipErrorInvalidConfiguration
         _lib.fwd(x, x, x, h, algo="window" if hl <= 8 else "direct")
+
+
+def test_a_token_of_the_most_sequences():
+    """A channel of 2^31 - 1 entries, which the kernel walks in steps that end beyond what 32 bits count."""
+    bs = (1 << 31) - 1
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 36 << 30:
+        pytest.skip("needs 36 GiB of device memory")
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x, f = (torch.empty(bs, 1, device=DEV, dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    state = torch.empty(bs, 1, device=DEV).normal_(generator=gen)
+    cuts = [slice(0, 3000), slice(bs // 2, bs // 2 + 70000), slice(bs - 200000, bs)]
+    before = [state[c].clone() for c in cuts]
+    y = _lib.scan_step(x, f, None, None, state)
+    for c, s in zip(cuts, before):
+        assert torch.equal(y[c], _lib.scan_step(x[c], f[c], None, None, s)) and torch.equal(state[c], s)
