@@ -673,7 +673,9 @@ int scan_step_launch(int dtype, const void *x, const void *f, const void *gate, 
                      int64_t bs, int D, hipStream_t st)
 {
     const ScanStep p = {x, f, gate, bias, state, y, strides[0], strides[1], strides[2], (int32_t)bs, D};
-    const dim3 grid((unsigned)((D + 255) / 256), (unsigned)(bs < 65535 ? bs : 65535)), block(256);
+    // (as many entries beside each other as a launch's 2^32 threads hold)
+    const int64_t across = (D + 255) / 256, most = ((1ll << 24) - 1) / across, deep = most < 65535 ? most : 65535;
+    const dim3 grid((unsigned)across, (unsigned)(bs < deep ? bs : deep)), block(256);
     switch (dtype) {
     case GCG_F32: return gate ? launch_main(scan_step_kernel<float, true>, grid, block, st, p) : launch_main(scan_step_kernel<float, false>, grid, block, st, p);
     case GCG_BF16: return gate ? launch_main(scan_step_kernel<bf16_t, true>, grid, block, st, p) : launch_main(scan_step_kernel<bf16_t, false>, grid, block, st, p);

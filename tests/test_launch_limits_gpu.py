@@ -74,3 +74,19 @@ def test_a_token_of_the_most_sequences():
     y = _lib.scan_step(x, f, None, None, state)
     for c, s in zip(cuts, before):
         assert torch.equal(y[c], _lib.scan_step(x[c], f[c], None, None, s)) and torch.equal(state[c], s)
+
+
+def test_a_token_of_many_wide_sequences():
+    """2^32 states, a thread each, would be more than a launch holds: a thread takes several."""
+    bs, D = 8200, 1 << 19
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 50 << 30:
+        pytest.skip("needs 50 GiB of device memory")
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x, f = (torch.empty(bs, D, device=DEV, dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    state = torch.empty(bs, D, device=DEV).normal_(generator=gen)
+    cuts = [slice(0, 20), slice(bs // 2, bs // 2 + 20), slice(bs - 30, bs)]
+    before = [state[c].clone() for c in cuts]
+    y = _lib.scan_step(x, f, None, None, state)
+    for c, s in zip(cuts, before):
+        assert torch.equal(y[c], _lib.scan_step(x[c], f[c], None, None, s)) and torch.equal(state[c], s)
