@@ -693,12 +693,18 @@ Two linear_gradients(const Tensor &dy, const Tensor &codes, const Tensor &scales
     }
     return {dx, dw};
 }
-// checks a weight in the tensors' type
-void check_weight(const Tensor &x, const Tensor &w)
+// checks a weight in the tensors' type; others: the norm's, whose gradients are formed of x's
+void check_weight(const Tensor &x, const Tensor &w, const Tensor &residual = {}, const Tensor &gain = {})
 {
     (void)product_dtype(x.scalar_type());
     TORCH_CHECK(w.dim() == 2 && w.size(1) == x.size(-1) && w.scalar_type() == x.scalar_type() && w.device() == x.device(),
                 "gcg: the weight must be a (out, in) matrix with the dtype and device of x");
+    if (!at::GradMode::is_enabled()) return;
+    const auto needs = [](const Tensor &t) { return t.defined() && t.requires_grad(); };
+    TORCH_CHECK(rows_of(x) <= GCG_PRODUCT8_MAX_K || !needs(w), "gcg: the weight's gradient is a sum over ", rows_of(x), " rows; at most ",
+                (int)GCG_PRODUCT8_MAX_K, " are supported");
+    TORCH_CHECK(w.size(0) <= GCG_PRODUCT8_MAX_K || !(needs(x) || needs(residual) || needs(gain)), "gcg: x's gradient is a sum over ", w.size(0),
+                " outputs; at most ", (int)GCG_PRODUCT8_MAX_K, " are supported");
 }
 
 struct LinearFloat8Node : torch::autograd::Function<LinearFloat8Node> {
@@ -850,8 +856,8 @@ Tensor linear_float8(const Tensor &x, const Tensor &w, at::ScalarType format)
 std::vector<Tensor> norm_linear_float8(const Tensor &x, const OptTensor &residual, const OptTensor &gain, const Tensor &w, double eps,
                                        at::ScalarType format)
 {
-    check_weight(x, w);
     const Tensor a = or_empty(residual), b = or_empty(gain);
+    check_weight(x, w, a, b);
     check_leaves({&x, &a, &b, &w});
     return NormLinearFloat8Node::apply(x, residual, gain, w, eps, format);
 }

@@ -51,11 +51,18 @@ def matmul_float8(a: Float8, b: Float8, dtype: torch.dtype = torch.bfloat16) -> 
     return _lib.matmul_float8(a.codes, a.scales, b.codes, b.scales, a.columns, dtype)
 
 
-def _check_weight(x: torch.Tensor, w: torch.Tensor) -> None:
+def _check_weight(x: torch.Tensor, w: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """others: the norm's, whose gradients are formed of x's."""
     if x.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"products of 8-bit tensors are bfloat16 or float16; got {x.dtype}")
     if w.dim() != 2 or x.dim() < 1 or w.shape[1] != x.shape[-1] or w.dtype != x.dtype or w.device != x.device:
         raise ValueError("the weight must be a (out, in) matrix with the dtype and device of x")
+    most = _lib.PRODUCT8_MAX_K
+    if (x.numel() > most or w.shape[0] > most) and torch.is_grad_enabled():
+        if w.requires_grad and x.shape[:-1].numel() > most:
+            raise ValueError(f"the weight's gradient is a sum over {x.shape[:-1].numel()} rows; at most {most} are supported")
+        if w.shape[0] > most and any(t is not None and t.requires_grad for t in (x, *others)):
+            raise ValueError(f"x's gradient is a sum over {w.shape[0]} outputs; at most {most} are supported")
 
 
 def _gradients(dy, x8, w, grad_dtype, need_dx, need_dw):
@@ -127,7 +134,8 @@ def linear_float8(x: torch.Tensor, w: Union[torch.Tensor, Float8], grad_dtype: t
     """x w^T (..., out) with both operands in 8 bits (``float8_e4m3fn``).
 
     x: (..., in) bfloat16 or float16.  w: (out, in) of x's dtype, differentiable as x is, or a ``Float8``, laid out once for inference.
-    ``grad_dtype``: the 8-bit type of y's gradient in the backward's products; ``float8_e5m2`` trades a bit of each number for range within a block."""
+    ``grad_dtype``: the 8-bit type of y's gradient in the backward's products; ``float8_e5m2`` trades a bit of each number for range within a block.
+    Sums go over 2^22 numbers at most: in, out where x's gradient is wanted, the rows where w's is."""
     x = x if x.is_contiguous() else x.contiguous()
     if isinstance(w, Float8):
         _no_gradient(x)
@@ -151,7 +159,7 @@ def norm_linear_float8(x: torch.Tensor, gain: Optional[torch.Tensor], w: Union[t
     if ready:
         _no_gradient(x, residual, gain)
     else:
-        _check_weight(x, w)
+        _check_weight(x, w, residual, gain)
         _lib.format_code(grad_dtype)
     if ready or (not torch.is_grad_enabled() and not _lib.forward_mode()):
         y, r = _lib.norm_linear_float8_infer(x, residual, gain, *(w if ready else to_float8(w)), eps)

@@ -189,3 +189,23 @@ def test_limits_agree_with_the_header():
     assert (value("GCG_PRODUCT8_MAX_K"), value("GCG_SCAN_MAX_TIME_STRIDE"), value("GCG_SCAN_MAX_WIDTH"), value("GCG_SCAN_MAX_ROWS")) == \
         (_lib.PRODUCT8_MAX_K, _lib.SCAN_MAX_TIME_STRIDE, _lib.SCAN_MAX_WIDTH, _lib.SCAN_MAX_ROWS)
     assert (value("GCG_E4M3"), value("GCG_E5M2")) == (_lib.GCG_E4M3, _lib.GCG_E5M2)
+
+
+def test_a_step_whose_gradients_sum_over_too_many_is_refused_before_it(gcg_lib):
+    """The weight's gradient sums over the rows and x's over the outputs, at most 2^22 of either: said by the forward, not after it."""
+    many = (1 << 22) + 1
+    x, w, wide = torch.zeros(many, 1).half(), torch.zeros(2, 1).half(), torch.zeros(many, 1).half()
+    needs = lambda t: t.clone().requires_grad_(True)                                                                           # noqa: E731
+    ops = torch.ops.gcg
+    for call in (lambda: linear_float8(x, needs(w)), lambda: linear_float8(x[:5].clone().requires_grad_(True), wide),
+                 lambda: linear_float8(x.reshape(1, many, 1), needs(w)), lambda: norm_linear_float8(x, None, needs(w)),
+                 lambda: norm_linear_float8(x[:5], needs(torch.ones(1).half()), wide), lambda: norm_linear_float8(x[:5], None, wide, residual=needs(x[:5])),
+                 lambda: ops.linear_float8(x, needs(w), E4M3), lambda: ops.linear_float8(needs(x[:5]), wide, E4M3),
+                 lambda: ops.norm_linear_float8(x, None, None, needs(w), 1e-6, E4M3)):
+        with pytest.raises((ValueError, RuntimeError), match="4194304"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="MI355X|CPU"):
+            call()                                                              # (nothing but the device is missing)
+    for call in (lambda: linear_float8(needs(x), w), lambda: linear_float8(x, wide), lambda: linear_float8(x[:-1], needs(w))):
+        with pytest.raises(RuntimeError, match="MI355X"):
+            call()
