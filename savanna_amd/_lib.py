@@ -288,6 +288,12 @@ def _run_plain(op, *args):
         return op(*args)
 
 
+def _refuse_lost_tangents(what: str, *args) -> None:
+    """The ctypes binding's part of ``_run_plain``."""
+    if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
+        refuse_tangents(what, *args)
+
+
 def native_nodes(t: torch.Tensor) -> bool:
     """Whether a layer's call on ``t`` may pass its Python autograd function by: the forward entry points below then hand a
     call whose gradients are recorded to the C++ form of that function (csrc/gcg_torch.cpp: same operators, same tensors
@@ -1449,6 +1455,7 @@ def rms_norm_float8(x, residual, w, eps: float):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.rms_norm_float8, x, residual, w, eps)
+    _refuse_lost_tangents("rms_norm_float8", x, residual, w)
     code = _rms_code(x, residual, w)
     codes, scales = _empty_float8(x.shape, torch.float8_e4m3fn, x.device)
     r = torch.empty_like(x) if residual is not None else None
@@ -1533,6 +1540,7 @@ def to_float8(x, format: torch.dtype):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.to_float8, x, format)
+    _refuse_lost_tangents("to_float8", x)
     _check_rows(x)
     f, code = format_code(format), dtype_code(x.dtype)
     codes, scales = _empty_float8(x.shape, format, x.device)
@@ -1644,6 +1652,7 @@ def linear_float8_infer(x, codes, scales, columns: int):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.linear_float8_infer, x, codes, scales, columns)
+    _refuse_lost_tangents("linear_float8_infer", x)
     _check_rows(x)
     _product_dtype(x.dtype)
     _check_float8(codes, scales, columns)
@@ -1666,6 +1675,7 @@ def norm_linear_float8_infer(x, residual, gain, codes, scales, columns: int, eps
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.norm_linear_float8_infer, x, residual, gain, codes, scales, columns, eps)
+    _refuse_lost_tangents("norm_linear_float8_infer", x, residual, gain)
     _product_dtype(x.dtype)
     a, a_scales, r, _ = rms_norm_float8(x, residual, gain, eps)
     if x.shape[-1] != columns:

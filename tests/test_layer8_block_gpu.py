@@ -360,3 +360,27 @@ def test_ctypes_binding_says_that_a_step_modifies_its_state(tmp_path):
             "else: raise AssertionError('a gradient of what is no longer there')\n"
             "with torch.inference_mode(): step(x, x, torch.zeros(3, 70, device='cuda:0'))\n") % os.path.dirname(here)
     subprocess.run([sys.executable, "-c", code], check=True, env={**os.environ, "GCG_BINDING": "ctypes"}, timeout=100)
+
+
+def test_ctypes_binding_refuses_tangents():
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys, torch; sys.path[:0] = [%r]\n"
+            "import torch.autograd.forward_ad as fwAD\n"
+            "from savanna_amd import _lib\n"
+            "from savanna_amd.operators.float8 import linear_float8, norm_linear_float8, to_float8\n"
+            "from savanna_amd.operators.norm import rms_norm_float8\n"
+            "from savanna_amd.operators.gated_recurrence import gated_recurrence_step\n"
+            "assert not _lib.TORCH_OPS\n"
+            "x, w = torch.randn(4, 300, device='cuda:0').bfloat16(), torch.randn(20, 300, device='cuda:0').bfloat16()\n"
+            "q, lost = to_float8(w), []\n"
+            "with fwAD.dual_level(), torch.no_grad():\n"
+            "    d = fwAD.make_dual(x, torch.ones_like(x))\n"
+            "    for name, f in dict(to_float8=lambda: to_float8(d), rms_norm_float8=lambda: rms_norm_float8(d), linear_float8=lambda: linear_float8(d, q),\n"
+            "                        norm_linear_float8=lambda: norm_linear_float8(x, None, q, residual=d), weight=lambda: rms_norm_float8(x, d[0]),\n"
+            "                        step=lambda: gated_recurrence_step(d, x, torch.zeros(4, 300, device='cuda:0'))).items():\n"
+            "        try: f()\n"
+            "        except NotImplementedError: continue\n"
+            "        lost.append(name)\n"
+            "    to_float8(x), rms_norm_float8(x), linear_float8(x, q), norm_linear_float8(x, None, q)\n"
+            "assert not lost, lost\n") % os.path.dirname(here)
+    subprocess.run([sys.executable, "-c", code], check=True, env={**os.environ, "GCG_BINDING": "ctypes"}, timeout=100)
