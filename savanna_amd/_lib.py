@@ -288,8 +288,8 @@ def _run_plain(op, *args):
         return op(*args)
 
 
-def _refuse_lost_tangents(what: str, *args) -> None:
-    """The ctypes binding's part of ``_run_plain``."""
+def refuse_lost_tangents(what: str, *args) -> None:
+    """``refuse_tangents`` for calls that may be traced: where a graph's end, or the ctypes binding, would drop them."""
     if forward_ad._current_level >= 0 and not torch.compiler.is_compiling():
         refuse_tangents(what, *args)
 
@@ -1455,7 +1455,7 @@ def rms_norm_float8(x, residual, w, eps: float):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.rms_norm_float8, x, residual, w, eps)
-    _refuse_lost_tangents("rms_norm_float8", x, residual, w)
+    refuse_lost_tangents("rms_norm_float8", x, residual, w)
     code = _rms_code(x, residual, w)
     codes, scales = _empty_float8(x.shape, torch.float8_e4m3fn, x.device)
     r = torch.empty_like(x) if residual is not None else None
@@ -1540,7 +1540,7 @@ def to_float8(x, format: torch.dtype):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.to_float8, x, format)
-    _refuse_lost_tangents("to_float8", x)
+    refuse_lost_tangents("to_float8", x)
     _check_rows(x)
     f, code = format_code(format), dtype_code(x.dtype)
     codes, scales = _empty_float8(x.shape, format, x.device)
@@ -1652,7 +1652,7 @@ def linear_float8_infer(x, codes, scales, columns: int):
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.linear_float8_infer, x, codes, scales, columns)
-    _refuse_lost_tangents("linear_float8_infer", x)
+    refuse_lost_tangents("linear_float8_infer", x)
     _check_rows(x)
     _product_dtype(x.dtype)
     _check_float8(codes, scales, columns)
@@ -1675,7 +1675,7 @@ def norm_linear_float8_infer(x, residual, gain, codes, scales, columns: int, eps
     _require_gpu(x)
     if TORCH_OPS:
         return _run_plain(torch.ops.gcg.norm_linear_float8_infer, x, residual, gain, codes, scales, columns, eps)
-    _refuse_lost_tangents("norm_linear_float8_infer", x, residual, gain)
+    refuse_lost_tangents("norm_linear_float8_infer", x, residual, gain)
     _product_dtype(x.dtype)
     a, a_scales, r, _ = rms_norm_float8(x, residual, gain, eps)
     if x.shape[-1] != columns:

@@ -35,7 +35,9 @@ def to_float8(x: torch.Tensor, dtype: torch.dtype = E4M3) -> Float8:
     at least, that brings the largest magnitude to at most 448 (``float8_e5m2``: 57344), and a code the element over it, rounded to nearest even.  A block
     that holds an infinity or a NaN has the scale 2^120 (``float8_e5m2``: 2^113); they become NaN (in ``float8_e5m2`` an infinity stays one) and
     numbers below 2^110 (2^96) zero.  Not differentiable: x's own graph is left alone."""
-    x = x.detach() if x.requires_grad else x
+    if x.requires_grad:
+        _lib.refuse_lost_tangents("to_float8", x)
+        x = x.detach()
     return Float8(*_lib.to_float8(x if x.is_contiguous() else x.contiguous(), dtype), x.shape[-1])
 
 

@@ -117,6 +117,7 @@ def rms_norm_float8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps:
     residual or the weight through it (``norm_linear_float8`` is the differentiable form, with the product).  r is, as the sum that it is."""
     recorded = residual is not None and torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad)
     if not recorded:
+        _lib.refuse_lost_tangents("rms_norm_float8", x, residual, weight)
         x, residual, weight = (t.detach() if t is not None and t.requires_grad else t for t in (x, residual, weight))
     x = x if x.is_contiguous() else x.contiguous()
     residual = residual if residual is None or residual.is_contiguous() else residual.contiguous()

@@ -384,3 +384,17 @@ def test_ctypes_binding_refuses_tangents():
             "    to_float8(x), rms_norm_float8(x), linear_float8(x, q), norm_linear_float8(x, None, q)\n"
             "assert not lost, lost\n") % os.path.dirname(here)
     subprocess.run([sys.executable, "-c", code], check=True, env={**os.environ, "GCG_BINDING": "ctypes"}, timeout=100)
+
+
+def test_no_lost_tangents_of_tensors_that_need_gradients():
+    """The graphs of these operators' arguments are left alone, their tangents are not."""
+    import torch.autograd.forward_ad as fwAD
+    x, w = (torch.randn(n, 300, device=DEV).bfloat16().requires_grad_(True) for n in (4, 1))
+    with fwAD.dual_level():
+        d, g = fwAD.make_dual(x, torch.ones_like(x)), fwAD.make_dual(w, torch.ones_like(w))[0]
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for f in (lambda: to_float8(d), lambda: rms_norm_float8(d), lambda: rms_norm_float8(x, g), lambda: rms_norm_float8(x.detach(), residual=d)):
+                    with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp|forward AD"):
+                        f()
+                to_float8(x), rms_norm_float8(x, w[0])
