@@ -349,3 +349,15 @@ def test_a_scale_that_is_no_number():
                 z = linear_float8(a, qb)
             bad[1], bad[:, 5] = False, True
             assert torch.equal(torch.isnan(z), bad) and torch.equal(z[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("M,N,K", [(1716, 1227, 15532), (1716, 1227, 15400), (274, 4257, 13982), (5149, 775, 16335), (2930, 795, 21788)])
+@pytest.mark.parametrize("fa,fb", [(E4M3, E4M3), (E5M2, E4M3), (E4M3, E5M2), (E5M2, E5M2)])
+def test_wide_tiles_in_parts(M, N, K, fa, fb):
+    """Weight gradients over many tokens: tiles of 256 x 256 in two to seven parts of the blocks, whose last has every length of the loop's rest
+    (test_product8_plan.py holds the plan)."""
+    a, b = whole(M, K, fa, K, 4), whole(N, K, fb, K + 1, 4)
+    want = a.float() @ b.float().t()                                # (fp32 holds these sums: below 2^15 * 16 * 16 = 2^23)
+    qa, qb = to_float8(a, fa), to_float8(b, fb)
+    for dtype in (torch.bfloat16, torch.float16, torch.bfloat16):
+        assert torch.equal(matmul_float8(qa, qb, dtype), want.to(dtype))

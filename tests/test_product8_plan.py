@@ -70,3 +70,33 @@ def test_what_a_tuning_build_is_told_is_taken_where_the_kernel_takes_it(plan):
             for parts in (None, -3, 0, 1, 2, 3, 7, 32, 1000, "x"):
                 check(M, N, K, plan(M, N, K, kernel, parts))
     assert plan(4096, 4096, 4096, WIDE, 2)[:2] == (WIDE, 2) and plan(8, 4096, 4096, TILE, 4)[:2] == (TILE, 4) and plan(100, 512, 512, TOKENS)[0] == TOKENS
+
+
+# Sizes at which the GPU tests check a kernel: by 256 x 256, by 256 x 128, by both, by 128 x 128, by groups of 64 rows; parts of the blocks
+PLANS = {
+    (4096, 4096, 128): (WIDE, 1, False), (3841, 4096, 640): (WIDE, 1, False), (4090, 4094, 1000): (WIDE, 1, False), (8200, 6000, 1300): (WIDE, 1, False),
+    (14673, 2327, 124): (WIDE, 1, False), (2357, 3272, 242): (WIDE, 1, False),
+    (1716, 1227, 15532): (WIDE, 4, False), (1716, 1227, 15400): (WIDE, 4, False), (274, 4257, 13982): (WIDE, 7, False), (5149, 775, 16335): (WIDE, 2, False),
+    (2930, 795, 21788): (WIDE, 4, False),
+    (12000, 11500, 1300): (WIDE, 1, True), (5003, 7683, 1301): (WIDE, 1, True), (70000, 257, 1300): (WIDE, 1, True), (16700, 1025, 900): (WIDE, 1, True),
+    (2048, 4096, 128): (TALL, 1, False), (1900, 3970, 1101): (TALL, 1, False), (7675, 2057, 766): (TALL, 1, False), (2040, 2048, 16384): (TALL, 2, False),
+    (1300, 2000, 7001): (TALL, 2, False), (600, 600, 17000): (TALL, 12, False),
+    (606, 11384, 1158): (TILE, 1, False), (150, 15000, 10000): (TILE, 2, False), (67, 14005, 6507): (TILE, 4, False), (200, 300, 20000): (TILE, 20, False),
+    (65, 64, 100): (TOKENS, 1, False), (300, 200, 5000): (TOKENS, 1, False), (1000, 1000, 8200): (TOKENS, 1, False), (1100, 33, 2000): (TOKENS, 1, False),
+    (1, 4097, 32768): (TOKENS, 1, False), (64, 9000, 16384): (TOKENS, 1, False),
+}
+
+
+@pytest.mark.parametrize("size", PLANS)
+def test_sizes_go_by_the_kernel_that_they_check(plan, size):
+    """A size that goes by another kernel after a change of the estimates leaves its kernel without this test: choose another one."""
+    kernel, parts, _, rest = plan(*size)
+    assert (kernel, parts, rest > 0) == PLANS[size]
+
+
+def test_the_parts_of_wide_tiles_end_in_every_rest_of_their_loop(plan):
+    ends = set()
+    for (M, N, K), (kernel, parts, _) in PLANS.items():
+        if kernel == WIDE and parts > 1:
+            ends.add(((K + 127) // 128 - (parts - 1) * plan(M, N, K)[2]) % 4)
+    assert ends == {0, 1, 2, 3}
