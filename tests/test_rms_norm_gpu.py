@@ -215,3 +215,18 @@ def test_the_stream_beside_8_bits_is_captured():
         res.detach() + 1
         rms_norm_float8(x, w, residual=res)
     del lives
+
+
+@pytest.mark.parametrize("dtype,wtype", TYPES)
+@pytest.mark.parametrize("rows,D", [(1, 1), (3, 7), (5, 128), (2, 511), (70, 513), (33, 1001), (23, 2054), (9, 2048), (5, 4096), (3, 8200), (2, 16384)])
+def test_output_in_8_bits_without_a_residual(rows, D, dtype, wtype):
+    """Tolerance and the share of other codes as with one."""
+    x, _, w, dy, _ = data((rows, D), dtype, wtype, seed=D + 1)
+    q = rms_norm_float8(x, w)
+    assert q.columns == D and q.codes.shape == (rows, (D + 127) // 128 * 128) and q.scales.shape == (rows, (D + 511) // 512 * 4)
+    assert not q.codes.view(torch.uint8)[:, D:].any() and (q.scales.view(torch.uint8)[:, (D + 127) // 128:] == 127).all()
+    y = reference(x, w, dy, None, 1e-6)[0][0]
+    ref, e = float8(y)
+    scale = torch.ldexp(torch.ones_like(e, dtype=torch.float64), e + 1).repeat_interleave(128, -1)[:, :D]
+    check(values(q), y, 2.0 ** -4 * y.abs() + 2.0 ** -10 * scale + F32 * y.abs(), "8 bits")
+    assert (values(q) != ref).double().mean() <= 2.0 ** -10 + 2 / ref.numel()
