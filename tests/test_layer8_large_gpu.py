@@ -75,9 +75,10 @@ def test_into_8_bits_and_back():
     assert not bits(codes_t[:, ROWS:]).any() and (bits(scales_t)[:, (ROWS + 127) // 128:] == 127).all()
 
 
-@pytest.mark.parametrize("M,N,K", [(70001, 32800, 200), (ROWS, 260, 4096), (129, ROWS, 4100)])
+@pytest.mark.parametrize("M,N,K", [(70001, 32800, 200), (ROWS, 260, 4096), (129, ROWS, 4100), (300, 300, 1 << 22), (70, 130, (1 << 22) - 100)])
 def test_products(M, N, K):
-    """Whole numbers, whose sums are exact: results, one operand or the other beyond 2^31."""
+    """Whole numbers, whose sums are exact (random ones of 2^22 products stay far below 2^24): results, one operand or the other beyond 2^31, and the longest
+    sums."""
     gen = torch.Generator(device=DEV).manual_seed(K)
     a, b = (torch.randint(-4, 5, (n, K), generator=gen, device=DEV, dtype=torch.int8).to(torch.bfloat16) for n in (M, N))
     y = matmul_float8(to_float8(a), to_float8(b))
