@@ -29,8 +29,9 @@ template <bool E5M2> __device__ __forceinline__ uint32_t f8_scale(uint32_t top)
 }
 // 2^(127 - b), which brings the block into range
 __device__ __forceinline__ float f8_down(uint32_t b) { return __uint_as_float((254u - b) << 23); }
-// 2^(b - 127); the byte 255, which no quantiser here writes, is no number, whatever it multiplies
-__device__ __forceinline__ float f8_up(uint32_t b) { return b == 255 ? __uint_as_float(0x7fc00000u) : b ? __uint_as_float(b << 23) : 0x1p-127f; }
+// 2^(b - 127), whose lowest is subnormal; the byte 255, which no quantiser here writes, is no number, whatever it multiplies.  (Both are the shifted
+// byte with the fraction's first bit set.)
+__device__ __forceinline__ float f8_up(uint32_t b) { return __uint_as_float(b << 23 | (b - 1u >= 254u ? 1u << 22 : 0u)); }
 
 // four codes in a word, rounded to nearest even; what is beyond the range is NaN (5 bits of exponent: infinity)
 template <bool E5M2> __device__ __forceinline__ uint32_t f8_codes(float a, float b, float c, float d, float down)
