@@ -525,8 +525,8 @@ template <typename T, bool GATE> __global__ __launch_bounds__(256) void scan_ste
 {
     const int ch = blockIdx.x * 256 + threadIdx.x;
     if (ch >= p.D) return;
-    for (int64_t b = blockIdx.y; b < p.bs; b += gridDim.y) {         // (a step beyond the last entry may pass 2^31)
-        const int64_t i = b * p.D + ch;
+    for (uint32_t b = blockIdx.y; b < (uint32_t)p.bs; b += gridDim.y) {         // (a step beyond the last entry may pass 2^31)
+        const int64_t i = (int64_t)b * p.D + ch;
         const float x = Elem<T>::load((const T *)p.x + b * p.sx + ch), f = Elem<T>::load((const T *)p.f + b * p.sf + ch);
         const float g = GATE ? Elem<T>::load((const T *)p.gate + b * p.sg + ch) : 1.f, before = p.state[i];
         float a, u;
