@@ -17,7 +17,10 @@
 // tickets earlier, are at work, and wait for earlier ones at most: every wait ends.
 //
 // Measured: 2 x 8192 x 4096 bf16 forward 117 us (4.7 TB/s), backward 204 + 4 for the bias (4.8), and 4 + 6 for clearing the words; 1 x 131072 x 512 fp32
-// forward 193 (5.6); 4 x 701 x 2560 f16 15.4: one after the other, all rows' arrival, the sums, the words' way, and all rows' leaving.
+// forward 193 (5.6); 4 x 701 x 2560 f16 16 (15.3 to 17.6): one after the other, all rows' arrival, the sums, the words' way, and all rows' leaving.  Rows off
+// the lines of memory take longer, and those on 2 bytes, one channel a lane, longest: of 4096, 4094, 4095 channels forward 119, 148, 168, backward 205, 291,
+// 369, with the clearing.  A token of 64, 256, 512, 1024 x 8192 bf16, launches
+// after each other on the same tensors: 4, 5.6, 13, 22.
 //
 // The backward needs the states inside a chunk again; the forward keeps the one before every kChunk rows (1 / 32 of a
 // 16-bit tensor), and the rest is made again from x and f, which it reads anyway.
@@ -540,7 +543,7 @@ template <typename T, bool GATE> __global__ __launch_bounds__(256) void scan_ste
 // ---- launches ---------------------------------------------------------------------------------------------------------------------
 // Rows of a chunk of the forward: 128, two workgroups a CU, which overlap one's loads with the other's sums.  256, one workgroup a CU, where the card
 // holds all of those at once and they are whole sequences, or those of 128 more than a CU's one or very many: what counts then is the chain of waits.
-// In chunks of 128 and 256: 4 x 701 x 2560 f16 17.8 and 15.9 us, 1 x 8192 x 1024 bf16 28.6 and 23.4, 16 x 256 x 1024 fp32 22.7 and 11.9; but
+// In chunks of 128 and 256, launches after each other: 4 x 701 x 2560 f16 17.8 and 15.9 us, 1 x 8192 x 1024 bf16 28.6 and 23.4, 16 x 256 x 1024 fp32 22.7 and 11.9; but
 // 1 x 512 x 4096 14.1 and 16.1, 64 x 256 x 4096 112 and 122, 2 x 8192 x 4096 118 and 131.  So also with many chunks after each other: 32768 x 128 fp32 36
 // and 25, 16384 x 256 bf16 26 and 23, 8192 x 512 20 and 21.
 int fwd_rows(int64_t bs, int64_t L, int64_t D)
