@@ -178,7 +178,7 @@ class LinearFloat8(nn.Module):
 
     ``lay_out()`` quantises the weight once for calls without gradients, as a serving program does after loading; until then, and after ``train()``,
     a move or cast of the module, ``load_state_dict`` or any change of the weight that torch counts, every call quantises it.  (It counts none that goes
-    by ``weight.data``, by a pointer, of a weight made in inference mode, or inside a traced program: call it again then.)"""
+    by ``weight.data``, a pointer or a replayed graph, of a weight made in inference mode, or inside a traced program: call it again then.)"""
 
     _laid_out_of = None             # the weight that was laid out, and torch's count of its modifications then
 
